@@ -41,6 +41,7 @@ typedef int trx_status;
 #define TRX_DEV_TIMEOUT    0x4u
 #define TRX_DEV_INTERNAL   0x8u   /* a launch found shared memory laid out unlike its plan */
 #define TRX_DEV_RANGE      0x10u  /* an index read from device memory (a position) was out of range */
+#define TRX_DEV_PAGES      0x20u  /* a page plan asked for more pages than are free */
 
 #define TRX_KIND_TERNARY   0    /* KIND_TERNARY,  model/layout.py:46 */
 #define TRX_KIND_Q8        1    /* KIND_Q8,       model/layout.py:47 (int8 weights, group 32) */
@@ -490,6 +491,120 @@ trx_status trx_attn_decode_tp(trx_ctx *ctx, const trx_attn_shape *shape, const f
                               const float *d_v, const float *d_qnorm_w, const float *d_knorm_w,
                               const float *d_rope_freq, void *d_kcache, void *d_vcache, const int32_t *d_pos,
                               float *d_out, const trx_tp_xfer *tp, cudaStream_t stream);
+
+/*
+ * Paged KV cache: many sequences of unequal lengths share a pool of pages (no counterpart in the
+ * reference, which decodes one sequence).  The pools of a layer are kpages and vpages
+ * [n_pages][page][n_kv][head_dim], 16-bit elements, 16-byte aligned; position p of sequence b lives
+ * in page tables[b][p / page] at p % page.  A step brings new rows for some sequences; row r of the
+ * step's tensors belongs to the sequence b with cu[b] <= r < cu[b + 1] and sits at position pos[r],
+ * cache slot slots[r] = page id * page + offset.
+ */
+#define TRX_TYPE_F32  0
+#define TRX_TYPE_F16  1
+#define TRX_TYPE_BF16 2
+
+typedef struct trx_pages {
+    uint32_t nseq;       /* sequences, at most 1024                                          */
+    uint32_t max_rows;   /* rows that slots and pos hold, at most 2^22                       */
+    uint32_t page;       /* positions per page: a power of two from 16 to 1024               */
+    uint32_t max_pages;  /* entries of a table row, at most 2^20; max_pages * page < 2^31    */
+    uint32_t n_pages;    /* pages of the pool; n_pages * page < 2^31                         */
+    int32_t *tables;     /* [nseq][max_pages] page ids                                       */
+    int32_t *lens;       /* [nseq] positions in the cache after the step                     */
+    int32_t *cu;         /* [nseq + 1] first row of every sequence, then the number of rows  */
+    int32_t *slots;      /* [max_rows] cache slot of every row                               */
+    int32_t *pos;        /* [max_rows] position of every row                                 */
+    int32_t *last;       /* [nseq] the sequence's last row (0 for one without rows)          */
+    int32_t *n_free;     /* [1] free pages left                                              */
+} trx_pages;
+
+/*
+ * The plan of a step, from the lengths alone, in one launch: sequence b has d_cached[b] positions in
+ * the cache and brings d_new[b] >= 0 more.  Its table's first ceil(cached / page) entries are read;
+ * if it has new rows the entries up to ceil((cached + new) / page) are filled with pages from the
+ * top of the free stack (d_free[0 .. *d_n_free), sequence after sequence).  Writes those table
+ * entries, lens, cu, slots, pos, last and n_free; slots and pos behind the last row and all other
+ * table entries are left as they were, d_free too.  d_cached may be pages->lens and d_n_free
+ * pages->n_free (a plan in place); otherwise the same call again gives the same plan.
+ * A negative or too large length, or more rows than max_rows, sets TRX_DEV_RANGE, too few free pages
+ * TRX_DEV_PAGES: cu and last are then zero (the step's other calls do nothing), lens is d_cached,
+ * n_free is *d_n_free.  A free-stack or table entry outside [0, n_pages) sets TRX_DEV_RANGE; its rows'
+ * slots are -1.
+ */
+trx_status trx_paged_plan(trx_ctx *ctx, const trx_pages *pages, const int32_t *d_cached, const int32_t *d_new,
+                          const int32_t *d_free, const int32_t *d_n_free, cudaStream_t stream);
+
+/*
+ * Give back the pages of the sequences with d_done[b] != 0: their ceil(d_lens[b] / page) pages go on
+ * top of the free stack d_free (room for n_pages) in sequence and table order, *d_n_free grows, the
+ * entries become -1 and d_lens[b] 0.  If the stack would overflow, or a table entry is outside
+ * [0, n_pages), TRX_DEV_RANGE is set and nothing changes.  Uses pages->tables only.
+ */
+trx_status trx_paged_release(trx_ctx *ctx, const trx_pages *pages, const int32_t *d_done, int32_t *d_lens,
+                             int32_t *d_free, int32_t *d_n_free, cudaStream_t stream);
+
+typedef struct trx_paged_shape {
+    uint32_t n_head;     /* query heads H                                                        */
+    uint32_t n_kv;       /* kv heads; H / n_kv is a whole number, at most 16                     */
+    uint32_t head_dim;   /* 64, 128 or 256                                                       */
+    uint32_t rope_dims;  /* rotated dims per head, a multiple of 8, <= head_dim                  */
+    int32_t  gated;      /* q rows hold [q | gate] per head: out *= sigmoid(gate)                */
+    float    eps;        /* epsilon of the q/k RMSNorms                                          */
+    uint32_t window;     /* 0: every earlier position is visible; else only the last `window`,   */
+    uint32_t sinks;      /*    the query's own among them, and the first `sinks` of the sequence */
+} trx_paged_shape;
+
+/*
+ * The new rows into the paged cache, and the queries ready for trx_attn_paged, in one launch:
+ * q[h] = RoPE(RMSNorm(q[h]) * qnorm_w), k = RoPE(RMSNorm(k) * knorm_w) (neox pairs over the first
+ * rope_dims, angle fp32(pos * rope_freq[i]), as trx_attn_decode), k and v rounded to cache_type and
+ * stored at the rows' slots, q to q_type in d_q_out [rows][H][head_dim].  d_q: rows of
+ * H * (gated ? 2 : 1) * head_dim floats at a row stride of q_ld floats; d_k, d_v: n_kv * head_dim at
+ * k_ld, v_ld; all 16-byte aligned, strides multiples of 4.  Rows are cu[nseq] at most max_rows; q_out
+ * behind them is left as it was.  A slot outside the pool sets TRX_DEV_RANGE and stores nothing.
+ * cache_type: TRX_TYPE_F16 or TRX_TYPE_BF16; q_type: the cache's type or TRX_TYPE_F32.
+ */
+trx_status trx_paged_append(trx_ctx *ctx, const trx_paged_shape *shape, const trx_pages *pages, const float *d_q,
+                            uint64_t q_ld, const float *d_k, uint64_t k_ld, const float *d_v, uint64_t v_ld,
+                            const float *d_qnorm_w, const float *d_knorm_w, const float *d_rope_freq, void *d_kpages,
+                            void *d_vpages, int32_t cache_type, void *d_q_out, int32_t q_type, cudaStream_t stream);
+
+/*
+ * Causal attention of every sequence's new rows over its pages, in one launch: row r of sequence b,
+ * head h (kv head h / (H / n_kv)), sees the positions j <= pos with pos - j < window or j < sinks
+ * (all when window is 0): out[r][h] = softmax(q . K^T / sqrt(head_dim)) V, times sigmoid(gate) when
+ * gated.  Decode (one new row), a prompt's chunk and a mixture of both are the same call.
+ * d_q [rows][H][head_dim] of q_type (as trx_paged_append writes it), d_out the same shape and type.
+ * q_type fp32 (fp16 cache only): queries and softmax weights enter the tensor cores as two fp16 parts
+ * each, so the result has fp32 rounding; 16-bit q_type (the cache's type): the weights are rounded to
+ * that type.  Sums, maxima and the output before its rounding are fp32 in both.  d_gate (NULL unless
+ * gated): the rows of d_q given to trx_paged_append, stride gate_ld floats.  max_new: a bound on the
+ * new rows of any sequence (rows only; it picks the kernel).  What the pools hold behind a sequence's
+ * length is never used; the positions below it have to be finite.  A sequence whose cu, lens or
+ * max_new do not fit sets TRX_DEV_RANGE and its rows are left as they were; a table entry outside
+ * [0, n_pages) sets TRX_DEV_RANGE and reads as zeros.  Rows behind the last are left as they were.
+ * Launches on the context's scratch: calls on one context must not overlap.
+ */
+trx_status trx_attn_paged(trx_ctx *ctx, const trx_paged_shape *shape, const trx_pages *pages, const void *d_q,
+                          int32_t q_type, const float *d_gate, uint64_t gate_ld, const void *d_kpages,
+                          const void *d_vpages, int32_t cache_type, uint32_t max_new, void *d_out,
+                          cudaStream_t stream);
+
+/*
+ * One token per row of logits [nrows][V] (type, row stride ld elements) with the row's own settings
+ * and random number (arrays of nrows): the tokens in descending order of logit, ties by index; of
+ * them the first top_k (<= 0: all); with weights exp((logit - max) / temperature), of those the
+ * shortest prefix whose share of the weight reaches top_p (>= 1: all); of those the ones with weight
+ * >= min_p (the largest weight is 1).  The token is the first, in index order, at which the running
+ * weight exceeds u times the weight of all kept (u in [0, 1)).  temperature <= 0: the largest logit,
+ * ties to the smallest index (as trx_argmax_rows).  NaN logits count as -inf; a row with no logit
+ * above -inf gives -1.  Weights are summed as integers (steps of 2^-40 or finer of the largest),
+ * so the token does not depend on the order of the sums.  V <= 2^22.  One launch, no scratch.
+ */
+trx_status trx_sample_rows(trx_ctx *ctx, const void *d_logits, int32_t type, uint64_t ld, uint32_t V, uint32_t nrows,
+                           const float *d_u, const float *d_temperature, const int32_t *d_top_k, const float *d_top_p,
+                           const float *d_min_p, int32_t *d_tokens, cudaStream_t stream);
 
 #ifdef __cplusplus
 }

@@ -15,7 +15,8 @@ ERRORS = {
     -1: "TRX_ERR_ARG", -2: "TRX_ERR_LAYOUT", -3: "TRX_ERR_OVERFLOW", -4: "TRX_ERR_CUDA",
     -5: "TRX_ERR_TIMEOUT", -6: "TRX_ERR_UNSUPPORTED",
 }
-DEV_OVERFLOW, DEV_BADBYTE, DEV_TIMEOUT, DEV_INTERNAL, DEV_RANGE = 0x1, 0x2, 0x4, 0x8, 0x10
+DEV_OVERFLOW, DEV_BADBYTE, DEV_TIMEOUT, DEV_INTERNAL, DEV_RANGE, DEV_PAGES = 0x1, 0x2, 0x4, 0x8, 0x10, 0x20
+TYPE_F32, TYPE_F16, TYPE_BF16 = 0, 1, 2
 
 # Every symbol the header declares (tests check the library exports all of them).
 SYMBOLS = (
@@ -29,7 +30,8 @@ SYMBOLS = (
     "trx_attn_decode_f32cache", "trx_matvec_f_rows", "trx_embed_lookup_rows", "trx_rmsnorm_rows", "trx_silu_mul",
     "trx_argmax_rows", "trx_advance_positions", "trx_attn_decode_rows", "trx_deltanet_step_rows",
     "trx_deltanet_int_step", "trx_matvec_fp_rows", "trx_matvec_f_rows_multi", "trx_deltanet_step_tp",
-    "trx_matvec_f_kseg_tp", "trx_matvec_f_rows_kseg",
+    "trx_matvec_f_kseg_tp", "trx_matvec_f_rows_kseg", "trx_paged_plan", "trx_paged_release", "trx_paged_append",
+    "trx_attn_paged", "trx_sample_rows",
 )
 
 TP_MAX = 8
@@ -49,7 +51,8 @@ class TrxDeviceError(RuntimeError):
         names = [n for b, n in ((DEV_OVERFLOW, "overflow"), (DEV_BADBYTE, "invalid trit5 byte"),
                                 (DEV_TIMEOUT, "bounded wait timed out"),
                                 (DEV_INTERNAL, "shared-memory layout mismatch"),
-                                (DEV_RANGE, "device-side index out of range")) if bits & b]
+                                (DEV_RANGE, "device-side index out of range"),
+                                (DEV_PAGES, "no free cache pages left")) if bits & b]
         super().__init__("device error: " + ", ".join(names or [hex(bits)]))
 
 
@@ -64,6 +67,21 @@ class DeltaNetShape(ctypes.Structure):
     """trx_deltanet_shape: one gated-DeltaNet layer's geometry."""
     _fields_ = [("n_k_heads", ctypes.c_uint32), ("k_head_dim", ctypes.c_uint32), ("n_v_heads", ctypes.c_uint32),
                 ("v_head_dim", ctypes.c_uint32), ("conv_kernel", ctypes.c_uint32), ("eps", ctypes.c_float)]
+
+
+class Pages(ctypes.Structure):
+    """trx_pages: the block tables of a paged KV cache and the plan of a step."""
+    _fields_ = [("nseq", ctypes.c_uint32), ("max_rows", ctypes.c_uint32), ("page", ctypes.c_uint32),
+                ("max_pages", ctypes.c_uint32), ("n_pages", ctypes.c_uint32), ("tables", ctypes.c_void_p),
+                ("lens", ctypes.c_void_p), ("cu", ctypes.c_void_p), ("slots", ctypes.c_void_p),
+                ("pos", ctypes.c_void_p), ("last", ctypes.c_void_p), ("n_free", ctypes.c_void_p)]
+
+
+class PagedShape(ctypes.Structure):
+    """trx_paged_shape: one attention layer's geometry over a paged cache."""
+    _fields_ = [("n_head", ctypes.c_uint32), ("n_kv", ctypes.c_uint32), ("head_dim", ctypes.c_uint32),
+                ("rope_dims", ctypes.c_uint32), ("gated", ctypes.c_int32), ("eps", ctypes.c_float),
+                ("window", ctypes.c_uint32), ("sinks", ctypes.c_uint32)]
 
 
 class TpXfer(ctypes.Structure):
@@ -99,6 +117,8 @@ def lib():
         L = ctypes.CDLL(LIB_PATH)
         E = ctypes.POINTER(Entry)
         T = ctypes.POINTER(TpXfer)
+        P = ctypes.POINTER(Pages)
+        PS = ctypes.POINTER(PagedShape)
         sig = {
             "trx_create": ([ctypes.POINTER(_vp), ctypes.c_int], ctypes.c_int),
             "trx_destroy": ([_vp], ctypes.c_int),
@@ -160,6 +180,14 @@ def lib():
             "trx_matvec_fp_rows": ([_vp, E, _vp, _vp, ctypes.c_int32, _vp, _vp, _vp], ctypes.c_int),
             "trx_matvec_f_rows_multi": ([_vp, E, ctypes.c_int, _vp, _vp, ctypes.c_int, _vp, ctypes.c_float, _vp, _vp,
                                          _vp], ctypes.c_int),
+            "trx_paged_plan": ([_vp, P, _vp, _vp, _vp, _vp, _vp], ctypes.c_int),
+            "trx_paged_release": ([_vp, P, _vp, _vp, _vp, _vp, _vp], ctypes.c_int),
+            "trx_paged_append": ([_vp, PS, P, _vp, ctypes.c_uint64, _vp, ctypes.c_uint64, _vp, ctypes.c_uint64, _vp,
+                                  _vp, _vp, _vp, _vp, ctypes.c_int32, _vp, ctypes.c_int32, _vp], ctypes.c_int),
+            "trx_attn_paged": ([_vp, PS, P, _vp, ctypes.c_int32, _vp, ctypes.c_uint64, _vp, _vp, ctypes.c_int32,
+                                ctypes.c_uint32, _vp, _vp], ctypes.c_int),
+            "trx_sample_rows": ([_vp, _vp, ctypes.c_int32, ctypes.c_uint64, ctypes.c_uint32, ctypes.c_uint32, _vp, _vp,
+                                 _vp, _vp, _vp, _vp, _vp], ctypes.c_int),
         }
         for name, (args, res) in sig.items():
             fn = getattr(L, name)

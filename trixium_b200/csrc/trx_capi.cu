@@ -1,4 +1,5 @@
 // C ABI of libtrixium_b200.so (declarations and contracts in include/trixium_b200.h).
+#include <cmath>
 #include <cstdint>
 #include <cstdlib>
 #include <new>
@@ -898,6 +899,159 @@ static trx_status deltanet_step(trx_ctx *ctx, const trx_deltanet_shape *sh, int3
     if (trx_status st = tp_resolve(tp, TP_PUSH, A.tp)) return st;
     if (A.tp.world && (nseq != 1 || A.tp.tag_out < 0)) return TRX_ERR_UNSUPPORTED;  // tagged words, one sequence
     return trx::launch_deltanet(A, ctx->err, stream);
+}
+
+static trx_status check_pages(const trx_pages *P) {
+    if (!P || P->nseq == 0 || P->max_rows == 0 || P->max_pages == 0 || P->n_pages == 0) return TRX_ERR_ARG;
+    if (P->page < 16 || P->page > 1024 || (P->page & (P->page - 1))) return TRX_ERR_UNSUPPORTED;
+    if (P->nseq > 1024 || P->max_rows > (1u << 22) || P->max_pages > (1u << 20)) return TRX_ERR_UNSUPPORTED;
+    if ((uint64_t)P->max_pages * P->page >= (1ull << 31) || (uint64_t)P->n_pages * P->page >= (1ull << 31))
+        return TRX_ERR_UNSUPPORTED;
+    if (!P->tables) return TRX_ERR_ARG;
+    return TRX_OK;
+}
+
+static trx_status check_paged_shape(const trx_paged_shape *sh) {
+    if (!sh || sh->n_head == 0 || sh->n_kv == 0 || sh->n_head % sh->n_kv || !(sh->eps >= 0.f)) return TRX_ERR_ARG;
+    if (sh->rope_dims > sh->head_dim) return TRX_ERR_ARG;
+    if (sh->head_dim != 64 && sh->head_dim != 128 && sh->head_dim != 256) return TRX_ERR_UNSUPPORTED;
+    if (sh->rope_dims % 8 || sh->n_head / sh->n_kv > 16 || sh->n_head > 1024) return TRX_ERR_UNSUPPORTED;
+    if (sh->window > (1u << 30) || sh->sinks > (1u << 30)) return TRX_ERR_UNSUPPORTED;
+    return TRX_OK;
+}
+
+static trx_status check_paged_types(int32_t cache_type, int32_t q_type) {
+    if (cache_type != TRX_TYPE_F16 && cache_type != TRX_TYPE_BF16) return TRX_ERR_ARG;
+    if (q_type != TRX_TYPE_F32 && q_type != cache_type) return TRX_ERR_ARG;
+    return TRX_OK;
+}
+
+trx_status trx_paged_plan(trx_ctx *ctx, const trx_pages *pages, const int32_t *d_cached, const int32_t *d_new,
+                          const int32_t *d_free, const int32_t *d_n_free, cudaStream_t stream) {
+    if (!ctx) return TRX_ERR_ARG;
+    if (trx_status s = check_pages(pages)) return s;
+    if (!d_cached || !d_new || !d_free || !d_n_free || !pages->lens || !pages->cu || !pages->slots || !pages->pos ||
+        !pages->last || !pages->n_free)
+        return TRX_ERR_ARG;
+    return trx::launch_paged_plan(*pages, d_cached, d_new, d_free, d_n_free, ctx->err, stream);
+}
+
+trx_status trx_paged_release(trx_ctx *ctx, const trx_pages *pages, const int32_t *d_done, int32_t *d_lens,
+                             int32_t *d_free, int32_t *d_n_free, cudaStream_t stream) {
+    if (!ctx) return TRX_ERR_ARG;
+    if (trx_status s = check_pages(pages)) return s;
+    if (!d_done || !d_lens || !d_free || !d_n_free) return TRX_ERR_ARG;
+    return trx::launch_paged_release(*pages, d_done, d_lens, d_free, d_n_free, ctx->err, stream);
+}
+
+trx_status trx_paged_append(trx_ctx *ctx, const trx_paged_shape *sh, const trx_pages *pages, const float *d_q,
+                            uint64_t q_ld, const float *d_k, uint64_t k_ld, const float *d_v, uint64_t v_ld,
+                            const float *d_qnorm_w, const float *d_knorm_w, const float *d_rope_freq, void *d_kpages,
+                            void *d_vpages, int32_t cache_type, void *d_q_out, int32_t q_type, cudaStream_t stream) {
+    if (!ctx) return TRX_ERR_ARG;
+    if (trx_status s = check_pages(pages)) return s;
+    if (trx_status s = check_paged_shape(sh)) return s;
+    if (trx_status s = check_paged_types(cache_type, q_type)) return s;
+    if (!d_q || !d_k || !d_v || !d_qnorm_w || !d_knorm_w || !d_kpages || !d_vpages || !d_q_out || !pages->cu ||
+        !pages->slots || !pages->pos || (sh->rope_dims && !d_rope_freq))
+        return TRX_ERR_ARG;
+    if (!aligned16(d_q) || !aligned16(d_k) || !aligned16(d_v) || !aligned16(d_qnorm_w) || !aligned16(d_knorm_w) ||
+        !aligned16(d_kpages) || !aligned16(d_vpages) || !aligned16(d_q_out))
+        return TRX_ERR_ARG;
+    const uint64_t qw = (uint64_t)sh->n_head * sh->head_dim * (sh->gated ? 2 : 1), kw = (uint64_t)sh->n_kv * sh->head_dim;
+    if (q_ld < qw || k_ld < kw || v_ld < kw || q_ld % 4 || k_ld % 4 || v_ld % 4) return TRX_ERR_ARG;
+    if (q_ld > (1ull << 40) || k_ld > (1ull << 40) || v_ld > (1ull << 40)) return TRX_ERR_UNSUPPORTED;
+    trx::PgAppendArgs A{};
+    A.q = d_q;
+    A.k = d_k;
+    A.v = d_v;
+    A.qn = d_qnorm_w;
+    A.kn = d_knorm_w;
+    A.freq = d_rope_freq;
+    A.q_ld = (long long)q_ld;
+    A.k_ld = (long long)k_ld;
+    A.v_ld = (long long)v_ld;
+    A.kp = d_kpages;
+    A.vp = d_vpages;
+    A.q_out = d_q_out;
+    A.cu = pages->cu;
+    A.slots = pages->slots;
+    A.pos = pages->pos;
+    A.nseq = (int)pages->nseq;
+    A.max_rows = (int)pages->max_rows;
+    A.H = (int)sh->n_head;
+    A.Hkv = (int)sh->n_kv;
+    A.hd = (int)sh->head_dim;
+    A.half = (int)sh->rope_dims / 2;
+    A.gated = sh->gated ? 1 : 0;
+    A.n_slots = (int)(pages->n_pages * pages->page);
+    A.eps = sh->eps;
+    return trx::launch_paged_append(A, cache_type, q_type, ctx->err, stream);
+}
+
+trx_status trx_attn_paged(trx_ctx *ctx, const trx_paged_shape *sh, const trx_pages *pages, const void *d_q,
+                          int32_t q_type, const float *d_gate, uint64_t gate_ld, const void *d_kpages,
+                          const void *d_vpages, int32_t cache_type, uint32_t max_new, void *d_out,
+                          cudaStream_t stream) {
+    if (!ctx) return TRX_ERR_ARG;
+    if (trx_status s = check_pages(pages)) return s;
+    if (trx_status s = check_paged_shape(sh)) return s;
+    if (trx_status s = check_paged_types(cache_type, q_type)) return s;
+    if (!d_q || !d_kpages || !d_vpages || !d_out || !pages->cu || !pages->lens || max_new == 0) return TRX_ERR_ARG;
+    if (!aligned16(d_q) || !aligned16(d_kpages) || !aligned16(d_vpages) || !aligned16(d_out) || !aligned16(d_gate))
+        return TRX_ERR_ARG;
+    if (q_type == TRX_TYPE_F32 && cache_type != TRX_TYPE_F16) return TRX_ERR_UNSUPPORTED;
+    if ((sh->gated != 0) != (d_gate != nullptr)) return TRX_ERR_ARG;
+    if (d_gate && (gate_ld < 2ull * sh->n_head * sh->head_dim || gate_ld % 4)) return TRX_ERR_ARG;
+    if (gate_ld > (1ull << 40)) return TRX_ERR_UNSUPPORTED;
+    trx::PgAttnArgs A{};
+    A.q = d_q;
+    A.gate = d_gate;
+    A.gate_ld = (long long)gate_ld;
+    A.kp = d_kpages;
+    A.vp = d_vpages;
+    A.tables = pages->tables;
+    A.lens = pages->lens;
+    A.cu = pages->cu;
+    A.out = d_out;
+    A.part = ctx->attn_part;
+    A.cnt = ctx->attn_cnt;
+    A.nseq = (int)pages->nseq;
+    A.max_rows = (int)pages->max_rows;
+    A.max_new = (int)(max_new < pages->max_rows ? max_new : pages->max_rows);
+    A.page_shift = 0;
+    while ((1u << A.page_shift) < pages->page) ++A.page_shift;
+    A.max_pages = (int)pages->max_pages;
+    A.n_pages = (int)pages->n_pages;
+    A.H = (int)sh->n_head;
+    A.Hkv = (int)sh->n_kv;
+    A.rep = A.H / A.Hkv;
+    A.window = (int)sh->window;
+    A.sinks = (int)sh->sinks;
+    A.scale_log2 = (float)(1.4426950408889634 / sqrt((double)sh->head_dim));
+    return trx::launch_attn_paged(A, (int)sh->head_dim, cache_type, q_type, kAttnPartFloats, (int)kAttnMaxKv, ctx->err,
+                                  stream);
+}
+
+trx_status trx_sample_rows(trx_ctx *ctx, const void *d_logits, int32_t type, uint64_t ld, uint32_t V, uint32_t nrows,
+                           const float *d_u, const float *d_temperature, const int32_t *d_top_k, const float *d_top_p,
+                           const float *d_min_p, int32_t *d_tokens, cudaStream_t stream) {
+    if (!ctx || !d_logits || !d_u || !d_temperature || !d_top_k || !d_top_p || !d_min_p || !d_tokens) return TRX_ERR_ARG;
+    if (type != TRX_TYPE_F32 && type != TRX_TYPE_F16 && type != TRX_TYPE_BF16) return TRX_ERR_ARG;
+    if (V == 0 || nrows == 0 || ld < V) return TRX_ERR_ARG;
+    if (V > (1u << 22) || nrows > (1u << 20) || ld > (1ull << 40)) return TRX_ERR_UNSUPPORTED;
+    trx::SampleArgs A{};
+    A.x = d_logits;
+    A.ld = (long long)ld;
+    A.V = (int)V;
+    A.nrows = (int)nrows;
+    A.u = d_u;
+    A.temp = d_temperature;
+    A.top_k = d_top_k;
+    A.top_p = d_top_p;
+    A.min_p = d_min_p;
+    A.tokens = d_tokens;
+    return trx::launch_sample_rows(A, type, stream);
 }
 
 }  // extern "C"

@@ -236,6 +236,50 @@ trx_status launch_quantize_tagged(const void *x, int n, int8_t *x8, int *e8, con
 trx_status launch_validate_t5(const uint8_t *w, int rows, int cols, uint32_t *err, cudaStream_t st);
 trx_status launch_build_lut(uint32_t *lut, cudaStream_t st);
 size_t lut_bytes();
+// Paged cache (trx_paged.cu, trx_paged_tc.cu).
+struct PgAttnArgs {
+    const void *q;             // [rows][H][hd]
+    const float *gate;         // raw q projection rows ([q | gate] per head), or nullptr
+    long long gate_ld;
+    const void *kp, *vp;       // pools [n_pages][page][Hkv][hd]
+    const int *tables, *lens, *cu;
+    void *out;                 // [rows][H][hd], the type of q
+    float *part;               // scratch partials: [2 * CTAs][query rows of a tile][hd + 2]
+    unsigned *cnt;             // [CTAs] arrival counts, zero between launches
+    int nseq, max_rows, max_new, page_shift, max_pages, n_pages;
+    int H, Hkv, rep, window, sinks;
+    int tq;                    // query tokens of a tile (set by the launch, with kt_shift)
+    int kt_shift;              // log2 of the key positions of a tile
+    float scale_log2;          // log2(e) / sqrt(hd)
+};
+trx_status launch_paged_plan(const trx_pages &P, const int *cached, const int *fresh, const int *free_pages,
+                             const int *n_free, uint32_t *err, cudaStream_t st);
+trx_status launch_paged_release(const trx_pages &P, const int *done, int *lens, int *free_pages, int *n_free,
+                                uint32_t *err, cudaStream_t st);
+struct PgAppendArgs {
+    const float *q, *k, *v, *qn, *kn, *freq;
+    long long q_ld, k_ld, v_ld;
+    void *kp, *vp, *q_out;
+    const int *cu, *slots, *pos;
+    int nseq, max_rows, H, Hkv, hd, half, gated;
+    int n_slots;
+    float eps;
+};
+trx_status launch_paged_append(const PgAppendArgs &A, int cache_type, int q_type, uint32_t *err, cudaStream_t st);
+// part_cap: floats of scratch; cnt_cap: arrival counts.
+trx_status launch_attn_paged(const PgAttnArgs &A, int hd, int cache_type, int q_type, size_t part_cap, int cnt_cap,
+                             uint32_t *err, cudaStream_t st);
+// Sampling (trx_sample.cu).
+struct SampleArgs {
+    const void *x;
+    long long ld;
+    int V, nrows;
+    const float *u, *temp;
+    const int *top_k;
+    const float *top_p, *min_p;
+    int *tokens;
+};
+trx_status launch_sample_rows(const SampleArgs &A, int type, cudaStream_t st);
 trx_status note_cuda(cudaError_t e);   // TRX_OK, or TRX_ERR_CUDA after recording e
 const char *last_cuda_error();
 

@@ -1,0 +1,709 @@
+// The paged KV cache of a server's step (sm_100a): the plan (block tables, slots and row offsets from
+// the sequences' lengths), the release of finished sequences' pages, the append of the new keys and
+// values, and attention over the pages for few query rows per kv head (decode).  The attention of
+// prompt chunks is in trx_paged_tc.cu.
+#include <cstdint>
+#include <cooperative_groups.h>
+#include <cuda_runtime.h>
+
+#include "trx_paged.cuh"
+
+namespace trx {
+namespace {
+namespace cg = cooperative_groups;
+
+// Plan ---------------------------------------------------------------------------------------------
+// have = ceil(cached / P), need = ceil((cached + new) / P) for a sequence with new rows.  Two prefix
+// sums over the sequences place everything: the rows give cu, the pages taken (need - have) give each
+// sequence its part of the free stack.  Both run as one 64-bit sum (rows in the low 33 bits).  The
+// kernel is latency: a few hundred bytes in, at most some hundred KB out.  One thread block, or a
+// cluster of up to 8 when there are many rows to write; every block of the cluster repeats the sums,
+// and the cluster barrier between the last read of the lengths and the first write lets lens and
+// n_free be the inputs' own buffers.
+constexpr int kPlanThreads = 1024;
+constexpr int kPlanRowBits = 33;
+
+__device__ __forceinline__ int pages_of(int positions, int shift) {
+    return (int)(((unsigned)positions + (1u << shift) - 1u) >> shift);
+}
+
+struct PlanSmem {
+    int cu[kPagedMaxSeq + 1];
+    int pg[kPagedMaxSeq + 1];  // pages taken by the sequences before
+    int cached[kPagedMaxSeq];
+    long long wsum[33];
+    int bad;
+};
+
+__device__ __forceinline__ int find_le(const int *a, int n, int v) {  // a[i] <= v < a[i + 1]
+    int lo = 0, hi = n;
+    while (hi - lo > 1) {
+        const int mid = (lo + hi) >> 1;
+        if (a[mid] <= v) lo = mid; else hi = mid;
+    }
+    return lo;
+}
+
+__global__ void __launch_bounds__(kPlanThreads)
+    paged_plan_kernel(const trx_pages P, int shift, const int *cached, const int *fresh, const int *free_pages,
+                      const int *n_free, uint32_t *err) {
+    __shared__ PlanSmem sm;
+    cg::cluster_group cluster = cg::this_cluster();
+    const int tid = threadIdx.x, nseq = (int)P.nseq;
+    const int crank = (int)cluster.block_rank(), nthr = (int)cluster.num_blocks() * kPlanThreads;
+    const bool writer = crank == 0;
+    pdl_trigger();
+    if (tid == 0) sm.bad = 0;
+    pdl_wait();
+    __syncthreads();
+    const int nf = *n_free;
+    int c = 0, n = 0, have = 0, need = 0;
+    if (tid < nseq) {
+        c = cached[tid];
+        n = fresh[tid];
+        if (c < 0 || n < 0 || n > (int)P.max_rows || (long long)c + n > (long long)P.max_pages << shift) {
+            sm.bad = TRX_DEV_RANGE;
+            n = 0;
+        } else {
+            have = pages_of(c, shift);
+            need = n ? pages_of(c + n, shift) : have;
+        }
+        sm.cached[tid] = c;
+    }
+    long long tot;
+    const long long ex = pg_block_scan((long long)n + ((long long)(need - have) << kPlanRowBits), sm.wsum, &tot);
+    const long long rows = tot & ((1ll << kPlanRowBits) - 1), taken = tot >> kPlanRowBits;
+    if (tid < nseq) {
+        sm.cu[tid] = (int)(ex & ((1ll << kPlanRowBits) - 1));
+        sm.pg[tid] = (int)(ex >> kPlanRowBits);
+    }
+    int bad = sm.bad;
+    if (nf < 0 || nf > (int)P.n_pages || rows > (long long)P.max_rows) bad |= TRX_DEV_RANGE;
+    if (!bad && taken > nf) bad = TRX_DEV_PAGES;
+    if (tid == 0) {
+        sm.cu[nseq] = bad ? 0 : (int)rows;
+        sm.pg[nseq] = bad ? 0 : (int)taken;
+    }
+    cluster.sync();  // all inputs read, the prefixes complete
+    if (writer) {
+        if (tid < nseq) {
+            P.cu[tid] = bad ? 0 : sm.cu[tid];
+            P.lens[tid] = bad ? c : c + n;
+            P.last[tid] = bad || n == 0 ? 0 : sm.cu[tid] + n - 1;
+        }
+        if (tid == 0) {
+            P.cu[nseq] = bad ? 0 : (int)rows;
+            *P.n_free = bad ? nf : nf - (int)taken;
+            if (bad) atomicOr(err, (unsigned)bad);
+        }
+    }
+    if (bad) return;
+    const int g = crank * kPlanThreads + tid;
+    for (int r = g; r < (int)rows; r += nthr) {
+        const int b = find_le(sm.cu, nseq, r);
+        const int cb = sm.cached[b], p = cb + r - sm.cu[b];
+        const int hb = pages_of(cb, shift), j = p >> shift;
+        int id;
+        if (j < hb)
+            id = P.tables[(size_t)b * P.max_pages + j];
+        else
+            id = free_pages[nf - 1 - (sm.pg[b] + j - hb)];
+        int slot = -1;
+        if ((unsigned)id < P.n_pages)
+            slot = (id << shift) + (p & ((1 << shift) - 1));
+        else
+            atomicOr(err, TRX_DEV_RANGE);
+        P.slots[r] = slot;
+        P.pos[r] = p;
+    }
+    for (int i = g; i < (int)taken; i += nthr) {
+        const int b = find_le(sm.pg, nseq, i);
+        P.tables[(size_t)b * P.max_pages + pages_of(sm.cached[b], shift) + i - sm.pg[b]] = free_pages[nf - 1 - i];
+    }
+}
+
+__global__ void __launch_bounds__(kPlanThreads)
+    paged_release_kernel(const trx_pages P, int shift, const int *done, int *lens, int *free_pages, int *n_free,
+                         uint32_t *err) {
+    __shared__ PlanSmem sm;
+    const int tid = threadIdx.x, nseq = (int)P.nseq;
+    pdl_trigger();
+    if (tid == 0) sm.bad = 0;
+    pdl_wait();
+    __syncthreads();
+    const int nf = *n_free;
+    int cnt = 0;
+    if (tid < nseq && done[tid]) {
+        const int len = lens[tid];
+        if (len < 0 || (long long)len > (long long)P.max_pages << shift)
+            sm.bad = 1;
+        else
+            cnt = pages_of(len, shift);
+    }
+    long long tot;
+    const long long ex = pg_block_scan(cnt, sm.wsum, &tot);
+    if (tid < nseq) sm.pg[tid] = (int)ex;
+    if (tid == 0) sm.pg[nseq] = (int)tot;
+    if (nf < 0 || (long long)nf + tot > (long long)P.n_pages) sm.bad = 1;
+    __syncthreads();
+    if (!sm.bad)
+        for (int i = tid; i < (int)tot; i += kPlanThreads) {
+            const int b = find_le(sm.pg, nseq, i);
+            if ((unsigned)P.tables[(size_t)b * P.max_pages + i - sm.pg[b]] >= P.n_pages) sm.bad = 1;
+        }
+    __syncthreads();
+    if (sm.bad) {
+        if (tid == 0) atomicOr(err, TRX_DEV_RANGE);
+        return;
+    }
+    for (int i = tid; i < (int)tot; i += kPlanThreads) {
+        const int b = find_le(sm.pg, nseq, i);
+        int *t = P.tables + (size_t)b * P.max_pages + i - sm.pg[b];
+        free_pages[nf + i] = *t;
+        *t = -1;
+    }
+    if (tid < nseq && done[tid]) lens[tid] = 0;
+    if (tid == 0) *n_free = nf + (int)tot;
+}
+
+// Append -------------------------------------------------------------------------------------------
+// A unit is 8 elements of a head: for u < half / 4 the pairs 4u..4u+3 and half+4u.. that the rotation
+// mixes, else 8 consecutive dims behind the rotated ones; hd / 8 neighbouring lanes hold a head, so the
+// norm is a shuffle over them and a rotation needs no exchange.  A block takes one row and a share of
+// its heads (y): its loads go out first, and meanwhile one thread per pair computes the row's cosines
+// and sines, which all heads share, into shared memory.  HBM-bound for chunks: 4 bytes in and 2 (or 4)
+// out per element.
+constexpr int kAppThreads = 256;
+
+template <typename T> __device__ __forceinline__ void store4(T *p, float4 v) {
+    const uint2 u = make_uint2(PgCvt<T>::pack(v.x, v.y), PgCvt<T>::pack(v.z, v.w));
+    *reinterpret_cast<uint2 *>(p) = u;
+}
+template <> __device__ __forceinline__ void store4<float>(float *p, float4 v) { *reinterpret_cast<float4 *>(p) = v; }
+
+__device__ __forceinline__ float4 mul4(float4 a, float s) { return make_float4(a.x * s, a.y * s, a.z * s, a.w * s); }
+__device__ __forceinline__ float4 mul4(float4 a, float4 b) {
+    return make_float4(a.x * b.x, a.y * b.y, a.z * b.z, a.w * b.w);
+}
+__device__ __forceinline__ float dot4(float4 a) { return a.x * a.x + a.y * a.y + a.z * a.z + a.w * a.w; }
+
+template <typename CT, typename QT, int HD>
+__global__ void __launch_bounds__(kAppThreads) paged_append_kernel(PgAppendArgs A, uint32_t *err) {
+    constexpr int UPH = HD / 8;               // lanes (units) per head
+    constexpr int HPB = kAppThreads / UPH;    // heads a block takes at a time
+    __shared__ __align__(16) float cs[HD / 2], sn[HD / 2];
+    const int tid = threadIdx.x, u = tid % UPH;
+    pdl_trigger();
+    const bool rot = u < A.half / 4;
+    const int d0 = rot ? 4 * u : 2 * A.half + 8 * (u - A.half / 4), d1 = rot ? A.half + 4 * u : d0 + 4;
+    const int heads = A.H + 2 * A.Hkv;
+    pdl_wait();
+    const float4 qw0 = *reinterpret_cast<const float4 *>(A.qn + d0), qw1 = *reinterpret_cast<const float4 *>(A.qn + d1);
+    const float4 kw0 = *reinterpret_cast<const float4 *>(A.kn + d0), kw1 = *reinterpret_cast<const float4 *>(A.kn + d1);
+    int rows = A.cu[A.nseq];
+    if (rows > A.max_rows || rows < 0) {
+        if (tid == 0 && blockIdx.x == 0 && blockIdx.y == 0) atomicOr(err, TRX_DEV_RANGE);
+        rows = rows < 0 ? 0 : A.max_rows;
+    }
+    for (int row = blockIdx.x; row < rows; row += gridDim.x) {
+        const int slot = A.slots[row], pos = A.pos[row];
+        const bool live = (unsigned)slot < (unsigned)A.n_slots;
+        if (!live && tid == 0 && blockIdx.y == 0) atomicOr(err, TRX_DEV_RANGE);
+        __syncthreads();  // the previous row's table is done with
+        if (tid < A.half) {
+            const float ang = __fmul_rn((float)pos, __ldg(A.freq + tid));
+            sincosf(ang, &sn[tid], &cs[tid]);
+        }
+        __syncthreads();
+        for (int h = blockIdx.y * HPB + tid / UPH; h < (heads + HPB - 1) / HPB * HPB; h += gridDim.y * HPB) {
+            // Whole groups of UPH lanes share a head; heads past the end do nothing but the shuffles.
+            const bool on = h < heads, is_q = h < A.H, is_k = !is_q && h < A.H + A.Hkv;
+            const float *src = is_q ? A.q + row * A.q_ld + (long long)h * HD * (A.gated ? 2 : 1)
+                                    : (is_k ? A.k + row * A.k_ld + (long long)(h - A.H) * HD
+                                            : A.v + row * A.v_ld + (long long)(h - A.H - A.Hkv) * HD);
+            float4 a = make_float4(0.f, 0.f, 0.f, 0.f), b = a;
+            if (on) {
+                a = *reinterpret_cast<const float4 *>(src + d0);
+                b = *reinterpret_cast<const float4 *>(src + d1);
+            }
+            float ss = dot4(a) + dot4(b);
+#pragma unroll
+            for (int o = UPH / 2; o; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+            if (!on) continue;
+            if (is_q || is_k) {
+                const float r = __fdiv_rn(1.0f, __fsqrt_rn(__fadd_rn(__fdiv_rn(ss, (float)HD), A.eps)));
+                a = mul4(mul4(a, r), is_q ? qw0 : kw0);
+                b = mul4(mul4(b, r), is_q ? qw1 : kw1);
+                if (rot) {
+                    const float4 c = *reinterpret_cast<const float4 *>(cs + 4 * u);
+                    const float4 s = *reinterpret_cast<const float4 *>(sn + 4 * u);
+                    const float4 x = a, y = b;
+                    a = make_float4(x.x * c.x - y.x * s.x, x.y * c.y - y.y * s.y, x.z * c.z - y.z * s.z,
+                                    x.w * c.w - y.w * s.w);
+                    b = make_float4(x.x * s.x + y.x * c.x, x.y * s.y + y.y * c.y, x.z * s.z + y.z * c.z,
+                                    x.w * s.w + y.w * c.w);
+                }
+            }
+            if (is_q) {
+                QT *dst = reinterpret_cast<QT *>(A.q_out) + ((size_t)row * A.H + h) * HD;
+                store4<QT>(dst + d0, a);
+                store4<QT>(dst + d1, b);
+            } else if (live) {
+                const int kh = is_k ? h - A.H : h - A.H - A.Hkv;
+                CT *dst = reinterpret_cast<CT *>(is_k ? A.kp : A.vp) + ((size_t)slot * A.Hkv + kh) * HD;
+                store4<CT>(dst + d0, a);
+                store4<CT>(dst + d1, b);
+            }
+        }
+    }
+}
+
+// Attention, few query rows ------------------------------------------------------------------------
+// One CTA of 4 warps walks its pieces (PgSched) in tiles of 64 key positions, 16 per warp, staged by
+// cp.async in a ring of three tiles.  Rows of the product are the query rows of one (query tile, kv
+// head): 16 / rep tokens x rep heads, padded to 16.  S = Q K^T and O += P V on mma.sync m16n8k16 with
+// fp32 accumulation, the softmax online per warp (running maximum and sum per row), the four warps
+// joined in a fixed order at the end of a piece.  fp32 queries: Q and P enter as two fp16 parts each
+// (x = hi + lo), so that products are exact to 2^-22.  Bound by the K/V stream: rep tokens' work per
+// byte is far below the tensor cores' rate even with 16 rows padded.
+constexpr int kDecThreads = 128;
+constexpr int kDecWarps = 4;
+constexpr int kDecTile = 64;
+constexpr int kDecStages = 3;
+
+template <int HD, bool SPLIT>
+struct DecSmem {
+    unsigned char k[kDecStages][kDecTile * HD * 2];
+    unsigned char v[kDecStages][kDecTile * HD * 2];
+    unsigned char q[SPLIT ? 2 : 1][16 * HD * 2];
+    union {
+        PgSchedSmem sched;
+        float o[16][HD];
+    };
+    float wm[kDecWarps][16], wl[kDecWarps][16], M[16], L[16];
+    int last;
+};
+
+template <typename CT>
+__device__ __forceinline__ void mma_16816(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1);
+template <>
+__device__ __forceinline__ void mma_16816<__half>(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+template <>
+__device__ __forceinline__ void mma_16816<__nv_bfloat16>(float (&d)[4], const uint32_t (&a)[4], uint32_t b0,
+                                                         uint32_t b1) {
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void ldsm4(uint32_t addr, uint32_t (&r)[4]) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+                 : "r"(addr)
+                 : "memory");
+}
+__device__ __forceinline__ void ldsm4t(uint32_t addr, uint32_t (&r)[4]) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+                 : "r"(addr)
+                 : "memory");
+}
+// 16 bytes to shared memory; zeros when n is 0.
+__device__ __forceinline__ void cp16z(uint32_t dst, const void *src, int n) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(n) : "memory");
+}
+
+// Byte offset of 16-byte piece c of row r in a tile of HD 16-bit elements per row: pieces are permuted
+// within each 128 bytes by the row, so that 8 rows' pieces of one column lie in different banks.
+template <int HD>
+__device__ __forceinline__ uint32_t tile_off(int r, int c) {
+    return (uint32_t)(r * HD * 2 + ((c ^ (r & 7)) << 4));
+}
+
+__device__ __forceinline__ float ex2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
+template <typename CT, typename QT>
+__device__ __forceinline__ void put_out(const PgAttnArgs &A, int hd, int row, int h, int d, float o) {
+    if (A.gate) {
+        const float g = A.gate[row * A.gate_ld + (long long)h * 2 * hd + hd + d];
+        o = __fdiv_rn(o, 1.0f + expf(-g));
+    }
+    QT *dst = reinterpret_cast<QT *>(A.out) + ((size_t)row * A.H + h) * hd + d;
+    if constexpr (sizeof(QT) == 4)
+        *dst = o;
+    else
+        *dst = PgCvt<QT>::from(o);
+}
+
+template <typename CT, typename QT, int HD>
+__global__ void __launch_bounds__(kDecThreads, HD == 256 ? 1 : 2) attn_paged_kernel(PgAttnArgs A, uint32_t *err) {
+    constexpr bool SPLIT = sizeof(QT) == 4;
+    extern __shared__ __align__(128) unsigned char smem_raw[];
+    using Smem = DecSmem<HD, SPLIT>;
+    Smem &sm = *reinterpret_cast<Smem *>(smem_raw);
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, c = lane & 3;
+    pdl_trigger();
+    pdl_wait();
+    pg_schedule(A, sm.sched, 1, err);
+    const PgSched S = sm.sched.S;
+    __syncthreads();
+    PgWalk W;
+    if (!W.start(A, S)) return;
+    PgWalk Ld = W;
+    int li = Ld.i0;
+    bool more = true;
+    const uint32_t kbase = smem_u32(sm.k), vbase = smem_u32(sm.v), qbase = smem_u32(sm.q);
+    constexpr uint32_t kStage = kDecTile * HD * 2;
+    constexpr int PPR = HD / 8;                // 16-byte pieces per row
+    constexpr int RPP = kDecThreads / PPR;     // rows per pass of the block
+    const int pc = tid % PPR, pr = tid / PPR;
+    const long long pitch = (long long)A.Hkv * HD;
+
+    // Stage the next key tile of the loader's walk into ring slot s.
+    auto issue = [&](int s) {
+        const int k0 = Ld.R.tile(li) * kDecTile, len = Ld.q.p0 + Ld.q.n;
+        const int *tab = A.tables + (long long)Ld.b * A.max_pages;
+#pragma unroll 4
+        for (int i = 0; i < kDecTile / RPP; ++i) {
+            const int r = pr + i * RPP, p = k0 + r;
+            int bytes = 0;
+            long long off = 0;
+            if (p < len) {
+                const int id = __ldg(tab + (p >> A.page_shift));
+                if ((unsigned)id < (unsigned)A.n_pages) {
+                    bytes = 16;
+                    off = (((long long)id << A.page_shift) + (p & ((1 << A.page_shift) - 1))) * pitch +
+                          (long long)Ld.kh * HD + pc * 8;
+                } else if (pc == 0) {
+                    atomicOr(err, TRX_DEV_RANGE);
+                }
+            }
+            cp16z(kbase + s * kStage + tile_off<HD>(r, pc), reinterpret_cast<const CT *>(A.kp) + off, bytes);
+            cp16z(vbase + s * kStage + tile_off<HD>(r, pc), reinterpret_cast<const CT *>(A.vp) + off, bytes);
+        }
+        if (++li == Ld.i1) {
+            more = Ld.next(A);
+            li = Ld.i0;
+        }
+    };
+#pragma unroll
+    for (int s = 0; s < kDecStages - 1; ++s) {
+        if (more) issue(s);
+        asm volatile("cp.async.commit_group;" ::: "memory");
+    }
+    int slot = 0;
+    do {
+        const int rows = W.rows(A);
+        const int row0 = W.q.row0 + W.t * A.tq, tok_pos = W.q.p0 + W.t * A.tq;
+        // The query rows, zeros behind them.
+        __syncthreads();
+        for (int i = tid; i < 16 * (HD / 8); i += kDecThreads) {
+            const int r = i / (HD / 8), pcq = i % (HD / 8);
+            uint4 hi = make_uint4(0u, 0u, 0u, 0u), lo = hi;
+            if (r < rows) {
+                const int tk = r / A.rep, h = W.kh * A.rep + r - tk * A.rep;
+                const QT *src = reinterpret_cast<const QT *>(A.q) + ((size_t)(row0 + tk) * A.H + h) * HD + pcq * 8;
+                if constexpr (SPLIT) {
+                    const float4 x = *reinterpret_cast<const float4 *>(src), y = *reinterpret_cast<const float4 *>(src + 4);
+                    const float f[8] = {x.x, x.y, x.z, x.w, y.x, y.y, y.z, y.w};
+                    uint32_t hw[4], lw[4];
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        hw[j] = PgCvt<CT>::pack(f[2 * j], f[2 * j + 1]);
+                        const float2 b = PgCvt<CT>::unpack(hw[j]);
+                        lw[j] = PgCvt<CT>::pack(f[2 * j] - b.x, f[2 * j + 1] - b.y);
+                    }
+                    hi = make_uint4(hw[0], hw[1], hw[2], hw[3]);
+                    lo = make_uint4(lw[0], lw[1], lw[2], lw[3]);
+                } else {
+                    hi = *reinterpret_cast<const uint4 *>(src);
+                }
+            }
+            *reinterpret_cast<uint4 *>(&sm.q[0][tile_off<HD>(r, pcq)]) = hi;
+            if constexpr (SPLIT) *reinterpret_cast<uint4 *>(&sm.q[SPLIT ? 1 : 0][tile_off<HD>(r, pcq)]) = lo;
+        }
+        float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
+        float o[HD / 8][4];
+#pragma unroll
+        for (int i = 0; i < HD / 8; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
+        // Positions of rows g and g + 8 (-1 behind the last: everything hidden).
+        const int qp[2] = {g < rows ? tok_pos + g / A.rep : -1, g + 8 < rows ? tok_pos + (g + 8) / A.rep : -1};
+        for (int it = W.i0; it < W.i1; ++it) {
+            asm volatile("cp.async.wait_group %0;" ::"n"(kDecStages - 2) : "memory");
+            __syncthreads();  // the tile has landed, and every warp is done with the slot refilled next
+            {
+                const int s2 = slot + kDecStages - 1;
+                if (more) issue(s2 >= kDecStages ? s2 - kDecStages : s2);
+                asm volatile("cp.async.commit_group;" ::: "memory");
+            }
+            const int k0 = W.R.tile(it) * kDecTile + warp * 16;
+            const uint32_t ks = kbase + slot * kStage, vs = vbase + slot * kStage;
+            float s0[4] = {0.f, 0.f, 0.f, 0.f}, s1[4] = {0.f, 0.f, 0.f, 0.f};
+            const int arow = (lane & 7) + ((lane >> 3) & 1) * 8, acol = lane >> 4;
+            const int brow = warp * 16 + (lane & 7) + (lane >> 4) * 8, bcol = (lane >> 3) & 1;
+#pragma unroll
+            for (int k = 0; k < HD / 16; ++k) {
+                uint32_t a[4], b[4];
+                ldsm4(qbase + tile_off<HD>(arow, 2 * k + acol), a);
+                ldsm4(ks + tile_off<HD>(brow, 2 * k + bcol), b);
+                mma_16816<CT>(s0, a, b[0], b[1]);
+                mma_16816<CT>(s1, a, b[2], b[3]);
+                if constexpr (SPLIT) {
+                    ldsm4(qbase + 16 * HD * 2 + tile_off<HD>(arow, 2 * k + acol), a);
+                    mma_16816<CT>(s0, a, b[0], b[1]);
+                    mma_16816<CT>(s1, a, b[2], b[3]);
+                }
+            }
+            // Row g: s0[0], s0[1] at positions k0 + 2c, + 1, s1[0], s1[1] at k0 + 8 + 2c; row g + 8: [2], [3].
+            uint32_t ph[4], pl[4];
+#pragma unroll
+            for (int rr = 0; rr < 2; ++rr) {
+                float x[4] = {s0[2 * rr], s0[2 * rr + 1], s1[2 * rr], s1[2 * rr + 1]};
+                float mx = -INFINITY;
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    const int kp = k0 + 2 * c + (j & 1) + (j >> 1) * 8;
+                    x[j] = pg_hidden(kp, qp[rr], A.window, A.sinks) ? -INFINITY : x[j] * A.scale_log2;
+                    mx = fmaxf(mx, x[j]);
+                }
+                mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
+                mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
+                const float mn = fmaxf(m[rr], mx), ms = mn == -INFINITY ? 0.f : mn;
+                const float al = ex2(m[rr] - ms);
+                float p[4], sum = 0.f;
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    p[j] = ex2(x[j] - ms);
+                    sum += p[j];
+                }
+                l[rr] = l[rr] * al + sum;
+                m[rr] = mn;
+#pragma unroll
+                for (int i = 0; i < HD / 8; ++i) {
+                    o[i][2 * rr] *= al;
+                    o[i][2 * rr + 1] *= al;
+                }
+                ph[rr] = PgCvt<CT>::pack(p[0], p[1]);
+                ph[2 + rr] = PgCvt<CT>::pack(p[2], p[3]);
+                if constexpr (SPLIT) {
+                    const float2 h0 = PgCvt<CT>::unpack(ph[rr]), h1 = PgCvt<CT>::unpack(ph[2 + rr]);
+                    pl[rr] = PgCvt<CT>::pack(p[0] - h0.x, p[1] - h0.y);
+                    pl[2 + rr] = PgCvt<CT>::pack(p[2] - h1.x, p[3] - h1.y);
+                }
+            }
+            const int vrow = warp * 16 + (lane & 7) + ((lane >> 3) & 1) * 8, vcol = lane >> 4;
+#pragma unroll
+            for (int i = 0; i < HD / 16; ++i) {
+                uint32_t b[4];
+                ldsm4t(vs + tile_off<HD>(vrow, 2 * i + vcol), b);
+                mma_16816<CT>(o[2 * i], ph, b[0], b[1]);
+                mma_16816<CT>(o[2 * i + 1], ph, b[2], b[3]);
+                if constexpr (SPLIT) {
+                    mma_16816<CT>(o[2 * i], pl, b[0], b[1]);
+                    mma_16816<CT>(o[2 * i + 1], pl, b[2], b[3]);
+                }
+            }
+            slot = slot + 1 == kDecStages ? 0 : slot + 1;
+        }
+        // The warps' parts of the piece, in their order.
+#pragma unroll
+        for (int rr = 0; rr < 2; ++rr) {
+            l[rr] += __shfl_xor_sync(0xffffffffu, l[rr], 1);
+            l[rr] += __shfl_xor_sync(0xffffffffu, l[rr], 2);
+            if (c == 0) {
+                sm.wm[warp][g + 8 * rr] = m[rr];
+                sm.wl[warp][g + 8 * rr] = l[rr];
+            }
+        }
+        __syncthreads();
+        float f[2];
+#pragma unroll
+        for (int rr = 0; rr < 2; ++rr) {
+            const int r = g + 8 * rr;
+            float M = -INFINITY;
+#pragma unroll
+            for (int w = 0; w < kDecWarps; ++w) M = fmaxf(M, sm.wm[w][r]);
+            f[rr] = m[rr] == -INFINITY ? 0.f : ex2(m[rr] - M);
+            if (warp == 0 && c == 0) {
+                float L = 0.f;
+                for (int w = 0; w < kDecWarps; ++w) {
+                    const float mw = sm.wm[w][r];
+                    if (mw != -INFINITY) L = fmaf(ex2(mw - M), sm.wl[w][r], L);
+                }
+                sm.M[r] = M;
+                sm.L[r] = L;
+            }
+        }
+        for (int w = 0; w < kDecWarps; ++w) {
+            if (warp == w) {
+#pragma unroll
+                for (int rr = 0; rr < 2; ++rr) {
+                    const int r = g + 8 * rr;
+                    if (r < rows)
+#pragma unroll
+                        for (int i = 0; i < HD / 8; ++i) {
+                            float2 *p = reinterpret_cast<float2 *>(&sm.o[r][8 * i + 2 * c]);
+                            float2 v = make_float2(f[rr] * o[i][2 * rr], f[rr] * o[i][2 * rr + 1]);
+                            if (w) {
+                                const float2 q = *p;
+                                v.x += q.x;
+                                v.y += q.y;
+                            }
+                            *p = v;
+                        }
+                }
+            }
+            __syncthreads();
+        }
+        if (W.whole()) {
+            for (int i = tid; i < rows * HD; i += kDecThreads) {
+                const int r = i / HD, d = i - r * HD, tk = r / A.rep;
+                const float L = sm.L[r];
+                put_out<CT, QT>(A, HD, row0 + tk, W.kh * A.rep + r - tk * A.rep, d, L > 0.f ? __fdiv_rn(sm.o[r][d], L) : 0.f);
+            }
+        } else {
+            // A cut item: this piece to scratch; the last CTA to arrive joins the pieces in CTA order.
+            const long long item0 = W.u - W.i1, item1 = item0 + W.R.cnt;
+            const int c0 = pg_owner(S, item0), c1 = pg_owner(S, item1 - 1);
+            constexpr size_t kPart = 16 * (HD + 2);
+            float *const mine = A.part + kPart * (2 * (size_t)blockIdx.x + ((int)blockIdx.x == c0 ? 1 : 0));
+            for (int i = tid; i < rows * HD; i += kDecThreads) mine[32 + i] = sm.o[i / HD][i % HD];
+            if (tid < rows) {
+                mine[tid] = sm.M[tid];
+                mine[16 + tid] = sm.L[tid];
+            }
+            __threadfence();
+            __syncthreads();
+            if (tid == 0) sm.last = atomicAdd(A.cnt + c0, 1u) == (unsigned)(c1 - c0);
+            __syncthreads();
+            if (sm.last) {
+                __threadfence();
+                auto slot_of = [&](int cc) { return A.part + kPart * (2 * (size_t)cc + (cc == c0 ? 1 : 0)); };
+                if (tid < rows) {
+                    float M = -INFINITY, L = 0.f;
+                    for (int cc = c0; cc <= c1; ++cc) M = fmaxf(M, __ldcg(slot_of(cc) + tid));
+                    for (int cc = c0; cc <= c1; ++cc) {
+                        const float mp = __ldcg(slot_of(cc) + tid);
+                        if (mp != -INFINITY) L = fmaf(ex2(mp - M), __ldcg(slot_of(cc) + 16 + tid), L);
+                    }
+                    sm.M[tid] = M;
+                    sm.L[tid] = L;
+                }
+                __syncthreads();
+                for (int i = tid; i < rows * HD; i += kDecThreads) {
+                    const int r = i / HD, d = i - r * HD, tk = r / A.rep;
+                    const float M = sm.M[r], L = sm.L[r];
+                    float acc = 0.f;
+                    for (int cc = c0; cc <= c1; ++cc) {
+                        const float *p = slot_of(cc);
+                        const float mp = __ldcg(p + r);
+                        if (mp != -INFINITY) acc = fmaf(ex2(mp - M), __ldcg(p + 32 + i), acc);
+                    }
+                    put_out<CT, QT>(A, HD, row0 + tk, W.kh * A.rep + r - tk * A.rep, d, L > 0.f ? __fdiv_rn(acc, L) : 0.f);
+                }
+                if (tid == 0) A.cnt[c0] = 0u;
+            }
+        }
+    } while (W.next(A));
+    asm volatile("cp.async.wait_group 0;" ::: "memory");
+}
+
+template <typename CT, typename QT, int HD>
+trx_status launch_dec(PgAttnArgs A, size_t part_cap, int cnt_cap, uint32_t *err, cudaStream_t st) {
+    constexpr size_t smem = sizeof(DecSmem<HD, sizeof(QT) == 4>);
+    static DevBits configured{0};
+    const cudaError_t e = once_per_device(configured, [] {
+        return cudaFuncSetAttribute(attn_paged_kernel<CT, QT, HD>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+    });
+    if (e != cudaSuccess) return note_cuda(e);
+    A.tq = 16 / A.rep;
+    A.kt_shift = 6;
+    int grid = device_sms() * (HD == 256 ? 1 : 2);
+    while (grid > 1 && ((size_t)grid * 2 * 16 * (HD + 2) > part_cap || grid > cnt_cap)) grid /= 2;
+    return note_cuda(launch_kernel(attn_paged_kernel<CT, QT, HD>, dim3(grid), dim3(kDecThreads), smem, st, A, err));
+}
+
+template <typename CT, typename QT>
+trx_status launch_dec_hd(const PgAttnArgs &A, int hd, size_t part_cap, int cnt_cap, uint32_t *err, cudaStream_t st) {
+    switch (hd) {
+        case 64: return launch_dec<CT, QT, 64>(A, part_cap, cnt_cap, err, st);
+        case 128: return launch_dec<CT, QT, 128>(A, part_cap, cnt_cap, err, st);
+        default: return launch_dec<CT, QT, 256>(A, part_cap, cnt_cap, err, st);
+    }
+}
+
+template <typename CT, typename QT>
+trx_status launch_app_hd(const PgAppendArgs &A, uint32_t *err, cudaStream_t st) {
+    // Blocks per row: enough to give every SM a block when there are few rows.
+    const int hpb = kAppThreads / (A.hd / 8), most = (A.H + 2 * A.Hkv + hpb - 1) / hpb;
+    int ny = (2 * device_sms() + A.max_rows - 1) / A.max_rows;
+    ny = ny < 1 ? 1 : (ny > most ? most : ny);
+    const int nx = A.max_rows < 65536 ? A.max_rows : 65536;
+    const dim3 grid(nx, ny), block(kAppThreads);
+    switch (A.hd) {
+        case 64: return note_cuda(launch_kernel(paged_append_kernel<CT, QT, 64>, grid, block, 0, st, A, err));
+        case 128: return note_cuda(launch_kernel(paged_append_kernel<CT, QT, 128>, grid, block, 0, st, A, err));
+        default: return note_cuda(launch_kernel(paged_append_kernel<CT, QT, 256>, grid, block, 0, st, A, err));
+    }
+}
+
+int shift_of(uint32_t page) {
+    int s = 0;
+    while ((1u << s) < page) ++s;
+    return s;
+}
+
+}  // namespace
+
+trx_status launch_paged_plan(const trx_pages &P, const int *cached, const int *fresh, const int *free_pages,
+                             const int *n_free, uint32_t *err, cudaStream_t st) {
+    // Blocks: one per 2048 rows, at most a portable cluster.
+    int nb = 1;
+    while (nb < 8 && (uint32_t)nb * 2048 < P.max_rows) nb *= 2;
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3(nb);
+    cfg.blockDim = dim3(kPlanThreads);
+    cfg.stream = st;
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = nb;
+    attr[0].val.clusterDim.y = 1;
+    attr[0].val.clusterDim.z = 1;
+    attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[1].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = pdl_enabled() ? 2 : 1;
+    return note_cuda(cudaLaunchKernelEx(&cfg, paged_plan_kernel, P, shift_of(P.page), cached, fresh, free_pages, n_free, err));
+}
+
+trx_status launch_paged_release(const trx_pages &P, const int *done, int *lens, int *free_pages, int *n_free,
+                                uint32_t *err, cudaStream_t st) {
+    return note_cuda(launch_kernel(paged_release_kernel, dim3(1), dim3(kPlanThreads), 0, st, P, shift_of(P.page), done,
+                                   lens, free_pages, n_free, err));
+}
+
+trx_status launch_paged_append(const PgAppendArgs &A, int cache_type, int q_type, uint32_t *err, cudaStream_t st) {
+    if (cache_type == TRX_TYPE_F16)
+        return q_type == TRX_TYPE_F32 ? launch_app_hd<__half, float>(A, err, st) : launch_app_hd<__half, __half>(A, err, st);
+    return q_type == TRX_TYPE_F32 ? launch_app_hd<__nv_bfloat16, float>(A, err, st)
+                                  : launch_app_hd<__nv_bfloat16, __nv_bfloat16>(A, err, st);
+}
+
+trx_status launch_attn_paged(const PgAttnArgs &A, int hd, int cache_type, int q_type, size_t part_cap, int cnt_cap,
+                             uint32_t *err, cudaStream_t st) {
+    if (cache_type == TRX_TYPE_BF16)
+        return launch_dec_hd<__nv_bfloat16, __nv_bfloat16>(A, hd, part_cap, cnt_cap, err, st);
+    return q_type == TRX_TYPE_F32 ? launch_dec_hd<__half, float>(A, hd, part_cap, cnt_cap, err, st)
+                                  : launch_dec_hd<__half, __half>(A, hd, part_cap, cnt_cap, err, st);
+}
+
+}  // namespace trx

@@ -1,0 +1,273 @@
+// Shared pieces of the paged-cache kernels (trx_paged.cu, trx_paged_tc.cu): the launch arguments, the
+// sequences' geometry, and the division of the attention work among CTAs.
+#pragma once
+#include <cstdint>
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <cuda_runtime.h>
+
+#include "trx_common.cuh"
+#include "trx_internal.h"
+
+namespace trx {
+
+constexpr int kPagedMaxSeq = 1024;  // sequences of one plan (the kernels keep a prefix of them in shared memory)
+
+// One sequence of an attention launch: its new rows [row0, row0 + n) at positions [p0, p0 + n).
+struct PgSeq {
+    int row0, n, p0;
+};
+
+// The sequence's rows and positions, or n = 0 for one whose offsets or length are out of range
+// (bad is then set; nothing outside the buffers is read or written for it).
+__device__ __forceinline__ PgSeq pg_seq(const PgAttnArgs &A, int b, bool &bad) {
+    PgSeq S;
+    const int c0 = A.cu[b], c1 = A.cu[b + 1], len = A.lens[b];
+    S.row0 = c0;
+    S.n = c1 - c0;
+    S.p0 = len - S.n;
+    if (c0 < 0 || c1 < c0 || c1 > A.max_rows || S.n > A.max_new || S.p0 < 0 ||
+        (S.n && (long long)len > (long long)A.max_pages << A.page_shift)) {
+        bad = true;
+        S.n = 0;
+    }
+    return S;
+}
+
+// The key tiles (KT positions each) that query tile t of a sequence reads: tile index i < ns is the
+// i-th sink tile, the rest are the tiles from w0 on.
+struct PgRange {
+    int ns, w0, cnt;
+    __device__ __forceinline__ int tile(int i) const { return i < ns ? i : w0 + i - ns; }
+};
+
+__device__ __forceinline__ PgRange pg_range(const PgAttnArgs &A, const PgSeq &S, int t) {
+    const int lo = S.p0 + t * A.tq, hi = S.p0 + min(S.n, (t + 1) * A.tq) - 1;
+    PgRange R;
+    R.w0 = A.window ? max(0, lo - A.window + 1) >> A.kt_shift : 0;
+    R.ns = A.window ? min((A.sinks + (1 << A.kt_shift) - 1) >> A.kt_shift, R.w0) : 0;
+    R.cnt = R.ns + (hi >> A.kt_shift) - R.w0 + 1;
+    return R;
+}
+
+// Division of the work.  The (query tile, kv head, key tile) units of all sequences form one line,
+// query tile major, key tile minor; CTA c of G takes units [c N / G, (c + 1) N / G).  An item is one
+// (query tile, kv head); a CTA's range cuts it into pieces.  An item in one piece is finished by its
+// CTA; the pieces of a cut item go to scratch as (max, sum, unnormalised output) and the CTA that
+// arrives last joins them in the order of the CTAs, so that the result does not depend on timing.
+// Every CTA finds its own range by scanning the sequences' lengths: no launch in front, and nothing of
+// the lengths has to be known on the host.
+struct PgSched {
+    long long N;               // units in all
+    int G;                     // CTAs that take part
+    long long u0, u1;          // this CTA's units
+    int b, t, kh, i;           // its first unit: sequence, query tile, kv head, index among the item's key tiles
+};
+
+struct PgSchedSmem {
+    int qpre[kPagedMaxSeq + 1];  // query tiles of the sequences before b
+    long long wsum[33];
+    PgSched S;
+    int bad;
+};
+
+// Block-wide exclusive sum of v (blockDim a multiple of 32, at most 1024 threads); total in *tot.
+__device__ __forceinline__ long long pg_block_scan(long long v, long long *wsum, long long *tot) {
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, nw = blockDim.x >> 5;
+    long long x = v;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const long long y = __shfl_up_sync(0xffffffffu, x, o);
+        if (lane >= o) x += y;
+    }
+    if (lane == 31) wsum[warp] = x;
+    __syncthreads();
+    if (warp == 0) {
+        long long w = lane < nw ? wsum[lane] : 0;
+        const long long w0 = w;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const long long y = __shfl_up_sync(0xffffffffu, w, o);
+            if (lane >= o) w += y;
+        }
+        if (lane < nw) wsum[lane] = w - w0;
+        if (lane == 31) wsum[32] = w;
+    }
+    __syncthreads();
+    const long long r = wsum[warp] + x - v;
+    *tot = wsum[32];
+    __syncthreads();
+    return r;
+}
+
+// The sequence that query tile q belongs to.
+__device__ __forceinline__ int pg_find(const int *qpre, int nseq, int q) {
+    int lo = 0, hi = nseq;  // qpre[lo] <= q < qpre[hi]
+    while (hi - lo > 1) {
+        const int mid = (lo + hi) >> 1;
+        if (qpre[mid] <= q) lo = mid; else hi = mid;
+    }
+    return lo;
+}
+
+// Every thread of the block: fills sm.S (see PgSched).  min_units: CTAs take part as long as each
+// gets this many units.
+__device__ __forceinline__ void pg_schedule(const PgAttnArgs &A, PgSchedSmem &sm, int min_units, uint32_t *err) {
+    const int tid = threadIdx.x, nt = blockDim.x;
+    if (tid == 0) sm.bad = 0;
+    __syncthreads();
+    long long carry = 0;
+    bool bad = false;
+    for (int b0 = 0; b0 < A.nseq; b0 += nt) {
+        const int b = b0 + tid;
+        int q = 0;
+        if (b < A.nseq) {
+            const PgSeq S = pg_seq(A, b, bad);
+            q = (S.n + A.tq - 1) / A.tq;
+        }
+        long long tot;
+        const long long ex = pg_block_scan(q, sm.wsum, &tot);
+        if (b < A.nseq) sm.qpre[b] = (int)(carry + ex);
+        carry += tot;
+    }
+    if (tid == 0) sm.qpre[A.nseq] = (int)carry;
+    if (bad) sm.bad = 1;
+    __syncthreads();
+    if (tid == 0 && sm.bad && blockIdx.x == 0) atomicOr(err, TRX_DEV_RANGE);
+    const int NQ = (int)carry;
+    // Units of query tile q (times the kv heads), its sequence and place.
+    auto units = [&](int q, int &b, int &t, PgRange &R) {
+        bool ignore = false;
+        b = pg_find(sm.qpre, A.nseq, q);
+        t = q - sm.qpre[b];
+        R = pg_range(A, pg_seq(A, b, ignore), t);
+        return (long long)R.cnt * A.Hkv;
+    };
+    long long N = 0;
+    for (int q0 = 0; q0 < NQ; q0 += nt) {
+        int b, t;
+        PgRange R;
+        long long tot;
+        pg_block_scan(q0 + tid < NQ ? units(q0 + tid, b, t, R) : 0, sm.wsum, &tot);
+        N += tot;
+    }
+    const long long gmax = (N + min_units - 1) / min_units;
+    const int G = (int)(gmax < (long long)gridDim.x ? gmax : (long long)gridDim.x);
+    const long long u0 = G ? (long long)blockIdx.x * N / G : 0, u1 = G ? (long long)(blockIdx.x + 1) * N / G : 0;
+    if (tid == 0) {
+        sm.S.N = N;
+        sm.S.G = G;
+        sm.S.u0 = u0;
+        sm.S.u1 = (int)blockIdx.x < G ? u1 : u0;
+    }
+    if ((int)blockIdx.x < G) {
+        long long base = 0;
+        for (int q0 = 0; q0 < NQ && base <= u0; q0 += nt) {
+            int b = 0, t = 0;
+            PgRange R{};
+            long long tot;
+            const long long u = q0 + tid < NQ ? units(q0 + tid, b, t, R) : 0;
+            const long long at = base + pg_block_scan(u, sm.wsum, &tot);
+            if (at <= u0 && u0 < at + u) {
+                sm.S.b = b;
+                sm.S.t = t;
+                sm.S.kh = (int)((u0 - at) / R.cnt);
+                sm.S.i = (int)((u0 - at) % R.cnt);
+            }
+            base += tot;
+        }
+    }
+    __syncthreads();
+}
+
+// The CTA that owns unit x.
+__device__ __forceinline__ int pg_owner(const PgSched &S, long long x) { return (int)(((x + 1) * S.G - 1) / S.N); }
+
+// A role's walk along its CTA's pieces.
+struct PgWalk {
+    PgSeq q;
+    PgRange R;
+    int b, t, kh, i0, i1;    // this piece: key tiles i0..i1-1 of the item's R.cnt
+    long long u, u1;         // units before the end of this piece, the end of the range
+
+    __device__ __forceinline__ void load(const PgAttnArgs &A) {
+        bool ignore = false;
+        q = pg_seq(A, b, ignore);
+        R = pg_range(A, q, t);
+    }
+    __device__ __forceinline__ void cut() {
+        const long long left = u1 - u;
+        i1 = (int)(left < R.cnt - i0 ? i0 + left : R.cnt);
+        u += i1 - i0;
+    }
+    // false: the CTA has no units.
+    __device__ __forceinline__ bool start(const PgAttnArgs &A, const PgSched &S) {
+        if (S.u0 >= S.u1) return false;
+        b = S.b;
+        t = S.t;
+        kh = S.kh;
+        i0 = S.i;
+        u = S.u0;
+        u1 = S.u1;
+        load(A);
+        cut();
+        return true;
+    }
+    __device__ __forceinline__ bool next(const PgAttnArgs &A) {
+        if (u >= u1) return false;
+        i0 = 0;
+        if (++kh == A.Hkv) {
+            kh = 0;
+            if (++t * A.tq >= q.n) {
+                t = 0;
+                bool ignore = false;
+                do { ++b; } while (b < A.nseq && pg_seq(A, b, ignore).n == 0);
+                if (b >= A.nseq) return false;
+            }
+            load(A);
+        }
+        cut();
+        return true;
+    }
+    __device__ __forceinline__ bool whole() const { return i0 == 0 && i1 == R.cnt; }
+    __device__ __forceinline__ int rows(const PgAttnArgs &A) const { return min(q.n - t * A.tq, A.tq) * A.rep; }
+};
+
+// Is key position k hidden from the query at position p?
+__device__ __forceinline__ bool pg_hidden(int k, int p, int window, int sinks) {
+    return k > p || (window && p - k >= window && k >= sinks);
+}
+
+template <typename CT> struct PgCvt;
+template <> struct PgCvt<__half> {
+    static __device__ __forceinline__ __half from(float x) { return __float2half_rn(x); }
+    static __device__ __forceinline__ float to(__half x) { return __half2float(x); }
+    static __device__ __forceinline__ uint32_t pack(float a, float b) {
+        const __half2 h = __floats2half2_rn(a, b);
+        uint32_t u;
+        memcpy(&u, &h, 4);
+        return u;
+    }
+    static __device__ __forceinline__ float2 unpack(uint32_t u) {
+        __half2 h;
+        memcpy(&h, &u, 4);
+        return __half22float2(h);
+    }
+};
+template <> struct PgCvt<__nv_bfloat16> {
+    static __device__ __forceinline__ __nv_bfloat16 from(float x) { return __float2bfloat16_rn(x); }
+    static __device__ __forceinline__ float to(__nv_bfloat16 x) { return __bfloat162float(x); }
+    static __device__ __forceinline__ uint32_t pack(float a, float b) {
+        const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
+        uint32_t u;
+        memcpy(&u, &h, 4);
+        return u;
+    }
+    static __device__ __forceinline__ float2 unpack(uint32_t u) {
+        __nv_bfloat162 h;
+        memcpy(&h, &u, 4);
+        return __bfloat1622float2(h);
+    }
+};
+
+}  // namespace trx

@@ -593,6 +593,174 @@ def deltanet_int_step(ctx, state, exp, maxabs, k, q, v, decay, beta, out=None):
     return out
 
 
+# Paged KV cache and sampling ---------------------------------------------------------------------------
+
+_TYPES = {torch.float32: _lib.TYPE_F32, torch.float16: _lib.TYPE_F16, torch.bfloat16: _lib.TYPE_BF16}
+
+
+def _stream_of(ctx):
+    """The current stream of the context's device, which has to be the current device (the library
+    launches on it)."""
+    if torch.cuda.current_device() != ctx.device.index:
+        raise ValueError(f"the context is on {ctx.device}, the current device is cuda:{torch.cuda.current_device()}")
+    return torch.cuda.current_stream().cuda_stream
+
+
+def _buf(t, dtype, n, name, dev):
+    """A contiguous tensor of at least n elements on the context's device."""
+    if not (t.dtype == dtype and t.device == dev and t.is_contiguous() and t.numel() >= n):
+        raise ValueError(f"{name}: expected a contiguous {dtype} tensor of at least {n} elements on {dev}, got "
+                         f"{t.dtype} {tuple(t.shape)} on {t.device} (contiguous={t.is_contiguous()})")
+    return t.data_ptr()
+
+
+def _mat(t, dtype, cols, name, dev):
+    """A matrix of `cols` columns whose rows may be apart (a slice of a wider one): pointer, row stride."""
+    if not (t.dtype == dtype and t.device == dev and t.dim() == 2 and t.shape[1] == cols and
+            (t.stride(1) == 1 or cols == 1) and (t.shape[0] <= 1 or t.stride(0) >= cols)):
+        raise ValueError(f"{name}: expected a {dtype} matrix of {cols} columns on {dev} with contiguous rows, got "
+                         f"{t.dtype} {tuple(t.shape)} strides {t.stride()} on {t.device}")
+    return t.data_ptr(), t.stride(0) if t.shape[0] > 1 else cols
+
+
+class PagedPlan:
+    """The block tables of nseq sequences over a pool of n_pages pages of `page` positions, and the
+    buffers that paged_plan fills for a step of at most max_rows new rows (trx_pages): tables
+    [nseq, max_pages] (-1 at first), lens [nseq], cu [nseq + 1], slots and pos [max_rows], last [nseq],
+    n_free [1], int32."""
+
+    def __init__(self, nseq, max_rows, max_pages, page, n_pages, device=None):
+        dev = self.device = torch.device("cuda", torch.cuda.current_device()) if device is None else torch.device(device)
+        if min(nseq, max_rows, max_pages, n_pages) < 1 or page < 16 or page & (page - 1):
+            raise ValueError("PagedPlan: sizes must be positive and the page a power of two of at least 16")
+        self.nseq, self.max_rows, self.max_pages, self.page, self.n_pages = nseq, max_rows, max_pages, page, n_pages
+        i32 = lambda *s: torch.zeros(*s, dtype=torch.int32, device=dev)
+        self.tables = torch.full((nseq, max_pages), -1, dtype=torch.int32, device=dev)
+        self.lens, self.cu, self.last, self.n_free = i32(nseq), i32(nseq + 1), i32(nseq), i32(1)
+        self.slots = torch.full((max_rows,), -1, dtype=torch.int32, device=dev)
+        self.pos = torch.full((max_rows,), -1, dtype=torch.int32, device=dev)
+        self._c = {}
+
+    def pages(self, rows=None):
+        """The trx_pages of this plan, for tensors of `rows` rows (default: max_rows)."""
+        rows = self.max_rows if rows is None else min(rows, self.max_rows)
+        c = self._c.get(rows)
+        if c is None:
+            c = self._c[rows] = _lib.Pages(self.nseq, rows, self.page, self.max_pages, self.n_pages,
+                                           *[t.data_ptr() for t in (self.tables, self.lens, self.cu, self.slots,
+                                                                    self.pos, self.last, self.n_free)])
+        return ctypes.byref(c)
+
+
+def paged_shape(n_head, n_kv, head_dim, rope_dims=None, gated=False, eps=1e-6, window=0, sinks=0):
+    return _lib.PagedShape(n_head, n_kv, head_dim, head_dim if rope_dims is None else rope_dims, 1 if gated else 0, eps,
+                           window, sinks)
+
+
+def paged_plan(ctx, plan, cached, new, free, n_free):
+    """The plan of a step (trx_paged_plan): cached and new [nseq] int32, the positions every sequence has
+    in the cache and the rows it brings; free [n_pages] and n_free [1] int32, the stack of free pages and
+    its height.  Fills plan's buffers and returns it.  cached may be plan.lens and n_free plan.n_free (in
+    place); free is not changed."""
+    dev = plan.device
+    _lib.check(_lib.lib().trx_paged_plan(
+        ctx.h, plan.pages(), _buf(cached, torch.int32, plan.nseq, "cached", dev),
+        _buf(new, torch.int32, plan.nseq, "new", dev), _buf(free, torch.int32, 1, "free", dev),
+        _buf(n_free, torch.int32, 1, "n_free", dev), _stream_of(ctx)), "trx_paged_plan")
+    return plan
+
+
+def paged_release(ctx, plan, done, lens, free, n_free):
+    """Give back the pages of the sequences with done[b] != 0 (trx_paged_release): they go on top of the
+    free stack, n_free grows, their table entries become -1 and lens 0, all in place."""
+    dev = plan.device
+    _lib.check(_lib.lib().trx_paged_release(
+        ctx.h, plan.pages(), _buf(done, torch.int32, plan.nseq, "done", dev),
+        _buf(lens, torch.int32, plan.nseq, "lens", dev), _buf(free, torch.int32, plan.n_pages, "free", dev),
+        _buf(n_free, torch.int32, 1, "n_free", dev), _stream_of(ctx)), "trx_paged_release")
+
+
+def _pools(shape, plan, kpages, vpages):
+    n = plan.n_pages * plan.page * shape.n_kv * shape.head_dim
+    if kpages.dtype not in (torch.float16, torch.bfloat16):
+        raise ValueError(f"kpages: expected float16 or bfloat16, got {kpages.dtype}")
+    return (_buf(kpages, kpages.dtype, n, "kpages", plan.device), _buf(vpages, kpages.dtype, n, "vpages", plan.device),
+            _TYPES[kpages.dtype])
+
+
+def paged_append(ctx, shape, plan, q, k, v, q_norm, k_norm, rope_freq, kpages, vpages, q_out=None, q_dtype=None):
+    """RMSNorm and RoPE of the step's new rows, keys and values into the pages, queries for attn_paged
+    (trx_paged_append).  q [rows, n_head*(1+gated)*head_dim], k, v [rows, n_kv*head_dim] float32 (rows may
+    be apart); kpages, vpages [n_pages, page, n_kv, head_dim] float16 or bfloat16.  Returns q_out [rows,
+    n_head, head_dim] of q_dtype (default: the pages' type; or float32)."""
+    dev, hd, f32 = plan.device, shape.head_dim, torch.float32
+    kp, vp, ct = _pools(shape, plan, kpages, vpages)
+    qp, q_ld = _mat(q, f32, shape.n_head * hd * (2 if shape.gated else 1), "q", dev)
+    kk, k_ld = _mat(k, f32, shape.n_kv * hd, "k", dev)
+    vv, v_ld = _mat(v, f32, shape.n_kv * hd, "v", dev)
+    rows = min(q.shape[0], k.shape[0], v.shape[0])
+    if q_out is None:
+        q_out = torch.empty(rows, shape.n_head, hd, dtype=q_dtype or kpages.dtype, device=dev)
+    if q_out.dtype not in (f32, kpages.dtype):
+        raise ValueError(f"q_out: expected float32 or {kpages.dtype}, got {q_out.dtype}")
+    rows = min(rows, q_out.shape[0])
+    if rows == 0:
+        return q_out
+    _lib.check(_lib.lib().trx_paged_append(
+        ctx.h, ctypes.byref(shape), plan.pages(rows), qp, q_ld, kk, k_ld, vv, v_ld, _buf(q_norm, f32, hd, "q_norm", dev),
+        _buf(k_norm, f32, hd, "k_norm", dev),
+        _buf(rope_freq, f32, shape.rope_dims // 2, "rope_freq", dev) if shape.rope_dims else None, kp, vp, ct,
+        _buf(q_out, q_out.dtype, rows * shape.n_head * hd, "q_out", dev), _TYPES[q_out.dtype], _stream_of(ctx)),
+        "trx_paged_append")
+    return q_out
+
+
+def attn_paged(ctx, shape, plan, q, kpages, vpages, gate=None, max_new=None, out=None):
+    """Causal attention of the step's new rows over their sequences' pages, decode and prompt chunks
+    alike (trx_attn_paged).  q [rows, n_head, head_dim] as paged_append returns it; gate: the raw q
+    projection given to paged_append (gated shapes only); max_new: a bound on the new rows of any
+    sequence (default: the rows of q).  Returns out, like q."""
+    dev, hd = plan.device, shape.head_dim
+    kp, vp, ct = _pools(shape, plan, kpages, vpages)
+    rows = q.shape[0]
+    if q.dtype not in _TYPES or (q.dtype != torch.float32 and q.dtype != kpages.dtype):
+        raise ValueError(f"q: expected float32 or {kpages.dtype}, got {q.dtype}")
+    if out is None:
+        out = torch.empty_like(q)
+    gp, g_ld = None, 0
+    if gate is not None:
+        gp, g_ld = _mat(gate, torch.float32, shape.n_head * 2 * hd, "gate", dev)
+        rows = min(rows, gate.shape[0])
+    n = rows * shape.n_head * hd
+    if rows == 0:
+        return out
+    _lib.check(_lib.lib().trx_attn_paged(
+        ctx.h, ctypes.byref(shape), plan.pages(rows), _buf(q, q.dtype, n, "q", dev), _TYPES[q.dtype], gp, g_ld, kp, vp,
+        ct, rows if max_new is None else max_new, _buf(out, q.dtype, n, "out", dev), _stream_of(ctx)), "trx_attn_paged")
+    return out
+
+
+def sample_rows(ctx, logits, u, temperature, top_k, top_p, min_p, tokens=None):
+    """One token per row of logits [n, vocab] (float32, float16 or bfloat16; rows may be apart) with the
+    row's own temperature (<= 0: greedy), top_k (<= 0: off), top_p (>= 1: off), min_p (<= 0: off) and random
+    number u in [0, 1) (trx_sample_rows); top_k int32, the others float32, [n] each.  Returns tokens [n]
+    int32 (-1 for a row without a logit above -inf)."""
+    if logits.dtype not in _TYPES or logits.dim() != 2:
+        raise ValueError(f"logits: expected a float32, float16 or bfloat16 matrix, got {logits.dtype} {tuple(logits.shape)}")
+    n, V = logits.shape
+    dev, f32 = ctx.device, torch.float32
+    lp, ld = _mat(logits, logits.dtype, V, "logits", dev)
+    if tokens is None:
+        tokens = torch.empty(n, dtype=torch.int32, device=dev)
+    if n == 0:
+        return tokens
+    _lib.check(_lib.lib().trx_sample_rows(
+        ctx.h, lp, _TYPES[logits.dtype], ld, V, n, _buf(u, f32, n, "u", dev), _buf(temperature, f32, n, "temperature", dev),
+        _buf(top_k, torch.int32, n, "top_k", dev), _buf(top_p, f32, n, "top_p", dev), _buf(min_p, f32, n, "min_p", dev),
+        _buf(tokens, torch.int32, n, "tokens", dev), _stream_of(ctx)), "trx_sample_rows")
+    return tokens
+
+
 def row_bytes(cols, kind):
     return int(_lib.lib().trx_row_bytes(cols, kind))
 
@@ -600,4 +768,5 @@ def row_bytes(cols, kind):
 __all__ = ["Context", "default_context", "DeviceTensor", "matvec_i8", "matvec_q8", "matvec_q8_f", "matvec_i8_rows", "quantize_pow2",
            "matvec_f", "matvec_fp", "matvec_swiglu", "hadamard_rotate", "validate_packed", "matvec_f_batch", "attn_decode", "attn_decode_static", "attn_shape",
            "deltanet_shape", "deltanet_step", "lmhead_argmax", "lmhead_argmax_key", "argmax_token", "matvec_f_multi", "embed_lookup",
-           "advance_position", "row_bytes", "L"]
+           "advance_position", "PagedPlan", "paged_shape", "paged_plan", "paged_release", "paged_append", "attn_paged",
+           "sample_rows", "row_bytes", "L"]
