@@ -913,8 +913,8 @@ static trx_status check_pages(const trx_pages *P) {
 
 static trx_status check_paged_shape(const trx_paged_shape *sh) {
     if (!sh || sh->n_head == 0 || sh->n_kv == 0 || sh->n_head % sh->n_kv || !(sh->eps >= 0.f)) return TRX_ERR_ARG;
-    if (sh->rope_dims > sh->head_dim) return TRX_ERR_ARG;
     if (sh->head_dim != 64 && sh->head_dim != 128 && sh->head_dim != 256) return TRX_ERR_UNSUPPORTED;
+    if (sh->rope_dims > sh->head_dim) return TRX_ERR_ARG;
     if (sh->rope_dims % 8 || sh->n_head / sh->n_kv > 16 || sh->n_head > 1024) return TRX_ERR_UNSUPPORTED;
     if (sh->window > (1u << 30) || sh->sinks > (1u << 30)) return TRX_ERR_UNSUPPORTED;
     return TRX_OK;

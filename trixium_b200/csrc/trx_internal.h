@@ -269,6 +269,11 @@ trx_status launch_paged_append(const PgAppendArgs &A, int cache_type, int q_type
 // part_cap: floats of scratch; cnt_cap: arrival counts.
 trx_status launch_attn_paged(const PgAttnArgs &A, int hd, int cache_type, int q_type, size_t part_cap, int cnt_cap,
                              uint32_t *err, cudaStream_t st);
+trx_status launch_attn_paged_tc(const PgAttnArgs &A, int hd, int cache_type, int q_type, size_t part_cap, int cnt_cap,
+                                uint32_t *err, cudaStream_t st);
+// A tiled TMA map of a row-major matrix of 16-bit elements (128-byte swizzle; trx_rows.cu): map points to
+// a CUtensorMap.  Elements outside the matrix read as zeros.
+bool encode_map_16bit(void *map, const void *base, uint64_t cols, uint64_t rows, uint32_t box_cols, uint32_t box_rows);
 // Sampling (trx_sample.cu).
 struct SampleArgs {
     const void *x;

@@ -238,6 +238,9 @@ __device__ __forceinline__ bool pg_hidden(int k, int p, int window, int sinks) {
     return k > p || (window && p - k >= window && k >= sinks);
 }
 
+template <typename CT> struct PgIsBf16 { static constexpr bool value = false; };
+template <> struct PgIsBf16<__nv_bfloat16> { static constexpr bool value = true; };
+
 template <typename CT> struct PgCvt;
 template <> struct PgCvt<__half> {
     static __device__ __forceinline__ __half from(float x) { return __float2half_rn(x); }

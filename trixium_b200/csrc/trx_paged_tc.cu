@@ -1,0 +1,667 @@
+// Attention of prompt chunks over a paged KV cache on the 5th-generation tensor cores (sm_100a
+// tcgen05, kind::f16): the same computation as attn_paged_kernel (trx_paged.cu), for sequences with
+// more than 16 query rows per kv head.
+//
+// Work: a query tile is 128 rows of one kv head, (token, head of the group) pairs in order: 128 / rep
+// tokens x rep heads (padded).  A CTA walks its pieces (PgSched): key tiles of KT positions of one
+// (query tile, kv head).  Per key tile S = Q K^T (M = 128, N = KT), the softmax in 32 bits, O += P V
+// (M = 128, N = head dim).  Warp roles:
+//  * warps 0-3: one query row per thread (its TMEM lane).  They put the query tile into shared memory,
+//    read S from tensor memory, keep the row's maximum and sum, write P (16 bits) over S as the A operand
+//    of the second product, and finish the piece.  O is rescaled only when a row's maximum has grown by
+//    more than 2^8 over the one in use: P then stays below 2^8, exact in any 16-bit float's exponent.
+//  * warp 4: the producer.  A key tile is gathered by TMA boxes of one page (or the tile's part of it) x
+//    64 dims, 128-byte swizzle; places behind the sequence's end come from outside the map, as zeros.
+//  * warp 5: issues the MMAs from one elected lane and commits them to the barriers below.
+// fp32 queries: Q = hi + lo and P = hi + lo in fp16, two MMAs per product, so products keep 2^-22.
+// V is read as the N-major B operand of the second product straight from its row-major tile; the rows
+// of a sequence's last page behind its end are overwritten with zeros first (0 times what lies there
+// would not be 0 if it is not finite).
+//
+// Head dims 64 and 128 run two CTAs per SM (at most 113 KB of shared memory, 256 TMEM columns each):
+// while one computes its softmax the other's MMAs run.  Head dim 256 has one CTA with two S buffers: the
+// next tile's S is computed while this one's softmax runs.
+#include <algorithm>
+#include <cstdint>
+#include <cstring>
+#include <cuda.h>
+#include <cuda_runtime.h>
+
+#include "trx_paged.cuh"
+
+namespace trx {
+namespace {
+
+constexpr int kTcThreads = 192;
+constexpr int kTcRows = 128;  // query rows of a tile: the MMA's M, the TMEM lanes
+
+template <int HD, bool SPLIT>
+struct TcCfg {
+    static constexpr int KT = HD == 64 ? 128 : (HD == 128 ? (SPLIT ? 64 : 128) : 64);
+    static constexpr int KT_SHIFT = KT == 128 ? 7 : 6;
+    static constexpr int NS = HD == 256 ? 2 : 1;                  // S buffers
+    static constexpr int KST = HD == 256 && !SPLIT ? 2 : 1;      // K and V tiles in shared memory
+    static constexpr int CTAS = HD == 256 ? 1 : 2;               // per SM
+    static constexpr int TMEM = HD == 256 ? 512 : 256;           // columns: O [HD], then S [NS][KT]
+    static constexpr int QBYTES = kTcRows * HD * 2, TBYTES = KT * HD * 2;
+    static constexpr int QOFF = 0, KOFF = QBYTES * (SPLIT ? 2 : 1), VOFF = KOFF + KST * TBYTES,
+                         END = VOFF + KST * TBYTES;  // multiples of 1024
+    static_assert(HD + NS * KT <= TMEM, "tensor memory holds O and every S");
+};
+
+struct TcBars {
+    uint64_t kfull[2], kfree[2];   // a K tile has landed; the MMAs that read it are complete
+    uint64_t vfull[2], vfree[2];   // the same for V
+    uint64_t sfull[2], pready[2];  // S is complete; P is in its place (4 warps)
+    uint64_t odone;                // a tile's P V is complete
+    uint64_t qready;               // the query tile is in shared memory (4 warps)
+    uint64_t join, fin;            // the softmax warps among themselves; every MMA of the block
+    uint32_t tmem;
+    volatile uint32_t dead;        // a wait ran out somewhere in the block
+    int last;
+};
+
+struct TcTail {  // behind the tiles
+    TcBars bars;
+    PgSchedSmem sched;
+};
+
+__device__ __forceinline__ void tc_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void tc_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
+
+// K-major operand tile, 128-byte swizzle: rows of 64 16-bit elements, 8-row groups 1024 bytes apart.
+__device__ __forceinline__ uint64_t desc_kmajor(uint32_t a) {
+    return (uint64_t)((a >> 4) & 0x3FFFu) | ((uint64_t)1u << 16) | ((uint64_t)(1024u >> 4) << 32) |
+           ((uint64_t)1u << 46) | ((uint64_t)2u << 61);
+}
+// N-major operand tile, 128-byte swizzle: 64 N elements contiguous, K rows 128 bytes apart in groups of 8
+// (1024 bytes apart), the next 64 N elements `block` bytes on.
+__device__ __forceinline__ uint64_t desc_nmajor(uint32_t a, uint32_t block) {
+    return (uint64_t)((a >> 4) & 0x3FFFu) | ((uint64_t)(block >> 4) << 16) | ((uint64_t)(1024u >> 4) << 32) |
+           ((uint64_t)1u << 46) | ((uint64_t)2u << 61);
+}
+// Instruction descriptor of kind::f16: D fp32, A and B fp16 (0) or bf16 (1), B N-major if bn, N, M = 128.
+template <typename CT>
+__device__ __forceinline__ uint32_t idesc_f16(int n, bool bn) {
+    constexpr uint32_t t = PgIsBf16<CT>::value ? 1u : 0u;
+    return (1u << 4) | (t << 7) | (t << 10) | ((bn ? 1u : 0u) << 16) | ((uint32_t)(n >> 3) << 17) |
+           ((uint32_t)(kTcRows >> 4) << 24);
+}
+
+// One elected lane of the converged warp issues (all lanes execute; operands are warp-uniform).
+__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, bool acc) {
+    asm volatile(
+        "{\n .reg .pred p, e;\n setp.ne.b32 p, %4, 0;\n elect.sync _|e, 0xffffffff;\n"
+        " @e tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}\n" ::"r"(d),
+        "l"(a), "l"(b), "r"(idesc), "r"((int)acc)
+        : "memory");
+}
+__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, bool acc) {
+    asm volatile(
+        "{\n .reg .pred p, e;\n setp.ne.b32 p, %4, 0;\n elect.sync _|e, 0xffffffff;\n"
+        " @e tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}\n" ::"r"(d),
+        "r"(a), "l"(b), "r"(idesc), "r"((int)acc)
+        : "memory");
+}
+__device__ __forceinline__ void commit(uint32_t bar) {
+    asm volatile(
+        "{\n .reg .pred e;\n elect.sync _|e, 0xffffffff;\n"
+        " @e tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n}\n" ::"r"(bar)
+        : "memory");
+}
+__device__ __forceinline__ void arrive(uint32_t bar) {
+    asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory");
+}
+__device__ __forceinline__ void load_box(uint32_t dst, const void *map, int x, int y, uint32_t bar) {
+    asm volatile(
+        "cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], "
+        "[%4];" ::"r"(dst),
+        "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(bar)
+        : "memory");
+}
+
+// Tensor memory, one lane per thread, 32 (or 16) consecutive columns.
+__device__ __forceinline__ void tm_ld32(uint32_t a, uint32_t (&v)[32]) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
+        "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
+        : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]), "=r"(v[8]),
+          "=r"(v[9]), "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15]), "=r"(v[16]),
+          "=r"(v[17]), "=r"(v[18]), "=r"(v[19]), "=r"(v[20]), "=r"(v[21]), "=r"(v[22]), "=r"(v[23]), "=r"(v[24]),
+          "=r"(v[25]), "=r"(v[26]), "=r"(v[27]), "=r"(v[28]), "=r"(v[29]), "=r"(v[30]), "=r"(v[31])
+        : "r"(a)
+        : "memory");
+}
+__device__ __forceinline__ void tm_st32(uint32_t a, const uint32_t (&o)[32]) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, "
+        "%15, %16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, %32};" ::"r"(a),
+        "r"(o[0]), "r"(o[1]), "r"(o[2]), "r"(o[3]), "r"(o[4]), "r"(o[5]), "r"(o[6]), "r"(o[7]), "r"(o[8]), "r"(o[9]),
+        "r"(o[10]), "r"(o[11]), "r"(o[12]), "r"(o[13]), "r"(o[14]), "r"(o[15]), "r"(o[16]), "r"(o[17]), "r"(o[18]),
+        "r"(o[19]), "r"(o[20]), "r"(o[21]), "r"(o[22]), "r"(o[23]), "r"(o[24]), "r"(o[25]), "r"(o[26]), "r"(o[27]),
+        "r"(o[28]), "r"(o[29]), "r"(o[30]), "r"(o[31])
+        : "memory");
+}
+__device__ __forceinline__ void tm_st16(uint32_t a, const uint32_t (&o)[16]) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, "
+        "%15, %16};" ::"r"(a),
+        "r"(o[0]), "r"(o[1]), "r"(o[2]), "r"(o[3]), "r"(o[4]), "r"(o[5]), "r"(o[6]), "r"(o[7]), "r"(o[8]), "r"(o[9]),
+        "r"(o[10]), "r"(o[11]), "r"(o[12]), "r"(o[13]), "r"(o[14]), "r"(o[15])
+        : "memory");
+}
+__device__ __forceinline__ void tm_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ void tm_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+
+__device__ __forceinline__ float ex2f(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
+struct TcMaps {
+    CUtensorMap k, v;
+};
+
+// 32 outputs of one row, dims d..d+31.
+template <typename QT>
+__device__ __forceinline__ void put32(const PgAttnArgs &A, int hd, int row, int h, int d, float (&o)[32]) {
+    if (A.gate) {
+        const float4 *g = reinterpret_cast<const float4 *>(A.gate + row * A.gate_ld + (long long)h * 2 * hd + hd + d);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const float4 v = g[i];
+            o[4 * i] = __fdividef(o[4 * i], 1.0f + expf(-v.x));
+            o[4 * i + 1] = __fdividef(o[4 * i + 1], 1.0f + expf(-v.y));
+            o[4 * i + 2] = __fdividef(o[4 * i + 2], 1.0f + expf(-v.z));
+            o[4 * i + 3] = __fdividef(o[4 * i + 3], 1.0f + expf(-v.w));
+        }
+    }
+    QT *dst = reinterpret_cast<QT *>(A.out) + ((size_t)row * A.H + h) * hd + d;
+    if constexpr (sizeof(QT) == 4) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+            reinterpret_cast<float4 *>(dst)[i] = make_float4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]);
+    } else {
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            reinterpret_cast<uint4 *>(dst)[i] =
+                make_uint4(PgCvt<QT>::pack(o[8 * i], o[8 * i + 1]), PgCvt<QT>::pack(o[8 * i + 2], o[8 * i + 3]),
+                           PgCvt<QT>::pack(o[8 * i + 4], o[8 * i + 5]), PgCvt<QT>::pack(o[8 * i + 6], o[8 * i + 7]));
+    }
+}
+
+template <typename CT, typename QT, int HD>
+__global__ void __launch_bounds__(kTcThreads, HD == 256 ? 1 : 2)
+    attn_paged_tc_kernel(const __grid_constant__ TcMaps maps, PgAttnArgs A, uint32_t *err) {
+    constexpr bool SPLIT = sizeof(QT) == 4;
+    using C = TcCfg<HD, SPLIT>;
+    constexpr int KT = C::KT, NS = C::NS, KST = C::KST;
+    extern __shared__ __align__(1024) unsigned char smem[];
+    TcTail &tail = *reinterpret_cast<TcTail *>(smem + C::END);
+    TcBars &bars = tail.bars;
+    PgSchedSmem &sched = tail.sched;
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const uint32_t sbase = smem_u32(smem);
+    if (sbase & 1023u) {  // the swizzled tiles need 1024-byte places
+        pdl_wait();
+        if (tid == 0) atomicOr(err, TRX_DEV_INTERNAL);
+        return;
+    }
+    if (tid == 0) {
+        for (int i = 0; i < 2; ++i) {
+            mbar_init(&bars.kfull[i], 1);
+            mbar_init(&bars.kfree[i], 1);
+            mbar_init(&bars.vfull[i], 1);
+            mbar_init(&bars.vfree[i], 1);
+            mbar_init(&bars.sfull[i], 1);
+            mbar_init(&bars.pready[i], 4);
+        }
+        mbar_init(&bars.odone, 1);
+        mbar_init(&bars.qready, 4);
+        mbar_init(&bars.join, 4);
+        mbar_init(&bars.fin, 1);
+        bars.dead = 0u;
+        mbar_fence_init();
+        tma_prefetch_map(&maps.k);
+        tma_prefetch_map(&maps.v);
+    }
+    pdl_wait();
+    // Tensor memory is taken only now that the kernel in front has ended, and the kernel behind is let in
+    // only once it is taken: a neighbour that allocates before it waits could otherwise hold what this
+    // one needs while it waits for this one.
+    if (warp == 5) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&bars.tmem)),
+                     "r"(C::TMEM)
+                     : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+    tc_before();
+    pg_schedule(A, sched, 1, err);  // barriers inside: the allocation and the barriers' set-up are visible behind it
+    tc_after();
+    pdl_trigger();
+    const uint32_t tmem = bars.tmem;
+    const PgSched &S = sched.S;
+    const uint32_t kfull = smem_u32(bars.kfull), kfree = smem_u32(bars.kfree), vfull = smem_u32(bars.vfull),
+                   vfree = smem_u32(bars.vfree), sfull = smem_u32(bars.sfull), pready = smem_u32(bars.pready),
+                   odone = smem_u32(&bars.odone), qready = smem_u32(&bars.qready), fin = smem_u32(&bars.fin);
+    // Every lane of a warp waits; false for all of them if any wait ran out.
+    auto wait = [&](uint32_t bar, uint32_t parity) {
+        const bool ok = __all_sync(0xffffffffu, mbar_wait_bounded_s(bar, parity & 1u, err));
+        if (!ok) bars.dead = 1u;
+        return ok;
+    };
+    PgWalk W;
+    const bool any = W.start(A, S);
+    if (any && warp == 4) {
+        // Producer.
+        const int br = min(1 << A.page_shift, KT), nb = KT / br;  // box rows, boxes per 64 dims
+        const int boxes = nb * (HD / 64);
+        const int beyond = A.n_pages << A.page_shift;  // a row outside the maps: zeros
+        int j = 0;
+        bool ok = true, more = true;
+        while (ok && more) {
+            const int *tab = A.tables + (long long)W.b * A.max_pages;
+            const int len = W.q.p0 + W.q.n;
+            for (int it = W.i0; ok && it < W.i1; ++it, ++j) {
+                const int st = j % KST, k0 = W.R.tile(it) * KT;
+                static_assert(KT / 16 * (HD / 64) <= 32, "a lane has one box");
+                int row = beyond;
+                if (lane < boxes) {
+                    const int p = k0 + (lane % nb) * br;
+                    if (p < len) {
+                        const int id = __ldg(tab + (p >> A.page_shift));
+                        if ((unsigned)id < (unsigned)A.n_pages)
+                            row = (id << A.page_shift) + (p & ((1 << A.page_shift) - 1));
+                        else
+                            atomicOr(err, TRX_DEV_RANGE);
+                    }
+                }
+                if (bars.dead) {
+                    ok = false;
+                    break;
+                }
+                for (int kind = 0; kind < 2; ++kind) {
+                    const uint32_t full = (kind ? vfull : kfull) + 8u * st, freed = (kind ? vfree : kfree) + 8u * st;
+                    if (j >= KST && !wait(freed, (uint32_t)(j / KST - 1))) {
+                        ok = false;
+                        break;
+                    }
+                    if (lane == 0) mbar_expect_tx_s(full, (uint32_t)C::TBYTES);
+                    __syncwarp();
+                    const uint32_t base = sbase + (kind ? C::VOFF : C::KOFF) + (uint32_t)(st * C::TBYTES);
+                    if (lane < boxes)
+                        load_box(base + (uint32_t)((lane / nb) * KT * 128 + (lane % nb) * br * 128),
+                                 kind ? &maps.v : &maps.k, W.kh * HD + 64 * (lane / nb), row, full);
+                    __syncwarp();
+                }
+            }
+            if (ok) more = W.next(A);
+        }
+        if (!ok) {
+            // Whatever was issued has landed before the block leaves (bounded; the timeout is recorded).
+            bars.dead = 1u;
+            for (int kind = 0; kind < 2; ++kind)
+                for (int st = 0; st < KST; ++st)
+                    for (int ph = 0; ph < 2; ++ph) mbar_wait_bounded_s((kind ? vfull : kfull) + 8u * st, ph, nullptr);
+        }
+    } else if (any && warp == 5) {
+        // MMA issue.
+        const uint32_t idq = idesc_f16<CT>(KT, false), idv = idesc_f16<CT>(HD, true);
+        int j = 0, jq = 0, j0 = 0;  // next tile of P V, of Q K^T, first of the piece
+        uint32_t piece = 0;
+        bool ok = true, more = true;
+        auto qk = [&] {  // S[jq % NS] = Q K(jq)^T
+            const int st = jq % KST;
+            if (!wait(kfull + 8u * st, (uint32_t)(jq / KST))) return false;
+            // P V of the tile that had this S buffer is complete (for a piece's first tiles: known from
+            // qready, and their phase may have passed).
+            if (jq - NS >= j0 && !wait(odone, (uint32_t)(jq - NS))) return false;
+            tc_after();
+            const uint32_t d = tmem + HD + (uint32_t)((jq % NS) * KT), ka = sbase + C::KOFF + (uint32_t)(st * C::TBYTES);
+#pragma unroll
+            for (int part = 0; part < (SPLIT ? 2 : 1); ++part)
+#pragma unroll
+                for (int k = 0; k < HD / 16; ++k)
+                    mma_ss(d, desc_kmajor(sbase + C::QOFF + part * C::QBYTES + (k / 4) * (kTcRows * 128) + (k % 4) * 32),
+                           desc_kmajor(ka + (k / 4) * (KT * 128) + (k % 4) * 32), idq, part || k);
+            commit(kfree + 8u * st);
+            commit(sfull + 8u * (jq % NS));
+            ++jq;
+            return true;
+        };
+        while (ok && more) {
+            if (!wait(qready, piece++)) {
+                ok = false;
+                break;
+            }
+            tc_after();
+            const int jend = j + W.i1 - W.i0;
+            j0 = j;
+            for (; ok && j < jend; ++j) {
+                if (bars.dead) {
+                    ok = false;
+                    break;
+                }
+                while (ok && jq < jend && jq < j + NS) ok = qk();
+                if (!ok) break;
+                const int st = j % KST;
+                if (!wait(vfull + 8u * st, (uint32_t)(j / KST)) || !wait(pready + 8u * (j % NS), (uint32_t)(j / NS))) {
+                    ok = false;
+                    break;
+                }
+                tc_after();
+                const uint32_t p = tmem + HD + (uint32_t)((j % NS) * KT), va = sbase + C::VOFF + (uint32_t)(st * C::TBYTES);
+#pragma unroll
+                for (int k = 0; k < KT / 16; ++k) {
+                    const uint64_t b = desc_nmajor(va + k * 2048, KT * 128);
+                    if constexpr (SPLIT) {
+                        mma_ts(tmem, p + 32 * (k / 2) + 8 * (k % 2), b, idv, j != j0 || k);
+                        mma_ts(tmem, p + 32 * (k / 2) + 8 * (k % 2) + 16, b, idv, true);
+                    } else {
+                        mma_ts(tmem, p + 8 * k, b, idv, j != j0 || k);
+                    }
+                }
+                commit(vfree + 8u * st);
+                commit(odone);
+            }
+            if (ok) more = W.next(A);
+        }
+        if (!ok) bars.dead = 1u;
+        commit(fin);  // every MMA is complete before the tensor memory is given back
+        mbar_wait_bounded_s(fin, 0u, nullptr);
+    } else if (any) {
+        // Softmax: query row tid of the piece's tile.
+        const int r = tid;
+        const uint32_t lanes = (uint32_t)(32 * warp) << 16;
+        int j = 0;
+        uint32_t joined = 0;
+        auto join = [&] {  // the four warps (bounded, unlike a block barrier)
+            __syncwarp();
+            if (lane == 0) arrive(smem_u32(&bars.join));
+            return wait(smem_u32(&bars.join), joined++);
+        };
+        bool ok = true, more = true;
+        while (ok && more) {
+            const int rows = W.rows(A), len = W.q.p0 + W.q.n;
+            const int row0 = W.q.row0 + W.t * A.tq, pos0 = W.q.p0 + W.t * A.tq;
+            const int tok = r / A.rep, head = W.kh * A.rep + r - tok * A.rep;
+            const int qpos = r < rows ? pos0 + tok : -1;
+            const int pmax = pos0 + (rows - 1) / A.rep;  // the tile's last position; pos0 its first
+            // The query tile, zeros behind its rows.  Every MMA that read the previous one is complete (its
+            // S was waited for).
+            for (int i = r; i < kTcRows * (HD / 8); i += kTcRows) {
+                const int qr = i / (HD / 8), c = i % (HD / 8);
+                uint4 hi = make_uint4(0u, 0u, 0u, 0u), lo = hi;
+                if (qr < rows) {
+                    const int tk = qr / A.rep, h = W.kh * A.rep + qr - tk * A.rep;
+                    const QT *src = reinterpret_cast<const QT *>(A.q) + ((size_t)(row0 + tk) * A.H + h) * HD + c * 8;
+                    if constexpr (SPLIT) {
+                        const float4 x = *reinterpret_cast<const float4 *>(src), y = *reinterpret_cast<const float4 *>(src + 4);
+                        const float f[8] = {x.x, x.y, x.z, x.w, y.x, y.y, y.z, y.w};
+                        uint32_t hw[4], lw[4];
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            hw[e] = PgCvt<CT>::pack(f[2 * e], f[2 * e + 1]);
+                            const float2 b = PgCvt<CT>::unpack(hw[e]);
+                            lw[e] = PgCvt<CT>::pack(f[2 * e] - b.x, f[2 * e + 1] - b.y);
+                        }
+                        hi = make_uint4(hw[0], hw[1], hw[2], hw[3]);
+                        lo = make_uint4(lw[0], lw[1], lw[2], lw[3]);
+                    } else {
+                        hi = *reinterpret_cast<const uint4 *>(src);
+                    }
+                }
+                const uint32_t off = (uint32_t)((c / 8) * (kTcRows * 128) + qr * 128 + (((c % 8) ^ (qr & 7)) << 4));
+                *reinterpret_cast<uint4 *>(smem + C::QOFF + off) = hi;
+                if constexpr (SPLIT) *reinterpret_cast<uint4 *>(smem + C::QOFF + C::QBYTES + off) = lo;
+            }
+            fence_proxy_async();
+            __syncwarp();
+            if (lane == 0) arrive(qready);
+            float m = -INFINITY, l = 0.f;
+            const int j0 = j;
+            for (int it = W.i0; it < W.i1; ++it, ++j) {
+                const int k0 = W.R.tile(it) * KT;
+                const uint32_t ts = tmem + lanes + HD + (uint32_t)((j % NS) * KT);
+                // Nothing of the tile is hidden from any row.
+                const bool open = k0 + KT - 1 <= pos0 &&
+                                  (!A.window || pmax - k0 < A.window || k0 + KT <= A.sinks);
+                if (!wait(sfull + 8u * (j % NS), (uint32_t)(j / NS))) {
+                    ok = false;
+                    break;
+                }
+                tc_after();
+                float mx = -INFINITY;
+#pragma unroll
+                for (int c = 0; c < KT / 32; ++c) {
+                    uint32_t v[32];
+                    tm_ld32(ts + 32 * c, v);
+                    tm_wait_ld();
+                    if (open) {
+#pragma unroll
+                        for (int e = 0; e < 32; ++e) mx = fmaxf(mx, __uint_as_float(v[e]));
+                    } else {
+#pragma unroll
+                        for (int e = 0; e < 32; ++e)
+                            mx = fmaxf(mx, pg_hidden(k0 + 32 * c + e, qpos, A.window, A.sinks) ? -INFINITY
+                                                                                              : __uint_as_float(v[e]));
+                    }
+                }
+                mx *= A.scale_log2;
+                if (r >= rows) mx = -INFINITY;
+                if (j == j0) {
+                    m = mx;
+                } else {
+                    const bool grow = mx > m + 8.f;
+                    if (__any_sync(0xffffffffu, grow)) {
+                        if (!wait(odone, (uint32_t)(j - 1))) {
+                            ok = false;
+                            break;
+                        }
+                        tc_after();
+                        // A row without a maximum so far has O = 0 and l = 0.
+                        const float f = grow && m != -INFINITY ? ex2f(m - mx) : 1.f;
+                        if (grow) m = mx;
+                        l *= f;
+#pragma unroll
+                        for (int c = 0; c < HD / 32; ++c) {
+                            uint32_t v[32];
+                            tm_ld32(tmem + lanes + 32 * c, v);
+                            tm_wait_ld();
+#pragma unroll
+                            for (int e = 0; e < 32; ++e) v[e] = __float_as_uint(__uint_as_float(v[e]) * f);
+                            tm_st32(tmem + lanes + 32 * c, v);
+                        }
+                        tm_wait_st();
+                    }
+                }
+                const float nm = m == -INFINITY ? 0.f : -m;
+                float sum[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                for (int c = 0; c < KT / 32; ++c) {
+                    uint32_t v[32], ph[16];
+                    tm_ld32(ts + 32 * c, v);
+                    tm_wait_ld();
+#pragma unroll
+                    for (int e = 0; e < 32; ++e) {
+                        float x = fmaf(__uint_as_float(v[e]), A.scale_log2, nm);
+                        if (!open && pg_hidden(k0 + 32 * c + e, qpos, A.window, A.sinks)) x = -INFINITY;
+                        const float p = ex2f(x);
+                        v[e] = __float_as_uint(p);
+                        sum[e & 3] += p;
+                    }
+#pragma unroll
+                    for (int e = 0; e < 16; ++e)
+                        ph[e] = PgCvt<CT>::pack(__uint_as_float(v[2 * e]), __uint_as_float(v[2 * e + 1]));
+                    if constexpr (SPLIT) {
+                        tm_st16(ts + 32 * c, ph);
+#pragma unroll
+                        for (int e = 0; e < 16; ++e) {
+                            const float2 b = PgCvt<CT>::unpack(ph[e]);
+                            ph[e] = PgCvt<CT>::pack(__uint_as_float(v[2 * e]) - b.x, __uint_as_float(v[2 * e + 1]) - b.y);
+                        }
+                        tm_st16(ts + 32 * c + 16, ph);
+                    } else {
+                        tm_st16(ts + 16 * c, ph);
+                    }
+                }
+                l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+                if (k0 + KT > len) {  // the rows of V behind the sequence's end
+                    if (!wait(vfull + 8u * (j % KST), (uint32_t)(j / KST))) {
+                        ok = false;
+                        break;
+                    }
+                    unsigned char *vt = smem + C::VOFF + (j % KST) * C::TBYTES;
+                    for (int i = r; i < (KT - (len - k0)) * (HD / 8); i += kTcRows) {
+                        const int vr = len - k0 + i / (HD / 8), c = i % (HD / 8);
+                        *reinterpret_cast<uint4 *>(vt + (c / 8) * (KT * 128) + vr * 128 + (c % 8) * 16) =
+                            make_uint4(0u, 0u, 0u, 0u);
+                    }
+                    fence_proxy_async();
+                }
+                tm_wait_st();
+                tc_before();
+                __syncwarp();
+                if (lane == 0) arrive(pready + 8u * (j % NS));
+            }
+            if (!ok) break;
+            if (!wait(odone, (uint32_t)(j - 1))) {
+                ok = false;
+                break;
+            }
+            tc_after();
+            if (W.whole()) {
+                const float inv = l > 0.f ? __fdiv_rn(1.0f, l) : 0.f;
+#pragma unroll 1
+                for (int c = 0; c < HD / 32; ++c) {
+                    uint32_t v[32];
+                    tm_ld32(tmem + lanes + 32 * c, v);
+                    tm_wait_ld();
+                    if (r < rows) {
+                        float o[32];
+#pragma unroll
+                        for (int e = 0; e < 32; ++e) o[e] = __uint_as_float(v[e]) * inv;
+                        put32<QT>(A, HD, row0 + tok, head, 32 * c, o);
+                    }
+                }
+            } else {
+                // A cut item (as in attn_paged_kernel): scratch [HD / 4][128 rows] of four dims, then the
+                // maxima and sums.
+                const long long item0 = W.u - W.i1, item1 = item0 + W.R.cnt;
+                const int c0 = pg_owner(S, item0), c1 = pg_owner(S, item1 - 1);
+                constexpr size_t kPart = kTcRows * (HD + 2);
+                auto slot_of = [&](int cc) { return A.part + kPart * (2 * (size_t)cc + (cc == c0 ? 1 : 0)); };
+                float *const mine = slot_of(blockIdx.x);
+#pragma unroll 1
+                for (int c = 0; c < HD / 32; ++c) {
+                    uint32_t v[32];
+                    tm_ld32(tmem + lanes + 32 * c, v);
+                    tm_wait_ld();
+#pragma unroll
+                    for (int e = 0; e < 8; ++e)
+                        reinterpret_cast<uint4 *>(mine)[(8 * c + e) * kTcRows + r] =
+                            make_uint4(v[4 * e], v[4 * e + 1], v[4 * e + 2], v[4 * e + 3]);
+                }
+                mine[kTcRows * HD + r] = m;
+                mine[kTcRows * (HD + 1) + r] = l;
+                __threadfence();
+                if (!join()) {
+                    ok = false;
+                    break;
+                }
+                if (r == 0) bars.last = atomicAdd(A.cnt + c0, 1u) == (unsigned)(c1 - c0);
+                if (!join()) {
+                    ok = false;
+                    break;
+                }
+                if (bars.last) {
+                    __threadfence();
+                    float M = -INFINITY, L = 0.f;
+                    for (int cc = c0; cc <= c1; ++cc) M = fmaxf(M, __ldcg(slot_of(cc) + kTcRows * HD + r));
+                    const float Ms = M == -INFINITY ? 0.f : M;
+                    for (int cc = c0; cc <= c1; ++cc) {
+                        const float *p = slot_of(cc) + kTcRows * HD + r;
+                        L = fmaf(ex2f(__ldcg(p) - Ms), __ldcg(p + kTcRows), L);
+                    }
+                    const float inv = L > 0.f ? __fdiv_rn(1.0f, L) : 0.f;
+#pragma unroll 1
+                    for (int c = 0; c < HD / 32; ++c) {
+                        float o[32];
+#pragma unroll
+                        for (int e = 0; e < 32; ++e) o[e] = 0.f;
+                        for (int cc = c0; cc <= c1; ++cc) {
+                            const float *p = slot_of(cc);
+                            const float w = ex2f(__ldcg(p + kTcRows * HD + r) - Ms);
+#pragma unroll
+                            for (int e = 0; e < 8; ++e) {
+                                const float4 x = __ldcg(reinterpret_cast<const float4 *>(p) + (8 * c + e) * kTcRows + r);
+                                o[4 * e] = fmaf(w, x.x, o[4 * e]);
+                                o[4 * e + 1] = fmaf(w, x.y, o[4 * e + 1]);
+                                o[4 * e + 2] = fmaf(w, x.z, o[4 * e + 2]);
+                                o[4 * e + 3] = fmaf(w, x.w, o[4 * e + 3]);
+                            }
+                        }
+#pragma unroll
+                        for (int e = 0; e < 32; ++e) o[e] *= inv;
+                        if (r < rows) put32<QT>(A, HD, row0 + tok, head, 32 * c, o);
+                    }
+                    if (r == 0) A.cnt[c0] = 0u;
+                }
+            }
+            tc_before();
+            more = W.next(A);
+        }
+        if (!ok) bars.dead = 1u;
+    }
+    tc_before();
+    __syncthreads();
+    if (warp == 5) {
+        tc_after();
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(C::TMEM) : "memory");
+    }
+}
+
+template <typename CT, typename QT, int HD>
+trx_status launch_tc(PgAttnArgs A, size_t part_cap, int cnt_cap, uint32_t *err, cudaStream_t st) {
+    using C = TcCfg<HD, sizeof(QT) == 4>;
+    static DevBits configured{0};
+    const cudaError_t e = once_per_device(configured, [] {
+        return cudaFuncSetAttribute(attn_paged_tc_kernel<CT, QT, HD>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                    (int)(C::END + sizeof(TcTail)));
+    });
+    if (e != cudaSuccess) return note_cuda(e);
+    A.tq = kTcRows / A.rep;
+    A.kt_shift = C::KT_SHIFT;
+    TcMaps maps;
+    const int page = 1 << A.page_shift;
+    const uint64_t cols = (uint64_t)A.Hkv * HD, rows = (uint64_t)A.n_pages << A.page_shift;
+    const uint32_t br = (uint32_t)std::min(page, C::KT);
+    if (!encode_map_16bit(&maps.k, A.kp, cols, rows, 64, br) || !encode_map_16bit(&maps.v, A.vp, cols, rows, 64, br))
+        return TRX_ERR_CUDA;
+    const int grid = device_sms() * C::CTAS;
+    if ((size_t)grid * 2 * kTcRows * (HD + 2) > part_cap || grid > cnt_cap) return TRX_ERR_UNSUPPORTED;
+    return note_cuda(launch_kernel(attn_paged_tc_kernel<CT, QT, HD>, dim3(grid), dim3(kTcThreads), C::END + sizeof(TcTail), st,
+                                   maps, A, err));
+}
+
+template <typename CT, typename QT>
+trx_status launch_tc_hd(const PgAttnArgs &A, int hd, size_t part_cap, int cnt_cap, uint32_t *err, cudaStream_t st) {
+    switch (hd) {
+        case 64: return launch_tc<CT, QT, 64>(A, part_cap, cnt_cap, err, st);
+        case 128: return launch_tc<CT, QT, 128>(A, part_cap, cnt_cap, err, st);
+        default: return launch_tc<CT, QT, 256>(A, part_cap, cnt_cap, err, st);
+    }
+}
+
+}  // namespace
+
+trx_status launch_attn_paged_tc(const PgAttnArgs &A, int hd, int cache_type, int q_type, size_t part_cap, int cnt_cap,
+                                uint32_t *err, cudaStream_t st) {
+    if (cache_type == TRX_TYPE_BF16)
+        return launch_tc_hd<__nv_bfloat16, __nv_bfloat16>(A, hd, part_cap, cnt_cap, err, st);
+    return q_type == TRX_TYPE_F32 ? launch_tc_hd<__half, float>(A, hd, part_cap, cnt_cap, err, st)
+                                  : launch_tc_hd<__half, __half>(A, hd, part_cap, cnt_cap, err, st);
+}
+
+}  // namespace trx
