@@ -12,15 +12,15 @@
 //    more than 2^8 over the one in use: P then stays below 2^8, exact in any 16-bit float's exponent.
 //  * warp 4: the producer.  A key tile is gathered by TMA boxes of one page (or the tile's part of it) x
 //    64 dims, 128-byte swizzle; places behind the sequence's end come from outside the map, as zeros.
-//  * warp 5: issues the MMAs from one elected lane and commits them to the barriers below.
+//  * warps 5 and 6: issue the MMAs of the first and of the second product, each from one elected lane. Two
+//    warps, since one's instructions between two MMAs (waits, commits) take as long as the MMAs.
 // fp32 queries: Q = hi + lo and P = hi + lo in fp16, two MMAs per product, so products keep 2^-22.
 // V is read as the N-major B operand of the second product straight from its row-major tile; the rows
 // of a sequence's last page behind its end are overwritten with zeros first (0 times what lies there
 // would not be 0 if it is not finite).
 //
-// Head dims 64 and 128 run two CTAs per SM (at most 113 KB of shared memory, 256 TMEM columns each):
-// while one computes its softmax the other's MMAs run.  Head dim 256 has one CTA with two S buffers: the
-// next tile's S is computed while this one's softmax runs.
+// Two S buffers: the next tile's S is computed while this one's softmax runs.  Head dims 64 and 128 run
+// two CTAs per SM (at most 113 KB of shared memory, 256 TMEM columns each), head dim 256 one.
 #include <algorithm>
 #include <cstdint>
 #include <cstring>
@@ -32,15 +32,14 @@
 namespace trx {
 namespace {
 
-constexpr int kTcThreads = 192;
+constexpr int kTcThreads = 256;
 constexpr int kTcRows = 128;  // query rows of a tile: the MMA's M, the TMEM lanes
 
 template <int HD, bool SPLIT>
 struct TcCfg {
-    static constexpr int KT = HD == 64 ? 128 : (HD == 128 ? (SPLIT ? 64 : 128) : 64);
-    static constexpr int KT_SHIFT = KT == 128 ? 7 : 6;
-    static constexpr int NS = HD == 256 ? 2 : 1;                  // S buffers
-    static constexpr int KST = HD == 256 && !SPLIT ? 2 : 1;      // K and V tiles in shared memory
+    static constexpr int KT = 64, KT_SHIFT = 6;                   // key positions of a tile
+    static constexpr int NS = 2;                                  // S buffers (the barriers' pairs)
+    static constexpr int KST = SPLIT && HD >= 128 ? 1 : 2;       // K and V tiles in shared memory
     static constexpr int CTAS = HD == 256 ? 1 : 2;               // per SM
     static constexpr int TMEM = HD == 256 ? 512 : 256;           // columns: O [HD], then S [NS][KT]
     static constexpr int QBYTES = kTcRows * HD * 2, TBYTES = KT * HD * 2;
@@ -50,12 +49,13 @@ struct TcCfg {
 };
 
 struct TcBars {
-    uint64_t kfull[2], kfree[2];   // a K tile has landed; the MMAs that read it are complete
-    uint64_t vfull[2], vfree[2];   // the same for V
-    uint64_t sfull[2], pready[2];  // S is complete; P is in its place (4 warps)
-    uint64_t odone;                // a tile's P V is complete
+    // Tile j of the CTA is phase j / KST of barrier j % KST, or phase j / 2 of barrier j % 2.
+    uint64_t kfull[2], vfull[2];   // the K, V tile has landed
+    uint64_t sfull[2];             // Q K^T is complete: S is there, the K tile is free
+    uint64_t pready[2];            // P is in the place of S (4 warps)
+    uint64_t odone[2];             // P V is complete: O, the V tile and the S buffer are free
     uint64_t qready;               // the query tile is in shared memory (4 warps)
-    uint64_t join, fin;            // the softmax warps among themselves; every MMA of the block
+    uint64_t join, fin[2];         // the softmax warps among themselves; every MMA of warps 5 and 6
     uint32_t tmem;
     volatile uint32_t dead;        // a wait ran out somewhere in the block
     int last;
@@ -88,19 +88,33 @@ __device__ __forceinline__ uint32_t idesc_f16(int n, bool bn) {
            ((uint32_t)(kTcRows >> 4) << 24);
 }
 
-// One elected lane of the converged warp issues (all lanes execute; operands are warp-uniform).
-__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, bool acc) {
+// Four MMAs (64 of K) issued by one elected lane of the converged warp (all lanes execute; operands are
+// warp-uniform).  A and B from shared memory, K-major: a step of 16 elements is 32 bytes.
+__device__ __forceinline__ void mma_ss4(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, bool acc) {
     asm volatile(
-        "{\n .reg .pred p, e;\n setp.ne.b32 p, %4, 0;\n elect.sync _|e, 0xffffffff;\n"
-        " @e tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}\n" ::"r"(d),
+        "{\n .reg .pred p, e, t;\n .reg .b64 a1, a2, a3, b1, b2, b3;\n setp.ne.b32 p, %4, 0;\n setp.eq.b32 t, 0, 0;\n"
+        " add.s64 a1, %1, 2;\n add.s64 a2, %1, 4;\n add.s64 a3, %1, 6;\n"
+        " add.s64 b1, %2, 2;\n add.s64 b2, %2, 4;\n add.s64 b3, %2, 6;\n"
+        " elect.sync _|e, 0xffffffff;\n"
+        " @e tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n"
+        " @e tcgen05.mma.cta_group::1.kind::f16 [%0], a1, b1, %3, t;\n"
+        " @e tcgen05.mma.cta_group::1.kind::f16 [%0], a2, b2, %3, t;\n"
+        " @e tcgen05.mma.cta_group::1.kind::f16 [%0], a3, b3, %3, t;\n}\n" ::"r"(d),
         "l"(a), "l"(b), "r"(idesc), "r"((int)acc)
         : "memory");
 }
-__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, bool acc) {
+// A from tensor memory at columns a0..a3, B N-major: a step of 16 rows is 2048 bytes.
+__device__ __forceinline__ void mma_ts4(uint32_t d, uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint64_t b,
+                                        uint32_t idesc, bool acc) {
     asm volatile(
-        "{\n .reg .pred p, e;\n setp.ne.b32 p, %4, 0;\n elect.sync _|e, 0xffffffff;\n"
-        " @e tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}\n" ::"r"(d),
-        "r"(a), "l"(b), "r"(idesc), "r"((int)acc)
+        "{\n .reg .pred p, e, t;\n .reg .b64 b1, b2, b3;\n setp.ne.b32 p, %7, 0;\n setp.eq.b32 t, 0, 0;\n"
+        " add.s64 b1, %5, 128;\n add.s64 b2, %5, 256;\n add.s64 b3, %5, 384;\n"
+        " elect.sync _|e, 0xffffffff;\n"
+        " @e tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %5, %6, p;\n"
+        " @e tcgen05.mma.cta_group::1.kind::f16 [%0], [%2], b1, %6, t;\n"
+        " @e tcgen05.mma.cta_group::1.kind::f16 [%0], [%3], b2, %6, t;\n"
+        " @e tcgen05.mma.cta_group::1.kind::f16 [%0], [%4], b3, %6, t;\n}\n" ::"r"(d),
+        "r"(a0), "r"(a1), "r"(a2), "r"(a3), "l"(b), "r"(idesc), "r"((int)acc)
         : "memory");
 }
 __device__ __forceinline__ void commit(uint32_t bar) {
@@ -159,6 +173,20 @@ __device__ __forceinline__ float ex2f(float x) {
     return y;
 }
 
+// Bounded wait on an mbarrier phase by the SM's own clock (2^29 cycles, about 0.3 s; then
+// TRX_DEV_TIMEOUT).
+__device__ __forceinline__ bool wait_phase(uint32_t bar, uint32_t parity, uint32_t *err) {
+    if (mbar_try_wait_s(bar, parity)) return true;
+    const long long t0 = clock64();
+    do {
+#pragma unroll 1
+        for (int i = 0; i < 16; ++i)
+            if (mbar_try_wait_s(bar, parity)) return true;
+    } while (clock64() - t0 < (1ll << 29));
+    if (err && (threadIdx.x & 31) == 0) atomicOr(err, TRX_DEV_TIMEOUT);
+    return false;
+}
+
 struct TcMaps {
     CUtensorMap k, v;
 };
@@ -191,6 +219,54 @@ __device__ __forceinline__ void put32(const PgAttnArgs &A, int hd, int row, int 
     }
 }
 
+// The query tile into shared memory (K-major, 128-byte swizzle), zeros behind its rows; eight (split: four)
+// 16-byte loads of a thread in flight at a time.
+template <typename CT, typename QT, int HD>
+__device__ __forceinline__ void load_query(const PgAttnArgs &A, unsigned char *smem, int r, int rows, int row0, int head0) {
+    constexpr bool SPLIT = sizeof(QT) == 4;
+    using C = TcCfg<HD, SPLIT>;
+    constexpr int PPR = HD / 8, B = SPLIT ? 4 : 8;  // pieces of 8 elements per row, loads in flight
+    const int inv = (65536 + A.rep - 1) / A.rep;    // qr / rep = qr * inv >> 16 for qr < 128, rep <= 16
+    const int c = r % PPR;
+    const uint32_t coff = (uint32_t)((c / 8) * (kTcRows * 128));
+    const QT *const src = reinterpret_cast<const QT *>(A.q) + ((long long)row0 * A.H + head0) * HD + c * 8;
+#pragma unroll 1
+    for (int i0 = 0; i0 < PPR; i0 += B) {
+        uint4 x[B], y[SPLIT ? B : 1];
+#pragma unroll
+        for (int b = 0; b < B; ++b) {
+            const int qr = (i0 + b) * (kTcRows / PPR) + r / PPR, tk = qr * inv >> 16;
+            const QT *p = src + (long long)(tk * A.H + qr - tk * A.rep) * HD;
+            x[b] = make_uint4(0u, 0u, 0u, 0u);
+            if (qr < rows) x[b] = *reinterpret_cast<const uint4 *>(p);
+            if constexpr (SPLIT) {
+                y[b] = make_uint4(0u, 0u, 0u, 0u);
+                if (qr < rows) y[b] = *reinterpret_cast<const uint4 *>(p + 4);
+            }
+        }
+#pragma unroll
+        for (int b = 0; b < B; ++b) {
+            const int qr = (i0 + b) * (kTcRows / PPR) + r / PPR;
+            unsigned char *const dst = smem + C::QOFF + coff + qr * 128 + (((c % 8) ^ (qr & 7)) << 4);
+            if constexpr (SPLIT) {
+                const uint32_t f[8] = {x[b].x, x[b].y, x[b].z, x[b].w, y[b].x, y[b].y, y[b].z, y[b].w};
+                uint32_t hw[4], lw[4];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const float f0 = __uint_as_float(f[2 * e]), f1 = __uint_as_float(f[2 * e + 1]);
+                    hw[e] = PgCvt<CT>::pack(f0, f1);
+                    const float2 h = PgCvt<CT>::unpack(hw[e]);
+                    lw[e] = PgCvt<CT>::pack(f0 - h.x, f1 - h.y);
+                }
+                *reinterpret_cast<uint4 *>(dst) = make_uint4(hw[0], hw[1], hw[2], hw[3]);
+                *reinterpret_cast<uint4 *>(dst + C::QBYTES) = make_uint4(lw[0], lw[1], lw[2], lw[3]);
+            } else {
+                *reinterpret_cast<uint4 *>(dst) = x[b];
+            }
+        }
+    }
+}
+
 template <typename CT, typename QT, int HD>
 __global__ void __launch_bounds__(kTcThreads, HD == 256 ? 1 : 2)
     attn_paged_tc_kernel(const __grid_constant__ TcMaps maps, PgAttnArgs A, uint32_t *err) {
@@ -211,16 +287,15 @@ __global__ void __launch_bounds__(kTcThreads, HD == 256 ? 1 : 2)
     if (tid == 0) {
         for (int i = 0; i < 2; ++i) {
             mbar_init(&bars.kfull[i], 1);
-            mbar_init(&bars.kfree[i], 1);
             mbar_init(&bars.vfull[i], 1);
-            mbar_init(&bars.vfree[i], 1);
             mbar_init(&bars.sfull[i], 1);
             mbar_init(&bars.pready[i], 4);
+            mbar_init(&bars.odone[i], 1);
         }
-        mbar_init(&bars.odone, 1);
         mbar_init(&bars.qready, 4);
         mbar_init(&bars.join, 4);
-        mbar_init(&bars.fin, 1);
+        mbar_init(&bars.fin[0], 1);
+        mbar_init(&bars.fin[1], 1);
         bars.dead = 0u;
         mbar_fence_init();
         tma_prefetch_map(&maps.k);
@@ -242,15 +317,17 @@ __global__ void __launch_bounds__(kTcThreads, HD == 256 ? 1 : 2)
     pdl_trigger();
     const uint32_t tmem = bars.tmem;
     const PgSched &S = sched.S;
-    const uint32_t kfull = smem_u32(bars.kfull), kfree = smem_u32(bars.kfree), vfull = smem_u32(bars.vfull),
-                   vfree = smem_u32(bars.vfree), sfull = smem_u32(bars.sfull), pready = smem_u32(bars.pready),
-                   odone = smem_u32(&bars.odone), qready = smem_u32(&bars.qready), fin = smem_u32(&bars.fin);
+    const uint32_t kfull = smem_u32(bars.kfull), vfull = smem_u32(bars.vfull), sfull = smem_u32(bars.sfull),
+                   pready = smem_u32(bars.pready), odone = smem_u32(bars.odone), qready = smem_u32(&bars.qready),
+                   fin = smem_u32(bars.fin);
     // Every lane of a warp waits; false for all of them if any wait ran out.
     auto wait = [&](uint32_t bar, uint32_t parity) {
-        const bool ok = __all_sync(0xffffffffu, mbar_wait_bounded_s(bar, parity & 1u, err));
+        const bool ok = __all_sync(0xffffffffu, wait_phase(bar, parity & 1u, err));
         if (!ok) bars.dead = 1u;
         return ok;
     };
+    // Tile j's phase of a pair of barriers.
+    auto wait2 = [&](uint32_t bar, int j) { return wait(bar + 8u * (j & 1), (uint32_t)(j >> 1)); };
     PgWalk W;
     const bool any = W.start(A, S);
     if (any && warp == 4) {
@@ -258,119 +335,123 @@ __global__ void __launch_bounds__(kTcThreads, HD == 256 ? 1 : 2)
         const int br = min(1 << A.page_shift, KT), nb = KT / br;  // box rows, boxes per 64 dims
         const int boxes = nb * (HD / 64);
         const int beyond = A.n_pages << A.page_shift;  // a row outside the maps: zeros
-        int j = 0;
-        bool ok = true, more = true;
-        while (ok && more) {
-            const int *tab = A.tables + (long long)W.b * A.max_pages;
-            const int len = W.q.p0 + W.q.n;
-            for (int it = W.i0; ok && it < W.i1; ++it, ++j) {
-                const int st = j % KST, k0 = W.R.tile(it) * KT;
-                static_assert(KT / 16 * (HD / 64) <= 32, "a lane has one box");
-                int row = beyond;
-                if (lane < boxes) {
-                    const int p = k0 + (lane % nb) * br;
-                    if (p < len) {
-                        const int id = __ldg(tab + (p >> A.page_shift));
-                        if ((unsigned)id < (unsigned)A.n_pages)
-                            row = (id << A.page_shift) + (p & ((1 << A.page_shift) - 1));
-                        else
-                            atomicOr(err, TRX_DEV_RANGE);
-                    }
-                }
-                if (bars.dead) {
-                    ok = false;
-                    break;
-                }
-                for (int kind = 0; kind < 2; ++kind) {
-                    const uint32_t full = (kind ? vfull : kfull) + 8u * st, freed = (kind ? vfree : kfree) + 8u * st;
-                    if (j >= KST && !wait(freed, (uint32_t)(j / KST - 1))) {
-                        ok = false;
-                        break;
-                    }
-                    if (lane == 0) mbar_expect_tx_s(full, (uint32_t)C::TBYTES);
-                    __syncwarp();
-                    const uint32_t base = sbase + (kind ? C::VOFF : C::KOFF) + (uint32_t)(st * C::TBYTES);
-                    if (lane < boxes)
-                        load_box(base + (uint32_t)((lane / nb) * KT * 128 + (lane % nb) * br * 128),
-                                 kind ? &maps.v : &maps.k, W.kh * HD + 64 * (lane / nb), row, full);
-                    __syncwarp();
-                }
+        static_assert(KT / 16 * (HD / 64) <= 32, "a lane has one box");
+        const int my_pos = (lane % nb) * br, my_dim = 64 * (lane / nb);
+        const uint32_t my_dst = sbase + (uint32_t)((lane / nb) * KT * 128 + my_pos * 128);
+        int it = W.i0;
+        bool more = true;
+        // This lane's first row of the walk's next tile, and its kv head's first column.
+        auto next_box = [&](int &row, int &col) {
+            const int p = W.R.tile(it) * KT + my_pos;
+            row = beyond;
+            col = W.kh * HD + my_dim;
+            if (lane < boxes && p < W.q.p0 + W.q.n) {
+                const int id = __ldg(A.tables + (long long)W.b * A.max_pages + (p >> A.page_shift));
+                if ((unsigned)id < (unsigned)A.n_pages)
+                    row = (id << A.page_shift) + (p & ((1 << A.page_shift) - 1));
+                else
+                    atomicOr(err, TRX_DEV_RANGE);
             }
-            if (ok) more = W.next(A);
+            if (++it == W.i1) {
+                more = W.next(A);
+                it = W.i0;
+            }
+        };
+        auto issue = [&](int j, int off, const CUtensorMap *map, uint32_t full, int row, int col) {
+            const int st = j % KST;
+            if (lane == 0) mbar_expect_tx_s(full + 8u * st, (uint32_t)C::TBYTES);
+            __syncwarp();
+            if (lane < boxes) load_box(my_dst + (uint32_t)(off + st * C::TBYTES), map, col, row, full + 8u * st);
+            __syncwarp();
+        };
+        // K runs a tile ahead of V (its place is free earlier), and the table is read a tile ahead of that.
+        int row, col, vrow = 0, vcol = 0;
+        next_box(row, col);
+        bool ok = true, tile = true;
+        for (int j = 0; ok; ++j) {
+            int nrow = 0, ncol = 0;
+            const bool next = tile && more;
+            if (next) next_box(nrow, ncol);
+            if (bars.dead) ok = false;
+            if (ok && tile) {
+                ok = j < KST || wait2(sfull, j - KST);
+                if (ok) issue(j, C::KOFF, &maps.k, kfull, row, col);
+            }
+            if (ok && j) {
+                ok = j - 1 < KST || wait2(odone, j - 1 - KST);
+                if (ok) issue(j - 1, C::VOFF, &maps.v, vfull, vrow, vcol);
+            }
+            if (!tile) break;
+            vrow = row;
+            vcol = col;
+            row = nrow;
+            col = ncol;
+            tile = next;
         }
         if (!ok) {
             // Whatever was issued has landed before the block leaves (bounded; the timeout is recorded).
             bars.dead = 1u;
             for (int kind = 0; kind < 2; ++kind)
                 for (int st = 0; st < KST; ++st)
-                    for (int ph = 0; ph < 2; ++ph) mbar_wait_bounded_s((kind ? vfull : kfull) + 8u * st, ph, nullptr);
+                    for (int ph = 0; ph < 2; ++ph) wait_phase((kind ? vfull : kfull) + 8u * st, ph, nullptr);
         }
     } else if (any && warp == 5) {
-        // MMA issue.
-        const uint32_t idq = idesc_f16<CT>(KT, false), idv = idesc_f16<CT>(HD, true);
-        int j = 0, jq = 0, j0 = 0;  // next tile of P V, of Q K^T, first of the piece
+        // S = Q K^T of every tile, as soon as its K tile and its S buffer allow.
+        const uint32_t idq = idesc_f16<CT>(KT, false);
+        const uint64_t qdesc = desc_kmajor(sbase + C::QOFF), kdesc = desc_kmajor(sbase + C::KOFF);
+        int j = 0;
         uint32_t piece = 0;
         bool ok = true, more = true;
-        auto qk = [&] {  // S[jq % NS] = Q K(jq)^T
-            const int st = jq % KST;
-            if (!wait(kfull + 8u * st, (uint32_t)(jq / KST))) return false;
-            // P V of the tile that had this S buffer is complete (for a piece's first tiles: known from
-            // qready, and their phase may have passed).
-            if (jq - NS >= j0 && !wait(odone, (uint32_t)(jq - NS))) return false;
-            tc_after();
-            const uint32_t d = tmem + HD + (uint32_t)((jq % NS) * KT), ka = sbase + C::KOFF + (uint32_t)(st * C::TBYTES);
-#pragma unroll
-            for (int part = 0; part < (SPLIT ? 2 : 1); ++part)
-#pragma unroll
-                for (int k = 0; k < HD / 16; ++k)
-                    mma_ss(d, desc_kmajor(sbase + C::QOFF + part * C::QBYTES + (k / 4) * (kTcRows * 128) + (k % 4) * 32),
-                           desc_kmajor(ka + (k / 4) * (KT * 128) + (k % 4) * 32), idq, part || k);
-            commit(kfree + 8u * st);
-            commit(sfull + 8u * (jq % NS));
-            ++jq;
-            return true;
-        };
         while (ok && more) {
-            if (!wait(qready, piece++)) {
-                ok = false;
-                break;
-            }
-            tc_after();
-            const int jend = j + W.i1 - W.i0;
-            j0 = j;
-            for (; ok && j < jend; ++j) {
-                if (bars.dead) {
-                    ok = false;
-                    break;
-                }
-                while (ok && jq < jend && jq < j + NS) ok = qk();
-                if (!ok) break;
+            ok = wait(qready, piece++);
+            for (int n = W.i1 - W.i0; ok && n; --n, ++j) {
                 const int st = j % KST;
-                if (!wait(vfull + 8u * st, (uint32_t)(j / KST)) || !wait(pready + 8u * (j % NS), (uint32_t)(j / NS))) {
-                    ok = false;
-                    break;
-                }
+                ok = wait(kfull + 8u * st, (uint32_t)(j / KST)) && (j < NS || wait2(odone, j - NS));
+                if (!ok) break;
                 tc_after();
-                const uint32_t p = tmem + HD + (uint32_t)((j % NS) * KT), va = sbase + C::VOFF + (uint32_t)(st * C::TBYTES);
+                const uint32_t d = tmem + HD + (uint32_t)((j % NS) * KT);
+                const uint64_t kb = kdesc + (uint64_t)((st * C::TBYTES) >> 4);
 #pragma unroll
-                for (int k = 0; k < KT / 16; ++k) {
-                    const uint64_t b = desc_nmajor(va + k * 2048, KT * 128);
-                    if constexpr (SPLIT) {
-                        mma_ts(tmem, p + 32 * (k / 2) + 8 * (k % 2), b, idv, j != j0 || k);
-                        mma_ts(tmem, p + 32 * (k / 2) + 8 * (k % 2) + 16, b, idv, true);
-                    } else {
-                        mma_ts(tmem, p + 8 * k, b, idv, j != j0 || k);
-                    }
-                }
-                commit(vfree + 8u * st);
-                commit(odone);
+                for (int part = SPLIT ? 1 : 0; part >= 0; --part)  // the small part first: the sums are cut off, not rounded
+#pragma unroll
+                    for (int c = 0; c < HD / 64; ++c)
+                        mma_ss4(d, qdesc + ((part * C::QBYTES + c * kTcRows * 128) >> 4), kb + ((c * KT * 128) >> 4), idq,
+                                (SPLIT && part == 0) || c);
+                commit(sfull + 8u * (j % NS));
             }
             if (ok) more = W.next(A);
         }
-        if (!ok) bars.dead = 1u;
         commit(fin);  // every MMA is complete before the tensor memory is given back
-        mbar_wait_bounded_s(fin, 0u, nullptr);
-    } else if (any) {
+        wait_phase(fin, 0u, nullptr);
+    } else if (any && warp == 6) {
+        // O += P V.
+        const uint32_t idv = idesc_f16<CT>(HD, true);
+        const uint64_t vdesc = desc_nmajor(sbase + C::VOFF, KT * 128);
+        int j = 0;
+        bool ok = true, more = true;
+        while (ok && more) {
+            bool first = true;
+            for (int n = W.i1 - W.i0; ok && n; --n, ++j) {
+                const int st = j % KST;
+                ok = wait(vfull + 8u * st, (uint32_t)(j / KST)) && wait2(pready, j);
+                if (!ok) break;
+                tc_after();
+                const uint32_t p = tmem + HD + (uint32_t)((j % NS) * KT);
+                const uint64_t vb = vdesc + (uint64_t)((st * C::TBYTES) >> 4);
+                if constexpr (SPLIT) {  // 16 columns of high parts, 16 of low parts, for each 32 positions
+                    mma_ts4(tmem, p + 16, p + 24, p + 48, p + 56, vb, idv, !first);
+                    mma_ts4(tmem, p, p + 8, p + 32, p + 40, vb, idv, true);
+                } else {
+                    mma_ts4(tmem, p, p + 8, p + 16, p + 24, vb, idv, !first);
+                }
+                commit(odone + 8u * (j & 1));
+                first = false;
+            }
+            if (ok) more = W.next(A);
+        }
+        commit(fin + 8u);
+        wait_phase(fin + 8u, 0u, nullptr);
+    } else if (any && warp < 4) {
         // Softmax: query row tid of the piece's tile.
         const int r = tid;
         const uint32_t lanes = (uint32_t)(32 * warp) << 16;
@@ -390,32 +471,7 @@ __global__ void __launch_bounds__(kTcThreads, HD == 256 ? 1 : 2)
             const int pmax = pos0 + (rows - 1) / A.rep;  // the tile's last position; pos0 its first
             // The query tile, zeros behind its rows.  Every MMA that read the previous one is complete (its
             // S was waited for).
-            for (int i = r; i < kTcRows * (HD / 8); i += kTcRows) {
-                const int qr = i / (HD / 8), c = i % (HD / 8);
-                uint4 hi = make_uint4(0u, 0u, 0u, 0u), lo = hi;
-                if (qr < rows) {
-                    const int tk = qr / A.rep, h = W.kh * A.rep + qr - tk * A.rep;
-                    const QT *src = reinterpret_cast<const QT *>(A.q) + ((size_t)(row0 + tk) * A.H + h) * HD + c * 8;
-                    if constexpr (SPLIT) {
-                        const float4 x = *reinterpret_cast<const float4 *>(src), y = *reinterpret_cast<const float4 *>(src + 4);
-                        const float f[8] = {x.x, x.y, x.z, x.w, y.x, y.y, y.z, y.w};
-                        uint32_t hw[4], lw[4];
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) {
-                            hw[e] = PgCvt<CT>::pack(f[2 * e], f[2 * e + 1]);
-                            const float2 b = PgCvt<CT>::unpack(hw[e]);
-                            lw[e] = PgCvt<CT>::pack(f[2 * e] - b.x, f[2 * e + 1] - b.y);
-                        }
-                        hi = make_uint4(hw[0], hw[1], hw[2], hw[3]);
-                        lo = make_uint4(lw[0], lw[1], lw[2], lw[3]);
-                    } else {
-                        hi = *reinterpret_cast<const uint4 *>(src);
-                    }
-                }
-                const uint32_t off = (uint32_t)((c / 8) * (kTcRows * 128) + qr * 128 + (((c % 8) ^ (qr & 7)) << 4));
-                *reinterpret_cast<uint4 *>(smem + C::QOFF + off) = hi;
-                if constexpr (SPLIT) *reinterpret_cast<uint4 *>(smem + C::QOFF + C::QBYTES + off) = lo;
-            }
+            load_query<CT, QT, HD>(A, smem, r, rows, row0, W.kh * A.rep);
             fence_proxy_async();
             __syncwarp();
             if (lane == 0) arrive(qready);
@@ -427,27 +483,24 @@ __global__ void __launch_bounds__(kTcThreads, HD == 256 ? 1 : 2)
                 // Nothing of the tile is hidden from any row.
                 const bool open = k0 + KT - 1 <= pos0 &&
                                   (!A.window || pmax - k0 < A.window || k0 + KT <= A.sinks);
-                if (!wait(sfull + 8u * (j % NS), (uint32_t)(j / NS))) {
+                if (!wait2(sfull, j)) {
                     ok = false;
                     break;
                 }
                 tc_after();
-                float mx = -INFINITY;
+                uint32_t v[KT];  // the row of S
+                tm_ld32(ts, *reinterpret_cast<uint32_t(*)[32]>(v));
+                tm_ld32(ts + 32, *reinterpret_cast<uint32_t(*)[32]>(v + 32));
+                tm_wait_ld();
+                if (!open) {
 #pragma unroll
-                for (int c = 0; c < KT / 32; ++c) {
-                    uint32_t v[32];
-                    tm_ld32(ts + 32 * c, v);
-                    tm_wait_ld();
-                    if (open) {
-#pragma unroll
-                        for (int e = 0; e < 32; ++e) mx = fmaxf(mx, __uint_as_float(v[e]));
-                    } else {
-#pragma unroll
-                        for (int e = 0; e < 32; ++e)
-                            mx = fmaxf(mx, pg_hidden(k0 + 32 * c + e, qpos, A.window, A.sinks) ? -INFINITY
-                                                                                              : __uint_as_float(v[e]));
-                    }
+                    for (int e = 0; e < KT; ++e)
+                        if (pg_hidden(k0 + e, qpos, A.window, A.sinks)) v[e] = 0xff800000u;
                 }
+                float mx4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+                for (int e = 0; e < KT; ++e) mx4[e & 3] = fmaxf(mx4[e & 3], __uint_as_float(v[e]));
+                float mx = fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3]));
                 mx *= A.scale_log2;
                 if (r >= rows) mx = -INFINITY;
                 if (j == j0) {
@@ -455,7 +508,7 @@ __global__ void __launch_bounds__(kTcThreads, HD == 256 ? 1 : 2)
                 } else {
                     const bool grow = mx > m + 8.f;
                     if (__any_sync(0xffffffffu, grow)) {
-                        if (!wait(odone, (uint32_t)(j - 1))) {
+                        if (!wait2(odone, j - 1)) {
                             ok = false;
                             break;
                         }
@@ -464,14 +517,14 @@ __global__ void __launch_bounds__(kTcThreads, HD == 256 ? 1 : 2)
                         const float f = grow && m != -INFINITY ? ex2f(m - mx) : 1.f;
                         if (grow) m = mx;
                         l *= f;
-#pragma unroll
+#pragma unroll 1
                         for (int c = 0; c < HD / 32; ++c) {
-                            uint32_t v[32];
-                            tm_ld32(tmem + lanes + 32 * c, v);
+                            uint32_t w[32];
+                            tm_ld32(tmem + lanes + 32 * c, w);
                             tm_wait_ld();
 #pragma unroll
-                            for (int e = 0; e < 32; ++e) v[e] = __float_as_uint(__uint_as_float(v[e]) * f);
-                            tm_st32(tmem + lanes + 32 * c, v);
+                            for (int e = 0; e < 32; ++e) w[e] = __float_as_uint(__uint_as_float(w[e]) * f);
+                            tm_st32(tmem + lanes + 32 * c, w);
                         }
                         tm_wait_st();
                     }
@@ -480,26 +533,23 @@ __global__ void __launch_bounds__(kTcThreads, HD == 256 ? 1 : 2)
                 float sum[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
                 for (int c = 0; c < KT / 32; ++c) {
-                    uint32_t v[32], ph[16];
-                    tm_ld32(ts + 32 * c, v);
-                    tm_wait_ld();
+                    uint32_t ph[16];
 #pragma unroll
-                    for (int e = 0; e < 32; ++e) {
-                        float x = fmaf(__uint_as_float(v[e]), A.scale_log2, nm);
-                        if (!open && pg_hidden(k0 + 32 * c + e, qpos, A.window, A.sinks)) x = -INFINITY;
-                        const float p = ex2f(x);
+                    for (int e = 32 * c; e < 32 * c + 32; ++e) {
+                        const float p = ex2f(fmaf(__uint_as_float(v[e]), A.scale_log2, nm));
                         v[e] = __float_as_uint(p);
                         sum[e & 3] += p;
                     }
 #pragma unroll
                     for (int e = 0; e < 16; ++e)
-                        ph[e] = PgCvt<CT>::pack(__uint_as_float(v[2 * e]), __uint_as_float(v[2 * e + 1]));
+                        ph[e] = PgCvt<CT>::pack(__uint_as_float(v[32 * c + 2 * e]), __uint_as_float(v[32 * c + 2 * e + 1]));
                     if constexpr (SPLIT) {
                         tm_st16(ts + 32 * c, ph);
 #pragma unroll
                         for (int e = 0; e < 16; ++e) {
                             const float2 b = PgCvt<CT>::unpack(ph[e]);
-                            ph[e] = PgCvt<CT>::pack(__uint_as_float(v[2 * e]) - b.x, __uint_as_float(v[2 * e + 1]) - b.y);
+                            ph[e] = PgCvt<CT>::pack(__uint_as_float(v[32 * c + 2 * e]) - b.x,
+                                                    __uint_as_float(v[32 * c + 2 * e + 1]) - b.y);
                         }
                         tm_st16(ts + 32 * c + 16, ph);
                     } else {
@@ -526,7 +576,7 @@ __global__ void __launch_bounds__(kTcThreads, HD == 256 ? 1 : 2)
                 if (lane == 0) arrive(pready + 8u * (j % NS));
             }
             if (!ok) break;
-            if (!wait(odone, (uint32_t)(j - 1))) {
+            if (!wait2(odone, j - 1)) {
                 ok = false;
                 break;
             }
