@@ -55,10 +55,9 @@ struct TcBars {
     uint64_t pready[2];            // P is in the place of S (4 warps)
     uint64_t odone[2];             // P V is complete: O, the V tile and the S buffer are free
     uint64_t qready;               // the query tile is in shared memory (4 warps)
-    uint64_t join, fin[2];         // the softmax warps among themselves; every MMA of warps 5 and 6
+    uint64_t fin[2];               // every MMA of warps 5 and 6
     uint32_t tmem;
     volatile uint32_t dead;        // a wait ran out somewhere in the block
-    int last;
 };
 
 struct TcTail {  // behind the tiles
@@ -219,13 +218,13 @@ __device__ __forceinline__ void put32(const PgAttnArgs &A, int hd, int row, int 
     }
 }
 
-// The query tile into shared memory (K-major, 128-byte swizzle), zeros behind its rows; eight (split: four)
+// The query tile into shared memory (K-major, 128-byte swizzle), zeros behind its rows; sixteen
 // 16-byte loads of a thread in flight at a time.
 template <typename CT, typename QT, int HD>
 __device__ __forceinline__ void load_query(const PgAttnArgs &A, unsigned char *smem, int r, int rows, int row0, int head0) {
     constexpr bool SPLIT = sizeof(QT) == 4;
     using C = TcCfg<HD, SPLIT>;
-    constexpr int PPR = HD / 8, B = SPLIT ? 4 : 8;  // pieces of 8 elements per row, loads in flight
+    constexpr int PPR = HD / 8, B = SPLIT || HD == 64 ? 8 : 16;  // pieces of 8 elements per row, of a batch
     const int inv = (65536 + A.rep - 1) / A.rep;    // qr / rep = qr * inv >> 16 for qr < 128, rep <= 16
     const int c = r % PPR;
     const uint32_t coff = (uint32_t)((c / 8) * (kTcRows * 128));
@@ -267,9 +266,103 @@ __device__ __forceinline__ void load_query(const PgAttnArgs &A, unsigned char *s
     }
 }
 
+// A row's output from its O in tensor memory (row < 0: none; every lane of the warp takes part).
+template <typename QT, int HD>
+__device__ __forceinline__ void finish_whole(const PgAttnArgs &A, uint32_t to, float l, int row, int head) {
+    const float inv = l > 0.f ? __fdiv_rn(1.0f, l) : 0.f;
+#pragma unroll 1
+    for (int c = 0; c < HD / 32; ++c) {
+        uint32_t v[32];
+        tm_ld32(to + 32 * c, v);
+        tm_wait_ld();
+        float o[32];
+#pragma unroll
+        for (int e = 0; e < 32; ++e) o[e] = __uint_as_float(v[e]) * inv;
+        if (row >= 0) put32<QT>(A, HD, row, head, 32 * c, o);
+    }
+}
+
+// A cut item: this piece's rows to scratch, [HD / 4][128 rows] of four dims, then the maxima and sums; the
+// last to arrive joins the pieces in the order of the CTAs (its own still from tensor memory).  The warps
+// arrive and join on their own, 32 rows each.
+template <typename QT, int HD>
+__device__ __forceinline__ void finish_cut(const PgAttnArgs &A, const PgSched &S, uint32_t to, long long item0,
+                                        long long item1, float m, float l, int row, int head) {
+    constexpr size_t kPart = kTcRows * (HD + 2);
+    const int r = threadIdx.x, lane = r & 31, me = (int)blockIdx.x;
+    const int c0 = pg_owner(S, item0), c1 = pg_owner(S, item1 - 1);
+    unsigned *const cnt = A.cnt + 4 * c0 + (r >> 5);
+    auto slot_of = [&](int cc) { return A.part + kPart * (2 * (size_t)cc + (cc == c0 ? 1 : 0)); };
+    {
+        float *const mine = slot_of(me);
+#pragma unroll 1
+        for (int c = 0; c < HD / 32; ++c) {
+            uint32_t v[32];
+            tm_ld32(to + 32 * c, v);
+            tm_wait_ld();
+#pragma unroll
+            for (int e = 0; e < 8; ++e)
+                reinterpret_cast<uint4 *>(mine)[(8 * c + e) * kTcRows + r] =
+                    make_uint4(v[4 * e], v[4 * e + 1], v[4 * e + 2], v[4 * e + 3]);
+        }
+        mine[kTcRows * HD + r] = m;
+        mine[kTcRows * (HD + 1) + r] = l;
+        __threadfence();
+        __syncwarp();
+        unsigned seen = 0;
+        if (lane == 0) seen = atomicAdd(cnt, 1u);
+        seen = __shfl_sync(0xffffffffu, seen, 0);
+        if (seen != (unsigned)(c1 - c0)) return;
+    }
+    __threadfence();
+    float M = m, L = 0.f;
+    for (int cc = c0; cc <= c1; ++cc)
+        if (cc != me) M = fmaxf(M, __ldcg(slot_of(cc) + kTcRows * HD + r));
+    const float Ms = M == -INFINITY ? 0.f : M;
+    for (int cc = c0; cc <= c1; ++cc) {
+        const float *p = slot_of(cc) + kTcRows * HD + r;
+        L = cc == me ? fmaf(ex2f(m - Ms), l, L) : fmaf(ex2f(__ldcg(p) - Ms), __ldcg(p + kTcRows), L);
+    }
+    const float inv = L > 0.f ? __fdiv_rn(1.0f, L) : 0.f;
+#pragma unroll 1
+    for (int c = 0; c < HD / 32; ++c) {
+        float o[32];
+#pragma unroll
+        for (int e = 0; e < 32; ++e) o[e] = 0.f;
+#pragma unroll 1
+        for (int cc = c0; cc <= c1; ++cc) {
+            uint32_t v[32];
+            float w;
+            if (cc == me) {
+                tm_ld32(to + 32 * c, v);
+                tm_wait_ld();
+                w = ex2f(m - Ms);
+            } else {
+                const float *p = slot_of(cc);
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    const uint4 x = __ldcg(reinterpret_cast<const uint4 *>(p) + (8 * c + e) * kTcRows + r);
+                    v[4 * e] = x.x;
+                    v[4 * e + 1] = x.y;
+                    v[4 * e + 2] = x.z;
+                    v[4 * e + 3] = x.w;
+                }
+                w = ex2f(__ldcg(p + kTcRows * HD + r) - Ms);
+            }
+#pragma unroll
+            for (int e = 0; e < 32; ++e) o[e] = fmaf(w, __uint_as_float(v[e]), o[e]);
+        }
+#pragma unroll
+        for (int e = 0; e < 32; ++e) o[e] *= inv;
+        if (row >= 0) put32<QT>(A, HD, row, head, 32 * c, o);
+    }
+    __syncwarp();
+    if (lane == 0) *cnt = 0u;
+}
+
 template <typename CT, typename QT, int HD>
 __global__ void __launch_bounds__(kTcThreads, HD == 256 ? 1 : 2)
-    attn_paged_tc_kernel(const __grid_constant__ TcMaps maps, PgAttnArgs A, uint32_t *err) {
+    attn_paged_tc_kernel(const __grid_constant__ TcMaps maps, const __grid_constant__ PgAttnArgs A, uint32_t *err) {
     constexpr bool SPLIT = sizeof(QT) == 4;
     using C = TcCfg<HD, SPLIT>;
     constexpr int KT = C::KT, NS = C::NS, KST = C::KST;
@@ -293,7 +386,6 @@ __global__ void __launch_bounds__(kTcThreads, HD == 256 ? 1 : 2)
             mbar_init(&bars.odone[i], 1);
         }
         mbar_init(&bars.qready, 4);
-        mbar_init(&bars.join, 4);
         mbar_init(&bars.fin[0], 1);
         mbar_init(&bars.fin[1], 1);
         bars.dead = 0u;
@@ -456,25 +548,21 @@ __global__ void __launch_bounds__(kTcThreads, HD == 256 ? 1 : 2)
         const int r = tid;
         const uint32_t lanes = (uint32_t)(32 * warp) << 16;
         int j = 0;
-        uint32_t joined = 0;
-        auto join = [&] {  // the four warps (bounded, unlike a block barrier)
-            __syncwarp();
-            if (lane == 0) arrive(smem_u32(&bars.join));
-            return wait(smem_u32(&bars.join), joined++);
-        };
-        bool ok = true, more = true;
-        while (ok && more) {
-            const int rows = W.rows(A), len = W.q.p0 + W.q.n;
-            const int row0 = W.q.row0 + W.t * A.tq, pos0 = W.q.p0 + W.t * A.tq;
-            const int tok = r / A.rep, head = W.kh * A.rep + r - tok * A.rep;
-            const int qpos = r < rows ? pos0 + tok : -1;
-            const int pmax = pos0 + (rows - 1) / A.rep;  // the tile's last position; pos0 its first
-            // The query tile, zeros behind its rows.  Every MMA that read the previous one is complete (its
-            // S was waited for).
-            load_query<CT, QT, HD>(A, smem, r, rows, row0, W.kh * A.rep);
+        bool ok = true;
+        // The walk's query tile; every MMA that read the one before is complete (its S was waited for).
+        auto fetch = [&] {
+            load_query<CT, QT, HD>(A, smem, r, W.rows(A), W.q.row0 + W.t * A.tq, W.kh * A.rep);
             fence_proxy_async();
             __syncwarp();
             if (lane == 0) arrive(qready);
+        };
+        fetch();
+        for (bool more = true; ok && more;) {
+            const int rows = W.rows(A), len = W.q.p0 + W.q.n;
+            const int pos0 = W.q.p0 + W.t * A.tq;
+            const int tok = r / A.rep, head = W.kh * A.rep + r - tok * A.rep;
+            const int qpos = r < rows ? pos0 + tok : -1;
+            const int pmax = pos0 + (rows - 1) / A.rep;  // the tile's last position; pos0 its first
             float m = -INFINITY, l = 0.f;
             const int j0 = j;
             for (int it = W.i0; it < W.i1; ++it, ++j) {
@@ -492,10 +580,11 @@ __global__ void __launch_bounds__(kTcThreads, HD == 256 ? 1 : 2)
                 tm_ld32(ts, *reinterpret_cast<uint32_t(*)[32]>(v));
                 tm_ld32(ts + 32, *reinterpret_cast<uint32_t(*)[32]>(v + 32));
                 tm_wait_ld();
-                if (!open) {
+                if (!open) {  // visible: e <= hi and (e >= lo or e < sk)
+                    const int hi = qpos - k0, lo = A.window ? hi - A.window + 1 : -1, sk = A.sinks - k0;
 #pragma unroll
                     for (int e = 0; e < KT; ++e)
-                        if (pg_hidden(k0 + e, qpos, A.window, A.sinks)) v[e] = 0xff800000u;
+                        if (e > hi || (e < lo && e >= sk)) v[e] = 0xff800000u;
                 }
                 float mx4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
@@ -576,91 +665,22 @@ __global__ void __launch_bounds__(kTcThreads, HD == 256 ? 1 : 2)
                 if (lane == 0) arrive(pready + 8u * (j % NS));
             }
             if (!ok) break;
+            // The next piece's query tile before this one is finished: its first S are computed meanwhile.
+            const bool whole = W.whole();
+            const int row = r < rows ? W.q.row0 + W.t * A.tq + tok : -1;
+            const long long item0 = W.u - W.i1, item1 = item0 + W.R.cnt;
+            more = W.next(A);
+            if (more) fetch();
             if (!wait2(odone, j - 1)) {
                 ok = false;
                 break;
             }
             tc_after();
-            if (W.whole()) {
-                const float inv = l > 0.f ? __fdiv_rn(1.0f, l) : 0.f;
-#pragma unroll 1
-                for (int c = 0; c < HD / 32; ++c) {
-                    uint32_t v[32];
-                    tm_ld32(tmem + lanes + 32 * c, v);
-                    tm_wait_ld();
-                    if (r < rows) {
-                        float o[32];
-#pragma unroll
-                        for (int e = 0; e < 32; ++e) o[e] = __uint_as_float(v[e]) * inv;
-                        put32<QT>(A, HD, row0 + tok, head, 32 * c, o);
-                    }
-                }
-            } else {
-                // A cut item (as in attn_paged_kernel): scratch [HD / 4][128 rows] of four dims, then the
-                // maxima and sums.
-                const long long item0 = W.u - W.i1, item1 = item0 + W.R.cnt;
-                const int c0 = pg_owner(S, item0), c1 = pg_owner(S, item1 - 1);
-                constexpr size_t kPart = kTcRows * (HD + 2);
-                auto slot_of = [&](int cc) { return A.part + kPart * (2 * (size_t)cc + (cc == c0 ? 1 : 0)); };
-                float *const mine = slot_of(blockIdx.x);
-#pragma unroll 1
-                for (int c = 0; c < HD / 32; ++c) {
-                    uint32_t v[32];
-                    tm_ld32(tmem + lanes + 32 * c, v);
-                    tm_wait_ld();
-#pragma unroll
-                    for (int e = 0; e < 8; ++e)
-                        reinterpret_cast<uint4 *>(mine)[(8 * c + e) * kTcRows + r] =
-                            make_uint4(v[4 * e], v[4 * e + 1], v[4 * e + 2], v[4 * e + 3]);
-                }
-                mine[kTcRows * HD + r] = m;
-                mine[kTcRows * (HD + 1) + r] = l;
-                __threadfence();
-                if (!join()) {
-                    ok = false;
-                    break;
-                }
-                if (r == 0) bars.last = atomicAdd(A.cnt + c0, 1u) == (unsigned)(c1 - c0);
-                if (!join()) {
-                    ok = false;
-                    break;
-                }
-                if (bars.last) {
-                    __threadfence();
-                    float M = -INFINITY, L = 0.f;
-                    for (int cc = c0; cc <= c1; ++cc) M = fmaxf(M, __ldcg(slot_of(cc) + kTcRows * HD + r));
-                    const float Ms = M == -INFINITY ? 0.f : M;
-                    for (int cc = c0; cc <= c1; ++cc) {
-                        const float *p = slot_of(cc) + kTcRows * HD + r;
-                        L = fmaf(ex2f(__ldcg(p) - Ms), __ldcg(p + kTcRows), L);
-                    }
-                    const float inv = L > 0.f ? __fdiv_rn(1.0f, L) : 0.f;
-#pragma unroll 1
-                    for (int c = 0; c < HD / 32; ++c) {
-                        float o[32];
-#pragma unroll
-                        for (int e = 0; e < 32; ++e) o[e] = 0.f;
-                        for (int cc = c0; cc <= c1; ++cc) {
-                            const float *p = slot_of(cc);
-                            const float w = ex2f(__ldcg(p + kTcRows * HD + r) - Ms);
-#pragma unroll
-                            for (int e = 0; e < 8; ++e) {
-                                const float4 x = __ldcg(reinterpret_cast<const float4 *>(p) + (8 * c + e) * kTcRows + r);
-                                o[4 * e] = fmaf(w, x.x, o[4 * e]);
-                                o[4 * e + 1] = fmaf(w, x.y, o[4 * e + 1]);
-                                o[4 * e + 2] = fmaf(w, x.z, o[4 * e + 2]);
-                                o[4 * e + 3] = fmaf(w, x.w, o[4 * e + 3]);
-                            }
-                        }
-#pragma unroll
-                        for (int e = 0; e < 32; ++e) o[e] *= inv;
-                        if (r < rows) put32<QT>(A, HD, row0 + tok, head, 32 * c, o);
-                    }
-                    if (r == 0) A.cnt[c0] = 0u;
-                }
-            }
+            if (whole)
+                finish_whole<QT, HD>(A, tmem + lanes, l, row, head);
+            else
+                finish_cut<QT, HD>(A, S, tmem + lanes, item0, item1, m, l, row, head);
             tc_before();
-            more = W.next(A);
         }
         if (!ok) bars.dead = 1u;
     }
@@ -690,7 +710,7 @@ trx_status launch_tc(PgAttnArgs A, size_t part_cap, int cnt_cap, uint32_t *err, 
     if (!encode_map_16bit(&maps.k, A.kp, cols, rows, 64, br) || !encode_map_16bit(&maps.v, A.vp, cols, rows, 64, br))
         return TRX_ERR_CUDA;
     const int grid = device_sms() * C::CTAS;
-    if ((size_t)grid * 2 * kTcRows * (HD + 2) > part_cap || grid > cnt_cap) return TRX_ERR_UNSUPPORTED;
+    if ((size_t)grid * 2 * kTcRows * (HD + 2) > part_cap || 4 * grid > cnt_cap) return TRX_ERR_UNSUPPORTED;
     return note_cuda(launch_kernel(attn_paged_tc_kernel<CT, QT, HD>, dim3(grid), dim3(kTcThreads), C::END + sizeof(TcTail), st,
                                    maps, A, err));
 }
