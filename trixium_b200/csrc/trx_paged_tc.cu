@@ -14,13 +14,15 @@
 //    64 dims, 128-byte swizzle; places behind the sequence's end come from outside the map, as zeros.
 //  * warps 5 and 6: issue the MMAs of the first and of the second product, each from one elected lane. Two
 //    warps, since one's instructions between two MMAs (waits, commits) take as long as the MMAs.
-// fp32 queries: Q = hi + lo and P = hi + lo in fp16, two MMAs per product, so products keep 2^-22.
+// fp32 queries: Q = hi + lo and P = hi + lo in fp16, two MMAs per product, so products keep 2^-22; each
+// tile's P V is added to an O in registers (head dim 256: tensor memory) by the softmax warps.
 // V is read as the N-major B operand of the second product straight from its row-major tile; the rows
 // of a sequence's last page behind its end are overwritten with zeros first (0 times what lies there
 // would not be 0 if it is not finite).
 //
 // Two S buffers: the next tile's S is computed while this one's softmax runs.  Head dims 64 and 128 run
-// two CTAs per SM (at most 113 KB of shared memory, 256 TMEM columns each), head dim 256 one.
+// two CTAs per SM (at most 113 KB of shared memory, 256 TMEM columns each), head dim 256 and fp32 queries
+// one.
 #include <algorithm>
 #include <cstdint>
 #include <cstring>
@@ -39,13 +41,18 @@ template <int HD, bool SPLIT>
 struct TcCfg {
     static constexpr int KT = 64, KT_SHIFT = 6;                   // key positions of a tile
     static constexpr int NS = 2;                                  // S buffers (the barriers' pairs)
-    static constexpr int KST = SPLIT && HD >= 128 ? 1 : 2;       // K and V tiles in shared memory
-    static constexpr int CTAS = HD == 256 ? 1 : 2;               // per SM
-    static constexpr int TMEM = HD == 256 ? 512 : 256;           // columns: O [HD], then S [NS][KT]
+    static constexpr int KST = SPLIT && HD == 256 ? 1 : 2;       // K and V tiles in shared memory
+    static constexpr int CTAS = SPLIT || HD == 256 ? 1 : 2;      // per SM
+    // Tensor memory.  16-bit: O [HD], S [2][KT].  Split: a tile's P V [NACC][NW], S [2][KT], and for head
+    // dim 256, whose O does not fit the registers, O [256] in front.
+    static constexpr bool REGO = SPLIT && HD <= 128;             // O in registers
+    static constexpr int NACC = REGO ? 2 : 1, NW = SPLIT && HD == 256 ? 128 : HD, NCH = HD / NW;
+    static constexpr int AOFF = SPLIT && !REGO ? HD : 0, SOFF = AOFF + NACC * NW;
+    static constexpr int TMEM = SOFF + NS * KT <= 256 ? 256 : 512;
     static constexpr int QBYTES = kTcRows * HD * 2, TBYTES = KT * HD * 2;
     static constexpr int QOFF = 0, KOFF = QBYTES * (SPLIT ? 2 : 1), VOFF = KOFF + KST * TBYTES,
                          END = VOFF + KST * TBYTES;  // multiples of 1024
-    static_assert(HD + NS * KT <= TMEM, "tensor memory holds O and every S");
+    static_assert(SOFF + NS * KT <= 512 && TMEM * CTAS <= 512, "tensor memory holds O and every S");
 };
 
 struct TcBars {
@@ -54,6 +61,7 @@ struct TcBars {
     uint64_t sfull[2];             // Q K^T is complete: S is there, the K tile is free
     uint64_t pready[2];            // P is in the place of S (4 warps)
     uint64_t odone[2];             // P V is complete: O, the V tile and the S buffer are free
+    uint64_t cdone[2], ofree[2];   // split: part n of P V is complete; it has been added to O (4 warps)
     uint64_t qready;               // the query tile is in shared memory (4 warps)
     uint64_t fin[2];               // every MMA of warps 5 and 6
     uint32_t tmem;
@@ -266,15 +274,15 @@ __device__ __forceinline__ void load_query(const PgAttnArgs &A, unsigned char *s
     }
 }
 
-// A row's output from its O in tensor memory (row < 0: none; every lane of the warp takes part).
-template <typename QT, int HD>
-__device__ __forceinline__ void finish_whole(const PgAttnArgs &A, uint32_t to, float l, int row, int head) {
+// A row's output from its O, 32 dims at a time from get (row < 0: none; every lane of the warp takes part).
+// REG: get reads registers, so the loops are unrolled.
+template <typename QT, int HD, bool REG, typename Get>
+__device__ __forceinline__ void finish_whole(const PgAttnArgs &A, Get &&get, float l, int row, int head) {
     const float inv = l > 0.f ? __fdiv_rn(1.0f, l) : 0.f;
-#pragma unroll 1
+#pragma unroll (REG ? HD / 32 : 1)
     for (int c = 0; c < HD / 32; ++c) {
         uint32_t v[32];
-        tm_ld32(to + 32 * c, v);
-        tm_wait_ld();
+        get(c, v);
         float o[32];
 #pragma unroll
         for (int e = 0; e < 32; ++e) o[e] = __uint_as_float(v[e]) * inv;
@@ -283,11 +291,11 @@ __device__ __forceinline__ void finish_whole(const PgAttnArgs &A, uint32_t to, f
 }
 
 // A cut item: this piece's rows to scratch, [HD / 4][128 rows] of four dims, then the maxima and sums; the
-// last to arrive joins the pieces in the order of the CTAs (its own still from tensor memory).  The warps
+// last to arrive joins the pieces in the order of the CTAs (its own still from get).  The warps
 // arrive and join on their own, 32 rows each.
-template <typename QT, int HD>
-__device__ __forceinline__ void finish_cut(const PgAttnArgs &A, const PgSched &S, uint32_t to, long long item0,
-                                        long long item1, float m, float l, int row, int head) {
+template <typename QT, int HD, bool REG, typename Get>
+__device__ __forceinline__ void finish_cut(const PgAttnArgs &A, const PgSched &S, Get &&get, long long item0,
+                                           long long item1, float m, float l, int row, int head) {
     constexpr size_t kPart = kTcRows * (HD + 2);
     const int r = threadIdx.x, lane = r & 31, me = (int)blockIdx.x;
     const int c0 = pg_owner(S, item0), c1 = pg_owner(S, item1 - 1);
@@ -295,11 +303,10 @@ __device__ __forceinline__ void finish_cut(const PgAttnArgs &A, const PgSched &S
     auto slot_of = [&](int cc) { return A.part + kPart * (2 * (size_t)cc + (cc == c0 ? 1 : 0)); };
     {
         float *const mine = slot_of(me);
-#pragma unroll 1
+#pragma unroll (REG ? HD / 32 : 1)
         for (int c = 0; c < HD / 32; ++c) {
             uint32_t v[32];
-            tm_ld32(to + 32 * c, v);
-            tm_wait_ld();
+            get(c, v);
 #pragma unroll
             for (int e = 0; e < 8; ++e)
                 reinterpret_cast<uint4 *>(mine)[(8 * c + e) * kTcRows + r] =
@@ -324,7 +331,7 @@ __device__ __forceinline__ void finish_cut(const PgAttnArgs &A, const PgSched &S
         L = cc == me ? fmaf(ex2f(m - Ms), l, L) : fmaf(ex2f(__ldcg(p) - Ms), __ldcg(p + kTcRows), L);
     }
     const float inv = L > 0.f ? __fdiv_rn(1.0f, L) : 0.f;
-#pragma unroll 1
+#pragma unroll (REG ? HD / 32 : 1)
     for (int c = 0; c < HD / 32; ++c) {
         float o[32];
 #pragma unroll
@@ -334,8 +341,7 @@ __device__ __forceinline__ void finish_cut(const PgAttnArgs &A, const PgSched &S
             uint32_t v[32];
             float w;
             if (cc == me) {
-                tm_ld32(to + 32 * c, v);
-                tm_wait_ld();
+                get(c, v);
                 w = ex2f(m - Ms);
             } else {
                 const float *p = slot_of(cc);
@@ -361,7 +367,7 @@ __device__ __forceinline__ void finish_cut(const PgAttnArgs &A, const PgSched &S
 }
 
 template <typename CT, typename QT, int HD>
-__global__ void __launch_bounds__(kTcThreads, HD == 256 ? 1 : 2)
+__global__ void __launch_bounds__(kTcThreads, HD == 256 || sizeof(QT) == 4 ? 1 : 2)
     attn_paged_tc_kernel(const __grid_constant__ TcMaps maps, const __grid_constant__ PgAttnArgs A, uint32_t *err) {
     constexpr bool SPLIT = sizeof(QT) == 4;
     using C = TcCfg<HD, SPLIT>;
@@ -384,6 +390,8 @@ __global__ void __launch_bounds__(kTcThreads, HD == 256 ? 1 : 2)
             mbar_init(&bars.sfull[i], 1);
             mbar_init(&bars.pready[i], 4);
             mbar_init(&bars.odone[i], 1);
+            mbar_init(&bars.cdone[i], 1);
+            mbar_init(&bars.ofree[i], 4);
         }
         mbar_init(&bars.qready, 4);
         mbar_init(&bars.fin[0], 1);
@@ -410,7 +418,8 @@ __global__ void __launch_bounds__(kTcThreads, HD == 256 ? 1 : 2)
     const uint32_t tmem = bars.tmem;
     const PgSched &S = sched.S;
     const uint32_t kfull = smem_u32(bars.kfull), vfull = smem_u32(bars.vfull), sfull = smem_u32(bars.sfull),
-                   pready = smem_u32(bars.pready), odone = smem_u32(bars.odone), qready = smem_u32(&bars.qready),
+                   pready = smem_u32(bars.pready), odone = smem_u32(bars.odone), cdone = smem_u32(C::NCH == 1 ? bars.odone : bars.cdone),
+                   ofree = smem_u32(bars.ofree), qready = smem_u32(&bars.qready),
                    fin = smem_u32(bars.fin);
     // Every lane of a warp waits; false for all of them if any wait ran out.
     auto wait = [&](uint32_t bar, uint32_t parity) {
@@ -501,7 +510,7 @@ __global__ void __launch_bounds__(kTcThreads, HD == 256 ? 1 : 2)
                 ok = wait(kfull + 8u * st, (uint32_t)(j / KST)) && (j < NS || wait2(odone, j - NS));
                 if (!ok) break;
                 tc_after();
-                const uint32_t d = tmem + HD + (uint32_t)((j % NS) * KT);
+                const uint32_t d = tmem + C::SOFF + (uint32_t)((j % NS) * KT);
                 const uint64_t kb = kdesc + (uint64_t)((st * C::TBYTES) >> 4);
 #pragma unroll
                 for (int part = SPLIT ? 1 : 0; part >= 0; --part)  // the small part first: the sums are cut off, not rounded
@@ -517,7 +526,7 @@ __global__ void __launch_bounds__(kTcThreads, HD == 256 ? 1 : 2)
         wait_phase(fin, 0u, nullptr);
     } else if (any && warp == 6) {
         // O += P V.
-        const uint32_t idv = idesc_f16<CT>(HD, true);
+        const uint32_t idv = idesc_f16<CT>(C::NW, true);
         const uint64_t vdesc = desc_nmajor(sbase + C::VOFF, KT * 128);
         int j = 0;
         bool ok = true, more = true;
@@ -528,11 +537,21 @@ __global__ void __launch_bounds__(kTcThreads, HD == 256 ? 1 : 2)
                 ok = wait(vfull + 8u * st, (uint32_t)(j / KST)) && wait2(pready, j);
                 if (!ok) break;
                 tc_after();
-                const uint32_t p = tmem + HD + (uint32_t)((j % NS) * KT);
+                const uint32_t p = tmem + C::SOFF + (uint32_t)((j % NS) * KT);
                 const uint64_t vb = vdesc + (uint64_t)((st * C::TBYTES) >> 4);
-                if constexpr (SPLIT) {  // 16 columns of high parts, 16 of low parts, for each 32 positions
-                    mma_ts4(tmem, p + 16, p + 24, p + 48, p + 56, vb, idv, !first);
-                    mma_ts4(tmem, p, p + 8, p + 32, p + 40, vb, idv, true);
+                if constexpr (SPLIT) {
+                    // 16 columns of high parts, 16 of low parts, for each 32 positions; alone, not onto O.
+                    for (int q = 0; ok && q < C::NCH; ++q) {
+                        const int n = j * C::NCH + q;
+                        ok = n < C::NACC || wait2(ofree, n - C::NACC);
+                        if (!ok) break;
+                        tc_after();
+                        const uint32_t d = tmem + C::AOFF + (uint32_t)((n % C::NACC) * C::NW);
+                        const uint64_t qb = vb + (uint64_t)((q * (C::NW / 64) * KT * 128) >> 4);
+                        mma_ts4(d, p + 16, p + 24, p + 48, p + 56, qb, idv, false);
+                        mma_ts4(d, p, p + 8, p + 32, p + 40, qb, idv, true);
+                        if constexpr (C::NCH > 1) commit(cdone + 8u * (n & 1));
+                    }
                 } else {
                     mma_ts4(tmem, p, p + 8, p + 16, p + 24, vb, idv, !first);
                 }
@@ -556,6 +575,53 @@ __global__ void __launch_bounds__(kTcThreads, HD == 256 ? 1 : 2)
             __syncwarp();
             if (lane == 0) arrive(qready);
         };
+        // Split: part n of P V (dims q NW..) onto O scaled by f.  The tensor cores cut their sums off instead of
+        // rounding them, which over the tiles of a row adds up to 2.6e-6 of the output (17 tiles of 64); so
+        // a tile is summed alone and joined by a rounded FMA.
+        float o[C::REGO ? HD : 1];
+        auto fold = [&](int n, int q, float f, bool first) {
+            if (!wait2(cdone, n)) return false;
+            tc_after();
+            const uint32_t ta = tmem + lanes + C::AOFF + (uint32_t)((n % C::NACC) * C::NW);
+#pragma unroll
+            for (int c = 0; c < C::NW / 32; ++c) {
+                uint32_t w[32];
+                tm_ld32(ta + 32 * c, w);
+                if constexpr (C::REGO) {
+                    tm_wait_ld();
+#pragma unroll
+                    for (int e = 0; e < 32; ++e) o[32 * c + e] = fmaf(o[32 * c + e], f, __uint_as_float(w[e]));
+                } else {
+                    const uint32_t to = tmem + lanes + (uint32_t)(q * C::NW + 32 * c);
+                    if (!first) {
+                        uint32_t x[32];
+                        tm_ld32(to, x);
+                        tm_wait_ld();
+#pragma unroll
+                        for (int e = 0; e < 32; ++e)
+                            w[e] = __float_as_uint(fmaf(__uint_as_float(x[e]), f, __uint_as_float(w[e])));
+                    } else {
+                        tm_wait_ld();
+                    }
+                    tm_st32(to, w);
+                }
+            }
+            if constexpr (!C::REGO) tm_wait_st();
+            tc_before();
+            __syncwarp();
+            if (lane == 0) arrive(ofree + 8u * (n & 1));
+            return true;
+        };
+        // 32 dims of this row's O.
+        auto get = [&](int c, uint32_t (&w)[32]) {
+            if constexpr (C::REGO) {
+#pragma unroll
+                for (int e = 0; e < 32; ++e) w[e] = __float_as_uint(o[32 * c + e]);
+            } else {
+                tm_ld32(tmem + lanes + 32 * c, w);
+                tm_wait_ld();
+            }
+        };
         fetch();
         for (bool more = true; ok && more;) {
             const int rows = W.rows(A), len = W.q.p0 + W.q.n;
@@ -563,11 +629,13 @@ __global__ void __launch_bounds__(kTcThreads, HD == 256 ? 1 : 2)
             const int tok = r / A.rep, head = W.kh * A.rep + r - tok * A.rep;
             const int qpos = r < rows ? pos0 + tok : -1;
             const int pmax = pos0 + (rows - 1) / A.rep;  // the tile's last position; pos0 its first
-            float m = -INFINITY, l = 0.f;
+            float m = -INFINITY, l = 0.f, fold_f = 0.f;
+#pragma unroll
+            for (int e = 0; e < (C::REGO ? HD : 1); ++e) o[e] = 0.f;
             const int j0 = j;
             for (int it = W.i0; it < W.i1; ++it, ++j) {
                 const int k0 = W.R.tile(it) * KT;
-                const uint32_t ts = tmem + lanes + HD + (uint32_t)((j % NS) * KT);
+                const uint32_t ts = tmem + lanes + C::SOFF + (uint32_t)((j % NS) * KT);
                 // Nothing of the tile is hidden from any row.
                 const bool open = k0 + KT - 1 <= pos0 &&
                                   (!A.window || pmax - k0 < A.window || k0 + KT <= A.sinks);
@@ -592,7 +660,13 @@ __global__ void __launch_bounds__(kTcThreads, HD == 256 ? 1 : 2)
                 float mx = fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3]));
                 mx *= A.scale_log2;
                 if (r >= rows) mx = -INFINITY;
-                if (j == j0) {
+                float f = 1.f;
+                if constexpr (SPLIT) {  // O = O f + P V, tile by tile
+                    const float mo = m;
+                    m = fmaxf(m, mx);
+                    f = m == -INFINITY ? 0.f : ex2f(mo - m);
+                    l *= f;
+                } else if (j == j0) {
                     m = mx;
                 } else {
                     const bool grow = mx > m + 8.f;
@@ -603,7 +677,7 @@ __global__ void __launch_bounds__(kTcThreads, HD == 256 ? 1 : 2)
                         }
                         tc_after();
                         // A row without a maximum so far has O = 0 and l = 0.
-                        const float f = grow && m != -INFINITY ? ex2f(m - mx) : 1.f;
+                        f = grow && m != -INFINITY ? ex2f(m - mx) : 1.f;
                         if (grow) m = mx;
                         l *= f;
 #pragma unroll 1
@@ -663,6 +737,15 @@ __global__ void __launch_bounds__(kTcThreads, HD == 256 ? 1 : 2)
                 tc_before();
                 __syncwarp();
                 if (lane == 0) arrive(pready + 8u * (j % NS));
+                if constexpr (SPLIT) {
+                    if constexpr (C::REGO) {  // the tile before, while this one's P V runs
+                        ok = j == j0 || fold(j - 1, 0, fold_f, false);
+                        fold_f = f;
+                    } else {
+                        for (int q = 0; ok && q < C::NCH; ++q) ok = fold(j * C::NCH + q, q, f, j == j0);
+                    }
+                    if (!ok) break;
+                }
             }
             if (!ok) break;
             // The next piece's query tile before this one is finished: its first S are computed meanwhile.
@@ -671,15 +754,16 @@ __global__ void __launch_bounds__(kTcThreads, HD == 256 ? 1 : 2)
             const long long item0 = W.u - W.i1, item1 = item0 + W.R.cnt;
             more = W.next(A);
             if (more) fetch();
-            if (!wait2(odone, j - 1)) {
-                ok = false;
-                break;
-            }
+            if constexpr (C::REGO)
+                ok = fold(j - 1, 0, fold_f, false);
+            else
+                ok = wait2(odone, j - 1);
+            if (!ok) break;
             tc_after();
             if (whole)
-                finish_whole<QT, HD>(A, tmem + lanes, l, row, head);
+                finish_whole<QT, HD, C::REGO>(A, get, l, row, head);
             else
-                finish_cut<QT, HD>(A, S, tmem + lanes, item0, item1, m, l, row, head);
+                finish_cut<QT, HD, C::REGO>(A, S, get, item0, item1, m, l, row, head);
             tc_before();
         }
         if (!ok) bars.dead = 1u;
