@@ -259,28 +259,35 @@ __global__ void __launch_bounds__(kAppThreads) paged_append_kernel(PgAppendArgs 
 }
 
 // Attention, few query rows ------------------------------------------------------------------------
-// One CTA of 4 warps walks its pieces (PgSched) in tiles of 64 key positions, 16 per warp, staged by
-// cp.async in a ring of three tiles.  Rows of the product are the query rows of one (query tile, kv
-// head): 16 / rep tokens x rep heads, padded to 16.  S = Q K^T and O += P V on mma.sync m16n8k16 with
-// fp32 accumulation, the softmax online per warp (running maximum and sum per row), the four warps
-// joined in a fixed order at the end of a piece.  fp32 queries: Q and P enter as two fp16 parts each
-// (x = hi + lo), so that products are exact to 2^-22.  Bound by the K/V stream: rep tokens' work per
-// byte is far below the tensor cores' rate even with 16 rows padded.
-constexpr int kDecThreads = 128;
+// A CTA walks its pieces (PgSched) in tiles of 64 key positions. Rows of the products are the query rows
+// of one (query tile, kv head): 16 / rep tokens x rep heads, padded to 16.
+//  * warp 4, the producer: key tiles by TMA (boxes of one page, or the tile's part of it, x 64 dims,
+//    128-byte swizzle; lanes 0-15 K, 16-31 V) through a ring, and each piece's query rows into one of two
+//    places, all ahead of the work.
+//  * warps 0-3: 16 positions each of every tile: S = Q K^T and O += P V on mma.sync m16n8k16 with fp32
+//    accumulation, the softmax online per warp (running maximum and sum per row). At the end of a piece
+//    the four are joined in a fixed order.
+// fp32 queries: Q and P enter as two fp16 parts each (x = hi + lo), so that products keep 2^-22.
+// Bound by the K/V stream: rep tokens' work per byte is far below the tensor cores' rate even with 16 rows
+// padded, so the ring (64 to 192 KB per SM in flight) and short ends of pieces are what matters.
+constexpr int kDecThreads = 160;
 constexpr int kDecWarps = 4;
 constexpr int kDecTile = 64;
-constexpr int kDecStages = 3;
 
 template <int HD, bool SPLIT>
 struct DecSmem {
-    unsigned char k[kDecStages][kDecTile * HD * 2];
-    unsigned char v[kDecStages][kDecTile * HD * 2];
-    unsigned char q[SPLIT ? 2 : 1][16 * HD * 2];
+    static constexpr int ST = HD == 64 ? 4 : 3;          // ring stages
+    static constexpr int TB = kDecTile * HD * 2;         // bytes of a K or V tile
+    static constexpr int QB = SPLIT && HD >= 128 ? 1 : 2;  // places for a piece's query rows
+    unsigned char kv[ST][2][TB];
+    unsigned char q[QB][SPLIT ? 2 : 1][16 * HD * 2];
     union {
         PgSchedSmem sched;
-        float o[16][HD];
+        float o[kDecWarps][4][HD];                       // four rows of every warp's O
     };
-    float wm[kDecWarps][16], wl[kDecWarps][16], M[16], L[16];
+    float wm[kDecWarps][16], wl[kDecWarps][16];
+    uint64_t full[ST], freed[ST], qfull[2], qfreed[2], join;
+    volatile uint32_t dead;
     int last;
 };
 
@@ -313,25 +320,15 @@ __device__ __forceinline__ void ldsm4t(uint32_t addr, uint32_t (&r)[4]) {
                  : "r"(addr)
                  : "memory");
 }
-// 16 bytes to shared memory; zeros when n is 0.
-__device__ __forceinline__ void cp16z(uint32_t dst, const void *src, int n) {
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(n) : "memory");
-}
 
-// Byte offset of 16-byte piece c of row r in a tile of HD 16-bit elements per row: pieces are permuted
-// within each 128 bytes by the row, so that 8 rows' pieces of one column lie in different banks.
-template <int HD>
+// Byte offset of 16-byte piece c of row r in a tile of ROWS rows as the 128-byte swizzle lays it: blocks of
+// 64 dims, pieces permuted within each 128 bytes by the row.
+template <int ROWS>
 __device__ __forceinline__ uint32_t tile_off(int r, int c) {
-    return (uint32_t)(r * HD * 2 + ((c ^ (r & 7)) << 4));
+    return (uint32_t)((c >> 3) * (ROWS * 128) + r * 128 + (((c & 7) ^ (r & 7)) << 4));
 }
 
-__device__ __forceinline__ float ex2(float x) {
-    float y;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-    return y;
-}
-
-template <typename CT, typename QT>
+template <typename QT>
 __device__ __forceinline__ void put_out(const PgAttnArgs &A, int hd, int row, int h, int d, float o) {
     if (A.gate) {
         const float g = A.gate[row * A.gate_ld + (long long)h * 2 * hd + hd + d];
@@ -345,108 +342,161 @@ __device__ __forceinline__ void put_out(const PgAttnArgs &A, int hd, int row, in
 }
 
 template <typename CT, typename QT, int HD>
-__global__ void __launch_bounds__(kDecThreads, HD == 256 ? 1 : 2) attn_paged_kernel(PgAttnArgs A, uint32_t *err) {
+__global__ void __launch_bounds__(kDecThreads, HD == 256 ? 1 : 2)
+    attn_paged_kernel(const __grid_constant__ PgMaps maps, const __grid_constant__ PgAttnArgs A, uint32_t *err) {
     constexpr bool SPLIT = sizeof(QT) == 4;
-    extern __shared__ __align__(128) unsigned char smem_raw[];
+    extern __shared__ __align__(1024) unsigned char smem_raw[];
     using Smem = DecSmem<HD, SPLIT>;
+    constexpr int ST = Smem::ST, TB = Smem::TB, QB = Smem::QB;
     Smem &sm = *reinterpret_cast<Smem *>(smem_raw);
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, c = lane & 3;
     pdl_trigger();
+    if (smem_u32(smem_raw) & 1023u) {  // the swizzled tiles need 1024-byte places
+        pdl_wait();
+        if (tid == 0) atomicOr(err, TRX_DEV_INTERNAL);
+        return;
+    }
+    if (tid == 0) {
+        for (int i = 0; i < ST; ++i) {
+            mbar_init(&sm.full[i], 1);
+            mbar_init(&sm.freed[i], kDecWarps);
+        }
+        for (int i = 0; i < 2; ++i) {
+            mbar_init(&sm.qfull[i], 1);
+            mbar_init(&sm.qfreed[i], kDecWarps);
+        }
+        mbar_init(&sm.join, kDecWarps);
+        sm.dead = 0u;
+        mbar_fence_init();
+        tma_prefetch_map(&maps.k);
+        tma_prefetch_map(&maps.v);
+    }
     pdl_wait();
-    pg_schedule(A, sm.sched, 1, err);
+    pg_schedule(A, sm.sched, 1, err);  // barriers inside: the set-up above is visible behind it
     const PgSched S = sm.sched.S;
     __syncthreads();
     PgWalk W;
     if (!W.start(A, S)) return;
-    PgWalk Ld = W;
-    int li = Ld.i0;
-    bool more = true;
-    const uint32_t kbase = smem_u32(sm.k), vbase = smem_u32(sm.v), qbase = smem_u32(sm.q);
-    constexpr uint32_t kStage = kDecTile * HD * 2;
-    constexpr int PPR = HD / 8;                // 16-byte pieces per row
-    constexpr int RPP = kDecThreads / PPR;     // rows per pass of the block
-    const int pc = tid % PPR, pr = tid / PPR;
-    const long long pitch = (long long)A.Hkv * HD;
-
-    // Stage the next key tile of the loader's walk into ring slot s.
-    auto issue = [&](int s) {
-        const int k0 = Ld.R.tile(li) * kDecTile, len = Ld.q.p0 + Ld.q.n;
-        const int *tab = A.tables + (long long)Ld.b * A.max_pages;
-#pragma unroll 4
-        for (int i = 0; i < kDecTile / RPP; ++i) {
-            const int r = pr + i * RPP, p = k0 + r;
-            int bytes = 0;
-            long long off = 0;
-            if (p < len) {
-                const int id = __ldg(tab + (p >> A.page_shift));
-                if ((unsigned)id < (unsigned)A.n_pages) {
-                    bytes = 16;
-                    off = (((long long)id << A.page_shift) + (p & ((1 << A.page_shift) - 1))) * pitch +
-                          (long long)Ld.kh * HD + pc * 8;
-                } else if (pc == 0) {
-                    atomicOr(err, TRX_DEV_RANGE);
-                }
-            }
-            cp16z(kbase + s * kStage + tile_off<HD>(r, pc), reinterpret_cast<const CT *>(A.kp) + off, bytes);
-            cp16z(vbase + s * kStage + tile_off<HD>(r, pc), reinterpret_cast<const CT *>(A.vp) + off, bytes);
-        }
-        if (++li == Ld.i1) {
-            more = Ld.next(A);
-            li = Ld.i0;
-        }
+    const uint32_t full = smem_u32(sm.full), freed = smem_u32(sm.freed), qfull = smem_u32(sm.qfull),
+                   qfreed = smem_u32(sm.qfreed), joinb = smem_u32(&sm.join);
+    auto wait = [&](uint32_t bar, uint32_t parity) {
+        const bool ok = __all_sync(0xffffffffu, wait_phase(bar, parity & 1u, err));
+        if (!ok) sm.dead = 1u;
+        return ok;
     };
-#pragma unroll
-    for (int s = 0; s < kDecStages - 1; ++s) {
-        if (more) issue(s);
-        asm volatile("cp.async.commit_group;" ::: "memory");
-    }
-    int slot = 0;
-    do {
-        const int rows = W.rows(A);
-        const int row0 = W.q.row0 + W.t * A.tq, tok_pos = W.q.p0 + W.t * A.tq;
-        // The query rows, zeros behind them.
-        __syncthreads();
-        for (int i = tid; i < 16 * (HD / 8); i += kDecThreads) {
-            const int r = i / (HD / 8), pcq = i % (HD / 8);
-            uint4 hi = make_uint4(0u, 0u, 0u, 0u), lo = hi;
-            if (r < rows) {
-                const int tk = r / A.rep, h = W.kh * A.rep + r - tk * A.rep;
-                const QT *src = reinterpret_cast<const QT *>(A.q) + ((size_t)(row0 + tk) * A.H + h) * HD + pcq * 8;
-                if constexpr (SPLIT) {
-                    const float4 x = *reinterpret_cast<const float4 *>(src), y = *reinterpret_cast<const float4 *>(src + 4);
-                    const float f[8] = {x.x, x.y, x.z, x.w, y.x, y.y, y.z, y.w};
-                    uint32_t hw[4], lw[4];
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) {
-                        hw[j] = PgCvt<CT>::pack(f[2 * j], f[2 * j + 1]);
-                        const float2 b = PgCvt<CT>::unpack(hw[j]);
-                        lw[j] = PgCvt<CT>::pack(f[2 * j] - b.x, f[2 * j + 1] - b.y);
-                    }
-                    hi = make_uint4(hw[0], hw[1], hw[2], hw[3]);
-                    lo = make_uint4(lw[0], lw[1], lw[2], lw[3]);
-                } else {
-                    hi = *reinterpret_cast<const uint4 *>(src);
-                }
+    if (warp == kDecWarps) {
+        // Producer.
+        const int br = min(1 << A.page_shift, kDecTile), nb = kDecTile / br;  // box rows, boxes per 64 dims
+        const int boxes = nb * (HD / 64), bi = lane & 15;
+        static_assert(kDecTile / 16 * (HD / 64) <= 16, "a lane has one box");
+        const int beyond = A.n_pages << A.page_shift;  // a row outside the maps: zeros
+        const int my_pos = (bi % nb) * br, my_dim = 64 * (bi / nb);
+        const uint32_t my_dst = smem_u32(sm.kv) + (uint32_t)((lane >> 4) * TB + (bi / nb) * (kDecTile * 128) + my_pos * 128);
+        const CUtensorMap *const map = lane < 16 ? &maps.k : &maps.v;
+        const bool mine = bi < boxes;
+        auto row_of = [&](const PgWalk &P, int it) {  // this lane's first row of tile it of a piece
+            const int p = P.R.tile(it) * kDecTile + my_pos;
+            int row = beyond;
+            if (mine && p < P.q.p0 + P.q.n) {
+                const int id = __ldg(A.tables + (long long)P.b * A.max_pages + (p >> A.page_shift));
+                if ((unsigned)id < (unsigned)A.n_pages)
+                    row = (id << A.page_shift) + (p & ((1 << A.page_shift) - 1));
+                else
+                    atomicOr(err, TRX_DEV_RANGE);
             }
-            *reinterpret_cast<uint4 *>(&sm.q[0][tile_off<HD>(r, pcq)]) = hi;
-            if constexpr (SPLIT) *reinterpret_cast<uint4 *>(&sm.q[SPLIT ? 1 : 0][tile_off<HD>(r, pcq)]) = lo;
+            return row;
+        };
+        int j = 0, piece = 0, it = W.i0;
+        bool ok = true;
+        int row = row_of(W, it);
+        for (;;) {
+            // The table is read a tile ahead.
+            PgWalk N = W;
+            int nit = it + 1;
+            const bool more = nit < W.i1 || N.next(A);
+            if (nit == W.i1) nit = N.i0;
+            const int nrow = more ? row_of(N, nit) : 0;
+            const int st = j % ST;
+            ok = !sm.dead && (j < ST || wait(freed + 8u * st, (uint32_t)(j / ST - 1)));
+            if (!ok) break;
+            if (lane == 0) mbar_expect_tx_s(full + 8u * st, 2u * TB);
+            __syncwarp();
+            if (mine) load_box(my_dst + (uint32_t)(st * 2 * TB), map, W.kh * HD + my_dim, row, full + 8u * st);
+            __syncwarp();
+            if (it == W.i0) {  // a new piece: its query rows, zeros behind them
+                const int qb = piece % QB;
+                ok = piece < QB || wait(qfreed + 8u * qb, (uint32_t)(piece / QB - 1));
+                if (!ok) break;
+                const int rows = W.rows(A), row0 = W.q.row0 + W.t * A.tq;
+#pragma unroll 2
+                for (int i = lane; i < 16 * (HD / 8); i += 32) {
+                    const int r = i / (HD / 8), pcq = i % (HD / 8);
+                    uint4 hi = make_uint4(0u, 0u, 0u, 0u), lo = hi;
+                    if (r < rows) {
+                        const int tk = r / A.rep, h = W.kh * A.rep + r - tk * A.rep;
+                        const QT *src = reinterpret_cast<const QT *>(A.q) + ((size_t)(row0 + tk) * A.H + h) * HD + pcq * 8;
+                        if constexpr (SPLIT) {
+                            const float4 x = *reinterpret_cast<const float4 *>(src), y = *reinterpret_cast<const float4 *>(src + 4);
+                            const float f[8] = {x.x, x.y, x.z, x.w, y.x, y.y, y.z, y.w};
+                            uint32_t hw[4], lw[4];
+#pragma unroll
+                            for (int e = 0; e < 4; ++e) {
+                                hw[e] = PgCvt<CT>::pack(f[2 * e], f[2 * e + 1]);
+                                const float2 b = PgCvt<CT>::unpack(hw[e]);
+                                lw[e] = PgCvt<CT>::pack(f[2 * e] - b.x, f[2 * e + 1] - b.y);
+                            }
+                            hi = make_uint4(hw[0], hw[1], hw[2], hw[3]);
+                            lo = make_uint4(lw[0], lw[1], lw[2], lw[3]);
+                        } else {
+                            hi = *reinterpret_cast<const uint4 *>(src);
+                        }
+                    }
+                    *reinterpret_cast<uint4 *>(&sm.q[qb][0][tile_off<16>(r, pcq)]) = hi;
+                    if constexpr (SPLIT) *reinterpret_cast<uint4 *>(&sm.q[qb][SPLIT ? 1 : 0][tile_off<16>(r, pcq)]) = lo;
+                }
+                __syncwarp();
+                if (lane == 0) arrive(qfull + 8u * qb);
+                ++piece;
+            }
+            ++j;
+            if (!more) break;
+            W = N;
+            it = nit;
+            row = nrow;
         }
+        if (!ok) {
+            // Whatever was issued has landed before the block leaves (bounded; the timeout is recorded).
+            sm.dead = 1u;
+            for (int st = 0; st < ST; ++st)
+                for (int ph = 0; ph < 2; ++ph) wait_phase(full + 8u * st, ph, nullptr);
+        }
+        return;
+    }
+    uint32_t joined = 0;
+    auto join = [&] {  // the four warps (bounded, unlike a block barrier)
+        __syncwarp();
+        if (lane == 0) arrive(joinb);
+        return wait(joinb, joined++);
+    };
+    int j = 0, piece = 0;
+    bool ok = true, more = true;
+    while (ok && more) {
+        const int rows = W.rows(A), len = W.q.p0 + W.q.n;
+        const int row0 = W.q.row0 + W.t * A.tq, tok_pos = W.q.p0 + W.t * A.tq;
+        const uint32_t qs = smem_u32(sm.q[piece % QB][0]);
+        if (!wait(qfull + 8u * (piece % QB), (uint32_t)(piece / QB))) break;
         float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
         float o[HD / 8][4];
 #pragma unroll
         for (int i = 0; i < HD / 8; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
         // Positions of rows g and g + 8 (-1 behind the last: everything hidden).
         const int qp[2] = {g < rows ? tok_pos + g / A.rep : -1, g + 8 < rows ? tok_pos + (g + 8) / A.rep : -1};
-        for (int it = W.i0; it < W.i1; ++it) {
-            asm volatile("cp.async.wait_group %0;" ::"n"(kDecStages - 2) : "memory");
-            __syncthreads();  // the tile has landed, and every warp is done with the slot refilled next
-            {
-                const int s2 = slot + kDecStages - 1;
-                if (more) issue(s2 >= kDecStages ? s2 - kDecStages : s2);
-                asm volatile("cp.async.commit_group;" ::: "memory");
-            }
+        for (int it = W.i0; it < W.i1; ++it, ++j) {
+            const int st = j % ST;
+            ok = wait(full + 8u * st, (uint32_t)(j / ST));
+            if (!ok) break;
             const int k0 = W.R.tile(it) * kDecTile + warp * 16;
-            const uint32_t ks = kbase + slot * kStage, vs = vbase + slot * kStage;
+            const uint32_t ks = smem_u32(sm.kv[st][0]), vs = ks + TB;
             float s0[4] = {0.f, 0.f, 0.f, 0.f}, s1[4] = {0.f, 0.f, 0.f, 0.f};
             float t0[4] = {0.f, 0.f, 0.f, 0.f}, t1[4] = {0.f, 0.f, 0.f, 0.f};  // the low parts' sums
             const int arow = (lane & 7) + ((lane >> 3) & 1) * 8, acol = lane >> 4;
@@ -454,45 +504,55 @@ __global__ void __launch_bounds__(kDecThreads, HD == 256 ? 1 : 2) attn_paged_ker
 #pragma unroll
             for (int k = 0; k < HD / 16; ++k) {
                 uint32_t a[4], b[4];
-                ldsm4(qbase + tile_off<HD>(arow, 2 * k + acol), a);
-                ldsm4(ks + tile_off<HD>(brow, 2 * k + bcol), b);
+                ldsm4(qs + tile_off<16>(arow, 2 * k + acol), a);
+                ldsm4(ks + tile_off<kDecTile>(brow, 2 * k + bcol), b);
                 mma_16816<CT>(s0, a, b[0], b[1]);
                 mma_16816<CT>(s1, a, b[2], b[3]);
                 if constexpr (SPLIT) {
-                    ldsm4(qbase + 16 * HD * 2 + tile_off<HD>(arow, 2 * k + acol), a);
+                    ldsm4(qs + 16 * HD * 2 + tile_off<16>(arow, 2 * k + acol), a);
                     mma_16816<CT>(t0, a, b[0], b[1]);
                     mma_16816<CT>(t1, a, b[2], b[3]);
                 }
             }
             if constexpr (SPLIT) {
 #pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    s0[j] += t0[j];
-                    s1[j] += t1[j];
+                for (int e = 0; e < 4; ++e) {
+                    s0[e] += t0[e];
+                    s1[e] += t1[e];
                 }
             }
-            float alpha[2];
+            // This warp's rows of V behind the sequence's end: zeros (0 times what lies there would not be 0
+            // if it is not finite).
+            if (k0 + 16 > len) {
+                const int z0 = max(0, len - k0);
+                for (int i = lane; i < (16 - z0) * (HD / 8); i += 32)
+                    *reinterpret_cast<uint4 *>(&sm.kv[st][1][tile_off<kDecTile>(warp * 16 + z0 + i / (HD / 8), i % (HD / 8))]) =
+                        make_uint4(0u, 0u, 0u, 0u);
+                fence_proxy_async();  // before the copy that refills the slot
+                __syncwarp();
+            }
             // Row g: s0[0], s0[1] at positions k0 + 2c, + 1, s1[0], s1[1] at k0 + 8 + 2c; row g + 8: [2], [3].
             uint32_t ph[4], pl[4];
+            float alpha[2];
 #pragma unroll
             for (int rr = 0; rr < 2; ++rr) {
                 float x[4] = {s0[2 * rr], s0[2 * rr + 1], s1[2 * rr], s1[2 * rr + 1]};
                 float mx = -INFINITY;
 #pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    const int kp = k0 + 2 * c + (j & 1) + (j >> 1) * 8;
-                    x[j] = pg_hidden(kp, qp[rr], A.window, A.sinks) ? -INFINITY : x[j] * A.scale_log2;
-                    mx = fmaxf(mx, x[j]);
+                for (int e = 0; e < 4; ++e) {
+                    const int kp = k0 + 2 * c + (e & 1) + (e >> 1) * 8;
+                    x[e] = pg_hidden(kp, qp[rr], A.window, A.sinks) ? -INFINITY : x[e] * A.scale_log2;
+                    mx = fmaxf(mx, x[e]);
                 }
                 mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
                 mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
                 const float mn = fmaxf(m[rr], mx), ms = mn == -INFINITY ? 0.f : mn;
-                const float al = ex2(m[rr] - ms);
+                const float al = ex2f(m[rr] - ms);
                 float p[4], sum = 0.f;
 #pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    p[j] = ex2(x[j] - ms);
-                    sum += p[j];
+                for (int e = 0; e < 4; ++e) {
+                    p[e] = ex2f(x[e] - ms);
+                    sum += p[e];
                 }
                 l[rr] = l[rr] * al + sum;
                 m[rr] = mn;
@@ -509,13 +569,13 @@ __global__ void __launch_bounds__(kDecThreads, HD == 256 ? 1 : 2) attn_paged_ker
 #pragma unroll
             for (int i = 0; i < HD / 16; ++i) {
                 uint32_t b[4];
-                ldsm4t(vs + tile_off<HD>(vrow, 2 * i + vcol), b);
+                ldsm4t(vs + tile_off<kDecTile>(vrow, 2 * i + vcol), b);
 #pragma unroll
                 for (int h = 0; h < 2; ++h) {
                     float(&d)[4] = o[2 * i + h];
                     if constexpr (SPLIT) {
                         // The tensor core cuts its sums off instead of rounding them: over hundreds of tiles
-                        // that adds up (1.8e-6 against 0.5e-6 at 30,000 positions), so each tile's product
+                        // that adds up (1.8e-6 against 0.4e-6 at 30,000 positions), so each tile's product
                         // is summed alone and added by a rounded FMA.
                         float t[4] = {0.f, 0.f, 0.f, 0.f};
                         mma_16816<CT>(t, pl, b[2 * h], b[2 * h + 1]);
@@ -533,9 +593,13 @@ __global__ void __launch_bounds__(kDecThreads, HD == 256 ? 1 : 2) attn_paged_ker
                     }
                 }
             }
-            slot = slot + 1 == kDecStages ? 0 : slot + 1;
+            __syncwarp();
+            if (lane == 0) arrive(freed + 8u * st);
         }
-        // The warps' parts of the piece, in their order.
+        if (!ok) break;
+        if (lane == 0) arrive(qfreed + 8u * (piece % QB));
+        ++piece;
+        // The warps' parts of the piece, joined in their order, four rows at a time.
 #pragma unroll
         for (int rr = 0; rr < 2; ++rr) {
             l[rr] += __shfl_xor_sync(0xffffffffu, l[rr], 1);
@@ -545,102 +609,93 @@ __global__ void __launch_bounds__(kDecThreads, HD == 256 ? 1 : 2) attn_paged_ker
                 sm.wl[warp][g + 8 * rr] = l[rr];
             }
         }
-        __syncthreads();
-        float f[2];
+        const bool whole = W.whole();
+        const long long item0 = W.u - W.i1, item1 = item0 + W.R.cnt;
+        const int kh = W.kh;
+        int c0 = 0, c1 = 0;
+        if (!whole) {
+            c0 = pg_owner(S, item0);
+            c1 = pg_owner(S, item1 - 1);
+        }
+        constexpr size_t kPart = 16 * (HD + 2);  // a cut piece in scratch: maxima, sums, then O by row
+        auto slot_of = [&](int cc) { return A.part + kPart * (2 * (size_t)cc + (cc == c0 ? 1 : 0)); };
+        float *const part = slot_of(blockIdx.x);
+        for (int r0 = 0; ok && r0 < rows; r0 += 4) {
+            // Lanes of rows r0..r0+3: g or g + 8.
+            const int rr = r0 >= 8 ? 1 : 0, lr = g + 8 * rr - r0;
+            if (lr >= 0 && lr < 4) {
 #pragma unroll
-        for (int rr = 0; rr < 2; ++rr) {
-            const int r = g + 8 * rr;
-            float M = -INFINITY;
+                for (int i = 0; i < HD / 8; ++i)
+                    *reinterpret_cast<float2 *>(&sm.o[warp][lr][8 * i + 2 * c]) =
+                        rr ? make_float2(o[i][2], o[i][3]) : make_float2(o[i][0], o[i][1]);
+            }
+            ok = join();
+            if (!ok) break;
+            const int nr = min(4, rows - r0);
+            for (int i = tid; i < nr * HD; i += 32 * kDecWarps) {
+                const int r = i / HD, d = i - r * HD, R = r0 + r, tk = R / A.rep;
+                float M = -INFINITY;
 #pragma unroll
-            for (int w = 0; w < kDecWarps; ++w) M = fmaxf(M, sm.wm[w][r]);
-            f[rr] = m[rr] == -INFINITY ? 0.f : ex2(m[rr] - M);
-            if (warp == 0 && c == 0) {
-                float L = 0.f;
+                for (int w = 0; w < kDecWarps; ++w) M = fmaxf(M, sm.wm[w][R]);
+                const float Ms = M == -INFINITY ? 0.f : M;
+                float L = 0.f, acc = 0.f;
+#pragma unroll
                 for (int w = 0; w < kDecWarps; ++w) {
-                    const float mw = sm.wm[w][r];
-                    if (mw != -INFINITY) L = fmaf(ex2(mw - M), sm.wl[w][r], L);
+                    const float e = ex2f(sm.wm[w][R] - Ms);
+                    L = fmaf(e, sm.wl[w][R], L);
+                    acc = fmaf(e, sm.o[w][r][d], acc);
                 }
-                sm.M[r] = M;
-                sm.L[r] = L;
-            }
-        }
-        for (int w = 0; w < kDecWarps; ++w) {
-            if (warp == w) {
-#pragma unroll
-                for (int rr = 0; rr < 2; ++rr) {
-                    const int r = g + 8 * rr;
-                    if (r < rows)
-#pragma unroll
-                        for (int i = 0; i < HD / 8; ++i) {
-                            float2 *p = reinterpret_cast<float2 *>(&sm.o[r][8 * i + 2 * c]);
-                            float2 v = make_float2(f[rr] * o[i][2 * rr], f[rr] * o[i][2 * rr + 1]);
-                            if (w) {
-                                const float2 q = *p;
-                                v.x += q.x;
-                                v.y += q.y;
-                            }
-                            *p = v;
-                        }
+                if (whole) {
+                    put_out<QT>(A, HD, row0 + tk, kh * A.rep + R - tk * A.rep, d, L > 0.f ? __fdiv_rn(acc, L) : 0.f);
+                } else {
+                    part[32 + R * HD + d] = acc;
+                    if (d == 0) {
+                        part[R] = M;
+                        part[16 + R] = L;
+                    }
                 }
             }
-            __syncthreads();
+            ok = join();
         }
-        if (W.whole()) {
-            for (int i = tid; i < rows * HD; i += kDecThreads) {
-                const int r = i / HD, d = i - r * HD, tk = r / A.rep;
-                const float L = sm.L[r];
-                put_out<CT, QT>(A, HD, row0 + tk, W.kh * A.rep + r - tk * A.rep, d, L > 0.f ? __fdiv_rn(sm.o[r][d], L) : 0.f);
-            }
-        } else {
-            // A cut item: this piece to scratch; the last CTA to arrive joins the pieces in CTA order.
-            const long long item0 = W.u - W.i1, item1 = item0 + W.R.cnt;
-            const int c0 = pg_owner(S, item0), c1 = pg_owner(S, item1 - 1);
-            constexpr size_t kPart = 16 * (HD + 2);
-            float *const mine = A.part + kPart * (2 * (size_t)blockIdx.x + ((int)blockIdx.x == c0 ? 1 : 0));
-            for (int i = tid; i < rows * HD; i += kDecThreads) mine[32 + i] = sm.o[i / HD][i % HD];
-            if (tid < rows) {
-                mine[tid] = sm.M[tid];
-                mine[16 + tid] = sm.L[tid];
-            }
+        if (!ok) break;
+        if (!whole) {
+            // The last CTA to arrive joins the pieces in CTA order.
             __threadfence();
-            __syncthreads();
+            ok = join();
+            if (!ok) break;
             if (tid == 0) sm.last = atomicAdd(A.cnt + c0, 1u) == (unsigned)(c1 - c0);
-            __syncthreads();
+            ok = join();
+            if (!ok) break;
             if (sm.last) {
                 __threadfence();
-                auto slot_of = [&](int cc) { return A.part + kPart * (2 * (size_t)cc + (cc == c0 ? 1 : 0)); };
-                if (tid < rows) {
-                    float M = -INFINITY, L = 0.f;
-                    for (int cc = c0; cc <= c1; ++cc) M = fmaxf(M, __ldcg(slot_of(cc) + tid));
-                    for (int cc = c0; cc <= c1; ++cc) {
-                        const float mp = __ldcg(slot_of(cc) + tid);
-                        if (mp != -INFINITY) L = fmaf(ex2(mp - M), __ldcg(slot_of(cc) + 16 + tid), L);
-                    }
-                    sm.M[tid] = M;
-                    sm.L[tid] = L;
-                }
-                __syncthreads();
-                for (int i = tid; i < rows * HD; i += kDecThreads) {
+                for (int i = tid; i < rows * HD; i += 32 * kDecWarps) {
                     const int r = i / HD, d = i - r * HD, tk = r / A.rep;
-                    const float M = sm.M[r], L = sm.L[r];
-                    float acc = 0.f;
+                    float M = -INFINITY;
+#pragma unroll 4
+                    for (int cc = c0; cc <= c1; ++cc) M = fmaxf(M, __ldcg(slot_of(cc) + r));
+                    const float Ms = M == -INFINITY ? 0.f : M;
+                    float L = 0.f, acc = 0.f;
+#pragma unroll 4
                     for (int cc = c0; cc <= c1; ++cc) {
                         const float *p = slot_of(cc);
-                        const float mp = __ldcg(p + r);
-                        if (mp != -INFINITY) acc = fmaf(ex2(mp - M), __ldcg(p + 32 + i), acc);
+                        const float e = ex2f(__ldcg(p + r) - Ms);
+                        L = fmaf(e, __ldcg(p + 16 + r), L);
+                        acc = fmaf(e, __ldcg(p + 32 + i), acc);
                     }
-                    put_out<CT, QT>(A, HD, row0 + tk, W.kh * A.rep + r - tk * A.rep, d, L > 0.f ? __fdiv_rn(acc, L) : 0.f);
+                    put_out<QT>(A, HD, row0 + tk, kh * A.rep + r - tk * A.rep, d, L > 0.f ? __fdiv_rn(acc, L) : 0.f);
                 }
                 if (tid == 0) A.cnt[c0] = 0u;
             }
         }
-    } while (W.next(A));
-    asm volatile("cp.async.wait_group 0;" ::: "memory");
+        more = W.next(A);
+    }
+    if (!ok) sm.dead = 1u;
 }
 
 template <typename CT, typename QT, int HD>
 trx_status launch_dec(PgAttnArgs A, size_t part_cap, int cnt_cap, uint32_t *err, cudaStream_t st) {
     constexpr size_t smem = sizeof(DecSmem<HD, sizeof(QT) == 4>);
+    static_assert(smem <= (HD == 256 ? 232448 : 115712), "one CTA (head dim 256) or two per SM");
     static DevBits configured{0};
     const cudaError_t e = once_per_device(configured, [] {
         return cudaFuncSetAttribute(attn_paged_kernel<CT, QT, HD>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
@@ -648,9 +703,14 @@ trx_status launch_dec(PgAttnArgs A, size_t part_cap, int cnt_cap, uint32_t *err,
     if (e != cudaSuccess) return note_cuda(e);
     A.tq = 16 / A.rep;
     A.kt_shift = 6;
-    int grid = device_sms() * (HD == 256 ? 1 : 2);
-    while (grid > 1 && ((size_t)grid * 2 * 16 * (HD + 2) > part_cap || grid > cnt_cap)) grid /= 2;
-    return note_cuda(launch_kernel(attn_paged_kernel<CT, QT, HD>, dim3(grid), dim3(kDecThreads), smem, st, A, err));
+    PgMaps maps;
+    const uint64_t cols = (uint64_t)A.Hkv * HD, rows = (uint64_t)A.n_pages << A.page_shift;
+    const uint32_t br = 1u << (A.page_shift < 6 ? A.page_shift : 6);
+    if (!encode_map_16bit(&maps.k, A.kp, cols, rows, 64, br) || !encode_map_16bit(&maps.v, A.vp, cols, rows, 64, br))
+        return TRX_ERR_CUDA;
+    const int grid = device_sms() * (HD == 256 ? 1 : 2);
+    if ((size_t)grid * 2 * 16 * (HD + 2) > part_cap || grid > cnt_cap) return TRX_ERR_UNSUPPORTED;
+    return note_cuda(launch_kernel(attn_paged_kernel<CT, QT, HD>, dim3(grid), dim3(kDecThreads), smem, st, maps, A, err));
 }
 
 template <typename CT, typename QT>

@@ -2,6 +2,7 @@
 // sequences' geometry, and the division of the attention work among CTAs.
 #pragma once
 #include <cstdint>
+#include <cuda.h>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
@@ -12,6 +13,42 @@
 namespace trx {
 
 constexpr int kPagedMaxSeq = 1024;  // sequences of one plan (the kernels keep a prefix of them in shared memory)
+
+// The pools as matrices of n_kv * head_dim columns, one row per slot.
+struct PgMaps {
+    CUtensorMap k, v;
+};
+
+__device__ __forceinline__ void arrive(uint32_t bar) {
+    asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory");
+}
+__device__ __forceinline__ void load_box(uint32_t dst, const void *map, int x, int y, uint32_t bar) {
+    asm volatile(
+        "cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], "
+        "[%4];" ::"r"(dst),
+        "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(bar)
+        : "memory");
+}
+
+// Bounded wait on an mbarrier phase by the SM's own clock (2^29 cycles, about 0.3 s; then
+// TRX_DEV_TIMEOUT).
+__device__ __forceinline__ bool wait_phase(uint32_t bar, uint32_t parity, uint32_t *err) {
+    if (mbar_try_wait_s(bar, parity)) return true;
+    const long long t0 = clock64();
+    do {
+#pragma unroll 1
+        for (int i = 0; i < 16; ++i)
+            if (mbar_try_wait_s(bar, parity)) return true;
+    } while (clock64() - t0 < (1ll << 29));
+    if (err && (threadIdx.x & 31) == 0) atomicOr(err, TRX_DEV_TIMEOUT);
+    return false;
+}
+
+__device__ __forceinline__ float ex2f(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
 
 // One sequence of an attention launch: its new rows [row0, row0 + n) at positions [p0, p0 + n).
 struct PgSeq {

@@ -130,17 +130,6 @@ __device__ __forceinline__ void commit(uint32_t bar) {
         " @e tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n}\n" ::"r"(bar)
         : "memory");
 }
-__device__ __forceinline__ void arrive(uint32_t bar) {
-    asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory");
-}
-__device__ __forceinline__ void load_box(uint32_t dst, const void *map, int x, int y, uint32_t bar) {
-    asm volatile(
-        "cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], "
-        "[%4];" ::"r"(dst),
-        "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(bar)
-        : "memory");
-}
-
 // Tensor memory, one lane per thread, 32 (or 16) consecutive columns.
 __device__ __forceinline__ void tm_ld32(uint32_t a, uint32_t (&v)[32]) {
     asm volatile(
@@ -173,30 +162,6 @@ __device__ __forceinline__ void tm_st16(uint32_t a, const uint32_t (&o)[16]) {
 }
 __device__ __forceinline__ void tm_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
 __device__ __forceinline__ void tm_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
-
-__device__ __forceinline__ float ex2f(float x) {
-    float y;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-    return y;
-}
-
-// Bounded wait on an mbarrier phase by the SM's own clock (2^29 cycles, about 0.3 s; then
-// TRX_DEV_TIMEOUT).
-__device__ __forceinline__ bool wait_phase(uint32_t bar, uint32_t parity, uint32_t *err) {
-    if (mbar_try_wait_s(bar, parity)) return true;
-    const long long t0 = clock64();
-    do {
-#pragma unroll 1
-        for (int i = 0; i < 16; ++i)
-            if (mbar_try_wait_s(bar, parity)) return true;
-    } while (clock64() - t0 < (1ll << 29));
-    if (err && (threadIdx.x & 31) == 0) atomicOr(err, TRX_DEV_TIMEOUT);
-    return false;
-}
-
-struct TcMaps {
-    CUtensorMap k, v;
-};
 
 // 32 outputs of one row, dims d..d+31.
 template <typename QT>
@@ -368,7 +333,7 @@ __device__ __forceinline__ void finish_cut(const PgAttnArgs &A, const PgSched &S
 
 template <typename CT, typename QT, int HD>
 __global__ void __launch_bounds__(kTcThreads, HD == 256 || sizeof(QT) == 4 ? 1 : 2)
-    attn_paged_tc_kernel(const __grid_constant__ TcMaps maps, const __grid_constant__ PgAttnArgs A, uint32_t *err) {
+    attn_paged_tc_kernel(const __grid_constant__ PgMaps maps, const __grid_constant__ PgAttnArgs A, uint32_t *err) {
     constexpr bool SPLIT = sizeof(QT) == 4;
     using C = TcCfg<HD, SPLIT>;
     constexpr int KT = C::KT, NS = C::NS, KST = C::KST;
@@ -787,7 +752,7 @@ trx_status launch_tc(PgAttnArgs A, size_t part_cap, int cnt_cap, uint32_t *err, 
     if (e != cudaSuccess) return note_cuda(e);
     A.tq = kTcRows / A.rep;
     A.kt_shift = C::KT_SHIFT;
-    TcMaps maps;
+    PgMaps maps;
     const int page = 1 << A.page_shift;
     const uint64_t cols = (uint64_t)A.Hkv * HD, rows = (uint64_t)A.n_pages << A.page_shift;
     const uint32_t br = (uint32_t)std::min(page, C::KT);
