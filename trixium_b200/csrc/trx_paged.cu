@@ -372,7 +372,7 @@ __global__ void __launch_bounds__(kDecThreads, HD == 256 ? 1 : 2)
         tma_prefetch_map(&maps.v);
     }
     pdl_wait();
-    pg_schedule(A, sm.sched, 1, err);  // barriers inside: the set-up above is visible behind it
+    pg_schedule(A, sm.sched, 2, err);  // barriers inside: the set-up above is visible behind it
     const PgSched S = sm.sched.S;
     __syncthreads();
     PgWalk W;
@@ -428,31 +428,42 @@ __global__ void __launch_bounds__(kDecThreads, HD == 256 ? 1 : 2)
                 ok = piece < QB || wait(qfreed + 8u * qb, (uint32_t)(piece / QB - 1));
                 if (!ok) break;
                 const int rows = W.rows(A), row0 = W.q.row0 + W.t * A.tq;
-#pragma unroll 2
-                for (int i = lane; i < 16 * (HD / 8); i += 32) {
-                    const int r = i / (HD / 8), pcq = i % (HD / 8);
-                    uint4 hi = make_uint4(0u, 0u, 0u, 0u), lo = hi;
-                    if (r < rows) {
-                        const int tk = r / A.rep, h = W.kh * A.rep + r - tk * A.rep;
-                        const QT *src = reinterpret_cast<const QT *>(A.q) + ((size_t)(row0 + tk) * A.H + h) * HD + pcq * 8;
-                        if constexpr (SPLIT) {
-                            const float4 x = *reinterpret_cast<const float4 *>(src), y = *reinterpret_cast<const float4 *>(src + 4);
-                            const float f[8] = {x.x, x.y, x.z, x.w, y.x, y.y, y.z, y.w};
-                            uint32_t hw[4], lw[4];
+                // Rows behind the last keep what was there: every position is hidden from them.
+                const QT *const src = reinterpret_cast<const QT *>(A.q) + ((long long)row0 * A.H + W.kh * A.rep) * HD;
+                const int inv = (65536 + A.rep - 1) / A.rep;  // r / rep = r * inv >> 16 for r < 16
+                constexpr int B = 4;                          // loads of a lane in flight
+                for (int i0 = lane; i0 < rows * (HD / 8); i0 += 32 * B) {
+                    uint4 x[B], y[SPLIT ? B : 1];
 #pragma unroll
-                            for (int e = 0; e < 4; ++e) {
-                                hw[e] = PgCvt<CT>::pack(f[2 * e], f[2 * e + 1]);
-                                const float2 b = PgCvt<CT>::unpack(hw[e]);
-                                lw[e] = PgCvt<CT>::pack(f[2 * e] - b.x, f[2 * e + 1] - b.y);
-                            }
-                            hi = make_uint4(hw[0], hw[1], hw[2], hw[3]);
-                            lo = make_uint4(lw[0], lw[1], lw[2], lw[3]);
-                        } else {
-                            hi = *reinterpret_cast<const uint4 *>(src);
+                    for (int e = 0; e < B; ++e) {
+                        const int i = i0 + 32 * e, r = i / (HD / 8), tk = r * inv >> 16;
+                        const QT *p = src + (long long)(tk * A.H + r - tk * A.rep) * HD + (i % (HD / 8)) * 8;
+                        if (r < rows) {
+                            x[e] = *reinterpret_cast<const uint4 *>(p);
+                            if constexpr (SPLIT) y[e] = *reinterpret_cast<const uint4 *>(p + 4);
                         }
                     }
-                    *reinterpret_cast<uint4 *>(&sm.q[qb][0][tile_off<16>(r, pcq)]) = hi;
-                    if constexpr (SPLIT) *reinterpret_cast<uint4 *>(&sm.q[qb][SPLIT ? 1 : 0][tile_off<16>(r, pcq)]) = lo;
+#pragma unroll
+                    for (int e = 0; e < B; ++e) {
+                        const int i = i0 + 32 * e, r = i / (HD / 8);
+                        if (r >= rows) break;
+                        const uint32_t off = tile_off<16>(r, i % (HD / 8));
+                        if constexpr (SPLIT) {
+                            const uint32_t f[8] = {x[e].x, x[e].y, x[e].z, x[e].w, y[e].x, y[e].y, y[e].z, y[e].w};
+                            uint32_t hw[4], lw[4];
+#pragma unroll
+                            for (int k = 0; k < 4; ++k) {
+                                const float f0 = __uint_as_float(f[2 * k]), f1 = __uint_as_float(f[2 * k + 1]);
+                                hw[k] = PgCvt<CT>::pack(f0, f1);
+                                const float2 h = PgCvt<CT>::unpack(hw[k]);
+                                lw[k] = PgCvt<CT>::pack(f0 - h.x, f1 - h.y);
+                            }
+                            *reinterpret_cast<uint4 *>(&sm.q[qb][0][off]) = make_uint4(hw[0], hw[1], hw[2], hw[3]);
+                            *reinterpret_cast<uint4 *>(&sm.q[qb][SPLIT ? 1 : 0][off]) = make_uint4(lw[0], lw[1], lw[2], lw[3]);
+                        } else {
+                            *reinterpret_cast<uint4 *>(&sm.q[qb][0][off]) = x[e];
+                        }
+                    }
                 }
                 __syncwarp();
                 if (lane == 0) arrive(qfull + 8u * qb);
@@ -617,7 +628,7 @@ __global__ void __launch_bounds__(kDecThreads, HD == 256 ? 1 : 2)
             c0 = pg_owner(S, item0);
             c1 = pg_owner(S, item1 - 1);
         }
-        constexpr size_t kPart = 16 * (HD + 2);  // a cut piece in scratch: maxima, sums, then O by row
+        constexpr size_t kPart = 16 * (HD + 2);  // a cut piece in scratch: maxima, sums, then O by row (16-byte places)
         auto slot_of = [&](int cc) { return A.part + kPart * (2 * (size_t)cc + (cc == c0 ? 1 : 0)); };
         float *const part = slot_of(blockIdx.x);
         for (int r0 = 0; ok && r0 < rows; r0 += 4) {
@@ -668,21 +679,35 @@ __global__ void __launch_bounds__(kDecThreads, HD == 256 ? 1 : 2)
             if (!ok) break;
             if (sm.last) {
                 __threadfence();
-                for (int i = tid; i < rows * HD; i += 32 * kDecWarps) {
+                // Four dims of a row per thread; the pieces of a round all in flight.
+                for (int i = 4 * tid; i < rows * HD; i += 4 * 32 * kDecWarps) {
                     const int r = i / HD, d = i - r * HD, tk = r / A.rep;
-                    float M = -INFINITY;
-#pragma unroll 4
-                    for (int cc = c0; cc <= c1; ++cc) M = fmaxf(M, __ldcg(slot_of(cc) + r));
-                    const float Ms = M == -INFINITY ? 0.f : M;
-                    float L = 0.f, acc = 0.f;
-#pragma unroll 4
-                    for (int cc = c0; cc <= c1; ++cc) {
-                        const float *p = slot_of(cc);
-                        const float e = ex2f(__ldcg(p + r) - Ms);
-                        L = fmaf(e, __ldcg(p + 16 + r), L);
-                        acc = fmaf(e, __ldcg(p + 32 + i), acc);
+                    float M = -INFINITY, L = 0.f, acc[4] = {0.f, 0.f, 0.f, 0.f};
+                    for (int cc = c0; cc <= c1; cc += 4) {
+                        float pm[4], pl[4];
+                        float4 po[4];
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            const float *p = slot_of(min(cc + e, c1));
+                            pm[e] = cc + e <= c1 ? __ldcg(p + r) : -INFINITY;
+                            pl[e] = __ldcg(p + 16 + r);
+                            po[e] = __ldcg(reinterpret_cast<const float4 *>(p + 32 + i));
+                        }
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            const float Mn = fmaxf(M, pm[e]), Ms = Mn == -INFINITY ? 0.f : Mn;
+                            const float f = ex2f(M - Ms), w = ex2f(pm[e] - Ms);
+                            M = Mn;
+                            L = fmaf(w, pl[e], L * f);
+                            acc[0] = fmaf(w, po[e].x, acc[0] * f);
+                            acc[1] = fmaf(w, po[e].y, acc[1] * f);
+                            acc[2] = fmaf(w, po[e].z, acc[2] * f);
+                            acc[3] = fmaf(w, po[e].w, acc[3] * f);
+                        }
                     }
-                    put_out<QT>(A, HD, row0 + tk, kh * A.rep + r - tk * A.rep, d, L > 0.f ? __fdiv_rn(acc, L) : 0.f);
+#pragma unroll
+                    for (int e = 0; e < 4; ++e)
+                        put_out<QT>(A, HD, row0 + tk, kh * A.rep + r - tk * A.rep, d + e, L > 0.f ? __fdiv_rn(acc[e], L) : 0.f);
                 }
                 if (tid == 0) A.cnt[c0] = 0u;
             }

@@ -88,15 +88,15 @@ __device__ __forceinline__ PgRange pg_range(const PgAttnArgs &A, const PgSeq &S,
 }
 
 // Division of the work.  The (query tile, kv head, key tile) units of all sequences form one line,
-// query tile major, key tile minor; CTA c of G takes units [c N / G, (c + 1) N / G).  An item is one
-// (query tile, kv head); a CTA's range cuts it into pieces.  An item in one piece is finished by its
-// CTA; the pieces of a cut item go to scratch as (max, sum, unnormalised output) and the CTA that
-// arrives last joins them in the order of the CTAs, so that the result does not depend on timing.
-// Every CTA finds its own range by scanning the sequences' lengths: no launch in front, and nothing of
-// the lengths has to be known on the host.
+// query tile major, key tile minor; G CTAs take N / G units each in order (the first N % G one more).
+// An item is one (query tile, kv head); a CTA's range cuts it into pieces.  An item in one piece is
+// finished by its CTA; the pieces of a cut item go to scratch as (max, sum, unnormalised output) and the
+// CTA that arrives last joins them in the order of the CTAs, so that the result does not depend on
+// timing.  Every CTA finds its own range by scanning the sequences' lengths: no launch in front, and
+// nothing of the lengths has to be known on the host.
 struct PgSched {
-    long long N;               // units in all
-    int G;                     // CTAs that take part
+    long long N, per;          // units in all, and of every CTA
+    int G, rem;                // CTAs that take part; the first rem have one unit more
     long long u0, u1;          // this CTA's units
     int b, t, kh, i;           // its first unit: sequence, query tile, kv head, index among the item's key tiles
 };
@@ -107,6 +107,11 @@ struct PgSchedSmem {
     PgSched S;
     int bad;
 };
+
+// 64-bit quotient by the 32-bit one where it suffices.
+__device__ __forceinline__ long long pg_div(long long a, long long b) {
+    return (a | b) >> 32 ? a / b : (long long)((uint32_t)a / (uint32_t)b);
+}
 
 // Block-wide exclusive sum of v (blockDim a multiple of 32, at most 1024 threads); total in *tot.
 __device__ __forceinline__ long long pg_block_scan(long long v, long long *wsum, long long *tot) {
@@ -147,78 +152,127 @@ __device__ __forceinline__ int pg_find(const int *qpre, int nseq, int q) {
     return lo;
 }
 
-// Every thread of the block: fills sm.S (see PgSched).  min_units: CTAs take part as long as each
-// gets this many units.
+// This CTA's range of N units (min_units: CTAs take part as long as each gets this many).
+__device__ __forceinline__ void pg_share(PgSched &S, long long N, int min_units) {
+    const long long gmax = pg_div(N + min_units - 1, min_units);
+    S.N = N;
+    S.G = (int)(gmax < (long long)gridDim.x ? gmax : (long long)gridDim.x);
+    S.per = S.G ? pg_div(N, S.G) : 0;
+    S.rem = (int)(N - S.per * S.G);
+    const int c = (int)blockIdx.x;
+    S.u0 = c * S.per + min(c, S.rem);
+    S.u1 = c < S.G ? S.u0 + S.per + (c < S.rem ? 1 : 0) : S.u0;
+}
+
+// The CTA that owns unit x.
+__device__ __forceinline__ int pg_owner(const PgSched &S, long long x) {
+    const long long big = (S.per + 1) * S.rem;
+    return (int)(x < big ? pg_div(x, S.per + 1) : S.rem + pg_div(x - big, S.per));
+}
+
+// Units of query tile q, its sequence b and place t there.
+__device__ __forceinline__ long long pg_units(const PgAttnArgs &A, const int *qpre, int q, int &b, int &t, PgRange &R) {
+    bool ignore = false;
+    b = pg_find(qpre, A.nseq, q);
+    t = q - qpre[b];
+    R = pg_range(A, pg_seq(A, b, ignore), t);
+    return (long long)R.cnt * A.Hkv;
+}
+
+__device__ __forceinline__ void pg_first(PgSched &S, long long at, int b, int t, int cnt) {
+    const long long d = S.u0 - at, kh = pg_div(d, cnt);
+    S.b = b;
+    S.t = t;
+    S.kh = (int)kh;
+    S.i = (int)(d - kh * cnt);
+}
+
+// Every thread of the block: fills sm.S (see PgSched).  Up to 32 sequences with up to 32 query tiles (a
+// decode step) are one warp's work; else the block scans.
 __device__ __forceinline__ void pg_schedule(const PgAttnArgs &A, PgSchedSmem &sm, int min_units, uint32_t *err) {
-    const int tid = threadIdx.x, nt = blockDim.x;
-    if (tid == 0) sm.bad = 0;
-    __syncthreads();
-    long long carry = 0;
-    bool bad = false;
-    for (int b0 = 0; b0 < A.nseq; b0 += nt) {
-        const int b = b0 + tid;
-        int q = 0;
-        if (b < A.nseq) {
-            const PgSeq S = pg_seq(A, b, bad);
-            q = (S.n + A.tq - 1) / A.tq;
+    const int tid = threadIdx.x, nt = blockDim.x, lane = tid & 31;
+    if (A.nseq <= 32) {
+        if (tid < 32) {
+            bool bad = false;
+            int q = 0;
+            if (lane < A.nseq) q = (pg_seq(A, lane, bad).n + A.tq - 1) / A.tq;
+            if (__any_sync(0xffffffffu, bad) && lane == 0 && blockIdx.x == 0) atomicOr(err, TRX_DEV_RANGE);
+            int x = q;
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+                const int y = __shfl_up_sync(0xffffffffu, x, o);
+                if (lane >= o) x += y;
+            }
+            sm.qpre[lane + 1] = x;  // beyond nseq: the total again
+            if (lane == 0) sm.qpre[0] = 0;
+            __syncwarp();
+            const int NQ = sm.qpre[32];
+            if (NQ <= 32) {
+                int b = 0, t = 0;
+                PgRange R{};
+                long long u = lane < NQ ? pg_units(A, sm.qpre, lane, b, t, R) : 0, v = u;
+#pragma unroll
+                for (int o = 1; o < 32; o <<= 1) {
+                    const long long y = __shfl_up_sync(0xffffffffu, v, o);
+                    if (lane >= o) v += y;
+                }
+                PgSched S;
+                pg_share(S, __shfl_sync(0xffffffffu, v, 31), min_units);
+                if (lane == 0) sm.S = S;
+                __syncwarp();
+                if (S.u0 < S.u1 && v - u <= S.u0 && S.u0 < v) pg_first(sm.S, v - u, b, t, R.cnt);
+            }
         }
-        long long tot;
-        const long long ex = pg_block_scan(q, sm.wsum, &tot);
-        if (b < A.nseq) sm.qpre[b] = (int)(carry + ex);
-        carry += tot;
+        __syncthreads();
+        if (sm.qpre[32] <= 32) return;
+    } else {
+        if (tid == 0) sm.bad = 0;
+        __syncthreads();
+        long long carry = 0;
+        bool bad = false;
+        for (int b0 = 0; b0 < A.nseq; b0 += nt) {
+            const int b = b0 + tid;
+            int q = 0;
+            if (b < A.nseq) q = (pg_seq(A, b, bad).n + A.tq - 1) / A.tq;
+            long long tot;
+            const long long ex = pg_block_scan(q, sm.wsum, &tot);
+            if (b < A.nseq) sm.qpre[b] = (int)(carry + ex);
+            carry += tot;
+        }
+        if (tid == 0) sm.qpre[A.nseq] = (int)carry;
+        if (bad) sm.bad = 1;
+        __syncthreads();
+        if (tid == 0 && sm.bad && blockIdx.x == 0) atomicOr(err, TRX_DEV_RANGE);
     }
-    if (tid == 0) sm.qpre[A.nseq] = (int)carry;
-    if (bad) sm.bad = 1;
-    __syncthreads();
-    if (tid == 0 && sm.bad && blockIdx.x == 0) atomicOr(err, TRX_DEV_RANGE);
-    const int NQ = (int)carry;
-    // Units of query tile q (times the kv heads), its sequence and place.
-    auto units = [&](int q, int &b, int &t, PgRange &R) {
-        bool ignore = false;
-        b = pg_find(sm.qpre, A.nseq, q);
-        t = q - sm.qpre[b];
-        R = pg_range(A, pg_seq(A, b, ignore), t);
-        return (long long)R.cnt * A.Hkv;
-    };
-    long long N = 0;
+    const int NQ = sm.qpre[A.nseq];
+    int b = 0, t = 0;
+    PgRange R{};
+    long long u = 0, at = 0, N = 0;  // of this thread's query tile in the last round
     for (int q0 = 0; q0 < NQ; q0 += nt) {
-        int b, t;
-        PgRange R;
         long long tot;
-        pg_block_scan(q0 + tid < NQ ? units(q0 + tid, b, t, R) : 0, sm.wsum, &tot);
+        u = q0 + tid < NQ ? pg_units(A, sm.qpre, q0 + tid, b, t, R) : 0;
+        at = N + pg_block_scan(u, sm.wsum, &tot);
         N += tot;
     }
-    const long long gmax = (N + min_units - 1) / min_units;
-    const int G = (int)(gmax < (long long)gridDim.x ? gmax : (long long)gridDim.x);
-    const long long u0 = G ? (long long)blockIdx.x * N / G : 0, u1 = G ? (long long)(blockIdx.x + 1) * N / G : 0;
-    if (tid == 0) {
-        sm.S.N = N;
-        sm.S.G = G;
-        sm.S.u0 = u0;
-        sm.S.u1 = (int)blockIdx.x < G ? u1 : u0;
-    }
-    if ((int)blockIdx.x < G) {
-        long long base = 0;
-        for (int q0 = 0; q0 < NQ && base <= u0; q0 += nt) {
-            int b = 0, t = 0;
-            PgRange R{};
-            long long tot;
-            const long long u = q0 + tid < NQ ? units(q0 + tid, b, t, R) : 0;
-            const long long at = base + pg_block_scan(u, sm.wsum, &tot);
-            if (at <= u0 && u0 < at + u) {
-                sm.S.b = b;
-                sm.S.t = t;
-                sm.S.kh = (int)((u0 - at) / R.cnt);
-                sm.S.i = (int)((u0 - at) % R.cnt);
+    if (tid == 0) pg_share(sm.S, N, min_units);
+    __syncthreads();
+    const long long u0 = sm.S.u0;
+    if (u0 < sm.S.u1) {
+        if (NQ <= nt) {
+            if (at <= u0 && u0 < at + u) pg_first(sm.S, at, b, t, R.cnt);
+        } else {
+            long long base = 0;
+            for (int q0 = 0; q0 < NQ && base <= u0; q0 += nt) {
+                long long tot;
+                u = q0 + tid < NQ ? pg_units(A, sm.qpre, q0 + tid, b, t, R) : 0;
+                at = base + pg_block_scan(u, sm.wsum, &tot);
+                if (at <= u0 && u0 < at + u) pg_first(sm.S, at, b, t, R.cnt);
+                base += tot;
             }
-            base += tot;
         }
     }
     __syncthreads();
 }
-
-// The CTA that owns unit x.
-__device__ __forceinline__ int pg_owner(const PgSched &S, long long x) { return (int)(((x + 1) * S.G - 1) / S.N); }
 
 // A role's walk along its CTA's pieces.
 struct PgWalk {
