@@ -1,16 +1,20 @@
 // Sampling of one token per row of logits (sm_100a): temperature, top-k, top-p and min-p from given
 // random numbers, in one launch.
 //
-// Order: descending by logit, ties by index.  Weights w = exp((x - max) / T), held as integers
-// round(w * 2^S) (S = 62 - ceil(log2 V), at most 50), so that every sum is exact whatever its order:
-// the borders of top-p and of the draw do not move with the division of the work.  The exponent and
-// exp are in 64 bits: with 152k tokens a 32-bit sum is off by more than many tokens' whole share.
+// Order: descending by logit, ties by index.  Weights w = exp((x - max) / T), held as integers of steps
+// 2^-S (S = 62 - ceil(log2 V), at most 50), each within 2^-30 of itself, so that every sum is exact
+// whatever its order: the borders of top-p and of the draw do not move with the division of the work.
+// (32-bit sums will not do: with 152k tokens they are off by more than many tokens' whole share.)
 //
-// A row is held by a cluster of C thread blocks (distributed shared memory joins their parts):
+// A row is held by a cluster of C thread blocks, its logits in their shared memory (a row too long for that
+// is read again in every pass); distributed shared memory joins the blocks' parts:
 //  1. max (and with it the greedy token) and min.
-//  2. top-k / top-p: a histogram over 2048 equal steps of max - x (counts, and weights for top-p).
-//     Equal steps order the tokens like their logits, and spread them better than the bits of a float
-//     would.  Block 0 finds the step in which the k-th token, or the last of the nucleus, lies.
+//  2. top-k / top-p: a histogram over 512 equal steps of max - x.  Equal steps order the tokens like their
+//     logits and spread them better than the bits of a float would.  With a small k it holds counts alone
+//     (top-p then has only the first k to look at); for top-p on the whole row it holds weights too, and
+//     the row's sum is formed.  Weights cost three atomics, so they are tried first over the weights above
+//     e^-10 only: a language model's logits have few of those.  Block 0 finds the step in which the k-th
+//     token, or the last of the nucleus, lies.
 //  3a. Few tokens up to that step (at most kList): they are gathered in block 0, which ranks them, cuts
 //     at k, p and min-p, and draws.
 //  3b. Otherwise the step is narrowed by histograms over the keys' bits until one key is left: the cut
@@ -31,15 +35,17 @@ namespace {
 namespace cg = cooperative_groups;
 using u64 = unsigned long long;
 
-constexpr int kThreadsS = 1024;
+constexpr int kThreadsS = 512;
 constexpr int kWarpsS = kThreadsS / 32;
-constexpr int kBins = 2048;
-constexpr int kList = 2048;
+constexpr int kBins = kThreadsS;  // a thread has one
+constexpr int kList = 1024;
 constexpr int kMaxCluster = 8;
+constexpr size_t kCacheMax = 80 * 1024;  // a block's part of the row: two blocks fit an SM
+constexpr float kNear = 10.f;     // the first histogram covers weights above e^-kNear
 
-// Order-preserving bits of a float (NaN counts as -inf).
+// Order-preserving bits of a float.
 __device__ __forceinline__ uint32_t key_of(float x) {
-    const uint32_t b = __float_as_uint(x != x ? -INFINITY : x);
+    const uint32_t b = __float_as_uint(x);
     return (b & 0x80000000u) ? ~b : (b | 0x80000000u);
 }
 __device__ __forceinline__ float val_of(uint32_t k) {
@@ -55,41 +61,55 @@ template <> __device__ __forceinline__ float load_f<__nv_bfloat16>(const __nv_bf
 }
 
 struct SmemS {
+    uint2 tab[32];                   // 2^(i / 32) in steps of 2^-31: as a whole number, as a float
     uint32_t cnt[kBins];             // this block's histogram
     uint32_t mlo[kBins], mhi[kBins]; // its weights, 64 bits in two words
-    uint32_t tcnt[kBins];            // block 0: the cluster's histogram
+    uint32_t tcnt[kBins];            // the cluster's histogram (every block forms it)
     u64 tmass[kBins];
     u64 list[kList], sorted[kList];  // block 0: gathered tokens (key << 32 | ~index)
     u64 best[kMaxCluster];           // every block's max, for the whole cluster
     uint32_t lo[kMaxCluster], hi[kMaxCluster];
+    u64 sum[kMaxCluster];            // every block's weight
     u64 wmass[kMaxCluster * kWarpsS];
     uint32_t wties[kMaxCluster * kWarpsS];
     u64 red[kWarpsS + 1];
     uint32_t redu[kWarpsS + 1];
-    // Block 0's findings, copied to every block.
-    int bin_k, bin_p, mode;
-    uint32_t key, nlist, found;
-    u64 base_cnt, base_mass, total;
+    int owner;
+    uint32_t nlist, found, got, nall, base;  // nall: block 0, tokens handed over
+    u64 base_cnt, base_mass;
 };
 
-// Weight function of a row.
+// Weight function of a row: round(2^((x - max) k) * 2^S) with k = log2(e) / T, in 32-bit operations only (64-bit
+// floats took three times as long).  t = 32 (x - max) k as a sum of two floats: x - max with its exact
+// rounding error, times k as two floats.  2^(t / 32) = 2^n * 2^(i / 32) * (1 + q), t = 32 n + i + r with |r| <= 1/2:
+// 2^(i / 32) from the table in steps of 2^-31, q = 2^(r / 32) - 1 = y + y^2 / 2 + y^3 / 6 + y^4 / 24 with
+// y = r ln2 / 32 <= 0.011 (the next term is below 2^-39), rounded at 2^-24 of itself: 2^-30 of the weight.
 struct Weigh {
-    float mx;
-    double inv, minp, scale;  // 1 / T, 2^S
+    float mx, kh, kl, lowest;  // 32 k in two floats; t below lowest rounds to 0
+    u64 minw;                  // min_p * 2^S, rounded up
+    int S;
+    const uint2 *tab;
     __device__ __forceinline__ u64 operator()(float x) const {
-        double w;
-        if (x == mx)
-            w = 1.0;
-        else if (x == -INFINITY)
-            w = 0.0;
-        else
-            w = exp(((double)x - (double)mx) * inv);
-        return (u64)__double2ull_rn(w * scale);
+        if (x == mx) return 1ull << S;
+        const float d = x - mx, c = d - x, dl = (x - (d - c)) - (mx + c);
+        const float t = d * kh;
+        if (!(t > lowest)) return 0;  // also x = -inf
+        const float tl = fmaf(d, kh, -t) + fmaf(d, kl, dl * kh);
+        const float magic = 12582912.f, big = t + magic;  // the nearest whole number in its low bits
+        const int n = __float_as_int(big) - __float_as_int(magic);
+        const float r = (t - (big - magic)) + tl;
+        const float y = r * (float)(0.6931471805599453 / 32);
+        const float q = fmaf(y * y, fmaf(y, fmaf(y, 1.f / 24, 1.f / 6), 0.5f), y);
+        const uint2 e = tab[n & 31];
+        const uint32_t m = e.x + (uint32_t)__float2int_rn(q * __uint_as_float(e.y));
+        const int sh = S - 31 + (n >> 5);
+        const u64 w = sh >= 0 ? (u64)m << sh : ((u64)m + (1ull << (-sh - 1))) >> -sh;
+        return w >> S && t != 0.f ? (1ull << S) - 1 : w;
     }
-    __device__ __forceinline__ bool enough(u64 w) const { return (double)w >= minp * scale; }
+    __device__ __forceinline__ bool enough(u64 w) const { return w >= minw; }
 };
 
-// Block-wide inclusive sums of (count, mass); every thread gets its own.
+// Block-wide inclusive sums; every thread gets its own, and the total.
 template <typename T>
 __device__ __forceinline__ T block_incl(T v, T *red, T *tot) {
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
@@ -101,20 +121,26 @@ __device__ __forceinline__ T block_incl(T v, T *red, T *tot) {
     if (lane == 31) red[warp] = v;
     __syncthreads();
     if (warp == 0) {
-        const T w0 = red[lane];
+        const T w0 = lane < kWarpsS ? red[lane] : 0;
         T w = w0;
 #pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
+        for (int o = 1; o < kWarpsS; o <<= 1) {
             const T y = __shfl_up_sync(0xffffffffu, w, o);
             if (lane >= o) w += y;
         }
-        red[lane] = w - w0;
-        if (lane == 31) red[32] = w;
+        if (lane < kWarpsS) red[lane] = w - w0;
+        if (lane == kWarpsS - 1) red[kWarpsS] = w;
     }
     __syncthreads();
     v += red[warp];
-    *tot = red[32];
+    *tot = red[kWarpsS];
     __syncthreads();
+    return v;
+}
+
+__device__ __forceinline__ u64 warp_sum(u64 v) {
+#pragma unroll
+    for (int o = 16; o; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
     return v;
 }
 
@@ -124,8 +150,8 @@ __device__ __forceinline__ void add_mass(SmemS &sm, int b, u64 w) {
     if (hi) atomicAdd(&sm.mhi[b], hi);
 }
 
-template <typename T>
-__global__ void __launch_bounds__(kThreadsS, 1) sample_kernel(SampleArgs A, int S) {
+template <typename T, bool CACHED>
+__global__ void __launch_bounds__(kThreadsS, 2) sample_kernel(SampleArgs A, int S) {
     extern __shared__ __align__(16) unsigned char smem_raw[];
     SmemS &sm = *reinterpret_cast<SmemS *>(smem_raw);
     cg::cluster_group cluster = cg::this_cluster();
@@ -133,194 +159,252 @@ __global__ void __launch_bounds__(kThreadsS, 1) sample_kernel(SampleArgs A, int 
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const int row = blockIdx.x / C, V = A.V;
     pdl_trigger();
+    asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");  // waited for before the first remote store
+    if (tid < 32) {
+        const double v = exp2((double)tid / 32) * 2147483648.0;
+        sm.tab[tid] = make_uint2((uint32_t)(v + 0.5), __float_as_uint((float)v));
+    }
     pdl_wait();
     const T *const x = reinterpret_cast<const T *>(A.x) + row * A.ld;
     const float temp = A.temp[row], u = A.u[row], topp = A.top_p[row];
     const int k = A.top_k[row];
-    // This warp's contiguous part, a multiple of 32 tokens.
+    // This warp's contiguous part, a multiple of 32 tokens; its e-th step of 32.
     const int part = ((V + C * kWarpsS - 1) / (C * kWarpsS) + 31) / 32 * 32;
     const int w0 = min(V, (rank * kWarpsS + warp) * part), w1 = min(V, w0 + part);
-
-    // 1. Max, min.
-    u64 best = 0;
-    uint32_t lo = 0xffffffffu;
-    for (int i = w0 + lane; i < w1; i += 32) {
-        const uint32_t key = key_of(load_f(x + i));
-        const u64 b = ((u64)key << 32) | (0xffffffffu - (uint32_t)i);
-        best = b > best ? b : best;
-        if (key > kKeyNegInf && key < lo) lo = key;
-    }
+    float *const cache = reinterpret_cast<float *>(smem_raw + sizeof(SmemS)) + warp * part - w0;
+    auto fetch = [&](int i) {
+        const float v = load_f(x + i);
+        return v != v ? -INFINITY : v;  // NaN counts as -inf
+    };
+    // 1. Max (the first of equal ones), min.
+    float vmax = -INFINITY, vmin = INFINITY;
+    int imax = 0x7fffffff;
+    for (int i0 = w0 + lane; i0 < w0 + part; i0 += 32 * 20) {  // twenty loads in flight
+        float v[20];
 #pragma unroll
-    for (int o = 16; o; o >>= 1) {
-        const u64 b = __shfl_xor_sync(0xffffffffu, best, o);
-        best = b > best ? b : best;
+        for (int e = 0; e < 20; ++e) v[e] = i0 + 32 * e < w1 ? fetch(i0 + 32 * e) : -INFINITY;
+#pragma unroll
+        for (int e = 0; e < 20; ++e) {
+            const int i = i0 + 32 * e;
+            if (i < w0 + part) {
+                if constexpr (CACHED) cache[i] = v[e];
+                if (v[e] > vmax) {
+                    vmax = v[e];
+                    imax = i;
+                }
+                if (v[e] != -INFINITY) vmin = fminf(vmin, v[e]);
+            }
+        }
     }
-    lo = __reduce_min_sync(0xffffffffu, lo);
-    if (lane == 0) {
-        sm.red[warp] = best;
-        sm.redu[warp] = lo;
-    }
-    cluster.sync();  // every block has started; red complete
-    if (warp == 0) {
-        best = sm.red[lane];
-        lo = __reduce_min_sync(0xffffffffu, sm.redu[lane]);
+    // f(index, logit) for every token of this thread (places behind the row: -inf), in index order by warp; a
+    // thread reads only what it stored.
+    auto each = [&](auto &&f) {
+#pragma unroll 4
+        for (int i = w0 + lane; i < w0 + part; i += 32) {
+            if constexpr (CACHED)
+                f(i, cache[i]);
+            else
+                f(i, i < w1 ? fetch(i) : -INFINITY);
+        }
+    };
+    {
+        u64 best = ((u64)key_of(vmax) << 32) | (0xffffffffu - (uint32_t)imax);
+        uint32_t lo = key_of(vmin);
 #pragma unroll
         for (int o = 16; o; o >>= 1) {
             const u64 b = __shfl_xor_sync(0xffffffffu, best, o);
             best = b > best ? b : best;
         }
-        if (lane < C) {
-            *cluster.map_shared_rank(&sm.best[rank], lane) = best;
-            *cluster.map_shared_rank(&sm.lo[rank], lane) = lo;
+        lo = __reduce_min_sync(0xffffffffu, lo);
+        if (lane == 0) {
+            sm.red[warp] = best;
+            sm.redu[warp] = lo;
+        }
+        asm volatile("barrier.cluster.wait.aligned;" ::: "memory");  // every block has started
+        __syncthreads();
+        if (warp == 0) {
+            best = lane < kWarpsS ? sm.red[lane] : 0;
+            lo = __reduce_min_sync(0xffffffffu, lane < kWarpsS ? sm.redu[lane] : 0xffffffffu);
+#pragma unroll
+            for (int o = 16; o; o >>= 1) {
+                const u64 b = __shfl_xor_sync(0xffffffffu, best, o);
+                best = b > best ? b : best;
+            }
+            if (lane < C) {
+                *cluster.map_shared_rank(&sm.best[rank], lane) = best;
+                *cluster.map_shared_rank(&sm.lo[rank], lane) = lo;
+            }
         }
     }
+    if (tid == 0) sm.got = sm.nall = 0;
     cluster.sync();
-    best = sm.best[0];
-    lo = sm.lo[0];
+    u64 best = sm.best[0];
+    uint32_t klo = sm.lo[0];
     for (int r = 1; r < C; ++r) {
         best = sm.best[r] > best ? sm.best[r] : best;
-        lo = min(lo, sm.lo[r]);
+        klo = min(klo, sm.lo[r]);
     }
     const uint32_t kmax = (uint32_t)(best >> 32);
     const bool none = kmax <= kKeyNegInf, greedy = !(temp > 0.f) || k == 1;
-    Weigh W;
-    W.mx = val_of(kmax);
-    W.inv = 1.0 / (double)temp;
-    W.scale = (double)(1ull << S);
-    W.minp = (double)A.min_p[row];
-    if (none || (greedy && (!(temp > 0.f) || W.minp <= 1.0))) {
+    const float minp = A.min_p[row];
+    if (none || (greedy && (!(temp > 0.f) || minp <= 1.f))) {
         if (rank == 0 && tid == 0) A.tokens[row] = none ? -1 : (int)(0xffffffffu - (uint32_t)best);
         return;
     }
+    Weigh W;
+    W.mx = val_of(kmax);
+    const double k32 = 32 * 1.4426950408889634 / (double)temp;
+    W.kh = (float)k32;
+    W.kl = (float)(k32 - (double)W.kh);
+    W.lowest = -32.f * (float)(S + 2);
+    W.S = S;
+    W.minw = minp <= 0.f ? 0 : (minp <= 1.f ? (u64)ceil((double)minp * (double)(1ull << S)) : ~0ull);
+    W.tab = sm.tab;
     const bool need_k = k > 0 && k < V, need_p = topp < 1.f;
     uint32_t thr = 0;           // kept: keys above thr, and the first `ties` with key thr
     uint32_t ties = 0xffffffffu;
     if (need_k || need_p) {
         // 2. Histogram over max - x.
-        const float span = fminf(36.f * temp, W.mx - val_of(lo));
-        const bool by_temp = span == 36.f * temp;  // then the last step holds only weights that round to 0
-        const float step = span > 0.f && span < INFINITY ? 2047.5f / span : 0.f;
-        auto bin_of = [&](float v) {
+        const float whole_span = W.mx - val_of(klo), rounds_to_0 = 36.f * temp;
+        float step = 0.f, span = 0.f;
+        bool by_weight = need_p && !(need_k && k <= kList);
+        auto bin_of = [&](float v) {  // kBins: beyond the histogram
             const float d = v == W.mx ? 0.f : W.mx - v;
-            return (int)fminf(d * step, (float)(kBins - 1));
+            return (int)fminf(d * step, (float)kBins);
         };
+        bool joined = false;
         auto clear = [&] {
-            for (int i = tid; i < kBins; i += kThreadsS) sm.cnt[i] = sm.mlo[i] = sm.mhi[i] = 0u;
+            if (joined) cluster.sync();  // the other blocks have read the last one
+            joined = false;
+            sm.cnt[tid] = sm.mlo[tid] = sm.mhi[tid] = 0u;
             __syncthreads();
         };
-        // The blocks' histograms into block 0's tcnt, tmass.
+        // The blocks' histograms into tcnt, tmass.
         auto join = [&] {
             cluster.sync();
-            SmemS *const s0 = cluster.map_shared_rank(&sm, 0);
-            for (int i = rank * (kBins / C) + tid; i < (rank + 1) * (kBins / C); i += kThreadsS) {
-                uint32_t n = 0;
-                u64 m = 0;
-                for (int r = 0; r < C; ++r) {
-                    const SmemS *const o = cluster.map_shared_rank(&sm, r);
-                    n += o->cnt[i];
-                    m += ((u64)o->mhi[i] << 32) + o->mlo[i];
-                }
-                s0->tcnt[i] = n;
-                s0->tmass[i] = m;
+            uint32_t n = 0;
+            u64 m = 0;
+            for (int r = 0; r < C; ++r) {
+                const SmemS *const o = cluster.map_shared_rank(&sm, r);
+                n += o->cnt[tid];
+                if (by_weight) m += ((u64)o->mhi[tid] << 32) + o->mlo[tid];
             }
-            cluster.sync();
+            sm.tcnt[tid] = n;
+            sm.tmass[tid] = m;
+            joined = true;
         };
-        // Block 0: the first step whose running count reaches n, or whose running weight reaches
-        // target (by_mass), with the count and weight before it: bin, base_cnt, base_mass.
+        // The first step whose running count reaches n, or whose running weight reaches target
+        // (by_mass), with the count and weight before it (base_cnt, base_mass) and the count up to it (nlist);
+        // kBins: none.  (A thread reads its own tcnt and tmass.)
         auto cross = [&](bool by_mass, u64 n, double target, u64 bc, u64 bm) {
-            u64 tc, tm;
-            const uint32_t c0 = sm.tcnt[2 * tid], c1 = sm.tcnt[2 * tid + 1];
-            const u64 m0 = sm.tmass[2 * tid], m1 = sm.tmass[2 * tid + 1];
-            const u64 ic = bc + block_incl<u64>((u64)c0 + c1, sm.red, &tc);
-            const u64 im = bm + block_incl<u64>(m0 + m1, sm.red, &tm);
-            const u64 ec = ic - c0 - c1, em = im - m0 - m1;
+            u64 tot;
+            const uint32_t c0 = sm.tcnt[tid];
+            const u64 m0 = sm.tmass[tid];
+            const u64 ic = bc + block_incl<u64>(c0, sm.red, &tot);
+            const u64 im = bm + (by_weight ? block_incl<u64>(m0, sm.red, &tot) : 0);
             if (tid == 0) sm.found = kBins;
             __syncthreads();
-            const bool h0 = by_mass ? (double)(em + m0) >= target : ec + c0 >= n;
-            const bool h1 = by_mass ? (double)im >= target : ic >= n;
-            if (h1) atomicMin(&sm.found, (uint32_t)(h0 ? 2 * tid : 2 * tid + 1));
+            if (by_mass ? (double)im >= target : ic >= n) atomicMin(&sm.found, (uint32_t)tid);
             __syncthreads();
-            if (sm.found / 2 == (uint32_t)tid) {
-                const bool second = sm.found & 1;
-                sm.base_cnt = second ? ec + c0 : ec;
-                sm.base_mass = second ? em + m0 : em;
-                sm.nlist = second ? (uint32_t)ic : (uint32_t)(ec + c0);
+            const int f = (int)sm.found;
+            if (f == tid) {
+                sm.base_cnt = ic - c0;
+                sm.base_mass = im - m0;
+                sm.nlist = (uint32_t)ic;
             }
             __syncthreads();
-            return (int)sm.found;
+            return f;
         };
-        clear();
-        for (int i = w0 + lane; i < w1; i += 32) {
-            const float v = val_of(key_of(load_f(x + i)));
-            const int b = bin_of(v);
-            atomicAdd(&sm.cnt[b], 1u);
-            if (need_p) {
-                const u64 w = W(v);
-                if (w) add_mass(sm, b, w);
-            }
-        }
-        join();
-        if (rank == 0) {
-            // mode 0: keep everything (by k and p), 1: gather the steps up to bin_k, 2: narrow.
-            u64 s = 0;
-            if (need_p) {
-                u64 t;
-                block_incl<u64>(sm.tmass[2 * tid] + sm.tmass[2 * tid + 1], sm.red, &t);
-                s = t;
-            }
-            const int bk = need_k ? cross(false, (u64)k, 0.0, 0, 0) : kBins;
-            const bool all_k = !need_k || bk >= kBins || (by_temp && bk == kBins - 1);
-            int bp = kBins;
-            if (all_k && need_p) bp = cross(true, 0, (double)topp * (double)s, 0, 0);
-            const bool all_p = !need_p || (all_k && (bp >= kBins || (by_temp && bp == kBins - 1)));
-            if (tid == 0) {
-                sm.mode = all_k && all_p ? 0 : (sm.nlist <= kList ? 1 : 2);
-                sm.bin_k = all_k ? -1 : bk;
-                sm.bin_p = all_k ? bp : -1;
-                sm.total = s;
-                sm.found = 0;
-            }
-            __syncthreads();
-            if (tid < C && tid) {
-                SmemS *const o = cluster.map_shared_rank(&sm, tid);
-                o->mode = sm.mode;
-                o->bin_k = sm.bin_k;
-                o->bin_p = sm.bin_p;
-                o->total = sm.total;
-            }
-        }
-        cluster.sync();
-        const int mode = sm.mode, bin_k = sm.bin_k, bin_p = sm.bin_p;
-        if (mode == 1) {
-            // 3a. The tokens up to the cut's step, in block 0.
-            SmemS *const s0 = cluster.map_shared_rank(&sm, 0);
-            const int cut = bin_k >= 0 ? bin_k : bin_p;
-            for (int i0 = w0; i0 < w1; i0 += 32) {
-                const int i = i0 + lane;
-                uint32_t key = 0;
-                bool in = false;
-                if (i < w1) {
-                    key = key_of(load_f(x + i));
-                    in = bin_of(val_of(key)) <= cut;
+        auto fill = [&] {
+            clear();
+            each([&](int i, float v) {
+                const int b = bin_of(v);
+                if (b >= kBins) return;
+                atomicAdd(&sm.cnt[b], 1u);
+                if (by_weight) {
+                    const u64 w = W(v);
+                    if (w) add_mass(sm, b, w);
                 }
-                const unsigned bal = __ballot_sync(0xffffffffu, in);
-                if (!bal) continue;
-                uint32_t at = 0;
-                if (lane == 0) at = atomicAdd(&s0->found, (uint32_t)__popc(bal));
-                at = __shfl_sync(0xffffffffu, at, 0) + __popc(bal & ((1u << lane) - 1u));
-                if (in && at < kList) s0->list[at] = ((u64)key << 32) | (0xffffffffu - (uint32_t)i);
+            });
+        };
+        u64 all = 0;  // the weight of the row
+        auto sum_row = [&] {  // complete behind the next join
+            u64 s = 0;
+            each([&](int i, float v) { s += W(v); });
+            s = warp_sum(s);
+            if (lane == 0) sm.red[warp] = s;
+            __syncthreads();
+            if (warp == 0) {
+                s = warp_sum(lane < kWarpsS ? sm.red[lane] : 0);
+                if (lane < C) *cluster.map_shared_rank(&sm.sum[rank], lane) = s;
             }
+        };
+        if (by_weight) sum_row();
+        int mode = 0, bin_k = -1, bin_p = -1;
+        for (int tier = by_weight ? 0 : 1;;) {
+            span = tier ? fminf(rounds_to_0, whole_span) : fminf(kNear * temp, whole_span);
+            const bool last = tier || !(span < fminf(rounds_to_0, whole_span));
+            // The last steps end short of kBins, so that only what rounds to no weight (or an infinity) is beyond.
+            step = span > 0.f && span < INFINITY ? (last ? kBins - 0.5f : (float)kBins) / span : 0.f;
+            fill();
+            join();
+            if (by_weight) {
+                all = 0;
+                for (int r = 0; r < C; ++r) all += sm.sum[r];
+            }
+            // mode 0: keep everything (by k and p), 1: gather the steps up to the cut, 2: narrow, 3: look
+            // further, 4: k keeps everything, look for p with weights.
+            const int bk = need_k ? cross(false, (u64)k, 0.0, 0, 0) : kBins;
+            const bool all_k = !need_k || (last && bk >= kBins);
+            int bp = kBins;
+            if (all_k && need_p && by_weight) bp = cross(true, 0, (double)topp * (double)all, 0, 0);
+            const int cut = all_k ? bp : bk;
+            mode = cut < kBins ? (sm.nlist <= kList ? 1 : 2) : (!last ? 3 : (need_p && !by_weight ? 4 : 0));
+            bin_k = all_k ? -1 : bk;
+            bin_p = all_k ? bp : -1;
+            if (mode < 3) break;
+            tier = 1;
+            if (mode == 4) {
+                by_weight = true;
+                sum_row();
+            }
+        }
+        if (mode == 1) {
+            // 3a. The tokens up to the cut's step: each block collects its own and hands them to block 0.
+            const int cut = bin_k >= 0 ? bin_k : bin_p;
+            u64 *const mine = rank ? sm.list : sm.sorted;
+            each([&](int i, float v) {
+                if (v != -INFINITY && bin_of(v) <= cut) {
+                    const uint32_t at = atomicAdd(&sm.got, 1u);
+                    if (at < kList) mine[at] = ((u64)key_of(v) << 32) | (0xffffffffu - (uint32_t)i);
+                }
+            });
+            __syncthreads();
+            SmemS *const s0 = cluster.map_shared_rank(&sm, 0);
+            const int got = min((int)sm.got, kList);
+            if (tid == 0) sm.base = atomicAdd(&s0->nall, (uint32_t)got);
+            __syncthreads();
+            for (int j = tid; j < got; j += kThreadsS)
+                if (sm.base + j < kList) s0->list[sm.base + j] = mine[j];
             cluster.sync();
             if (rank) return;
-            const int n = min((int)sm.found, kList);
+            const int n = min((int)sm.nall, kList);
+            const int n2 = (n + 1) & ~1;
+            if (tid == 0 && n < n2) sm.list[n] = 0;
+            __syncthreads();
+            const ulonglong2 *const l2 = reinterpret_cast<const ulonglong2 *>(sm.list);
             for (int j = tid; j < n; j += kThreadsS) {
                 const u64 e = sm.list[j];
                 int r = 0;
-                for (int q = 0; q < n; ++q) r += sm.list[q] > e;
+#pragma unroll 4
+                for (int q = 0; q < n2 / 2; ++q) {
+                    const ulonglong2 o = l2[q];
+                    r += (o.x > e) + (o.y > e);
+                }
                 sm.sorted[r] = e;
             }
             __syncthreads();
-            const int nk = need_k && bin_k >= 0 ? min(n, k) : n;
+            const int nk = bin_k >= 0 ? min(n, k) : n;
             // Two consecutive ranks per thread.
             u64 e[2], w[2];
 #pragma unroll
@@ -331,32 +415,35 @@ __global__ void __launch_bounds__(kThreadsS, 1) sample_kernel(SampleArgs A, int 
             }
             u64 sk;
             const u64 inc = block_incl<u64>(w[0] + w[1], sm.red, &sk);
-            const double target = (double)topp * (double)(bin_k >= 0 ? sk : sm.total);
+            const double target = (double)topp * (double)(bin_k >= 0 ? sk : all);
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
-                const u64 before = inc - w[1] - (h ? 0 : w[0]);
-                if ((need_p && !(2 * tid + h == 0) && (double)before >= target) || !W.enough(w[h])) w[h] = 0;
+                const u64 before = inc - (h ? 0 : w[0]) - w[1];
+                if ((need_p && 2 * tid + h && (double)before >= target) || !W.enough(w[h])) e[h] = 0;
             }
+            if (!e[0]) w[0] = 0;
+            if (!e[1]) w[1] = 0;
             u64 tot;
             block_incl<u64>(w[0] + w[1], sm.red, &tot);
             // The draw: the first in index order whose running weight passes u * tot.
             u64 goal = (u64)((double)u * (double)tot);
             goal = tot && goal >= tot ? tot - 1 : goal;
             __syncthreads();
+            // list: pairs of (index, weight); kept ones are a prefix of the order.
 #pragma unroll
             for (int h = 0; h < 2; ++h)
                 if (2 * tid + h < n) {
                     sm.sorted[2 * tid + h] = w[h];
                     sm.list[2 * tid + h] = w[h] ? 0xffffffffu - (uint32_t)e[h] : 0xffffffffffffffffull;
                 }
+            const int kept = __syncthreads_count(w[0] != 0) + __syncthreads_count(w[1] != 0);
             if (tid == 0) sm.found = 0xffffffffu;
             __syncthreads();
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                if (2 * tid + h >= n || !w[h]) continue;
-                const u64 me = sm.list[2 * tid + h];
+            for (int j = tid; j < kept; j += kThreadsS) {
+                const u64 me = sm.list[j];
                 u64 run = 0;
-                for (int q = 0; q < n; ++q) run += sm.list[q] <= me ? sm.sorted[q] : 0;
+#pragma unroll 4
+                for (int q = 0; q < kept; ++q) run += sm.list[q] <= me ? sm.sorted[q] : 0;
                 if (run > goal) atomicMin(&sm.found, (uint32_t)me);
             }
             __syncthreads();
@@ -366,47 +453,34 @@ __global__ void __launch_bounds__(kThreadsS, 1) sample_kernel(SampleArgs A, int 
         if (mode == 2) {
             // 3b. Narrow the step of the cut: first for k, then (with the weight of the first k as the
             // whole) for p.
-            u64 whole = sm.total;
+            u64 whole = all;
+            if (need_p && !by_weight) {
+                by_weight = true;
+                fill();
+                join();
+            }
             for (int pass = 0; pass < 2; ++pass) {
                 const bool by_mass = pass == 1;
                 if (by_mass ? !need_p : bin_k < 0) continue;
                 const double target = (double)topp * (double)whole;
-                u64 bc = 0, bm = 0;  // block 0: counts and weights before the range
                 int b = by_mass ? bin_p : bin_k;
                 if (by_mass && b < 0) {
                     // k was narrowed first: the step of p among the row's steps again.
-                    clear();
-                    for (int i = w0 + lane; i < w1; i += 32) {
-                        const float v = val_of(key_of(load_f(x + i)));
-                        const u64 w = W(v);
-                        const int bb = bin_of(v);
-                        atomicAdd(&sm.cnt[bb], 1u);
-                        if (w) add_mass(sm, bb, w);
-                    }
+                    fill();
                     join();
-                    if (rank == 0) {
-                        const int f = cross(true, 0, target, 0, 0);
-                        if (tid < C) cluster.map_shared_rank(&sm, tid)->bin_p = f;
-                    }
-                    cluster.sync();
-                    b = sm.bin_p;
-                    if (b >= kBins) continue;
                 }
-                if (rank == 0) {
-                    // The step's base, from the row's steps (tcnt and tmass still hold them).
-                    cross(by_mass, (u64)k, target, 0, 0);
-                    bc = sm.base_cnt;
-                    bm = sm.base_mass;
-                }
+                // The step and its base, from the row's steps (tcnt and tmass hold them).
+                b = cross(by_mass, (u64)k, target, 0, 0);
+                if (b >= kBins) continue;
+                u64 bc = sm.base_cnt, bm = sm.base_mass;  // counts and weights before the range
                 // The keys of the step.
                 uint32_t kl = 0xffffffffu, kh = 0;
-                for (int i = w0 + lane; i < w1; i += 32) {
-                    const uint32_t key = key_of(load_f(x + i));
-                    if (bin_of(val_of(key)) == b) {
-                        kl = min(kl, key);
-                        kh = max(kh, key);
+                each([&](int i, float v) {
+                    if (v != -INFINITY && bin_of(v) == b) {
+                        kl = min(kl, key_of(v));
+                        kh = max(kh, key_of(v));
                     }
-                }
+                });
                 kl = __reduce_min_sync(0xffffffffu, kl);
                 kh = __reduce_max_sync(0xffffffffu, kh);
                 __syncthreads();
@@ -416,8 +490,8 @@ __global__ void __launch_bounds__(kThreadsS, 1) sample_kernel(SampleArgs A, int 
                 }
                 __syncthreads();
                 if (warp == 0) {
-                    kl = __reduce_min_sync(0xffffffffu, sm.redu[lane]);
-                    kh = __reduce_max_sync(0xffffffffu, (uint32_t)sm.red[lane]);
+                    kl = __reduce_min_sync(0xffffffffu, lane < kWarpsS ? sm.redu[lane] : 0xffffffffu);
+                    kh = __reduce_max_sync(0xffffffffu, lane < kWarpsS ? (uint32_t)sm.red[lane] : 0u);
                     if (lane < C) {
                         *cluster.map_shared_rank(&sm.lo[rank], lane) = kl;
                         *cluster.map_shared_rank(&sm.hi[rank], lane) = kh;
@@ -434,30 +508,20 @@ __global__ void __launch_bounds__(kThreadsS, 1) sample_kernel(SampleArgs A, int 
                     int shift = 0;
                     while (((kh - kl) >> shift) >= (uint32_t)kBins) ++shift;
                     clear();
-                    for (int i = w0 + lane; i < w1; i += 32) {
-                        const uint32_t key = key_of(load_f(x + i));
-                        if (key < kl || key > kh) continue;
+                    each([&](int i, float v) {
+                        const uint32_t key = key_of(v);
+                        if (key < kl || key > kh) return;
                         const int bb = (int)((kh - key) >> shift);
                         atomicAdd(&sm.cnt[bb], 1u);
                         if (need_p) {
-                            const u64 w = W(val_of(key));
+                            const u64 w = W(v);
                             if (w) add_mass(sm, bb, w);
                         }
-                    }
+                    });
                     join();
-                    if (rank == 0) {
-                        const int f = cross(by_mass, (u64)k, target, bc, bm);
-                        bc = sm.base_cnt;
-                        bm = sm.base_mass;
-                        if (tid < C) {
-                            SmemS *const o = cluster.map_shared_rank(&sm, tid);
-                            o->key = (uint32_t)f;
-                            o->base_cnt = bc;
-                            o->base_mass = bm;
-                        }
-                    }
-                    cluster.sync();
-                    const uint32_t f = sm.key;
+                    const uint32_t f = (uint32_t)cross(by_mass, (u64)k, target, bc, bm);
+                    bc = sm.base_cnt;
+                    bm = sm.base_mass;
                     kh -= f << shift;
                     if (shift == 0) break;
                     const uint32_t width = (1u << shift) - 1u;
@@ -466,13 +530,13 @@ __global__ void __launch_bounds__(kThreadsS, 1) sample_kernel(SampleArgs A, int 
                 const u64 wt = W(val_of(kh));
                 if (!by_mass) {
                     thr = kh;
-                    ties = (uint32_t)((u64)k - sm.base_cnt);
-                    whole = sm.base_mass + (u64)ties * wt;
+                    ties = (uint32_t)((u64)k - bc);
+                    whole = bm + (u64)ties * wt;
                 } else {
                     // Ties before which the running weight is still below the target.
                     uint32_t n = 0xffffffffu;
                     if (wt) {
-                        const double left = target - (double)sm.base_mass;
+                        const double left = target - (double)bm;
                         n = left <= 0.0 ? 1u : (uint32_t)ceil(left / (double)wt);
                         n = n ? n : 1u;
                     }
@@ -483,24 +547,22 @@ __global__ void __launch_bounds__(kThreadsS, 1) sample_kernel(SampleArgs A, int 
                         ties = min(ties, n);
                     }
                 }
-                cluster.sync();  // sm.key, base_* are read before the next pass writes them
             }
         }
     }
     // 4. The draw over the row.
     u64 mass = 0;
     uint32_t nt = 0;
-    for (int i = w0 + lane; i < w1; i += 32) {
-        const uint32_t key = key_of(load_f(x + i));
+    each([&](int i, float v) {
+        const uint32_t key = key_of(v);
         if (key > thr) {
-            const u64 w = W(val_of(key));
+            const u64 w = W(v);
             if (W.enough(w)) mass += w;
-        } else if (key == thr) {
+        } else if (key == thr && v != -INFINITY) {
             ++nt;
         }
-    }
-#pragma unroll
-    for (int o = 16; o; o >>= 1) mass += __shfl_xor_sync(0xffffffffu, mass, o);
+    });
+    mass = warp_sum(mass);
     nt = __reduce_add_sync(0xffffffffu, nt);
     if (lane < C) {
         SmemS *const o = cluster.map_shared_rank(&sm, lane);
@@ -521,29 +583,30 @@ __global__ void __launch_bounds__(kThreadsS, 1) sample_kernel(SampleArgs A, int 
     const u64 im = block_incl<u64>(mine, sm.red, &tot);
     u64 goal = (u64)((double)u * (double)tot);
     goal = tot && goal >= tot ? tot - 1 : goal;
-    if (tid == 0) sm.mode = -1;
+    if (tid == 0) sm.owner = -1;
     __syncthreads();
     if (mine && im > goal && im - mine <= goal) {
-        sm.mode = tid;
+        sm.owner = tid;
         sm.base_mass = im - mine;
         sm.base_cnt = et;
     }
     __syncthreads();
-    const int owner = sm.mode;
+    const int owner = sm.owner;
     if (owner < 0) {
         if (rank == 0 && tid == 0) A.tokens[row] = -1;
         return;
     }
     if (owner / kWarpsS != rank || owner % kWarpsS != warp) return;
     u64 run = sm.base_mass, seen = sm.base_cnt;
-    for (int i0 = w0; i0 < w1; i0 += 32) {
-        const int i = i0 + lane;
-        const uint32_t key = i < w1 ? key_of(load_f(x + i)) : 0u;
-        const bool tie = i < w1 && key == thr;
+    bool done = false;
+    each([&](int i, float v) {
+        if (done) return;
+        const uint32_t key = key_of(v);
+        const bool tie = key == thr && v != -INFINITY;
         const unsigned bal = __ballot_sync(0xffffffffu, tie);
         u64 w = 0;
-        if (i < w1 && key > thr) {
-            w = W(val_of(key));
+        if (key > thr) {
+            w = W(v);
             if (!W.enough(w)) w = 0;
         } else if (tie && seen + __popc(bal & ((1u << lane) - 1u)) < ties) {
             w = wt;
@@ -557,30 +620,26 @@ __global__ void __launch_bounds__(kThreadsS, 1) sample_kernel(SampleArgs A, int 
         const unsigned hit = __ballot_sync(0xffffffffu, run + s > goal);
         if (hit) {
             if (lane == __ffs(hit) - 1) A.tokens[row] = i;
+            done = true;
             return;
         }
         run += __shfl_sync(0xffffffffu, s, 31);
         seen += __popc(bal);
-    }
+    });
 }
 
-template <typename T>
-trx_status launch_t(const SampleArgs &A, cudaStream_t st) {
+template <typename T, bool CACHED>
+cudaError_t launch_e(const SampleArgs &A, int S, int C, size_t cache, cudaStream_t st) {
     static DevBits configured{0};
     cudaError_t e = once_per_device(configured, [] {
-        return cudaFuncSetAttribute(sample_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)sizeof(SmemS));
+        return cudaFuncSetAttribute(sample_kernel<T, CACHED>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                    (int)(sizeof(SmemS) + kCacheMax));
     });
-    if (e != cudaSuccess) return note_cuda(e);
-    int bits = 0;
-    while ((1 << bits) < A.V) ++bits;
-    const int S = 62 - bits < 50 ? 62 - bits : 50;
-    // Blocks per row: a power of two that fills the SMs, none with less than two tokens per thread.
-    int C = 1;
-    while (C < kMaxCluster && (long long)A.nrows * C * 2 <= device_sms() * 2 && A.V > C * 2 * kThreadsS) C *= 2;
+    if (e != cudaSuccess) return e;
     cudaLaunchConfig_t cfg{};
     cfg.gridDim = dim3((unsigned)A.nrows * C);
     cfg.blockDim = dim3(kThreadsS);
-    cfg.dynamicSmemBytes = sizeof(SmemS);
+    cfg.dynamicSmemBytes = sizeof(SmemS) + cache;
     cfg.stream = st;
     cudaLaunchAttribute attr[2];
     attr[0].id = cudaLaunchAttributeClusterDimension;
@@ -591,7 +650,23 @@ trx_status launch_t(const SampleArgs &A, cudaStream_t st) {
     attr[1].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = attr;
     cfg.numAttrs = pdl_enabled() ? 2 : 1;
-    return note_cuda(cudaLaunchKernelEx(&cfg, sample_kernel<T>, A, S));
+    return cudaLaunchKernelEx(&cfg, sample_kernel<T, CACHED>, A, S);
+}
+
+template <typename T>
+trx_status launch_t(const SampleArgs &A, cudaStream_t st) {
+    int bits = 0;
+    while ((1 << bits) < A.V) ++bits;
+    const int S = 62 - bits < 50 ? 62 - bits : 50;
+    // Blocks per row: a power of two that fills the SMs (two blocks each), none with less than two tokens per
+    // thread; more for a row that would not fit the blocks' shared memory otherwise.
+    auto bytes = [&](int C) {  // of a block's part of the row
+        return (size_t)((A.V + C * kWarpsS - 1) / (C * kWarpsS) + 31) / 32 * 32 * kWarpsS * 4;
+    };
+    int C = 1;
+    while (C < kMaxCluster && A.V > C * 2 * kThreadsS && ((long long)A.nrows * C < device_sms() || bytes(C) > kCacheMax))
+        C *= 2;
+    return note_cuda(bytes(C) <= kCacheMax ? launch_e<T, true>(A, S, C, bytes(C), st) : launch_e<T, false>(A, S, C, 0, st));
 }
 
 }  // namespace
