@@ -9,17 +9,17 @@
 // A row is held by a cluster of C thread blocks, its logits in their shared memory (a row too long for that
 // is read again in every pass); distributed shared memory joins the blocks' parts:
 //  1. max (and with it the greedy token) and min.
-//  2. top-k / top-p: a histogram over 512 equal steps of max - x.  Equal steps order the tokens like their
-//     logits and spread them better than the bits of a float would.  With a small k it holds counts alone
-//     (top-p then has only the first k to look at); for top-p on the whole row it holds weights too, and
-//     the row's sum is formed.  Weights cost three atomics, so they are tried first over the weights above
-//     e^-10 only: a language model's logits have few of those.  Block 0 finds the step in which the k-th
-//     token, or the last of the nucleus, lies.
-//  3a. Few tokens up to that step (at most kList): they are gathered in block 0, which ranks them, cuts
-//     at k, p and min-p, and draws.
-//  3b. Otherwise the step is narrowed by histograms over the keys' bits until one key is left: the cut
-//     is that key and how many of its ties (in index order) are kept.
-//  4. (3b, or no top-k and top-p) The draw over the whole row: each warp sums its contiguous part, the
+//  2. top-k / top-p: counts over 512 equal steps of max - x, down to where weights round to 0.  Equal steps
+//     order the tokens like their logits and spread them better than the bits of a float would.
+//  3. top-k: the step with the k-th token follows from the counts.  If few tokens lie up to it (at most
+//     kList), block 0 takes them over, ranks them, cuts at k, p and min-p, and draws.  Otherwise the step
+//     is narrowed by histograms over the keys' bits until one key is left: the cut is that key and how many of
+//     its ties (in index order) are kept.
+//     top-p over more than that: the steps' counts and mean places tell, to a fraction of a step, where the
+//     nucleus ends; one pass then sums exactly the weights of the row, above that step and in it, and
+//     collects the step's tokens, which block 0 ranks (or the step is narrowed, if they are too many).  Should
+//     the end lie in a neighbouring step after all, the pass is repeated there.
+//  4. Unless block 0 has drawn: the draw over the whole row: each warp sums its contiguous part, the
 //     parts' prefix tells which warp holds the token, and that warp scans its part again.
 #include <cstdint>
 #include <cooperative_groups.h>
@@ -41,7 +41,6 @@ constexpr int kBins = kThreadsS;  // a thread has one
 constexpr int kList = 1024;
 constexpr int kMaxCluster = 8;
 constexpr size_t kCacheMax = 80 * 1024;  // a block's part of the row: two blocks fit an SM
-constexpr float kNear = 10.f;     // the first histogram covers weights above e^-kNear
 
 // Order-preserving bits of a float.
 __device__ __forceinline__ uint32_t key_of(float x) {
@@ -63,20 +62,23 @@ template <> __device__ __forceinline__ float load_f<__nv_bfloat16>(const __nv_bf
 struct SmemS {
     uint2 tab[32];                   // 2^(i / 32) in steps of 2^-31: as a whole number, as a float
     uint32_t cnt[kBins];             // this block's histogram
-    uint32_t mlo[kBins], mhi[kBins]; // its weights, 64 bits in two words
+    uint32_t mlo[kBins], mhi[kBins]; // its weights, 64 bits in two words; in step 2 mlo: the places within a step
     uint32_t tcnt[kBins];            // the cluster's histogram (every block forms it)
     u64 tmass[kBins];
     u64 list[kList], sorted[kList];  // block 0: gathered tokens (key << 32 | ~index)
     u64 best[kMaxCluster];           // every block's max, for the whole cluster
     uint32_t lo[kMaxCluster], hi[kMaxCluster];
-    u64 sum[kMaxCluster];            // every block's weight
+    u64 sum[kMaxCluster][3];         // every block's weight: the row's, above a step, in it
     u64 wmass[kMaxCluster * kWarpsS];
     uint32_t wties[kMaxCluster * kWarpsS];
-    u64 red[kWarpsS + 1];
+    u64 red[kWarpsS + 1], part[kWarpsS][3];
+    double redd[kWarpsS + 1];
     uint32_t redu[kWarpsS + 1];
     int owner;
     uint32_t nlist, found, got, nall, base;  // nall: block 0, tokens handed over
     u64 base_cnt, base_mass;
+    double est[kBins + 1];           // estimated running weight before a step
+    uint32_t cut_key, cut_ties;
 };
 
 // Weight function of a row: round(2^((x - max) k) * 2^S) with k = log2(e) / T, in 32-bit operations only (64-bit
@@ -102,9 +104,7 @@ struct Weigh {
         const float q = fmaf(y * y, fmaf(y, fmaf(y, 1.f / 24, 1.f / 6), 0.5f), y);
         const uint2 e = tab[n & 31];
         const uint32_t m = e.x + (uint32_t)__float2int_rn(q * __uint_as_float(e.y));
-        const int sh = S - 31 + (n >> 5);
-        const u64 w = sh >= 0 ? (u64)m << sh : ((u64)m + (1ull << (-sh - 1))) >> -sh;
-        return w >> S && t != 0.f ? (1ull << S) - 1 : w;
+        return ((u64)m << 31) >> (62 - S - (n >> 5));
     }
     __device__ __forceinline__ bool enough(u64 w) const { return w >= minw; }
 };
@@ -245,7 +245,7 @@ __global__ void __launch_bounds__(kThreadsS, 2) sample_kernel(SampleArgs A, int 
         klo = min(klo, sm.lo[r]);
     }
     const uint32_t kmax = (uint32_t)(best >> 32);
-    const bool none = kmax <= kKeyNegInf, greedy = !(temp > 0.f) || k == 1;
+    const bool none = kmax <= kKeyNegInf, greedy = !(temp > 0.f) || k == 1 || topp <= 0.f;
     const float minp = A.min_p[row];
     if (none || (greedy && (!(temp > 0.f) || minp <= 1.f))) {
         if (rank == 0 && tid == 0) A.tokens[row] = none ? -1 : (int)(0xffffffffu - (uint32_t)best);
@@ -256,7 +256,7 @@ __global__ void __launch_bounds__(kThreadsS, 2) sample_kernel(SampleArgs A, int 
     const double k32 = 32 * 1.4426950408889634 / (double)temp;
     W.kh = (float)k32;
     W.kl = (float)(k32 - (double)W.kh);
-    W.lowest = -32.f * (float)(S + 2);
+    W.lowest = -32.f * (float)S;  // shifts stay below 64
     W.S = S;
     W.minw = minp <= 0.f ? 0 : (minp <= 1.f ? (u64)ceil((double)minp * (double)(1ull << S)) : ~0ull);
     W.tab = sm.tab;
@@ -264,14 +264,15 @@ __global__ void __launch_bounds__(kThreadsS, 2) sample_kernel(SampleArgs A, int 
     uint32_t thr = 0;           // kept: keys above thr, and the first `ties` with key thr
     uint32_t ties = 0xffffffffu;
     if (need_k || need_p) {
-        // 2. Histogram over max - x.
-        const float whole_span = W.mx - val_of(klo), rounds_to_0 = 36.f * temp;
-        float step = 0.f, span = 0.f;
-        bool by_weight = need_p && !(need_k && k <= kList);
-        auto bin_of = [&](float v) {  // kBins: beyond the histogram
+        // 2. Counts over max - x.
+        const float span = fminf(36.f * temp, W.mx - val_of(klo));
+        // The last step ends short of kBins, so that only what rounds to no weight (or an infinity) is beyond.
+        const float step = span > 0.f && span < INFINITY ? (kBins - 0.5f) / span : 0.f;
+        auto place = [&](float v) {  // in steps; kBins: beyond
             const float d = v == W.mx ? 0.f : W.mx - v;
-            return (int)fminf(d * step, (float)kBins);
+            return fminf(d * step, (float)kBins);
         };
+        auto bin_of = [&](float v) { return (int)place(v); };
         bool joined = false;
         auto clear = [&] {
             if (joined) cluster.sync();  // the other blocks have read the last one
@@ -287,7 +288,7 @@ __global__ void __launch_bounds__(kThreadsS, 2) sample_kernel(SampleArgs A, int 
             for (int r = 0; r < C; ++r) {
                 const SmemS *const o = cluster.map_shared_rank(&sm, r);
                 n += o->cnt[tid];
-                if (by_weight) m += ((u64)o->mhi[tid] << 32) + o->mlo[tid];
+                if (need_p) m += ((u64)o->mhi[tid] << 32) + o->mlo[tid];
             }
             sm.tcnt[tid] = n;
             sm.tmass[tid] = m;
@@ -298,83 +299,29 @@ __global__ void __launch_bounds__(kThreadsS, 2) sample_kernel(SampleArgs A, int 
         // kBins: none.  (A thread reads its own tcnt and tmass.)
         auto cross = [&](bool by_mass, u64 n, double target, u64 bc, u64 bm) {
             u64 tot;
-            const uint32_t c0 = sm.tcnt[tid];
-            const u64 m0 = sm.tmass[tid];
-            const u64 ic = bc + block_incl<u64>(c0, sm.red, &tot);
-            const u64 im = bm + (by_weight ? block_incl<u64>(m0, sm.red, &tot) : 0);
+            const u64 own = by_mass ? sm.tmass[tid] : sm.tcnt[tid], base = by_mass ? bm : bc;
+            const u64 inc = base + block_incl<u64>(own, sm.red, &tot);
             if (tid == 0) sm.found = kBins;
             __syncthreads();
-            if (by_mass ? (double)im >= target : ic >= n) atomicMin(&sm.found, (uint32_t)tid);
+            if (by_mass ? (double)inc >= target : inc >= n) atomicMin(&sm.found, (uint32_t)tid);
             __syncthreads();
             const int f = (int)sm.found;
             if (f == tid) {
-                sm.base_cnt = ic - c0;
-                sm.base_mass = im - m0;
-                sm.nlist = (uint32_t)ic;
+                sm.base_cnt = by_mass ? 0 : inc - own;
+                sm.base_mass = by_mass ? inc - own : 0;
+                sm.nlist = (uint32_t)inc;
             }
             __syncthreads();
             return f;
         };
-        auto fill = [&] {
-            clear();
-            each([&](int i, float v) {
-                const int b = bin_of(v);
-                if (b >= kBins) return;
-                atomicAdd(&sm.cnt[b], 1u);
-                if (by_weight) {
-                    const u64 w = W(v);
-                    if (w) add_mass(sm, b, w);
-                }
-            });
-        };
-        u64 all = 0;  // the weight of the row
-        auto sum_row = [&] {  // complete behind the next join
-            u64 s = 0;
-            each([&](int i, float v) { s += W(v); });
-            s = warp_sum(s);
-            if (lane == 0) sm.red[warp] = s;
-            __syncthreads();
-            if (warp == 0) {
-                s = warp_sum(lane < kWarpsS ? sm.red[lane] : 0);
-                if (lane < C) *cluster.map_shared_rank(&sm.sum[rank], lane) = s;
-            }
-        };
-        if (by_weight) sum_row();
-        int mode = 0, bin_k = -1, bin_p = -1;
-        for (int tier = by_weight ? 0 : 1;;) {
-            span = tier ? fminf(rounds_to_0, whole_span) : fminf(kNear * temp, whole_span);
-            const bool last = tier || !(span < fminf(rounds_to_0, whole_span));
-            // The last steps end short of kBins, so that only what rounds to no weight (or an infinity) is beyond.
-            step = span > 0.f && span < INFINITY ? (last ? kBins - 0.5f : (float)kBins) / span : 0.f;
-            fill();
-            join();
-            if (by_weight) {
-                all = 0;
-                for (int r = 0; r < C; ++r) all += sm.sum[r];
-            }
-            // mode 0: keep everything (by k and p), 1: gather the steps up to the cut, 2: narrow, 3: look
-            // further, 4: k keeps everything, look for p with weights.
-            const int bk = need_k ? cross(false, (u64)k, 0.0, 0, 0) : kBins;
-            const bool all_k = !need_k || (last && bk >= kBins);
-            int bp = kBins;
-            if (all_k && need_p && by_weight) bp = cross(true, 0, (double)topp * (double)all, 0, 0);
-            const int cut = all_k ? bp : bk;
-            mode = cut < kBins ? (sm.nlist <= kList ? 1 : 2) : (!last ? 3 : (need_p && !by_weight ? 4 : 0));
-            bin_k = all_k ? -1 : bk;
-            bin_p = all_k ? bp : -1;
-            if (mode < 3) break;
-            tier = 1;
-            if (mode == 4) {
-                by_weight = true;
-                sum_row();
-            }
-        }
-        if (mode == 1) {
-            // 3a. The tokens up to the cut's step: each block collects its own and hands them to block 0.
-            const int cut = bin_k >= 0 ? bin_k : bin_p;
+        // This block's tokens of the row for which in(logit) holds into block 0's list (at most kList in all;
+        // nall counts them all).
+        auto collect = [&](auto &&in) {
             u64 *const mine = rank ? sm.list : sm.sorted;
+            if (tid == 0) sm.got = 0;
+            __syncthreads();
             each([&](int i, float v) {
-                if (v != -INFINITY && bin_of(v) <= cut) {
+                if (in(v)) {
                     const uint32_t at = atomicAdd(&sm.got, 1u);
                     if (at < kList) mine[at] = ((u64)key_of(v) << 32) | (0xffffffffu - (uint32_t)i);
                 }
@@ -382,14 +329,14 @@ __global__ void __launch_bounds__(kThreadsS, 2) sample_kernel(SampleArgs A, int 
             __syncthreads();
             SmemS *const s0 = cluster.map_shared_rank(&sm, 0);
             const int got = min((int)sm.got, kList);
-            if (tid == 0) sm.base = atomicAdd(&s0->nall, (uint32_t)got);
+            if (tid == 0) sm.base = atomicAdd(&s0->nall, sm.got);
             __syncthreads();
             for (int j = tid; j < got; j += kThreadsS)
                 if (sm.base + j < kList) s0->list[sm.base + j] = mine[j];
-            cluster.sync();
-            if (rank) return;
-            const int n = min((int)sm.nall, kList);
-            const int n2 = (n + 1) & ~1;
+        };
+        // Block 0: its list in order into sorted; returns the number.
+        auto rank_list = [&] {
+            const int n = min((int)sm.nall, kList), n2 = (n + 1) & ~1;
             if (tid == 0 && n < n2) sm.list[n] = 0;
             __syncthreads();
             const ulonglong2 *const l2 = reinterpret_cast<const ulonglong2 *>(sm.list);
@@ -404,7 +351,84 @@ __global__ void __launch_bounds__(kThreadsS, 2) sample_kernel(SampleArgs A, int 
                 sm.sorted[r] = e;
             }
             __syncthreads();
-            const int nk = bin_k >= 0 ? min(n, k) : n;
+            return n;
+        };
+        // The key in which step b is cut: by histograms over the bits of its keys.  bc, bm: counts and
+        // weights before the step, on return before that key.
+        auto narrow = [&](int b, bool by_mass, double target, u64 &bc, u64 &bm) {
+            uint32_t kl = 0xffffffffu, kh = 0;
+            each([&](int i, float v) {
+                if (v != -INFINITY && bin_of(v) == b) {
+                    kl = min(kl, key_of(v));
+                    kh = max(kh, key_of(v));
+                }
+            });
+            kl = __reduce_min_sync(0xffffffffu, kl);
+            kh = __reduce_max_sync(0xffffffffu, kh);
+            __syncthreads();
+            if (lane == 0) {
+                sm.redu[warp] = kl;
+                sm.red[warp] = kh;
+            }
+            __syncthreads();
+            if (warp == 0) {
+                kl = __reduce_min_sync(0xffffffffu, lane < kWarpsS ? sm.redu[lane] : 0xffffffffu);
+                kh = __reduce_max_sync(0xffffffffu, lane < kWarpsS ? (uint32_t)sm.red[lane] : 0u);
+                if (lane < C) {
+                    *cluster.map_shared_rank(&sm.lo[rank], lane) = kl;
+                    *cluster.map_shared_rank(&sm.hi[rank], lane) = kh;
+                }
+            }
+            cluster.sync();
+            joined = false;  // behind a barrier: the last histogram has been read
+            kl = sm.lo[0];
+            kh = sm.hi[0];
+            for (int r = 1; r < C; ++r) {
+                kl = min(kl, sm.lo[r]);
+                kh = max(kh, sm.hi[r]);
+            }
+            for (;;) {
+                int shift = 0;
+                while (((kh - kl) >> shift) >= (uint32_t)kBins) ++shift;
+                clear();
+                each([&](int i, float v) {
+                    const uint32_t key = key_of(v);
+                    if (key < kl || key > kh) return;
+                    const int bb = (int)((kh - key) >> shift);
+                    atomicAdd(&sm.cnt[bb], 1u);
+                    if (by_mass) {
+                        const u64 w = W(v);
+                        if (w) add_mass(sm, bb, w);
+                    }
+                });
+                join();
+                const uint32_t f = (uint32_t)cross(by_mass, (u64)k, target, bc, bm);
+                bc = sm.base_cnt;
+                bm = sm.base_mass;
+                kh -= f << shift;
+                if (shift == 0) return kh;
+                const uint32_t width = (1u << shift) - 1u;
+                if (kh - kl > width) kl = kh - width;
+            }
+        };
+
+        clear();
+        each([&](int i, float v) {
+            const float at = place(v);
+            const int b = (int)at;
+            if (b >= kBins) return;
+            atomicAdd(&sm.cnt[b], 1u);
+            if (need_p) atomicAdd(&sm.mlo[b], (uint32_t)((at - (float)b) * 4096.f));
+        });
+        join();
+        int bin_k = kBins;
+        if (need_k) bin_k = cross(false, (u64)k, 0.0, 0, 0);
+        if (bin_k < kBins && sm.nlist <= kList) {
+            // 3. The first k are among few tokens: block 0 finishes the row.
+            collect([&](float v) { return v != -INFINITY && bin_of(v) <= bin_k; });
+            cluster.sync();
+            if (rank) return;
+            const int n = rank_list(), nk = min(n, k);
             // Two consecutive ranks per thread.
             u64 e[2], w[2];
 #pragma unroll
@@ -415,7 +439,7 @@ __global__ void __launch_bounds__(kThreadsS, 2) sample_kernel(SampleArgs A, int 
             }
             u64 sk;
             const u64 inc = block_incl<u64>(w[0] + w[1], sm.red, &sk);
-            const double target = (double)topp * (double)(bin_k >= 0 ? sk : all);
+            const double target = (double)topp * (double)sk;
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
                 const u64 before = inc - (h ? 0 : w[0]) - w[1];
@@ -429,7 +453,7 @@ __global__ void __launch_bounds__(kThreadsS, 2) sample_kernel(SampleArgs A, int 
             u64 goal = (u64)((double)u * (double)tot);
             goal = tot && goal >= tot ? tot - 1 : goal;
             __syncthreads();
-            // list: pairs of (index, weight); kept ones are a prefix of the order.
+            // list: indices, sorted: weights; kept ones are a prefix of the order.
 #pragma unroll
             for (int h = 0; h < 2; ++h)
                 if (2 * tid + h < n) {
@@ -450,103 +474,138 @@ __global__ void __launch_bounds__(kThreadsS, 2) sample_kernel(SampleArgs A, int 
             if (tid == 0) A.tokens[row] = (int)sm.found;
             return;
         }
-        if (mode == 2) {
-            // 3b. Narrow the step of the cut: first for k, then (with the weight of the first k as the
-            // whole) for p.
-            u64 whole = all;
-            if (need_p && !by_weight) {
-                by_weight = true;
-                fill();
-                join();
+        // The estimate of top-p, from the same counts (before a narrowing replaces them): the running weight
+        // before every step, a step's weight as its count at its mean place.
+        double est_all = 0.0;
+        int guess = kBins;
+        if (need_p) {
+            const uint32_t n = sm.tcnt[tid];
+            const double at = n ? tid + (double)sm.tmass[tid] / (4096.0 * n) : 0.0;
+            const double est = n ? n * (step > 0.f ? exp(-at / ((double)step * (double)temp)) : 1.0) : 0.0;
+            double tot;
+            const double inc = block_incl<double>(est, sm.redd, &tot);
+            sm.est[tid + 1] = inc;
+            if (tid == 0) sm.est[0] = 0.0;
+            __syncthreads();
+            est_all = tot;
+            if (bin_k < kBins) {  // the first k only: a part of step bin_k
+                const double part = (double)(k - (long long)sm.base_cnt) / (double)sm.tcnt[bin_k];
+                est_all = sm.est[bin_k] + part * (sm.est[bin_k + 1] - sm.est[bin_k]);
             }
-            for (int pass = 0; pass < 2; ++pass) {
-                const bool by_mass = pass == 1;
-                if (by_mass ? !need_p : bin_k < 0) continue;
-                const double target = (double)topp * (double)whole;
-                int b = by_mass ? bin_p : bin_k;
-                if (by_mass && b < 0) {
-                    // k was narrowed first: the step of p among the row's steps again.
-                    fill();
-                    join();
-                }
-                // The step and its base, from the row's steps (tcnt and tmass hold them).
-                b = cross(by_mass, (u64)k, target, 0, 0);
-                if (b >= kBins) continue;
-                u64 bc = sm.base_cnt, bm = sm.base_mass;  // counts and weights before the range
-                // The keys of the step.
-                uint32_t kl = 0xffffffffu, kh = 0;
+            if (tid == 0) sm.found = kBins - 1;
+            __syncthreads();
+            if (inc >= (double)topp * est_all) atomicMin(&sm.found, (uint32_t)tid);
+            __syncthreads();
+            guess = (int)sm.found;
+            __syncthreads();
+        }
+        if (bin_k < kBins) {
+            u64 bc = sm.base_cnt, bm = 0;
+            thr = narrow(bin_k, false, 0.0, bc, bm);
+            ties = (uint32_t)((u64)k - bc);
+        }
+        if (need_p) {
+            const u64 wk = thr ? (u64)ties * W(val_of(thr)) : 0;  // of the ties at the k-th token's key
+            u64 all, above, in;
+            double target;
+            for (int tries = 0;; ++tries) {
+                // Exactly: the weight kept by k, above the step, in the step; and the step's tokens.
+                u64 sa = 0, sb = 0, sc = 0;
                 each([&](int i, float v) {
-                    if (v != -INFINITY && bin_of(v) == b) {
-                        kl = min(kl, key_of(v));
-                        kh = max(kh, key_of(v));
+                    const int b = bin_of(v);
+                    if (key_of(v) > thr || b == guess) {
+                        const u64 w = W(v);
+                        if (key_of(v) > thr) sa += w;
+                        if (b < guess) sb += w;
+                        if (b == guess) sc += w;
                     }
                 });
-                kl = __reduce_min_sync(0xffffffffu, kl);
-                kh = __reduce_max_sync(0xffffffffu, kh);
+                sa = warp_sum(sa);
+                sb = warp_sum(sb);
+                sc = warp_sum(sc);
                 __syncthreads();
                 if (lane == 0) {
-                    sm.redu[warp] = kl;
-                    sm.red[warp] = kh;
+                    sm.part[warp][0] = sa;
+                    sm.part[warp][1] = sb;
+                    sm.part[warp][2] = sc;
                 }
                 __syncthreads();
                 if (warp == 0) {
-                    kl = __reduce_min_sync(0xffffffffu, lane < kWarpsS ? sm.redu[lane] : 0xffffffffu);
-                    kh = __reduce_max_sync(0xffffffffu, lane < kWarpsS ? (uint32_t)sm.red[lane] : 0u);
-                    if (lane < C) {
-                        *cluster.map_shared_rank(&sm.lo[rank], lane) = kl;
-                        *cluster.map_shared_rank(&sm.hi[rank], lane) = kh;
+                    for (int q = 0; q < 3; ++q) {
+                        const u64 v = warp_sum(lane < kWarpsS ? sm.part[lane][q] : 0);
+                        if (lane < C) *cluster.map_shared_rank(&sm.sum[rank][q], lane) = v;
+                    }
+                }
+                collect([&](float v) { return v != -INFINITY && bin_of(v) == guess; });
+                cluster.sync();
+                joined = false;
+                all = wk;
+                above = in = 0;
+                for (int r = 0; r < C; ++r) {
+                    all += sm.sum[r][0];
+                    above += sm.sum[r][1];
+                    in += sm.sum[r][2];
+                }
+                target = (double)topp * (double)all;
+                int next = guess;
+                if (guess && (double)above >= target) --next;
+                else if (guess < kBins - 1 && (double)(above + in) < target) ++next;
+                if (next == guess || tries >= 2 * kBins) break;
+                guess = next;
+                cluster.sync();  // the sums have been read
+                if (tid == 0) sm.nall = 0;
+                cluster.sync();
+            }
+            uint32_t key, nties;
+            if (*cluster.map_shared_rank(&sm.nall, 0) <= kList) {
+                if (rank == 0) {
+                    const int n = rank_list();
+                    u64 e[2], w[2];
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) {
+                        const int r = 2 * tid + h;
+                        e[h] = r < n ? sm.sorted[r] : 0;
+                        w[h] = r < n ? W(val_of((uint32_t)(e[h] >> 32))) : 0;
+                    }
+                    u64 tot;
+                    const u64 inc = above + block_incl<u64>(w[0] + w[1], sm.red, &tot);
+                    if (tid == 0) sm.found = sm.nlist = 0;
+                    __syncthreads();
+                    // The last rank before which the running weight is below the target.
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) {
+                        const u64 before = inc - (h ? 0 : w[0]) - w[1];
+                        if (e[h] && (double)before < target) atomicMax(&sm.found, (uint32_t)(2 * tid + h));
+                    }
+                    __syncthreads();
+                    const uint32_t last = sm.found, lk = (uint32_t)(sm.sorted[last] >> 32);
+#pragma unroll
+                    for (int h = 0; h < 2; ++h)
+                        if (2 * tid + h <= (int)last && (uint32_t)(e[h] >> 32) == lk) atomicAdd(&sm.nlist, 1u);
+                    __syncthreads();
+                    if (tid < C) {
+                        SmemS *const o = cluster.map_shared_rank(&sm, tid);
+                        o->cut_key = lk;
+                        o->cut_ties = sm.nlist;
                     }
                 }
                 cluster.sync();
-                kl = sm.lo[0];
-                kh = sm.hi[0];
-                for (int r = 1; r < C; ++r) {
-                    kl = min(kl, sm.lo[r]);
-                    kh = max(kh, sm.hi[r]);
-                }
-                for (;;) {
-                    int shift = 0;
-                    while (((kh - kl) >> shift) >= (uint32_t)kBins) ++shift;
-                    clear();
-                    each([&](int i, float v) {
-                        const uint32_t key = key_of(v);
-                        if (key < kl || key > kh) return;
-                        const int bb = (int)((kh - key) >> shift);
-                        atomicAdd(&sm.cnt[bb], 1u);
-                        if (need_p) {
-                            const u64 w = W(v);
-                            if (w) add_mass(sm, bb, w);
-                        }
-                    });
-                    join();
-                    const uint32_t f = (uint32_t)cross(by_mass, (u64)k, target, bc, bm);
-                    bc = sm.base_cnt;
-                    bm = sm.base_mass;
-                    kh -= f << shift;
-                    if (shift == 0) break;
-                    const uint32_t width = (1u << shift) - 1u;
-                    if (kh - kl > width) kl = kh - width;
-                }
-                const u64 wt = W(val_of(kh));
-                if (!by_mass) {
-                    thr = kh;
-                    ties = (uint32_t)((u64)k - bc);
-                    whole = bm + (u64)ties * wt;
-                } else {
-                    // Ties before which the running weight is still below the target.
-                    uint32_t n = 0xffffffffu;
-                    if (wt) {
-                        const double left = target - (double)bm;
-                        n = left <= 0.0 ? 1u : (uint32_t)ceil(left / (double)wt);
-                        n = n ? n : 1u;
-                    }
-                    if (kh > thr) {
-                        thr = kh;
-                        ties = n;
-                    } else if (kh == thr) {
-                        ties = min(ties, n);
-                    }
-                }
+                key = sm.cut_key;
+                nties = sm.cut_ties;
+            } else {
+                u64 bc = 0, bm = above;
+                key = narrow(guess, true, target, bc, bm);
+                // Ties before which the running weight is still below the target.
+                const u64 wt = W(val_of(key));
+                const double left = target - (double)bm;
+                nties = wt ? (left <= 0.0 ? 1u : (uint32_t)fmin(ceil(left / (double)wt), 4294967295.0)) : 0xffffffffu;
+                nties = nties ? nties : 1u;
+            }
+            if (key > thr) {
+                thr = key;
+                ties = nties;
+            } else if (key == thr) {
+                ties = min(ties, nties);
             }
         }
     }
