@@ -598,29 +598,40 @@ def deltanet_int_step(ctx, state, exp, maxabs, k, q, v, decay, beta, out=None):
 _TYPES = {torch.float32: _lib.TYPE_F32, torch.float16: _lib.TYPE_F16, torch.bfloat16: _lib.TYPE_BF16}
 
 
+# The calls below are made hundreds of times per step, so their checks touch each tensor as little as they can.
+_raw_stream, _current_device = torch._C._cuda_getCurrentRawStream, torch._C._cuda_getDevice
+
+
 def _stream_of(ctx):
     """The current stream of the context's device, which has to be the current device (the library
     launches on it)."""
-    if torch.cuda.current_device() != ctx.device.index:
-        raise ValueError(f"the context is on {ctx.device}, the current device is cuda:{torch.cuda.current_device()}")
-    return torch.cuda.current_stream().cuda_stream
+    dev = ctx.device.index or 0
+    if _current_device() != dev:
+        raise ValueError(f"the context is on {ctx.device}, the current device is cuda:{_current_device()}")
+    return _raw_stream(dev)
 
 
 def _buf(t, dtype, n, name, dev):
-    """A contiguous tensor of at least n elements on the context's device."""
-    if not (t.dtype == dtype and t.device == dev and t.is_contiguous() and t.numel() >= n):
-        raise ValueError(f"{name}: expected a contiguous {dtype} tensor of at least {n} elements on {dev}, got "
-                         f"{t.dtype} {tuple(t.shape)} on {t.device} (contiguous={t.is_contiguous()})")
-    return t.data_ptr()
+    """A contiguous tensor of at least n elements on the context's device: its pointer."""
+    if t.dtype is dtype and t.device == dev and t.is_contiguous() and t.numel() >= n:
+        return t.data_ptr()
+    raise ValueError(f"{name}: expected a contiguous {dtype} tensor of at least {n} elements on {dev}, got "
+                     f"{t.dtype} {tuple(t.shape)} on {t.device} (contiguous={t.is_contiguous()})")
 
 
 def _mat(t, dtype, cols, name, dev):
-    """A matrix of `cols` columns whose rows may be apart (a slice of a wider one): pointer, row stride."""
-    if not (t.dtype == dtype and t.device == dev and t.dim() == 2 and t.shape[1] == cols and
-            (t.stride(1) == 1 or cols == 1) and (t.shape[0] <= 1 or t.stride(0) >= cols)):
-        raise ValueError(f"{name}: expected a {dtype} matrix of {cols} columns on {dev} with contiguous rows, got "
-                         f"{t.dtype} {tuple(t.shape)} strides {t.stride()} on {t.device}")
-    return t.data_ptr(), t.stride(0) if t.shape[0] > 1 else cols
+    """A matrix of `cols` columns whose rows may be apart (a slice of a wider one): pointer, row stride, rows."""
+    shape = t.shape
+    if t.dtype is dtype and t.device == dev and len(shape) == 2 and shape[1] == cols:
+        s0, s1 = t.stride()
+        rows = shape[0]
+        if s1 == 1 or cols == 1:
+            if rows <= 1:
+                return t.data_ptr(), cols, rows
+            if s0 >= cols:
+                return t.data_ptr(), s0, rows
+    raise ValueError(f"{name}: expected a {dtype} matrix of {cols} columns on {dev} with contiguous rows, got "
+                     f"{t.dtype} {tuple(shape)} strides {t.stride()} on {t.device}")
 
 
 class PagedPlan:
@@ -646,10 +657,10 @@ class PagedPlan:
         rows = self.max_rows if rows is None else min(rows, self.max_rows)
         c = self._c.get(rows)
         if c is None:
-            c = self._c[rows] = _lib.Pages(self.nseq, rows, self.page, self.max_pages, self.n_pages,
-                                           *[t.data_ptr() for t in (self.tables, self.lens, self.cu, self.slots,
-                                                                    self.pos, self.last, self.n_free)])
-        return ctypes.byref(c)
+            c = self._c[rows] = ctypes.byref(_lib.Pages(
+                self.nseq, rows, self.page, self.max_pages, self.n_pages,
+                *[t.data_ptr() for t in (self.tables, self.lens, self.cu, self.slots, self.pos, self.last, self.n_free)]))
+        return c
 
 
 def paged_shape(n_head, n_kv, head_dim, rope_dims=None, gated=False, eps=1e-6, window=0, sinks=0):
@@ -693,25 +704,25 @@ def paged_append(ctx, shape, plan, q, k, v, q_norm, k_norm, rope_freq, kpages, v
     (trx_paged_append).  q [rows, n_head*(1+gated)*head_dim], k, v [rows, n_kv*head_dim] float32 (rows may
     be apart); kpages, vpages [n_pages, page, n_kv, head_dim] float16 or bfloat16.  Returns q_out [rows,
     n_head, head_dim] of q_dtype (default: the pages' type; or float32)."""
-    dev, hd, f32 = plan.device, shape.head_dim, torch.float32
+    dev, hd, f32, n_head, n_kv = plan.device, shape.head_dim, torch.float32, shape.n_head, shape.n_kv
     kp, vp, ct = _pools(shape, plan, kpages, vpages)
-    qp, q_ld = _mat(q, f32, shape.n_head * hd * (2 if shape.gated else 1), "q", dev)
-    kk, k_ld = _mat(k, f32, shape.n_kv * hd, "k", dev)
-    vv, v_ld = _mat(v, f32, shape.n_kv * hd, "v", dev)
-    rows = min(q.shape[0], k.shape[0], v.shape[0])
+    qp, q_ld, rows = _mat(q, f32, n_head * hd * (2 if shape.gated else 1), "q", dev)
+    kk, k_ld, k_rows = _mat(k, f32, n_kv * hd, "k", dev)
+    vv, v_ld, v_rows = _mat(v, f32, n_kv * hd, "v", dev)
+    rows = min(rows, k_rows, v_rows)
     if q_out is None:
-        q_out = torch.empty(rows, shape.n_head, hd, dtype=q_dtype or kpages.dtype, device=dev)
-    if q_out.dtype not in (f32, kpages.dtype):
-        raise ValueError(f"q_out: expected float32 or {kpages.dtype}, got {q_out.dtype}")
+        q_out = torch.empty(rows, n_head, hd, dtype=q_dtype or kpages.dtype, device=dev)
+    qt = q_out.dtype
+    if qt is not f32 and qt is not kpages.dtype:
+        raise ValueError(f"q_out: expected float32 or {kpages.dtype}, got {qt}")
     rows = min(rows, q_out.shape[0])
     if rows == 0:
         return q_out
     _lib.check(_lib.lib().trx_paged_append(
-        ctx.h, ctypes.byref(shape), plan.pages(rows), qp, q_ld, kk, k_ld, vv, v_ld, _buf(q_norm, f32, hd, "q_norm", dev),
+        ctx.h, shape, plan.pages(rows), qp, q_ld, kk, k_ld, vv, v_ld, _buf(q_norm, f32, hd, "q_norm", dev),
         _buf(k_norm, f32, hd, "k_norm", dev),
         _buf(rope_freq, f32, shape.rope_dims // 2, "rope_freq", dev) if shape.rope_dims else None, kp, vp, ct,
-        _buf(q_out, q_out.dtype, rows * shape.n_head * hd, "q_out", dev), _TYPES[q_out.dtype], _stream_of(ctx)),
-        "trx_paged_append")
+        _buf(q_out, qt, rows * n_head * hd, "q_out", dev), _TYPES[qt], _stream_of(ctx)), "trx_paged_append")
     return q_out
 
 
@@ -720,23 +731,23 @@ def attn_paged(ctx, shape, plan, q, kpages, vpages, gate=None, max_new=None, out
     alike (trx_attn_paged).  q [rows, n_head, head_dim] as paged_append returns it; gate: the raw q
     projection given to paged_append (gated shapes only); max_new: a bound on the new rows of any
     sequence (default: the rows of q).  Returns out, like q."""
-    dev, hd = plan.device, shape.head_dim
+    dev, width, qt = plan.device, shape.n_head * shape.head_dim, q.dtype
     kp, vp, ct = _pools(shape, plan, kpages, vpages)
     rows = q.shape[0]
-    if q.dtype not in _TYPES or (q.dtype != torch.float32 and q.dtype != kpages.dtype):
-        raise ValueError(f"q: expected float32 or {kpages.dtype}, got {q.dtype}")
+    if qt is not torch.float32 and qt is not kpages.dtype:
+        raise ValueError(f"q: expected float32 or {kpages.dtype}, got {qt}")
     if out is None:
         out = torch.empty_like(q)
     gp, g_ld = None, 0
     if gate is not None:
-        gp, g_ld = _mat(gate, torch.float32, shape.n_head * 2 * hd, "gate", dev)
-        rows = min(rows, gate.shape[0])
-    n = rows * shape.n_head * hd
+        gp, g_ld, g_rows = _mat(gate, torch.float32, 2 * width, "gate", dev)
+        rows = min(rows, g_rows)
     if rows == 0:
         return out
     _lib.check(_lib.lib().trx_attn_paged(
-        ctx.h, ctypes.byref(shape), plan.pages(rows), _buf(q, q.dtype, n, "q", dev), _TYPES[q.dtype], gp, g_ld, kp, vp,
-        ct, rows if max_new is None else max_new, _buf(out, q.dtype, n, "out", dev), _stream_of(ctx)), "trx_attn_paged")
+        ctx.h, shape, plan.pages(rows), _buf(q, qt, rows * width, "q", dev), _TYPES[qt], gp, g_ld, kp, vp, ct,
+        rows if max_new is None else max_new, _buf(out, qt, rows * width, "out", dev), _stream_of(ctx)),
+        "trx_attn_paged")
     return out
 
 
@@ -749,7 +760,7 @@ def sample_rows(ctx, logits, u, temperature, top_k, top_p, min_p, tokens=None):
         raise ValueError(f"logits: expected a float32, float16 or bfloat16 matrix, got {logits.dtype} {tuple(logits.shape)}")
     n, V = logits.shape
     dev, f32 = ctx.device, torch.float32
-    lp, ld = _mat(logits, logits.dtype, V, "logits", dev)
+    lp, ld, _ = _mat(logits, logits.dtype, V, "logits", dev)
     if tokens is None:
         tokens = torch.empty(n, dtype=torch.int32, device=dev)
     if n == 0:
