@@ -1,0 +1,113 @@
+"""Serving sequences of unequal lengths over a paged cache (trixium_b200.decoder.PagedDecoder): greedy
+tokens equal the batch-1 decoder's (itself pinned to the oracle model) whatever the chunks, the slots and
+the pages; sampled tokens are those of the sampler's definition on the step's logits."""
+import numpy as np
+import pytest
+import torch
+
+from test_sample_gpu import draw
+
+pytestmark = pytest.mark.gpu
+
+PROMPTS = [[5, 17, 300, 42, 999, 0, 7], [1], [640, 12, 12, 7, 800, 33, 4, 4, 90, 1, 2, 77, 650, 13, 8, 9, 10, 11, 2], [3, 2]]
+
+
+def weights(name, seed=5):
+    from trixium_b200 import decoder as D
+    return D.SyntheticWeights(D.CONFIGS[name], seed=seed)
+
+
+@pytest.mark.parametrize("name", ["tiny", "tiny-kv1", "tiny-hd256", "tiny-kseg"])
+@pytest.mark.parametrize("max_rows,graph", [(64, False), (5, True)])
+def test_greedy_tokens_match_decoder(name, max_rows, graph):
+    from trixium_b200 import decoder as D
+    w = weights(name)
+    want = [D.Decoder(w, max_pos=64).generate(p, 12) for p in PROMPTS]
+    pd = D.PagedDecoder(w, len(PROMPTS), max_pos=64, max_rows=max_rows)
+    if graph:
+        pd.capture()
+    assert pd.generate(PROMPTS, 12) == want
+    assert pd.plan.n_free.item() == pd.n_pages and pd.lens == [0] * len(PROMPTS)
+    assert sorted(pd.free.tolist()) == list(range(pd.n_pages))
+    assert pd.generate(PROMPTS[::-1], 12) == want[::-1]  # the pages come back in another order
+
+
+def test_more_prompts_than_slots_and_few_pages():
+    from trixium_b200 import decoder as D
+    w = weights("tiny")
+    prompts = PROMPTS * 2
+    want = [D.Decoder(w, max_pos=64).generate(p, 6) for p in PROMPTS] * 2
+    pd = D.PagedDecoder(w, 2, max_pos=32, n_pages=4, max_rows=8)
+    assert pd.generate(prompts, 6) == want
+
+
+def test_long_prompt_in_chunks():
+    """A prompt longer than the tile sizes, in chunks that end inside pages and tiles, beside a short one."""
+    from trixium_b200 import decoder as D
+    w = weights("tiny")
+    rng = np.random.default_rng(3)
+    prompts = [rng.integers(0, 1000, 330).tolist(), rng.integers(0, 1000, 21).tolist()]
+    want = [D.Decoder(w, max_pos=400).generate(p, 4) for p in prompts]
+    for rows in (150, 37):
+        pd = D.PagedDecoder(w, 2, max_pos=400, page=32, max_rows=rows)
+        assert pd.generate(prompts, 4) == want, rows
+
+
+def test_sampled_tokens_are_the_definition_on_the_logits():
+    from trixium_b200 import decoder as D
+    pd = D.PagedDecoder(weights("tiny"), 3, max_pos=64, max_rows=32)
+    cfg = [dict(temperature=0.9, top_k=50, top_p=0.9), dict(), dict(temperature=1.2, min_p=0.02)]
+    for s, c in enumerate(cfg):
+        pd.set_sampling(s, **c)
+    tokens = [PROMPTS[0], PROMPTS[2], PROMPTS[3]]
+    for step in range(5):
+        pd.rand.copy_(torch.rand(3, generator=torch.Generator().manual_seed(step)))
+        pd.step(tokens)
+        x, u = pd.logits.double().cpu().numpy(), pd.rand.double().cpu().numpy()
+        f = lambda v: float(np.float32(v))
+        want = [draw(x[s], u[s], f(c.get("temperature", 0)), c.get("top_k", 0), f(c.get("top_p", 1.0)), f(c.get("min_p", 0)))
+                for s, c in enumerate(cfg)]
+        assert pd.tok.tolist() == want, step
+        tokens = [None] * 3
+    assert pd.ctx.errors() == 0
+    pd.finish(range(3))
+    a = pd.generate(PROMPTS, 8, sampling=[dict(temperature=1.0)] * 4, seed=1)
+    assert a == pd.generate(PROMPTS, 8, sampling=[dict(temperature=1.0)] * 4, seed=1)
+    assert a != pd.generate(PROMPTS, 8, sampling=[dict(temperature=1.0)] * 4, seed=2)
+
+
+def test_window_and_sinks_that_cover_everything_change_nothing():
+    from trixium_b200 import decoder as D
+    w = weights("tiny")
+
+    def run(**kw):
+        pd = D.PagedDecoder(w, 4, max_pos=64, max_rows=64, **kw)
+        return pd.generate(PROMPTS, 6), pd.logits.clone()
+    full, logits = run()
+    assert run(window=64)[0] == full
+    assert run(window=4, sinks=64)[0] == full
+    assert not torch.equal(run(window=4)[1], logits)  # (a random model's greedy tokens need not change)
+
+
+def test_refusals_and_running_out_of_pages():
+    from trixium_b200 import _lib, decoder as D
+    with pytest.raises(ValueError, match="DeltaNet"):
+        D.PagedDecoder(weights("tiny-hybrid"), 2)
+    w = weights("tiny")
+    with pytest.raises(ValueError):
+        D.PagedDecoder(w, 0)
+    with pytest.raises(ValueError):
+        D.PagedDecoder(w, 8, max_rows=4)
+    pd = D.PagedDecoder(w, 2, max_pos=32, max_rows=16, n_pages=1)
+    with pytest.raises(ValueError):
+        pd.generate([[]], 3)
+    with pytest.raises(ValueError):
+        pd.step([[1] * 20, []])
+    with pytest.raises(ValueError):
+        pd.step([[1]])
+    with pytest.raises(ValueError):
+        pd.generate([[1] * 33], 1)
+    pd = D.PagedDecoder(w, 2, max_pos=32, max_rows=16, n_pages=1)
+    with pytest.raises(_lib.TrxDeviceError) as e:
+        pd.generate([[1, 2], [3]], 4)
+    assert e.value.bits & _lib.DEV_PAGES

@@ -511,9 +511,209 @@ class BatchDecoder:
         return out.t().cpu().tolist()
 
 
+class PagedDecoder:
+    """Decoding of sequences of unequal lengths over a paged KV cache (attention-only configs): nseq slots
+    share a pool of n_pages pages; a step takes up to max_rows new rows, prompt chunks and single tokens of
+    decoding sequences together, each sequence at its own length.  A step is the page plan
+    (trx_paged_plan), then per layer the batched projections of BatchDecoder over groups of 32 rows, the
+    append (trx_paged_append) and one attention call for all rows (trx_attn_paged, queries in fp32 as the
+    other decoders keep them), then the LM head over every sequence's last row and the sampler
+    (trx_sample_rows; temperature 0, the default, is the greedy token).  window and sinks limit what a row
+    sees (trx_paged_shape).  finish() returns a slot's pages to the pool."""
+
+    def __init__(self, weights: SyntheticWeights, nseq, ctx=None, max_pos=4096, page=16, n_pages=None, max_rows=256,
+                 window=0, sinks=0):
+        cfg = self.cfg = weights.cfg
+        if any(cfg.layer_type(l) == "d" for l in range(cfg.n_layer)):
+            raise ValueError("PagedDecoder: DeltaNet layers have no paged form (BatchDecoder takes them)")
+        if not 1 <= nseq <= 1024:
+            raise ValueError("PagedDecoder: 1 <= nseq <= 1024")
+        if max_rows < nseq:
+            raise ValueError("PagedDecoder: max_rows must hold a row of every sequence")
+        for lw in weights.layers:
+            d = lw["down"]
+            if isinstance(d, list) and (len(d) != 2 or any(t.kind == L.KIND_Q8 for t in d)):
+                raise ValueError("PagedDecoder: a K-segmented tensor needs two ternary segments")
+        self.w, self.nseq, self.max_pos, self.max_rows = weights, nseq, max_pos, max_rows
+        self.ctx = ctx or ops.default_context()
+        dev = weights.emb.device
+        f32 = lambda *shape: torch.zeros(*shape, dtype=torch.float32, device=dev)
+        i32 = lambda *shape: torch.zeros(*shape, dtype=torch.int32, device=dev)
+        E, R = cfg.hidden, max_rows
+        max_pages = -(-max_pos // page)
+        self.n_pages = n_pages = n_pages or nseq * max_pages
+        self.plan = ops.PagedPlan(nseq, R, max_pages, page, n_pages, device=dev)
+        self.free = torch.arange(n_pages - 1, -1, -1, dtype=torch.int32, device=dev)
+        self.plan.n_free.fill_(n_pages)
+        self.shape = ops.paged_shape(cfg.n_head, cfg.n_kv, cfg.head_dim, rope_dims=cfg.rope_dims or cfg.head_dim,
+                                     gated=cfg.attn_gated, eps=cfg.eps, window=window, sinks=sinks)
+        pool = lambda: torch.zeros(n_pages, page, cfg.n_kv, cfg.head_dim, dtype=torch.float16, device=dev)
+        self.kp, self.vp = [pool() for _ in range(cfg.n_layer)], [pool() for _ in range(cfg.n_layer)]
+        self.x, self.h = f32(R, E), f32(nseq, E)
+        self.q, self.k, self.v = f32(R, cfg.q_rows), f32(R, cfg.kv_rows), f32(R, cfg.kv_rows)
+        self.qr, self.attn = f32(R, cfg.n_head, cfg.head_dim), f32(R, cfg.n_head, cfg.head_dim)
+        self.g, self.u, self.act = f32(R, cfg.ffn), f32(R, cfg.ffn), f32(R, cfg.ffn)
+        self.logits = f32(nseq, cfg.vocab)
+        self.rows_tok, self.new, self.tok = i32(R), i32(nseq), i32(nseq)
+        # Sampling settings of every slot, and the step's random numbers.
+        self.temperature, self.top_k, self.top_p, self.min_p = f32(nseq), i32(nseq), f32(nseq) + 1, f32(nseq)
+        self.rand = f32(nseq)
+        self.lens = [0] * nseq  # host copy of plan.lens
+        self.graph = None
+
+    def set_sampling(self, slot, temperature=0.0, top_k=0, top_p=1.0, min_p=0.0):
+        """Settings of one slot (trx_sample_rows): temperature 0 greedy, top_k 0, top_p 1, min_p 0 off."""
+        self.temperature[slot], self.top_k[slot], self.top_p[slot], self.min_p[slot] = temperature, top_k, top_p, min_p
+
+    def enqueue_step(self, rows, max_new):
+        """The kernels of a step on the current stream: self.new rows per slot (rows in all, at most
+        max_new of any), their tokens in self.rows_tok, into self.logits and self.tok."""
+        cfg, w, ctx, plan = self.cfg, self.w, self.ctx, self.plan
+        groups = [slice(r, min(r + 32, rows)) for r in range(0, rows, 32)]
+        ops.paged_plan(ctx, plan, plan.lens, self.new, self.free, plan.n_free)
+        ops.embed_lookup_rows(ctx, w.emb, self.rows_tok[:rows], self.x)
+        q, k, v, qr, attn = self.q[:rows], self.k[:rows], self.v[:rows], self.qr[:rows], self.attn[:rows]
+        flat = attn.view(rows, -1)
+        for l, lw in enumerate(w.layers):
+            p, ffn = lw["in"], lw["ffn_packed"]
+            for g in groups:
+                ops.matvec_f_rows_multi(ctx, p.entries, p.data, self.x[g], [self.q[g], self.k[g], self.v[g]],
+                                        norm_w=lw["attn_norm"], eps=cfg.eps)
+            ops.paged_append(ctx, self.shape, plan, q, k, v, lw["q_norm"], lw["k_norm"], w.rope_freq, self.kp[l],
+                             self.vp[l], q_out=qr)
+            ops.attn_paged(ctx, self.shape, plan, qr, self.kp[l], self.vp[l], gate=q if cfg.attn_gated else None,
+                           max_new=max_new, out=attn)
+            for g in groups:
+                ops.matvec_f_rows(ctx, lw["out"], flat[g], out=self.x[g], resid=self.x[g])
+            for g in groups:
+                ops.matvec_f_rows_multi(ctx, ffn.entries, ffn.data, self.x[g], [self.g[g], self.u[g]],
+                                        norm_w=lw["ffn_norm"], eps=cfg.eps)
+            ops.silu_mul(ctx, self.g[:rows], self.u[:rows], self.act)
+            for g in groups:
+                if isinstance(lw["down"], list):
+                    ops.matvec_f_rows_kseg(ctx, lw["down"], self.act[g], out=self.x[g], resid=self.x[g])
+                else:
+                    ops.matvec_f_rows(ctx, lw["down"], self.act[g], out=self.x[g], resid=self.x[g])
+        # Every slot's last row (row 0 for one without rows: its token is not used).
+        ops.embed_lookup_rows(ctx, self.x, plan.last, self.h)
+        ops.rmsnorm_rows(ctx, self.h, w.out_norm, cfg.eps, y=self.x[:self.nseq])
+        for r in range(0, self.nseq, 32):
+            g = slice(r, min(r + 32, self.nseq))
+            ops.matvec_f_rows(ctx, w.lm_head, self.x[g], out=self.logits[g])
+        ops.sample_rows(ctx, self.logits, self.rand, self.temperature, self.top_k, self.top_p, self.min_p,
+                        tokens=self.tok)
+
+    def step(self, tokens):
+        """One step: tokens[s], the new tokens of slot s (a list; empty: the slot waits; None: its last
+        sampled token).  Afterwards self.tok[s] is the token that follows, on the device."""
+        counts = [1 if t is None else len(t) for t in tokens]
+        rows, top = sum(counts), max(counts, default=0)
+        if len(counts) != self.nseq or rows > self.max_rows:
+            raise ValueError(f"PagedDecoder: {len(counts)} slots and {rows} rows, expected {self.nseq} slots and at most "
+                             f"{self.max_rows} rows")
+        if any(n + c > self.max_pos for n, c in zip(self.lens, counts)):
+            raise ValueError(f"PagedDecoder: a sequence would pass max_pos = {self.max_pos}")
+        if rows == 0:
+            return
+        self.lens = [n + c for n, c in zip(self.lens, counts)]
+        if self.graph is not None and all(t is None for t in tokens):
+            self.graph.replay()
+            return
+        host = [t for seq in tokens for t in ([0] if seq is None else seq)]
+        self.rows_tok[:rows].copy_(torch.tensor(host, dtype=torch.int32))
+        self.new.copy_(torch.tensor(counts, dtype=torch.int32))
+        fed = [s for s, t in enumerate(tokens) if t is None]
+        if fed:  # rows whose token is still on the device only
+            first = np.concatenate([[0], np.cumsum(counts)])
+            idx = torch.tensor(np.stack([first[fed], fed]).astype(np.int64)).to(self.tok.device)
+            self.rows_tok[idx[0]] = self.tok[idx[1]]
+        self.enqueue_step(rows, top)
+
+    def finish(self, slots):
+        """Return the pages of these slots to the pool; the slots are empty again."""
+        done = torch.zeros(self.nseq, dtype=torch.int32)
+        done[list(slots)] = 1
+        ops.paged_release(self.ctx, self.plan, done.to(self.tok.device), self.plan.lens, self.free, self.plan.n_free)
+        for s in slots:
+            self.lens[s] = 0
+
+    def capture(self):
+        """Capture the step in which every slot feeds its last sampled token as a CUDA graph (lengths,
+        tables, tokens and settings live on the device)."""
+        def one():
+            self.rows_tok[:self.nseq].copy_(self.tok)
+            self.enqueue_step(self.nseq, 1)
+        self.new.fill_(1)
+        s = torch.cuda.Stream()
+        s.wait_stream(torch.cuda.current_stream())
+        live = [self.plan.lens, self.plan.tables, self.plan.n_free, self.tok]
+        saved = [t.clone() for t in live]
+        with torch.cuda.stream(s):
+            self.plan.lens.zero_()  # the warm-up writes to pages of the free stack only
+            one()
+            torch.cuda.synchronize()
+        for t, c in zip(live, saved):
+            t.copy_(c)
+        self.graph = torch.cuda.CUDAGraph()
+        with torch.cuda.stream(s):
+            with torch.cuda.graph(self.graph, stream=s):
+                self.new.fill_(1)
+                one()
+        torch.cuda.synchronize()
+        return self.graph
+
+    def generate(self, prompts, n_new, sampling=None, seed=0):
+        """n_new tokens after every prompt (any number of them, any lengths): prompts enter free slots in
+        order, in chunks that share the steps' rows with the decoding slots; a finished sequence's slot and
+        pages go to the next prompt.  sampling: per prompt a dict for set_sampling (None: greedy), the
+        random numbers from `seed`.  Returns [prompts][n_new] ids."""
+        if any(len(p) == 0 for p in prompts) or n_new < 1:
+            raise ValueError("PagedDecoder: prompts must hold a token, and n_new be at least 1")
+        if any(self.lens):
+            raise ValueError("PagedDecoder: generate needs empty slots (finish)")
+        gen = torch.Generator(device=self.tok.device)
+        gen.manual_seed(seed)
+        out = torch.empty(len(prompts), n_new, dtype=torch.int32, device=self.tok.device)
+        slots = [None] * self.nseq   # (prompt, prompt tokens fed, tokens made)
+        waiting = list(range(len(prompts)))
+        while waiting or any(slots):
+            for s in range(self.nseq):
+                if slots[s] is None and waiting:
+                    i = waiting.pop(0)
+                    slots[s] = [i, 0, 0]
+                    self.set_sampling(s, **((sampling[i] if sampling else None) or {}))
+            tokens = [[] for _ in slots]
+            room = self.max_rows
+            for s, t in enumerate(slots):   # decoding sequences first
+                if t and t[2]:
+                    tokens[s] = None
+                    room -= 1
+            for s, t in enumerate(slots):
+                if t and not t[2]:
+                    tokens[s] = prompts[t[0]][t[1]:t[1] + room]
+                    t[1] += len(tokens[s])
+                    room -= len(tokens[s])
+            torch.rand(self.nseq, generator=gen, out=self.rand)
+            self.step(tokens)
+            done = []
+            for s, t in enumerate(slots):
+                if t and t[1] == len(prompts[t[0]]):
+                    out[t[0], t[2]:t[2] + 1].copy_(self.tok[s:s + 1])
+                    t[2] += 1
+                    if t[2] == n_new:
+                        done.append(s)
+                        slots[s] = None
+            if done:
+                self.finish(done)
+        self.ctx.raise_on_error()
+        return out.cpu().tolist()
+
+
 def main(argv=None):
     """Decode timing on synthetic weights: python -m trixium_b200.decoder --config qwen3-8b
-    --context 1024 --tokens 64 [--eager].  Prints one JSON line (ms and tok/s per token)."""
+    --context 1024 --tokens 64 [--eager].  Prints one JSON line (ms and tok/s per token).  --sequences N
+    serves N sequences over a paged cache (PagedDecoder), their context fed as prompts in chunks of --rows:
+    the line also holds the prompts' tokens per second."""
     import argparse
     import json
     ap = argparse.ArgumentParser(description=main.__doc__)
@@ -522,8 +722,12 @@ def main(argv=None):
     ap.add_argument("--tokens", type=int, default=64)
     ap.add_argument("--warmup", type=int, default=3)
     ap.add_argument("--eager", action="store_true", help="launch the kernels directly (no CUDA graph)")
+    ap.add_argument("--sequences", type=int, default=0, help="serve this many sequences over a paged cache")
+    ap.add_argument("--rows", type=int, default=256, help="new rows of a paged step")
     a = ap.parse_args(argv)
     cfg = CONFIGS[a.config]
+    if a.sequences:
+        return _serve(cfg, a)
     dec = Decoder(SyntheticWeights(cfg, seed=0), max_pos=a.context + a.tokens + a.warmup + 8)
     dec.set_states(1)
     dec.fill_context(a.context)
@@ -544,6 +748,39 @@ def main(argv=None):
     print(json.dumps({"config": a.config, "context": a.context, "tokens": a.tokens, "graph": not a.eager,
                       "ms_per_token": round(ms, 4), "tok_s": round(1000.0 / ms, 1),
                       "launches_per_token": dec.launches_per_step()}))
+
+
+def _serve(cfg, a):
+    import json
+    n = a.sequences
+    dec = PagedDecoder(SyntheticWeights(cfg, seed=0), n, max_pos=a.context + a.tokens + a.warmup + 8,
+                       max_rows=max(a.rows, n))
+    prompts = np.random.default_rng(0).integers(0, cfg.vocab, (n, a.context)).tolist()
+    e = [torch.cuda.Event(enable_timing=True) for _ in range(3)]
+    chunk = max(1, dec.max_rows // n)
+    dec.step([p[:1] for p in prompts])  # warm-up
+    dec.finish(range(n))
+    torch.cuda.synchronize()
+    e[0].record()
+    for c in range(0, a.context, chunk):
+        dec.step([p[c:c + chunk] for p in prompts])
+    e[1].record()
+    if not a.eager:
+        dec.capture()
+    for _ in range(a.warmup):
+        dec.step([None] * n)
+    torch.cuda.synchronize()
+    t0, t1 = e[2], torch.cuda.Event(enable_timing=True)
+    t0.record()
+    for _ in range(a.tokens):
+        dec.step([None] * n)
+    t1.record()
+    torch.cuda.synchronize()
+    dec.ctx.raise_on_error()
+    ms = t0.elapsed_time(t1) / a.tokens
+    print(json.dumps({"config": a.config, "sequences": n, "context": a.context, "tokens": a.tokens, "graph": not a.eager,
+                      "prompt_tok_s": round(1000.0 * n * a.context / e[0].elapsed_time(e[1]), 1),
+                      "ms_per_step": round(ms, 4), "tok_s": round(1000.0 * n / ms, 1)}))
 
 
 if __name__ == "__main__":
