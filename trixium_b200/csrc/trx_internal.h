@@ -274,6 +274,8 @@ trx_status launch_attn_paged_tc(const PgAttnArgs &A, int hd, int cache_type, int
 // A tiled TMA map of a row-major matrix of 16-bit elements (128-byte swizzle; trx_rows.cu): map points to
 // a CUtensorMap.  Elements outside the matrix read as zeros.
 bool encode_map_16bit(void *map, const void *base, uint64_t cols, uint64_t rows, uint32_t box_cols, uint32_t box_rows);
+// The same for four dimensions (innermost first; strides in bytes of all but the innermost).
+bool encode_map_16bit_4d(void *map, const void *base, const uint64_t *dims, const uint64_t *strides, const uint32_t *box);
 // Sampling (trx_sample.cu).
 struct SampleArgs {
     const void *x;

@@ -14,9 +14,10 @@ namespace trx {
 
 constexpr int kPagedMaxSeq = 1024;  // sequences of one plan (the kernels keep a prefix of them in shared memory)
 
-// The pools as matrices of n_kv * head_dim columns, one row per slot.
+// The pools as matrices of n_kv * head_dim columns, one row per slot; the queries (16-bit ones of the
+// tcgen05 kernel) as [rows][n_kv][rep][head_dim].
 struct PgMaps {
-    CUtensorMap k, v;
+    CUtensorMap k, v, q;
 };
 
 __device__ __forceinline__ void arrive(uint32_t bar) {
@@ -27,6 +28,14 @@ __device__ __forceinline__ void load_box(uint32_t dst, const void *map, int x, i
         "cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], "
         "[%4];" ::"r"(dst),
         "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(bar)
+        : "memory");
+}
+
+__device__ __forceinline__ void load_box4(uint32_t dst, const void *map, int x, int y, int z, int w, uint32_t bar) {
+    asm volatile(
+        "cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], "
+        "[%6];" ::"r"(dst),
+        "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(z), "r"(w), "r"(bar)
         : "memory");
 }
 

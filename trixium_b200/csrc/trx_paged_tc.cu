@@ -6,8 +6,8 @@
 // tokens x rep heads (padded).  A CTA walks its pieces (PgSched): key tiles of KT positions of one
 // (query tile, kv head).  Per key tile S = Q K^T (M = 128, N = KT), the softmax in 32 bits, O += P V
 // (M = 128, N = head dim).  Warp roles:
-//  * warps 0-3: one query row per thread (its TMEM lane).  They put the query tile into shared memory,
-//    read S from tensor memory, keep the row's maximum and sum, write P (16 bits) over S as the A operand
+//  * warps 0-3: one query row per thread (its TMEM lane).  They put an fp32 query tile into shared memory (a
+//    16-bit one comes by TMA), read S from tensor memory, keep the row's maximum and sum, write P (16 bits) over S as the A operand
 //    of the second product, and finish the piece.  O is rescaled only when a row's maximum has grown by
 //    more than 2^8 over the one in use: P then stays below 2^8, exact in any 16-bit float's exponent.
 //  * warp 4: the producer.  A key tile is gathered by TMA boxes of one page (or the tile's part of it) x
@@ -62,7 +62,7 @@ struct TcBars {
     uint64_t pready[2];            // P is in the place of S (4 warps)
     uint64_t odone[2];             // P V is complete: O, the V tile and the S buffer are free
     uint64_t cdone[2], ofree[2];   // split: part n of P V is complete; it has been added to O (4 warps)
-    uint64_t qready;               // the query tile is in shared memory (4 warps)
+    uint64_t qready;               // the query tile is in shared memory (split: 4 warps; else by TMA)
     uint64_t fin[2];               // every MMA of warps 5 and 6
     uint32_t tmem;
     volatile uint32_t dead;        // a wait ran out somewhere in the block
@@ -191,50 +191,44 @@ __device__ __forceinline__ void put32(const PgAttnArgs &A, int hd, int row, int 
     }
 }
 
-// The query tile into shared memory (K-major, 128-byte swizzle), zeros behind its rows; sixteen
-// 16-byte loads of a thread in flight at a time.
+// The fp32 query tile into shared memory as two fp16 parts (K-major, 128-byte swizzle), zeros behind its rows;
+// sixteen 16-byte loads of a thread in flight at a time.
 template <typename CT, typename QT, int HD>
 __device__ __forceinline__ void load_query(const PgAttnArgs &A, unsigned char *smem, int r, int rows, int row0, int head0) {
-    constexpr bool SPLIT = sizeof(QT) == 4;
-    using C = TcCfg<HD, SPLIT>;
-    constexpr int PPR = HD / 8, B = SPLIT || HD == 64 ? 8 : 16;  // pieces of 8 elements per row, of a batch
-    const int inv = (65536 + A.rep - 1) / A.rep;    // qr / rep = qr * inv >> 16 for qr < 128, rep <= 16
+    using C = TcCfg<HD, true>;
+    constexpr int PPR = HD / 8, B = 8;            // pieces of 8 elements per row, of a batch
+    const int inv = (65536 + A.rep - 1) / A.rep;  // qr / rep = qr * inv >> 16 for qr < 128, rep <= 16
     const int c = r % PPR;
     const uint32_t coff = (uint32_t)((c / 8) * (kTcRows * 128));
     const QT *const src = reinterpret_cast<const QT *>(A.q) + ((long long)row0 * A.H + head0) * HD + c * 8;
 #pragma unroll 1
     for (int i0 = 0; i0 < PPR; i0 += B) {
-        uint4 x[B], y[SPLIT ? B : 1];
+        uint4 x[B], y[B];
 #pragma unroll
         for (int b = 0; b < B; ++b) {
             const int qr = (i0 + b) * (kTcRows / PPR) + r / PPR, tk = qr * inv >> 16;
             const QT *p = src + (long long)(tk * A.H + qr - tk * A.rep) * HD;
-            x[b] = make_uint4(0u, 0u, 0u, 0u);
-            if (qr < rows) x[b] = *reinterpret_cast<const uint4 *>(p);
-            if constexpr (SPLIT) {
-                y[b] = make_uint4(0u, 0u, 0u, 0u);
-                if (qr < rows) y[b] = *reinterpret_cast<const uint4 *>(p + 4);
+            x[b] = y[b] = make_uint4(0u, 0u, 0u, 0u);
+            if (qr < rows) {
+                x[b] = *reinterpret_cast<const uint4 *>(p);
+                y[b] = *reinterpret_cast<const uint4 *>(p + 4);
             }
         }
 #pragma unroll
         for (int b = 0; b < B; ++b) {
             const int qr = (i0 + b) * (kTcRows / PPR) + r / PPR;
             unsigned char *const dst = smem + C::QOFF + coff + qr * 128 + (((c % 8) ^ (qr & 7)) << 4);
-            if constexpr (SPLIT) {
-                const uint32_t f[8] = {x[b].x, x[b].y, x[b].z, x[b].w, y[b].x, y[b].y, y[b].z, y[b].w};
-                uint32_t hw[4], lw[4];
+            const uint32_t f[8] = {x[b].x, x[b].y, x[b].z, x[b].w, y[b].x, y[b].y, y[b].z, y[b].w};
+            uint32_t hw[4], lw[4];
 #pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    const float f0 = __uint_as_float(f[2 * e]), f1 = __uint_as_float(f[2 * e + 1]);
-                    hw[e] = PgCvt<CT>::pack(f0, f1);
-                    const float2 h = PgCvt<CT>::unpack(hw[e]);
-                    lw[e] = PgCvt<CT>::pack(f0 - h.x, f1 - h.y);
-                }
-                *reinterpret_cast<uint4 *>(dst) = make_uint4(hw[0], hw[1], hw[2], hw[3]);
-                *reinterpret_cast<uint4 *>(dst + C::QBYTES) = make_uint4(lw[0], lw[1], lw[2], lw[3]);
-            } else {
-                *reinterpret_cast<uint4 *>(dst) = x[b];
+            for (int e = 0; e < 4; ++e) {
+                const float f0 = __uint_as_float(f[2 * e]), f1 = __uint_as_float(f[2 * e + 1]);
+                hw[e] = PgCvt<CT>::pack(f0, f1);
+                const float2 h = PgCvt<CT>::unpack(hw[e]);
+                lw[e] = PgCvt<CT>::pack(f0 - h.x, f1 - h.y);
             }
+            *reinterpret_cast<uint4 *>(dst) = make_uint4(hw[0], hw[1], hw[2], hw[3]);
+            *reinterpret_cast<uint4 *>(dst + C::QBYTES) = make_uint4(lw[0], lw[1], lw[2], lw[3]);
         }
     }
 }
@@ -358,13 +352,14 @@ __global__ void __launch_bounds__(kTcThreads, HD == 256 || sizeof(QT) == 4 ? 1 :
             mbar_init(&bars.cdone[i], 1);
             mbar_init(&bars.ofree[i], 4);
         }
-        mbar_init(&bars.qready, 4);
+        mbar_init(&bars.qready, SPLIT ? 4 : 1);
         mbar_init(&bars.fin[0], 1);
         mbar_init(&bars.fin[1], 1);
         bars.dead = 0u;
         mbar_fence_init();
         tma_prefetch_map(&maps.k);
         tma_prefetch_map(&maps.v);
+        if (!SPLIT) tma_prefetch_map(&maps.q);
     }
     pdl_wait();
     // Tensor memory is taken only now that the kernel in front has ended, and the kernel behind is let in
@@ -377,7 +372,7 @@ __global__ void __launch_bounds__(kTcThreads, HD == 256 || sizeof(QT) == 4 ? 1 :
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
     }
     tc_before();
-    pg_schedule(A, sched, 1, err);  // barriers inside: the allocation and the barriers' set-up are visible behind it
+    pg_schedule(A, sched, 4, err);  // barriers inside: the allocation and the barriers' set-up are visible behind it
     tc_after();
     pdl_trigger();
     const uint32_t tmem = bars.tmem;
@@ -469,6 +464,18 @@ __global__ void __launch_bounds__(kTcThreads, HD == 256 || sizeof(QT) == 4 ? 1 :
         uint32_t piece = 0;
         bool ok = true, more = true;
         while (ok && more) {
+            if constexpr (!SPLIT) {
+                // The piece's query tile (rows of other sequences or zeros behind its own, whose results are not
+                // used), once the MMAs that read the one before are complete.
+                ok = j == 0 || wait2(sfull, j - 1);
+                if (!ok) break;
+                if (lane == 0) mbar_expect_tx_s(qready, (uint32_t)(A.tq * A.rep * HD * 2));
+                __syncwarp();
+                if (lane < HD / 64)
+                    load_box4(sbase + C::QOFF + (uint32_t)(lane * kTcRows * 128), &maps.q, 64 * lane, 0, W.kh,
+                              W.q.row0 + W.t * A.tq, qready);
+                __syncwarp();
+            }
             ok = wait(qready, piece++);
             for (int n = W.i1 - W.i0; ok && n; --n, ++j) {
                 const int st = j % KST;
@@ -487,6 +494,8 @@ __global__ void __launch_bounds__(kTcThreads, HD == 256 || sizeof(QT) == 4 ? 1 :
             }
             if (ok) more = W.next(A);
         }
+        if (!SPLIT && !ok)  // a query tile on its way has landed
+            for (int ph = 0; ph < 2; ++ph) wait_phase(qready, ph, nullptr);
         commit(fin);  // every MMA is complete before the tensor memory is given back
         wait_phase(fin, 0u, nullptr);
     } else if (any && warp == 6) {
@@ -534,11 +543,13 @@ __global__ void __launch_bounds__(kTcThreads, HD == 256 || sizeof(QT) == 4 ? 1 :
         int j = 0;
         bool ok = true;
         // The walk's query tile; every MMA that read the one before is complete (its S was waited for).
-        auto fetch = [&] {
-            load_query<CT, QT, HD>(A, smem, r, W.rows(A), W.q.row0 + W.t * A.tq, W.kh * A.rep);
-            fence_proxy_async();
-            __syncwarp();
-            if (lane == 0) arrive(qready);
+        auto fetch = [&] {  // split: warp 5 brings 16-bit queries
+            if constexpr (SPLIT) {
+                load_query<CT, QT, HD>(A, smem, r, W.rows(A), W.q.row0 + W.t * A.tq, W.kh * A.rep);
+                fence_proxy_async();
+                __syncwarp();
+                if (lane == 0) arrive(qready);
+            }
         };
         // Split: part n of P V (dims q NW..) onto O scaled by f.  The tensor cores cut their sums off instead of
         // rounding them, which over the tiles of a row adds up to 2.6e-6 of the output (17 tiles of 64); so
@@ -758,6 +769,12 @@ trx_status launch_tc(PgAttnArgs A, size_t part_cap, int cnt_cap, uint32_t *err, 
     const uint32_t br = (uint32_t)std::min(page, C::KT);
     if (!encode_map_16bit(&maps.k, A.kp, cols, rows, 64, br) || !encode_map_16bit(&maps.v, A.vp, cols, rows, 64, br))
         return TRX_ERR_CUDA;
+    if (sizeof(QT) == 2) {
+        const uint64_t dims[4] = {HD, (uint64_t)A.rep, (uint64_t)A.Hkv, (uint64_t)A.max_rows};
+        const uint64_t strides[3] = {HD * 2ull, (uint64_t)A.rep * HD * 2, (uint64_t)A.H * HD * 2};
+        const uint32_t box[4] = {64, (uint32_t)A.rep, 1, (uint32_t)A.tq};
+        if (!encode_map_16bit_4d(&maps.q, A.q, dims, strides, box)) return TRX_ERR_CUDA;
+    }
     const int grid = device_sms() * C::CTAS;
     if ((size_t)grid * 2 * kTcRows * (HD + 2) > part_cap || 4 * grid > cnt_cap) return TRX_ERR_UNSUPPORTED;
     return note_cuda(launch_kernel(attn_paged_tc_kernel<CT, QT, HD>, dim3(grid), dim3(kTcThreads), C::END + sizeof(TcTail), st,

@@ -826,6 +826,16 @@ bool encode_map_16bit(void *map, const void *base, uint64_t cols, uint64_t rows,
              CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
+bool encode_map_16bit_4d(void *map, const void *base, const uint64_t *dims, const uint64_t *strides, const uint32_t *box) {
+    const EncodeTiledFn2 f = encode_fn();
+    if (!f) return false;
+    const cuuint64_t d[4] = {dims[0], dims[1], dims[2], dims[3]}, st[3] = {strides[0], strides[1], strides[2]};
+    const cuuint32_t b[4] = {box[0], box[1], box[2], box[3]}, es[4] = {1, 1, 1, 1};
+    return f(static_cast<CUtensorMap *>(map), CU_TENSOR_MAP_DATA_TYPE_UINT16, 4, const_cast<void *>(base), d, st, b, es,
+             CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+             CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
 // Slots of [activation tiles][codes][scales] (1024-byte multiples, 1024-aligned in the window) after
 // the barriers; trit5: around the LUT at window 0x10000.
 static bool rows_plan(int kind, int BN, int G, int reserved, RowsPlan &P) {
