@@ -394,32 +394,32 @@ __global__ void __launch_bounds__(kDecThreads, HD == 256 ? 1 : 2)
         const uint32_t my_dst = smem_u32(sm.kv) + (uint32_t)((lane >> 4) * TB + (bi / nb) * (kDecTile * 128) + my_pos * 128);
         const CUtensorMap *const map = lane < 16 ? &maps.k : &maps.v;
         const bool mine = bi < boxes;
-        auto row_of = [&](const PgWalk &P, int it) {  // this lane's first row of tile it of a piece
-            const int p = P.R.tile(it) * kDecTile + my_pos;
-            int row = beyond;
-            if (mine && p < P.q.p0 + P.q.n) {
-                const int id = __ldg(A.tables + (long long)P.b * A.max_pages + (p >> A.page_shift));
-                if ((unsigned)id < (unsigned)A.n_pages)
-                    row = (id << A.page_shift) + (p & ((1 << A.page_shift) - 1));
-                else
-                    atomicOr(err, TRX_DEV_RANGE);
-            }
-            return row;
+        // This lane's table entry of tile it of a piece (-1 behind the sequence's end); looked at only when the box
+        // is sent, so that the load's time is not waited for.
+        auto pos_of = [&](const PgWalk &P, int it) { return P.R.tile(it) * kDecTile + my_pos; };
+        auto id_of = [&](const PgWalk &P, int it) {
+            const int p = pos_of(P, it);
+            return mine && p < P.q.p0 + P.q.n ? __ldg(A.tables + (long long)P.b * A.max_pages + (p >> A.page_shift)) : -1;
         };
         int j = 0, piece = 0, it = W.i0;
         bool ok = true;
-        int row = row_of(W, it);
+        int id = id_of(W, it);
         for (;;) {
             // The table is read a tile ahead.
             PgWalk N = W;
             int nit = it + 1;
             const bool more = nit < W.i1 || N.next(A);
             if (nit == W.i1) nit = N.i0;
-            const int nrow = more ? row_of(N, nit) : 0;
+            const int nid = more ? id_of(N, nit) : 0;
             const int st = j % ST;
             ok = !sm.dead && (j < ST || wait(freed + 8u * st, (uint32_t)(j / ST - 1)));
             if (!ok) break;
             if (lane == 0) mbar_expect_tx_s(full + 8u * st, 2u * TB);
+            int row = beyond;
+            if ((unsigned)id < (unsigned)A.n_pages)
+                row = (id << A.page_shift) + (pos_of(W, it) & ((1 << A.page_shift) - 1));
+            else if (mine && pos_of(W, it) < W.q.p0 + W.q.n)
+                atomicOr(err, TRX_DEV_RANGE);
             __syncwarp();
             if (mine) load_box(my_dst + (uint32_t)(st * 2 * TB), map, W.kh * HD + my_dim, row, full + 8u * st);
             __syncwarp();
@@ -473,7 +473,7 @@ __global__ void __launch_bounds__(kDecThreads, HD == 256 ? 1 : 2)
             if (!more) break;
             W = N;
             it = nit;
-            row = nrow;
+            id = nid;
         }
         if (!ok) {
             // Whatever was issued has landed before the block leaves (bounded; the timeout is recorded).

@@ -237,6 +237,7 @@ __device__ __forceinline__ void load_query(const PgAttnArgs &A, unsigned char *s
 // REG: get reads registers, so the loops are unrolled.
 template <typename QT, int HD, bool REG, typename Get>
 __device__ __forceinline__ void finish_whole(const PgAttnArgs &A, Get &&get, float l, int row, int head) {
+    if (!__any_sync(0xffffffffu, row >= 0)) return;
     const float inv = l > 0.f ? __fdiv_rn(1.0f, l) : 0.f;
 #pragma unroll (REG ? HD / 32 : 1)
     for (int c = 0; c < HD / 32; ++c) {
@@ -256,6 +257,7 @@ template <typename QT, int HD, bool REG, typename Get>
 __device__ __forceinline__ void finish_cut(const PgAttnArgs &A, const PgSched &S, Get &&get, long long item0,
                                            long long item1, float m, float l, int row, int head) {
     constexpr size_t kPart = kTcRows * (HD + 2);
+    if (!__any_sync(0xffffffffu, row >= 0)) return;  // none of this warp's rows exist (the same in every piece)
     const int r = threadIdx.x, lane = r & 31, me = (int)blockIdx.x;
     const int c0 = pg_owner(S, item0), c1 = pg_owner(S, item1 - 1);
     unsigned *const cnt = A.cnt + 4 * c0 + (r >> 5);
@@ -290,36 +292,48 @@ __device__ __forceinline__ void finish_cut(const PgAttnArgs &A, const PgSched &S
         L = cc == me ? fmaf(ex2f(m - Ms), l, L) : fmaf(ex2f(__ldcg(p) - Ms), __ldcg(p + kTcRows), L);
     }
     const float inv = L > 0.f ? __fdiv_rn(1.0f, L) : 0.f;
+    constexpr int GC = HD == 256 ? 2 : 1;  // 32 dims at a time, or 64: loads in flight
 #pragma unroll (REG ? HD / 32 : 1)
-    for (int c = 0; c < HD / 32; ++c) {
-        float o[32];
+    for (int c = 0; c < HD / 32; c += GC) {
+        float o[GC][32];
 #pragma unroll
-        for (int e = 0; e < 32; ++e) o[e] = 0.f;
+        for (int g = 0; g < GC; ++g)
+#pragma unroll
+            for (int e = 0; e < 32; ++e) o[g][e] = 0.f;
 #pragma unroll 1
         for (int cc = c0; cc <= c1; ++cc) {
-            uint32_t v[32];
+            uint32_t v[GC][32];
             float w;
             if (cc == me) {
-                get(c, v);
+#pragma unroll
+                for (int g = 0; g < GC; ++g) get(c + g, v[g]);
                 w = ex2f(m - Ms);
             } else {
                 const float *p = slot_of(cc);
+                w = __ldcg(p + kTcRows * HD + r);
 #pragma unroll
-                for (int e = 0; e < 8; ++e) {
-                    const uint4 x = __ldcg(reinterpret_cast<const uint4 *>(p) + (8 * c + e) * kTcRows + r);
-                    v[4 * e] = x.x;
-                    v[4 * e + 1] = x.y;
-                    v[4 * e + 2] = x.z;
-                    v[4 * e + 3] = x.w;
-                }
-                w = ex2f(__ldcg(p + kTcRows * HD + r) - Ms);
+                for (int g = 0; g < GC; ++g)
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) {
+                        const uint4 x = __ldcg(reinterpret_cast<const uint4 *>(p) + (8 * (c + g) + e) * kTcRows + r);
+                        v[g][4 * e] = x.x;
+                        v[g][4 * e + 1] = x.y;
+                        v[g][4 * e + 2] = x.z;
+                        v[g][4 * e + 3] = x.w;
+                    }
+                w = ex2f(w - Ms);
             }
 #pragma unroll
-            for (int e = 0; e < 32; ++e) o[e] = fmaf(w, __uint_as_float(v[e]), o[e]);
+            for (int g = 0; g < GC; ++g)
+#pragma unroll
+                for (int e = 0; e < 32; ++e) o[g][e] = fmaf(w, __uint_as_float(v[g][e]), o[g][e]);
         }
 #pragma unroll
-        for (int e = 0; e < 32; ++e) o[e] *= inv;
-        if (row >= 0) put32<QT>(A, HD, row, head, 32 * c, o);
+        for (int g = 0; g < GC; ++g) {
+#pragma unroll
+            for (int e = 0; e < 32; ++e) o[g][e] *= inv;
+            if (row >= 0) put32<QT>(A, HD, row, head, 32 * (c + g), o[g]);
+        }
     }
     __syncwarp();
     if (lane == 0) *cnt = 0u;
@@ -401,22 +415,27 @@ __global__ void __launch_bounds__(kTcThreads, HD == 256 || sizeof(QT) == 4 ? 1 :
         const uint32_t my_dst = sbase + (uint32_t)((lane / nb) * KT * 128 + my_pos * 128);
         int it = W.i0;
         bool more = true;
-        // This lane's first row of the walk's next tile, and its kv head's first column.
-        auto next_box = [&](int &row, int &col) {
+        // Of the walk's next tile: this lane's page (its table entry, or -1 behind the sequence's end; used only
+        // when the box is sent, so that the load's time is not waited for), place in it, and first column.
+        struct Box {
+            int id, at, col;
+            bool in;
+        };
+        auto next_box = [&](Box &B) {
             const int p = W.R.tile(it) * KT + my_pos;
-            row = beyond;
-            col = W.kh * HD + my_dim;
-            if (lane < boxes && p < W.q.p0 + W.q.n) {
-                const int id = __ldg(A.tables + (long long)W.b * A.max_pages + (p >> A.page_shift));
-                if ((unsigned)id < (unsigned)A.n_pages)
-                    row = (id << A.page_shift) + (p & ((1 << A.page_shift) - 1));
-                else
-                    atomicOr(err, TRX_DEV_RANGE);
-            }
+            B.in = lane < boxes && p < W.q.p0 + W.q.n;
+            B.id = B.in ? __ldg(A.tables + (long long)W.b * A.max_pages + (p >> A.page_shift)) : -1;
+            B.at = p & ((1 << A.page_shift) - 1);
+            B.col = W.kh * HD + my_dim;
             if (++it == W.i1) {
                 more = W.next(A);
                 it = W.i0;
             }
+        };
+        auto row_of = [&](const Box &B) {
+            if ((unsigned)B.id < (unsigned)A.n_pages) return (B.id << A.page_shift) + B.at;
+            if (B.in) atomicOr(err, TRX_DEV_RANGE);
+            return beyond;
         };
         auto issue = [&](int j, int off, const CUtensorMap *map, uint32_t full, int row, int col) {
             const int st = j % KST;
@@ -426,17 +445,19 @@ __global__ void __launch_bounds__(kTcThreads, HD == 256 || sizeof(QT) == 4 ? 1 :
             __syncwarp();
         };
         // K runs a tile ahead of V (its place is free earlier), and the table is read a tile ahead of that.
-        int row, col, vrow = 0, vcol = 0;
-        next_box(row, col);
+        Box box, nbox{};
+        next_box(box);
+        int vrow = 0, vcol = 0;
         bool ok = true, tile = true;
         for (int j = 0; ok; ++j) {
-            int nrow = 0, ncol = 0;
+            int row = 0;
             const bool next = tile && more;
-            if (next) next_box(nrow, ncol);
+            if (next) next_box(nbox);
             if (bars.dead) ok = false;
             if (ok && tile) {
                 ok = j < KST || wait2(sfull, j - KST);
-                if (ok) issue(j, C::KOFF, &maps.k, kfull, row, col);
+                row = row_of(box);
+                if (ok) issue(j, C::KOFF, &maps.k, kfull, row, box.col);
             }
             if (ok && j) {
                 ok = j - 1 < KST || wait2(odone, j - 1 - KST);
@@ -444,9 +465,8 @@ __global__ void __launch_bounds__(kTcThreads, HD == 256 || sizeof(QT) == 4 ? 1 :
             }
             if (!tile) break;
             vrow = row;
-            vcol = col;
-            row = nrow;
-            col = ncol;
+            vcol = box.col;
+            box = nbox;
             tile = next;
         }
         if (!ok) {
