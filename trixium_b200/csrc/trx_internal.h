@@ -271,10 +271,8 @@ trx_status launch_attn_paged(const PgAttnArgs &A, int hd, int cache_type, int q_
                              uint32_t *err, cudaStream_t st);
 trx_status launch_attn_paged_tc(const PgAttnArgs &A, int hd, int cache_type, int q_type, size_t part_cap, int cnt_cap,
                                 uint32_t *err, cudaStream_t st);
-// A tiled TMA map of a row-major matrix of 16-bit elements (128-byte swizzle; trx_rows.cu): map points to
-// a CUtensorMap.  Elements outside the matrix read as zeros.
-bool encode_map_16bit(void *map, const void *base, uint64_t cols, uint64_t rows, uint32_t box_cols, uint32_t box_rows);
-// The same for four dimensions (innermost first; strides in bytes of all but the innermost).
+// A tiled TMA map over four dimensions of 16-bit elements (innermost first; strides in bytes of all but the
+// innermost; 128-byte swizzle; trx_rows.cu): map points to a CUtensorMap.  Elements outside read as zeros.
 bool encode_map_16bit_4d(void *map, const void *base, const uint64_t *dims, const uint64_t *strides, const uint32_t *box);
 // Sampling (trx_sample.cu).
 struct SampleArgs {

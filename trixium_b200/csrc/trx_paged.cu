@@ -261,8 +261,8 @@ __global__ void __launch_bounds__(kAppThreads) paged_append_kernel(PgAppendArgs 
 // Attention, few query rows ------------------------------------------------------------------------
 // A CTA walks its pieces (PgSched) in tiles of 64 key positions. Rows of the products are the query rows
 // of one (query tile, kv head): 16 / rep tokens x rep heads, padded to 16.
-//  * warp 4, the producer: key tiles by TMA (boxes of one page, or the tile's part of it, x 64 dims,
-//    128-byte swizzle; lanes 0-15 K, 16-31 V) through a ring, and each piece's query rows into one of two
+//  * warp 4, the producer: key tiles by TMA (boxes of one page, or the tile's part of it, see PgMaps;
+//    lanes 0-15 K, 16-31 V) through a ring, and each piece's query rows into one of two
 //    places, all ahead of the work.
 //  * warps 0-3: 16 positions each of every tile: S = Q K^T and O += P V on mma.sync m16n8k16 with fp32
 //    accumulation, the softmax online per warp (running maximum and sum per row). At the end of a piece
@@ -321,11 +321,11 @@ __device__ __forceinline__ void ldsm4t(uint32_t addr, uint32_t (&r)[4]) {
                  : "memory");
 }
 
-// Byte offset of 16-byte piece c of row r in a tile of ROWS rows as the 128-byte swizzle lays it: blocks of
-// 64 dims, pieces permuted within each 128 bytes by the row.
-template <int ROWS>
+// Byte offset of 16-byte piece c of row r of a tile: groups of 8 rows, in each the 64-dim blocks of 8 rows x
+// 128 bytes, pieces permuted within the 128 bytes by the row (the swizzle).
+template <int HD>
 __device__ __forceinline__ uint32_t tile_off(int r, int c) {
-    return (uint32_t)((c >> 3) * (ROWS * 128) + r * 128 + (((c & 7) ^ (r & 7)) << 4));
+    return (uint32_t)((r >> 3) * (HD * 16) + (c >> 3) * 1024 + (r & 7) * 128 + (((c & 7) ^ (r & 7)) << 4));
 }
 
 template <typename QT>
@@ -386,12 +386,12 @@ __global__ void __launch_bounds__(kDecThreads, HD == 256 ? 1 : 2)
     };
     if (warp == kDecWarps) {
         // Producer.
-        const int br = min(1 << A.page_shift, kDecTile), nb = kDecTile / br;  // box rows, boxes per 64 dims
-        const int boxes = nb * (HD / 64), bi = lane & 15;
-        static_assert(kDecTile / 16 * (HD / 64) <= 16, "a lane has one box");
+        const int br = min(1 << A.page_shift, kDecTile), boxes = kDecTile / br;  // rows of a box, boxes of a tile
+        const int bi = lane & 15;
+        static_assert(kDecTile / 16 <= 16, "a lane has one box");
         const int beyond = A.n_pages << A.page_shift;  // a row outside the maps: zeros
-        const int my_pos = (bi % nb) * br, my_dim = 64 * (bi / nb);
-        const uint32_t my_dst = smem_u32(sm.kv) + (uint32_t)((lane >> 4) * TB + (bi / nb) * (kDecTile * 128) + my_pos * 128);
+        const int my_pos = bi * br;
+        const uint32_t my_dst = smem_u32(sm.kv) + (uint32_t)((lane >> 4) * TB + my_pos * HD * 2);
         const CUtensorMap *const map = lane < 16 ? &maps.k : &maps.v;
         const bool mine = bi < boxes;
         // This lane's table entry of tile it of a piece (-1 behind the sequence's end); looked at only when the box
@@ -421,7 +421,7 @@ __global__ void __launch_bounds__(kDecThreads, HD == 256 ? 1 : 2)
             else if (mine && pos_of(W, it) < W.q.p0 + W.q.n)
                 atomicOr(err, TRX_DEV_RANGE);
             __syncwarp();
-            if (mine) load_box(my_dst + (uint32_t)(st * 2 * TB), map, W.kh * HD + my_dim, row, full + 8u * st);
+            if (mine) load_box4(my_dst + (uint32_t)(st * 2 * TB), map, 0, 0, W.kh * (HD / 64), row / 8, full + 8u * st);
             __syncwarp();
             if (it == W.i0) {  // a new piece: its query rows, zeros behind them
                 const int qb = piece % QB;
@@ -447,7 +447,7 @@ __global__ void __launch_bounds__(kDecThreads, HD == 256 ? 1 : 2)
                     for (int e = 0; e < B; ++e) {
                         const int i = i0 + 32 * e, r = i / (HD / 8);
                         if (r >= rows) break;
-                        const uint32_t off = tile_off<16>(r, i % (HD / 8));
+                        const uint32_t off = tile_off<HD>(r, i % (HD / 8));
                         if constexpr (SPLIT) {
                             const uint32_t f[8] = {x[e].x, x[e].y, x[e].z, x[e].w, y[e].x, y[e].y, y[e].z, y[e].w};
                             uint32_t hw[4], lw[4];
@@ -515,12 +515,12 @@ __global__ void __launch_bounds__(kDecThreads, HD == 256 ? 1 : 2)
 #pragma unroll
             for (int k = 0; k < HD / 16; ++k) {
                 uint32_t a[4], b[4];
-                ldsm4(qs + tile_off<16>(arow, 2 * k + acol), a);
-                ldsm4(ks + tile_off<kDecTile>(brow, 2 * k + bcol), b);
+                ldsm4(qs + tile_off<HD>(arow, 2 * k + acol), a);
+                ldsm4(ks + tile_off<HD>(brow, 2 * k + bcol), b);
                 mma_16816<CT>(s0, a, b[0], b[1]);
                 mma_16816<CT>(s1, a, b[2], b[3]);
                 if constexpr (SPLIT) {
-                    ldsm4(qs + 16 * HD * 2 + tile_off<16>(arow, 2 * k + acol), a);
+                    ldsm4(qs + 16 * HD * 2 + tile_off<HD>(arow, 2 * k + acol), a);
                     mma_16816<CT>(t0, a, b[0], b[1]);
                     mma_16816<CT>(t1, a, b[2], b[3]);
                 }
@@ -537,7 +537,7 @@ __global__ void __launch_bounds__(kDecThreads, HD == 256 ? 1 : 2)
             if (k0 + 16 > len) {
                 const int z0 = max(0, len - k0);
                 for (int i = lane; i < (16 - z0) * (HD / 8); i += 32)
-                    *reinterpret_cast<uint4 *>(&sm.kv[st][1][tile_off<kDecTile>(warp * 16 + z0 + i / (HD / 8), i % (HD / 8))]) =
+                    *reinterpret_cast<uint4 *>(&sm.kv[st][1][tile_off<HD>(warp * 16 + z0 + i / (HD / 8), i % (HD / 8))]) =
                         make_uint4(0u, 0u, 0u, 0u);
                 fence_proxy_async();  // before the copy that refills the slot
                 __syncwarp();
@@ -580,7 +580,7 @@ __global__ void __launch_bounds__(kDecThreads, HD == 256 ? 1 : 2)
 #pragma unroll
             for (int i = 0; i < HD / 16; ++i) {
                 uint32_t b[4];
-                ldsm4t(vs + tile_off<kDecTile>(vrow, 2 * i + vcol), b);
+                ldsm4t(vs + tile_off<HD>(vrow, 2 * i + vcol), b);
 #pragma unroll
                 for (int h = 0; h < 2; ++h) {
                     float(&d)[4] = o[2 * i + h];
@@ -729,10 +729,7 @@ trx_status launch_dec(PgAttnArgs A, size_t part_cap, int cnt_cap, uint32_t *err,
     A.tq = 16 / A.rep;
     A.kt_shift = 6;
     PgMaps maps;
-    const uint64_t cols = (uint64_t)A.Hkv * HD, rows = (uint64_t)A.n_pages << A.page_shift;
-    const uint32_t br = 1u << (A.page_shift < 6 ? A.page_shift : 6);
-    if (!encode_map_16bit(&maps.k, A.kp, cols, rows, 64, br) || !encode_map_16bit(&maps.v, A.vp, cols, rows, 64, br))
-        return TRX_ERR_CUDA;
+    if (!pg_encode_pools<HD>(maps, A, 1u << (A.page_shift < 6 ? A.page_shift : 6))) return TRX_ERR_CUDA;
     const int grid = device_sms() * (HD == 256 ? 1 : 2);
     if ((size_t)grid * 2 * 16 * (HD + 2) > part_cap || grid > cnt_cap) return TRX_ERR_UNSUPPORTED;
     return note_cuda(launch_kernel(attn_paged_kernel<CT, QT, HD>, dim3(grid), dim3(kDecThreads), smem, st, maps, A, err));

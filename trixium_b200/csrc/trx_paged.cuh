@@ -14,23 +14,25 @@ namespace trx {
 
 constexpr int kPagedMaxSeq = 1024;  // sequences of one plan (the kernels keep a prefix of them in shared memory)
 
-// The pools as matrices of n_kv * head_dim columns, one row per slot; the queries (16-bit ones of the
-// tcgen05 kernel) as [rows][n_kv][rep][head_dim].
+// The pools as [8 slots][slot of 8][64 dims of a head][dim], one box a page's (or a tile's part of it) slots of
+// one kv head: a single copy lays them as groups of 8 slots, in each group the head's 64-dim blocks of 8 rows
+// x 128 bytes.  (A box per 64 dims cost 80 cycles of the producer each: 1,300 for a tile of head dim 256 in
+// pages of 16.)  The queries (16-bit ones of the tcgen05 kernel) as [rows][n_kv][rep][head_dim].
 struct PgMaps {
     CUtensorMap k, v, q;
 };
 
+template <int HD>
+inline bool pg_encode_pools(PgMaps &maps, const PgAttnArgs &A, uint32_t box_rows) {
+    const uint64_t pitch = (uint64_t)A.Hkv * HD * 2, groups = ((uint64_t)A.n_pages << A.page_shift) / 8;
+    const uint64_t dims[4] = {64, 8, (uint64_t)A.Hkv * HD / 64, groups}, strides[3] = {pitch, 128, 8 * pitch};
+    const uint32_t box[4] = {64, 8, HD / 64, box_rows / 8};
+    return encode_map_16bit_4d(&maps.k, A.kp, dims, strides, box) && encode_map_16bit_4d(&maps.v, A.vp, dims, strides, box);
+}
+
 __device__ __forceinline__ void arrive(uint32_t bar) {
     asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory");
 }
-__device__ __forceinline__ void load_box(uint32_t dst, const void *map, int x, int y, uint32_t bar) {
-    asm volatile(
-        "cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], "
-        "[%4];" ::"r"(dst),
-        "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(bar)
-        : "memory");
-}
-
 __device__ __forceinline__ void load_box4(uint32_t dst, const void *map, int x, int y, int z, int w, uint32_t bar) {
     asm volatile(
         "cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], "

@@ -10,8 +10,8 @@
 //    16-bit one comes by TMA), read S from tensor memory, keep the row's maximum and sum, write P (16 bits) over S as the A operand
 //    of the second product, and finish the piece.  O is rescaled only when a row's maximum has grown by
 //    more than 2^8 over the one in use: P then stays below 2^8, exact in any 16-bit float's exponent.
-//  * warp 4: the producer.  A key tile is gathered by TMA boxes of one page (or the tile's part of it) x
-//    64 dims, 128-byte swizzle; places behind the sequence's end come from outside the map, as zeros.
+//  * warp 4: the producer.  A key tile is gathered by TMA boxes of one page (or the tile's part of it, see
+//    PgMaps); places behind the sequence's end come from outside the map, as zeros.
 //  * warps 5 and 6: issue the MMAs of the first and of the second product, each from one elected lane. Two
 //    warps, since one's instructions between two MMAs (waits, commits) take as long as the MMAs.
 // fp32 queries: Q = hi + lo and P = hi + lo in fp16, two MMAs per product, so products keep 2^-22; each
@@ -76,15 +76,16 @@ struct TcTail {  // behind the tiles
 __device__ __forceinline__ void tc_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void tc_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
 
-// K-major operand tile, 128-byte swizzle: rows of 64 16-bit elements, 8-row groups 1024 bytes apart.
-__device__ __forceinline__ uint64_t desc_kmajor(uint32_t a) {
-    return (uint64_t)((a >> 4) & 0x3FFFu) | ((uint64_t)1u << 16) | ((uint64_t)(1024u >> 4) << 32) |
+// K-major operand tile, 128-byte swizzle: rows of 64 16-bit elements in groups of 8 (1024 bytes), `group` bytes
+// apart.
+__device__ __forceinline__ uint64_t desc_kmajor(uint32_t a, uint32_t group) {
+    return (uint64_t)((a >> 4) & 0x3FFFu) | ((uint64_t)1u << 16) | ((uint64_t)(group >> 4) << 32) |
            ((uint64_t)1u << 46) | ((uint64_t)2u << 61);
 }
-// N-major operand tile, 128-byte swizzle: 64 N elements contiguous, K rows 128 bytes apart in groups of 8
-// (1024 bytes apart), the next 64 N elements `block` bytes on.
-__device__ __forceinline__ uint64_t desc_nmajor(uint32_t a, uint32_t block) {
-    return (uint64_t)((a >> 4) & 0x3FFFu) | ((uint64_t)(block >> 4) << 16) | ((uint64_t)(1024u >> 4) << 32) |
+// N-major operand tile, 128-byte swizzle: 64 N elements contiguous, K rows 128 bytes apart in groups of 8,
+// `group` bytes apart, the next 64 N elements `block` bytes on.
+__device__ __forceinline__ uint64_t desc_nmajor(uint32_t a, uint32_t group, uint32_t block) {
+    return (uint64_t)((a >> 4) & 0x3FFFu) | ((uint64_t)(block >> 4) << 16) | ((uint64_t)(group >> 4) << 32) |
            ((uint64_t)1u << 46) | ((uint64_t)2u << 61);
 }
 // Instruction descriptor of kind::f16: D fp32, A and B fp16 (0) or bf16 (1), B N-major if bn, N, M = 128.
@@ -110,18 +111,20 @@ __device__ __forceinline__ void mma_ss4(uint32_t d, uint64_t a, uint64_t b, uint
         "l"(a), "l"(b), "r"(idesc), "r"((int)acc)
         : "memory");
 }
-// A from tensor memory at columns a0..a3, B N-major: a step of 16 rows is 2048 bytes.
+// A from tensor memory at columns a0..a3, B N-major: a step of 16 rows is two groups.
+template <int HD>
 __device__ __forceinline__ void mma_ts4(uint32_t d, uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint64_t b,
                                         uint32_t idesc, bool acc) {
+    constexpr int step = 2 * (HD / 64) * 1024 / 16;
     asm volatile(
         "{\n .reg .pred p, e, t;\n .reg .b64 b1, b2, b3;\n setp.ne.b32 p, %7, 0;\n setp.eq.b32 t, 0, 0;\n"
-        " add.s64 b1, %5, 128;\n add.s64 b2, %5, 256;\n add.s64 b3, %5, 384;\n"
+        " add.s64 b1, %5, %8;\n add.s64 b2, %5, %9;\n add.s64 b3, %5, %10;\n"
         " elect.sync _|e, 0xffffffff;\n"
         " @e tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %5, %6, p;\n"
         " @e tcgen05.mma.cta_group::1.kind::f16 [%0], [%2], b1, %6, t;\n"
         " @e tcgen05.mma.cta_group::1.kind::f16 [%0], [%3], b2, %6, t;\n"
         " @e tcgen05.mma.cta_group::1.kind::f16 [%0], [%4], b3, %6, t;\n}\n" ::"r"(d),
-        "r"(a0), "r"(a1), "r"(a2), "r"(a3), "l"(b), "r"(idesc), "r"((int)acc)
+        "r"(a0), "r"(a1), "r"(a2), "r"(a3), "l"(b), "r"(idesc), "r"((int)acc), "n"(step), "n"(2 * step), "n"(3 * step)
         : "memory");
 }
 __device__ __forceinline__ void commit(uint32_t bar) {
@@ -407,18 +410,17 @@ __global__ void __launch_bounds__(kTcThreads, HD == 256 || sizeof(QT) == 4 ? 1 :
     const bool any = W.start(A, S);
     if (any && warp == 4) {
         // Producer.
-        const int br = min(1 << A.page_shift, KT), nb = KT / br;  // box rows, boxes per 64 dims
-        const int boxes = nb * (HD / 64);
+        const int br = min(1 << A.page_shift, KT), boxes = KT / br;  // rows of a box, boxes of a tile
         const int beyond = A.n_pages << A.page_shift;  // a row outside the maps: zeros
-        static_assert(KT / 16 * (HD / 64) <= 32, "a lane has one box");
-        const int my_pos = (lane % nb) * br, my_dim = 64 * (lane / nb);
-        const uint32_t my_dst = sbase + (uint32_t)((lane / nb) * KT * 128 + my_pos * 128);
+        static_assert(KT / 16 <= 32, "a lane has one box");
+        const int my_pos = lane * br;
+        const uint32_t my_dst = sbase + (uint32_t)(my_pos * HD * 2);
         int it = W.i0;
         bool more = true;
         // Of the walk's next tile: this lane's page (its table entry, or -1 behind the sequence's end; used only
-        // when the box is sent, so that the load's time is not waited for), place in it, and first column.
+        // when the box is sent, so that the load's time is not waited for), place in it, and kv head.
         struct Box {
-            int id, at, col;
+            int id, at, kh;
             bool in;
         };
         auto next_box = [&](Box &B) {
@@ -426,7 +428,7 @@ __global__ void __launch_bounds__(kTcThreads, HD == 256 || sizeof(QT) == 4 ? 1 :
             B.in = lane < boxes && p < W.q.p0 + W.q.n;
             B.id = B.in ? __ldg(A.tables + (long long)W.b * A.max_pages + (p >> A.page_shift)) : -1;
             B.at = p & ((1 << A.page_shift) - 1);
-            B.col = W.kh * HD + my_dim;
+            B.kh = W.kh;
             if (++it == W.i1) {
                 more = W.next(A);
                 it = W.i0;
@@ -437,17 +439,18 @@ __global__ void __launch_bounds__(kTcThreads, HD == 256 || sizeof(QT) == 4 ? 1 :
             if (B.in) atomicOr(err, TRX_DEV_RANGE);
             return beyond;
         };
-        auto issue = [&](int j, int off, const CUtensorMap *map, uint32_t full, int row, int col) {
+        auto issue = [&](int j, int off, const CUtensorMap *map, uint32_t full, int row, int kh) {
             const int st = j % KST;
             if (lane == 0) mbar_expect_tx_s(full + 8u * st, (uint32_t)C::TBYTES);
             __syncwarp();
-            if (lane < boxes) load_box(my_dst + (uint32_t)(off + st * C::TBYTES), map, col, row, full + 8u * st);
+            if (lane < boxes)
+                load_box4(my_dst + (uint32_t)(off + st * C::TBYTES), map, 0, 0, kh * (HD / 64), row / 8, full + 8u * st);
             __syncwarp();
         };
         // K runs a tile ahead of V (its place is free earlier), and the table is read a tile ahead of that.
         Box box, nbox{};
         next_box(box);
-        int vrow = 0, vcol = 0;
+        int vrow = 0, vkh = 0;
         bool ok = true, tile = true;
         for (int j = 0; ok; ++j) {
             int row = 0;
@@ -457,15 +460,15 @@ __global__ void __launch_bounds__(kTcThreads, HD == 256 || sizeof(QT) == 4 ? 1 :
             if (ok && tile) {
                 ok = j < KST || wait2(sfull, j - KST);
                 row = row_of(box);
-                if (ok) issue(j, C::KOFF, &maps.k, kfull, row, box.col);
+                if (ok) issue(j, C::KOFF, &maps.k, kfull, row, box.kh);
             }
             if (ok && j) {
                 ok = j - 1 < KST || wait2(odone, j - 1 - KST);
-                if (ok) issue(j - 1, C::VOFF, &maps.v, vfull, vrow, vcol);
+                if (ok) issue(j - 1, C::VOFF, &maps.v, vfull, vrow, vkh);
             }
             if (!tile) break;
             vrow = row;
-            vcol = box.col;
+            vkh = box.kh;
             box = nbox;
             tile = next;
         }
@@ -479,7 +482,7 @@ __global__ void __launch_bounds__(kTcThreads, HD == 256 || sizeof(QT) == 4 ? 1 :
     } else if (any && warp == 5) {
         // S = Q K^T of every tile, as soon as its K tile and its S buffer allow.
         const uint32_t idq = idesc_f16<CT>(KT, false);
-        const uint64_t qdesc = desc_kmajor(sbase + C::QOFF), kdesc = desc_kmajor(sbase + C::KOFF);
+        const uint64_t qdesc = desc_kmajor(sbase + C::QOFF, 1024), kdesc = desc_kmajor(sbase + C::KOFF, HD / 64 * 1024);
         int j = 0;
         uint32_t piece = 0;
         bool ok = true, more = true;
@@ -508,7 +511,7 @@ __global__ void __launch_bounds__(kTcThreads, HD == 256 || sizeof(QT) == 4 ? 1 :
                 for (int part = SPLIT ? 1 : 0; part >= 0; --part)  // the small part first: the sums are cut off, not rounded
 #pragma unroll
                     for (int c = 0; c < HD / 64; ++c)
-                        mma_ss4(d, qdesc + ((part * C::QBYTES + c * kTcRows * 128) >> 4), kb + ((c * KT * 128) >> 4), idq,
+                        mma_ss4(d, qdesc + ((part * C::QBYTES + c * kTcRows * 128) >> 4), kb + ((c * 1024) >> 4), idq,
                                 (SPLIT && part == 0) || c);
                 commit(sfull + 8u * (j % NS));
             }
@@ -521,7 +524,7 @@ __global__ void __launch_bounds__(kTcThreads, HD == 256 || sizeof(QT) == 4 ? 1 :
     } else if (any && warp == 6) {
         // O += P V.
         const uint32_t idv = idesc_f16<CT>(C::NW, true);
-        const uint64_t vdesc = desc_nmajor(sbase + C::VOFF, KT * 128);
+        const uint64_t vdesc = desc_nmajor(sbase + C::VOFF, HD / 64 * 1024, 1024);
         int j = 0;
         bool ok = true, more = true;
         while (ok && more) {
@@ -541,13 +544,13 @@ __global__ void __launch_bounds__(kTcThreads, HD == 256 || sizeof(QT) == 4 ? 1 :
                         if (!ok) break;
                         tc_after();
                         const uint32_t d = tmem + C::AOFF + (uint32_t)((n % C::NACC) * C::NW);
-                        const uint64_t qb = vb + (uint64_t)((q * (C::NW / 64) * KT * 128) >> 4);
-                        mma_ts4(d, p + 16, p + 24, p + 48, p + 56, qb, idv, false);
-                        mma_ts4(d, p, p + 8, p + 32, p + 40, qb, idv, true);
+                        const uint64_t qb = vb + (uint64_t)((q * (C::NW / 64) * 1024) >> 4);
+                        mma_ts4<HD>(d, p + 16, p + 24, p + 48, p + 56, qb, idv, false);
+                        mma_ts4<HD>(d, p, p + 8, p + 32, p + 40, qb, idv, true);
                         if constexpr (C::NCH > 1) commit(cdone + 8u * (n & 1));
                     }
                 } else {
-                    mma_ts4(tmem, p, p + 8, p + 16, p + 24, vb, idv, !first);
+                    mma_ts4<HD>(tmem, p, p + 8, p + 16, p + 24, vb, idv, !first);
                 }
                 commit(odone + 8u * (j & 1));
                 first = false;
@@ -724,7 +727,7 @@ __global__ void __launch_bounds__(kTcThreads, HD == 256 || sizeof(QT) == 4 ? 1 :
                     unsigned char *vt = smem + C::VOFF + (j % KST) * C::TBYTES;
                     for (int i = r; i < (KT - (len - k0)) * (HD / 8); i += kTcRows) {
                         const int vr = len - k0 + i / (HD / 8), c = i % (HD / 8);
-                        *reinterpret_cast<uint4 *>(vt + (c / 8) * (KT * 128) + vr * 128 + (c % 8) * 16) =
+                        *reinterpret_cast<uint4 *>(vt + (vr / 8) * (HD * 16) + (c / 8) * 1024 + (vr % 8) * 128 + (c % 8) * 16) =
                             make_uint4(0u, 0u, 0u, 0u);
                     }
                     fence_proxy_async();
@@ -784,11 +787,7 @@ trx_status launch_tc(PgAttnArgs A, size_t part_cap, int cnt_cap, uint32_t *err, 
     A.tq = kTcRows / A.rep;
     A.kt_shift = C::KT_SHIFT;
     PgMaps maps;
-    const int page = 1 << A.page_shift;
-    const uint64_t cols = (uint64_t)A.Hkv * HD, rows = (uint64_t)A.n_pages << A.page_shift;
-    const uint32_t br = (uint32_t)std::min(page, C::KT);
-    if (!encode_map_16bit(&maps.k, A.kp, cols, rows, 64, br) || !encode_map_16bit(&maps.v, A.vp, cols, rows, 64, br))
-        return TRX_ERR_CUDA;
+    if (!pg_encode_pools<HD>(maps, A, (uint32_t)std::min(1 << A.page_shift, C::KT))) return TRX_ERR_CUDA;
     if (sizeof(QT) == 2) {
         const uint64_t dims[4] = {HD, (uint64_t)A.rep, (uint64_t)A.Hkv, (uint64_t)A.max_rows};
         const uint64_t strides[3] = {HD * 2ull, (uint64_t)A.rep * HD * 2, (uint64_t)A.H * HD * 2};

@@ -816,16 +816,6 @@ static bool encode(CUtensorMap *m, const void *base, const cuuint64_t *dims, con
            CUDA_SUCCESS;
 }
 
-bool encode_map_16bit(void *map, const void *base, uint64_t cols, uint64_t rows, uint32_t box_cols, uint32_t box_rows) {
-    const EncodeTiledFn2 f = encode_fn();
-    if (!f) return false;
-    const cuuint64_t dims[2] = {cols, rows}, strides[1] = {cols * 2};
-    const cuuint32_t box[2] = {box_cols, box_rows}, es[2] = {1, 1};
-    return f(static_cast<CUtensorMap *>(map), CU_TENSOR_MAP_DATA_TYPE_UINT16, 2, const_cast<void *>(base), dims, strides,
-             box, es, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-             CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
-}
-
 bool encode_map_16bit_4d(void *map, const void *base, const uint64_t *dims, const uint64_t *strides, const uint32_t *box) {
     const EncodeTiledFn2 f = encode_fn();
     if (!f) return false;
