@@ -52,6 +52,10 @@ struct TcCfg {
     static constexpr int QBYTES = kTcRows * HD * 2, TBYTES = KT * HD * 2;
     static constexpr int QOFF = 0, KOFF = QBYTES * (SPLIT ? 2 : 1), VOFF = KOFF + KST * TBYTES,
                          END = VOFF + KST * TBYTES;  // multiples of 1024
+    // Gates through shared memory (a ring of three pieces of 16 dims per row, behind the tail) where there is
+    // room for it: head dim 256 with 16-bit queries.
+    static constexpr bool RING = !SPLIT && HD == 256;
+    static constexpr int GBYTES = RING ? 3 * kTcRows * 64 : 0;
     static_assert(SOFF + NS * KT <= 512 && TMEM * CTAS <= 512, "tensor memory holds O and every S");
 };
 
@@ -72,6 +76,8 @@ struct TcTail {  // behind the tiles
     TcBars bars;
     PgSchedSmem sched;
 };
+static_assert(sizeof(TcTail) % 16 == 0 && TcCfg<256, false>::END + sizeof(TcTail) + TcCfg<256, false>::GBYTES <= 232448,
+              "the gates' ring is aligned and fits");
 
 __device__ __forceinline__ void tc_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void tc_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
@@ -166,20 +172,85 @@ __device__ __forceinline__ void tm_st16(uint32_t a, const uint32_t (&o)[16]) {
 __device__ __forceinline__ void tm_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
 __device__ __forceinline__ void tm_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
-// 32 outputs of one row, dims d..d+31.
-template <typename QT>
-__device__ __forceinline__ void put32(const PgAttnArgs &A, int hd, int row, int h, int d, float (&o)[32]) {
-    if (A.gate) {
-        const float4 *g = reinterpret_cast<const float4 *>(A.gate + row * A.gate_ld + (long long)h * 2 * hd + hd + d);
+// The gates of a piece on their way to a warp's ring: 16 dims of its 32 rows at a time, each row's 64 bytes read
+// by four lanes together, kept swizzled so that a lane per row reads them without conflicts.  Loads by the thread
+// of a row at the time of use (32 lines per access, one round trip per 32 dims) made the end of a piece of 128
+// gated rows x 256 dims take 38,000 cycles; this way 25,000 (1,137 rows of 24 gated heads: 114 to 101 us).
+struct GateRing {
+    uint32_t at;       // shared address of the warp's ring
+    long long row0;    // the piece's first row and head, its rows
+    int head0, rows;
+    int next, slot;    // the next 16 dims to be sent for; the slot of the next to be used
+    __device__ __forceinline__ void send(const PgAttnArgs &A, int hd, int s) {
+        const int lane = threadIdx.x & 31, inv = (65536 + A.rep - 1) / A.rep;
+        if (16 * next < hd) {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            const float4 v = g[i];
-            o[4 * i] = __fdividef(o[4 * i], 1.0f + expf(-v.x));
-            o[4 * i + 1] = __fdividef(o[4 * i + 1], 1.0f + expf(-v.y));
-            o[4 * i + 2] = __fdividef(o[4 * i + 2], 1.0f + expf(-v.z));
-            o[4 * i + 3] = __fdividef(o[4 * i + 3], 1.0f + expf(-v.w));
+            for (int i = 0; i < 4; ++i) {
+                const int wr = 8 * i + (lane >> 2), r = (threadIdx.x & ~31) + wr, tok = r * inv >> 16, u = lane & 3;
+                const float *g = A.gate + (row0 + tok) * A.gate_ld + (long long)(head0 + r - tok * A.rep) * 2 * hd + hd +
+                                 16 * next + 4 * u;
+                if (r < rows)
+                    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(at + s * (kTcRows * 64) + wr * 64 +
+                                                                                   ((u ^ (wr >> 1 & 3)) << 4)),
+                                 "l"(g)
+                                 : "memory");
+            }
+        }
+        asm volatile("cp.async.commit_group;" ::: "memory");
+        ++next;
+    }
+    __device__ __forceinline__ void drain() const { asm volatile("cp.async.wait_all;" ::: "memory"); }
+    // The first three of a piece; what an unfinished piece left on its way lands first.
+    __device__ __forceinline__ void start(const PgAttnArgs &A, int hd) {
+        drain();
+        __syncwarp();
+        next = slot = 0;
+        for (int s = 0; s < 3; ++s) send(A, hd, s);
+    }
+    // The next 16 gates of this lane's row; another 16 dims are sent for.
+    __device__ __forceinline__ void take(const PgAttnArgs &A, int hd, float4 (&g)[4]) {
+        const int lane = threadIdx.x & 31;
+        asm volatile("cp.async.wait_group 2;" ::: "memory");
+        __syncwarp();
+#pragma unroll
+        for (int u = 0; u < 4; ++u)
+            asm volatile("ld.shared.v4.f32 {%0, %1, %2, %3}, [%4];"
+                         : "=f"(g[u].x), "=f"(g[u].y), "=f"(g[u].z), "=f"(g[u].w)
+                         : "r"(at + slot * (kTcRows * 64) + lane * 64 + ((u ^ (lane >> 1 & 3)) << 4))
+                         : "memory");
+        __syncwarp();
+        send(A, hd, slot);
+        slot = slot == 2 ? 0 : slot + 1;
+    }
+};
+
+// 32 outputs of one row (row < 0: none; every lane of the warp takes part), dims d..d+31.
+template <typename QT, bool RING>
+__device__ __forceinline__ void put32(const PgAttnArgs &A, GateRing &G, int hd, int row, int h, int d, float (&o)[32]) {
+    if (A.gate) {
+        const float4 *gp = nullptr;
+        if constexpr (!RING)
+            gp = reinterpret_cast<const float4 *>(A.gate + (row < 0 ? 0 : row) * A.gate_ld + (long long)h * 2 * hd + hd + d);
+#pragma unroll
+        for (int n = 0; n < 2; ++n) {
+            float4 g[4];
+            if constexpr (RING) {
+                G.take(A, hd, g);
+            } else {
+#pragma unroll
+                for (int i = 0; i < 4; ++i) g[i] = gp[4 * n + i];
+            }
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                float *const v = &o[16 * n + 4 * i];
+                v[0] = __fdividef(v[0], 1.0f + expf(-g[i].x));
+                v[1] = __fdividef(v[1], 1.0f + expf(-g[i].y));
+                v[2] = __fdividef(v[2], 1.0f + expf(-g[i].z));
+                v[3] = __fdividef(v[3], 1.0f + expf(-g[i].w));
+            }
         }
     }
+    if (row < 0) return;
     QT *dst = reinterpret_cast<QT *>(A.out) + ((size_t)row * A.H + h) * hd + d;
     if constexpr (sizeof(QT) == 4) {
 #pragma unroll
@@ -238,8 +309,8 @@ __device__ __forceinline__ void load_query(const PgAttnArgs &A, unsigned char *s
 
 // A row's output from its O, 32 dims at a time from get (row < 0: none; every lane of the warp takes part).
 // REG: get reads registers, so the loops are unrolled.
-template <typename QT, int HD, bool REG, typename Get>
-__device__ __forceinline__ void finish_whole(const PgAttnArgs &A, Get &&get, float l, int row, int head) {
+template <typename QT, int HD, bool REG, bool RING, typename Get>
+__device__ __forceinline__ void finish_whole(const PgAttnArgs &A, GateRing &G, Get &&get, float l, int row, int head) {
     if (!__any_sync(0xffffffffu, row >= 0)) return;
     const float inv = l > 0.f ? __fdiv_rn(1.0f, l) : 0.f;
 #pragma unroll (REG ? HD / 32 : 1)
@@ -249,15 +320,15 @@ __device__ __forceinline__ void finish_whole(const PgAttnArgs &A, Get &&get, flo
         float o[32];
 #pragma unroll
         for (int e = 0; e < 32; ++e) o[e] = __uint_as_float(v[e]) * inv;
-        if (row >= 0) put32<QT>(A, HD, row, head, 32 * c, o);
+        put32<QT, RING>(A, G, HD, row, head, 32 * c, o);
     }
 }
 
 // A cut item: this piece's rows to scratch, [HD / 4][128 rows] of four dims, then the maxima and sums; the
 // last to arrive joins the pieces in the order of the CTAs (its own still from get).  The warps
 // arrive and join on their own, 32 rows each.
-template <typename QT, int HD, bool REG, typename Get>
-__device__ __forceinline__ void finish_cut(const PgAttnArgs &A, const PgSched &S, Get &&get, long long item0,
+template <typename QT, int HD, bool REG, bool RING, typename Get>
+__device__ __forceinline__ void finish_cut(const PgAttnArgs &A, const PgSched &S, GateRing &G, Get &&get, long long item0,
                                            long long item1, float m, float l, int row, int head) {
     constexpr size_t kPart = kTcRows * (HD + 2);
     if (!__any_sync(0xffffffffu, row >= 0)) return;  // none of this warp's rows exist (the same in every piece)
@@ -286,14 +357,24 @@ __device__ __forceinline__ void finish_cut(const PgAttnArgs &A, const PgSched &S
         if (seen != (unsigned)(c1 - c0)) return;
     }
     __threadfence();
-    float M = m, L = 0.f;
-    for (int cc = c0; cc <= c1; ++cc)
-        if (cc != me) M = fmaxf(M, __ldcg(slot_of(cc) + kTcRows * HD + r));
-    const float Ms = M == -INFINITY ? 0.f : M;
-    for (int cc = c0; cc <= c1; ++cc) {
-        const float *p = slot_of(cc) + kTcRows * HD + r;
-        L = cc == me ? fmaf(ex2f(m - Ms), l, L) : fmaf(ex2f(__ldcg(p) - Ms), __ldcg(p + kTcRows), L);
+    // The pieces' maxima and sums, four pieces' loads at a time.
+    float M = -INFINITY, L = 0.f;
+    for (int cc = c0; cc <= c1; cc += 4) {
+        float pm[4], pl[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            const float *p = slot_of(min(cc + e, c1)) + kTcRows * HD + r;
+            pm[e] = cc + e <= c1 ? __ldcg(p) : -INFINITY;
+            pl[e] = __ldcg(p + kTcRows);
+        }
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            const float Mn = fmaxf(M, pm[e]), Mz = Mn == -INFINITY ? 0.f : Mn;
+            L = fmaf(ex2f(pm[e] - Mz), pl[e], L * ex2f(M - Mz));
+            M = Mn;
+        }
     }
+    const float Ms = M == -INFINITY ? 0.f : M;
     const float inv = L > 0.f ? __fdiv_rn(1.0f, L) : 0.f;
     constexpr int GC = HD == 256 ? 2 : 1;  // 32 dims at a time, or 64: loads in flight
 #pragma unroll (REG ? HD / 32 : 1)
@@ -335,7 +416,7 @@ __device__ __forceinline__ void finish_cut(const PgAttnArgs &A, const PgSched &S
         for (int g = 0; g < GC; ++g) {
 #pragma unroll
             for (int e = 0; e < 32; ++e) o[g][e] *= inv;
-            if (row >= 0) put32<QT>(A, HD, row, head, 32 * (c + g), o[g]);
+            put32<QT, RING>(A, G, HD, row, head, 32 * (c + g), o[g]);
         }
     }
     __syncwarp();
@@ -621,6 +702,8 @@ __global__ void __launch_bounds__(kTcThreads, HD == 256 || sizeof(QT) == 4 ? 1 :
                 tm_wait_ld();
             }
         };
+        GateRing G;
+        if (C::RING) G.at = smem_u32(smem + C::END + sizeof(TcTail)) + warp * (32 * 64);
         fetch();
         for (bool more = true; ok && more;) {
             const int rows = W.rows(A), len = W.q.p0 + W.q.n;
@@ -628,6 +711,12 @@ __global__ void __launch_bounds__(kTcThreads, HD == 256 || sizeof(QT) == 4 ? 1 :
             const int tok = r / A.rep, head = W.kh * A.rep + r - tok * A.rep;
             const int qpos = r < rows ? pos0 + tok : -1;
             const int pmax = pos0 + (rows - 1) / A.rep;  // the tile's last position; pos0 its first
+            if (C::RING && A.gate) {
+                G.row0 = W.q.row0 + W.t * A.tq;
+                G.head0 = W.kh * A.rep;
+                G.rows = rows;
+                G.start(A, HD);
+            }
             float m = -INFINITY, l = 0.f, fold_f = 0.f;
 #pragma unroll
             for (int e = 0; e < (C::REGO ? HD : 1); ++e) o[e] = 0.f;
@@ -760,11 +849,12 @@ __global__ void __launch_bounds__(kTcThreads, HD == 256 || sizeof(QT) == 4 ? 1 :
             if (!ok) break;
             tc_after();
             if (whole)
-                finish_whole<QT, HD, C::REGO>(A, get, l, row, head);
+                finish_whole<QT, HD, C::REGO, C::RING>(A, G, get, l, row, head);
             else
-                finish_cut<QT, HD, C::REGO>(A, S, get, item0, item1, m, l, row, head);
+                finish_cut<QT, HD, C::REGO, C::RING>(A, S, G, get, item0, item1, m, l, row, head);
             tc_before();
         }
+        if (C::RING && A.gate) G.drain();
         if (!ok) bars.dead = 1u;
     }
     tc_before();
@@ -781,7 +871,7 @@ trx_status launch_tc(PgAttnArgs A, size_t part_cap, int cnt_cap, uint32_t *err, 
     static DevBits configured{0};
     const cudaError_t e = once_per_device(configured, [] {
         return cudaFuncSetAttribute(attn_paged_tc_kernel<CT, QT, HD>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                    (int)(C::END + sizeof(TcTail)));
+                                    (int)(C::END + sizeof(TcTail) + C::GBYTES));
     });
     if (e != cudaSuccess) return note_cuda(e);
     A.tq = kTcRows / A.rep;
@@ -796,7 +886,7 @@ trx_status launch_tc(PgAttnArgs A, size_t part_cap, int cnt_cap, uint32_t *err, 
     }
     const int grid = device_sms() * C::CTAS;
     if ((size_t)grid * 2 * kTcRows * (HD + 2) > part_cap || 4 * grid > cnt_cap) return TRX_ERR_UNSUPPORTED;
-    return note_cuda(launch_kernel(attn_paged_tc_kernel<CT, QT, HD>, dim3(grid), dim3(kTcThreads), C::END + sizeof(TcTail), st,
+    return note_cuda(launch_kernel(attn_paged_tc_kernel<CT, QT, HD>, dim3(grid), dim3(kTcThreads), C::END + sizeof(TcTail) + C::GBYTES, st,
                                    maps, A, err));
 }
 
