@@ -523,22 +523,23 @@ typedef struct trx_pages {
  * The plan of a step, from the lengths alone, in one launch: sequence b has d_cached[b] positions in
  * the cache and brings d_new[b] >= 0 more.  Its table's first ceil(cached / page) entries are read;
  * if it has new rows the entries up to ceil((cached + new) / page) are filled with pages from the
- * top of the free stack (d_free[0 .. *d_n_free), sequence after sequence).  Writes those table
- * entries, lens, cu, slots, pos, last and n_free; slots and pos behind the last row and all other
+ * top of the free stack (d_free[0 .. *d_n_free), of free_cap entries at most), sequence after sequence.
+ * Writes those table entries, lens, cu, slots, pos, last and n_free; slots and pos behind the last row and all other
  * table entries are left as they were, d_free too.  d_cached may be pages->lens and d_n_free
  * pages->n_free (a plan in place); otherwise the same call again gives the same plan.
- * A negative or too large length, or more rows than max_rows, sets TRX_DEV_RANGE, too few free pages
+ * A negative or too large length, or more rows than max_rows, or a stack higher than free_cap or n_pages, sets TRX_DEV_RANGE, too few free pages
  * TRX_DEV_PAGES: cu and last are then zero (the step's other calls do nothing), lens is d_cached,
  * n_free is *d_n_free.  A free-stack or table entry outside [0, n_pages) sets TRX_DEV_RANGE; its rows'
  * slots are -1.
  */
 trx_status trx_paged_plan(trx_ctx *ctx, const trx_pages *pages, const int32_t *d_cached, const int32_t *d_new,
-                          const int32_t *d_free, const int32_t *d_n_free, cudaStream_t stream);
+                          const int32_t *d_free, uint32_t free_cap, const int32_t *d_n_free, cudaStream_t stream);
 
 /*
  * Give back the pages of the sequences with d_done[b] != 0: their ceil(d_lens[b] / page) pages go on
  * top of the free stack d_free (room for n_pages) in sequence and table order, *d_n_free grows, the
- * entries become -1 and d_lens[b] 0.  If the stack would overflow, or a table entry is outside
+ * entries become -1 and d_lens[b] 0.  A page belongs to one sequence: one that two tables name would come
+ * back twice.  If the stack would overflow, or a table entry is outside
  * [0, n_pages), TRX_DEV_RANGE is set and nothing changes.  Uses pages->tables only.
  */
 trx_status trx_paged_release(trx_ctx *ctx, const trx_pages *pages, const int32_t *d_done, int32_t *d_lens,
@@ -575,9 +576,11 @@ trx_status trx_paged_append(trx_ctx *ctx, const trx_paged_shape *shape, const tr
  * head h (kv head h / (H / n_kv)), sees the positions j <= pos with pos - j < window or j < sinks
  * (all when window is 0): out[r][h] = softmax(q . K^T / sqrt(head_dim)) V, times sigmoid(gate) when
  * gated.  Decode (one new row), a prompt's chunk and a mixture of both are the same call.
- * d_q [rows][H][head_dim] of q_type (as trx_paged_append writes it), d_out the same shape and type.
+ * d_q [max_rows][H][head_dim] of q_type (as trx_paged_append writes it), d_out the same shape and type: d_q
+ * may be read, without effect, behind the last row, up to max_rows.
  * q_type fp32 (fp16 cache only): queries and softmax weights enter the tensor cores as two fp16 parts
- * each, so the result has fp32 rounding; 16-bit q_type (the cache's type): the weights are rounded to
+ * each (an element of q, below 65504, within the larger of 2^-22 of itself and 2^-25), so the result has
+ * fp32 rounding; 16-bit q_type (the cache's type): the weights are rounded to
  * that type.  Sums, maxima and the output before its rounding are fp32 in both.  d_gate (NULL unless
  * gated): the rows of d_q given to trx_paged_append, stride gate_ld floats.  max_new: a bound on the
  * new rows of any sequence (rows only; it picks the kernel).  What the pools hold behind a sequence's
@@ -599,7 +602,7 @@ trx_status trx_attn_paged(trx_ctx *ctx, const trx_paged_shape *shape, const trx_
  * >= min_p (the largest weight is 1).  The token is the first, in index order, at which the running
  * weight exceeds u times the weight of all kept (u in [0, 1)).  temperature <= 0: the largest logit,
  * ties to the smallest index (as trx_argmax_rows).  NaN logits count as -inf; a row with no logit
- * above -inf gives -1.  Weights are summed as integers (steps of 2^-40 or finer of the largest),
+ * above -inf, or with min_p above 1, gives -1.  Weights are summed as integers (steps of 2^-40 or finer of the largest),
  * so the token does not depend on the order of the sums.  V <= 2^22.  One launch, no scratch.
  */
 trx_status trx_sample_rows(trx_ctx *ctx, const void *d_logits, int32_t type, uint64_t ld, uint32_t V, uint32_t nrows,

@@ -38,7 +38,7 @@ BAD_SHAPES = [(dict(n_head=0), ARG), (dict(n_kv=0), ARG), (dict(n_head=7), ARG),
 
 
 def call_plan(L, pg, ctx=P, args=(P, P, P, P)):
-    return L.trx_paged_plan(ctx, pg, *args, N)
+    return L.trx_paged_plan(ctx, pg, *args[:3], 10, args[3], N)
 
 
 def call_append(L, sh, pg, q=P, qld=1024, k=P, kld=256, v=P, vld=256, qn=P, kn=P, f=P, kp=P, vp=P, ct=1, qo=P, qt=1):
@@ -84,7 +84,7 @@ def test_null_and_misaligned_pointers_are_refused():
         assert call_attn(L, shape(), pages(), **{f: ODD}) == ARG
     for f in ("cu", "lens"):
         assert call_attn(L, shape(), pages(**{f: None})) == ARG
-    assert L.trx_paged_plan(P, None, P, P, P, P, N) == ARG
+    assert L.trx_paged_plan(P, None, P, P, P, 10, P, N) == ARG
 
 
 def test_strides_and_types_are_refused():
@@ -138,6 +138,37 @@ def test_python_checks_name_the_argument():
         ops._mat(torch.zeros(1, 6).expand(4, 6), torch.float32, 6, "q", dev)
     with pytest.raises(ValueError):
         ops.PagedPlan(2, 8, 2, 24, 10, device="cpu")
+
+
+def test_plans_keep_their_buffers_and_device(monkeypatch):
+    """A plan's buffers cannot be replaced (the library holds their addresses), and a plan on another device
+    than the context's is refused before anything is launched."""
+    from trixium_b200 import ops
+    plan = ops.PagedPlan(2, 8, 2, 16, 10, device="cpu")
+    for name in ("lens", "tables", "max_rows", "other"):
+        with pytest.raises(AttributeError, match=name):
+            setattr(plan, name, torch.zeros(2, dtype=torch.int32))
+    plan.lens.fill_(3)
+
+    class Ctx:
+        device, h = torch.device("cuda", 0), None
+    monkeypatch.setattr(ops, "_current_device", lambda: 0)
+    monkeypatch.setattr(ops, "_raw_stream", lambda dev: 0)
+    z = torch.zeros(10, dtype=torch.int32)
+    with pytest.raises(ValueError, match="plan on cpu"):
+        ops.paged_plan(Ctx, plan, z, z, z, z)
+    with pytest.raises(ValueError, match="plan on cpu"):
+        ops.paged_release(Ctx, plan, z, z, z, z)
+    x, w = torch.zeros(8, 256), torch.zeros(64)
+    pool = torch.zeros(10, 16, 2, 64, dtype=torch.float16)
+    shape = ops.paged_shape(4, 2, 64)
+    with pytest.raises(ValueError, match="plan on cpu"):
+        ops.paged_append(Ctx, shape, plan, x, x[:, :128], x[:, 128:], w, w, w, pool, pool)
+    with pytest.raises(ValueError, match="plan on cpu"):
+        ops.attn_paged(Ctx, shape, plan, x.view(8, 4, 64), pool, pool)
+    with pytest.raises(ValueError, match="plan on cuda:1"):
+        ops._stream_of(Ctx, torch.device("cuda", 1))
+    assert ops._stream_of(Ctx, torch.device("cuda", 0)) == 0
     with pytest.raises(ValueError):
         ops.PagedPlan(0, 8, 2, 16, 10, device="cpu")
     p = ops.PagedPlan(2, 8, 2, 16, 10, device="cpu")

@@ -107,6 +107,17 @@ def test_plan_that_does_not_fit_does_nothing(ops, ctx, bad):
     assert plan.tables.tolist() == tables and plan.slots.tolist() == [-1] * rows
 
 
+def test_plan_free_stack_shorter_than_its_height(ops, ctx):
+    """n_free beyond the stack's own tensor is refused; nothing behind it is read."""
+    from trixium_b200 import _lib
+    plan = ops.PagedPlan(1, 40, 4, 16, 6)
+    ops.paged_plan(ctx, plan, i32([0]), i32([20]), i32([1, 2]), i32([3]))
+    assert ctx.errors() == _lib.DEV_RANGE
+    assert plan.cu.tolist() == [0, 0] and plan.tables.tolist() == [[-1] * 4]
+    ops.paged_plan(ctx, plan, i32([0]), i32([20]), i32([1, 2]), i32([2]))
+    assert ctx.errors() == 0 and plan.tables.tolist() == [[2, 1, -1, -1]]
+
+
 def test_plan_bad_page_id(ops, ctx):
     from trixium_b200 import _lib
     plan = ops.PagedPlan(2, 40, 4, 16, 6)
@@ -350,6 +361,78 @@ def test_attention_on_another_stream_and_in_a_graph(ops, ctx, new):
         torch.cuda.synchronize()
         C.check(q, out)
     assert ctx.errors() == 0
+
+
+@pytest.mark.parametrize("cache,qt", TYPES)
+@pytest.mark.parametrize("window,sinks", [(2 ** 30, 2 ** 30), (1, 2 ** 30), (2 ** 30, 0)])
+def test_attention_largest_window_and_sinks(ops, ctx, cache, qt, window, sinks):
+    run_case(ops, ctx, 4, 2, 64, getattr(torch, cache), getattr(torch, qt), [150, 1, 0], [400, 129, 5], 16, window, sinks)
+
+
+@pytest.mark.parametrize("new", [1, 2, 40])
+def test_attention_many_sequences(ops, ctx, new):
+    """The most sequences a plan takes, every third one idle."""
+    n = [0 if b % 3 == 2 else new for b in range(1024)]
+    run_case(ops, ctx, 4, 1, 64, torch.float16, torch.float16, n, [c + b % 50 for b, c in enumerate(n)], 16, max_new=new)
+
+
+@pytest.mark.parametrize("qt", ["float16", "float32"])
+@pytest.mark.parametrize("new", [1, 60])
+def test_attention_of_two_contexts_at_once(ops, ctx, new, qt):
+    """Two contexts on two streams, launches in turn: each the bits it gives alone."""
+    other = ops.Context(0)
+    made = []
+    for c, seed in ((ctx, 1), (other, 2)):
+        C = R.Cache(ops, [3000, 700, 64], [new, 1, 1], 2, 128, 16, torch.float16, seed)
+        q = torch.randn(C.rows, 8, 128, device="cuda").to(getattr(torch, qt))
+        shape = ops.paged_shape(8, 2, 128, rope_dims=0)
+        made.append((c, C, shape, q, ops.attn_paged(c, shape, C.plan, q, C.kp, C.vp), torch.cuda.Stream()))
+    torch.cuda.synchronize()
+    outs = []
+    for _ in range(20):
+        for c, C, shape, q, alone, s in made:
+            with torch.cuda.stream(s):
+                outs.append((ops.attn_paged(c, shape, C.plan, q, C.kp, C.vp), alone))
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for a, b in outs)
+    assert ctx.errors() == 0 and other.errors() == 0
+    other.close()
+
+
+@pytest.mark.parametrize("new", [1, 80])
+def test_pages_behind_4_billion_bytes(ops, ctx, new):
+    """A pool of more than 2^31 elements, the sequence's pages at both of its ends."""
+    kv, hd, page, L = 8, 256, 16, 100
+    n_pages = 2 ** 31 // (kv * hd * page) + 40
+    kp = torch.empty(n_pages, page, kv, hd, dtype=torch.bfloat16, device="cuda")
+    vp = torch.empty_like(kp)
+    g = torch.Generator(device="cuda").manual_seed(0)
+    k, v = [torch.randn(L, kv, hd, generator=g, device="cuda").bfloat16() for _ in range(2)]
+    ids = [n_pages - 1, 0, n_pages - 2, n_pages - 30, 1, n_pages - 3, n_pages - 31]
+    plan = ops.PagedPlan(1, new, len(ids), page, n_pages)
+    free = i32(ids[::-1])
+    old = L - new
+    have = R.pages_of(old, page)
+    plan.tables[0, :have] = i32(ids[:have])
+    for p in range(old):
+        kp[ids[p // page], p % page], vp[ids[p // page], p % page] = k[p], v[p]
+    ops.paged_plan(ctx, plan, i32([old]), i32([new]), free, i32([len(ids) - have]))
+    shape = ops.paged_shape(kv * 2, kv, hd, rope_dims=0, eps=0.0)
+    one = torch.ones(hd, device="cuda")
+    q = torch.randn(new, kv * 2 * hd, generator=g, device="cuda")
+    raw = torch.randn(new, kv * hd, generator=g, device="cuda")
+    qr = ops.paged_append(ctx, shape, plan, q, raw, v[old:].float().view(new, -1), one, one, None, kp, vp)
+    assert ctx.errors() == 0
+    for p in range(old, L):
+        assert torch.equal(vp[ids[p // page], p % page], v[p])
+        k[p] = kp[ids[p // page], p % page]
+    ref = R.rotate(raw.view(new, kv, hd), plan.pos, one[:0], one, 0.0)
+    assert bool(((k[old:].double() - ref).abs() <= ref.abs() * (2.0 ** -8 + 2.0 ** -20)).all())
+    out = ops.attn_paged(ctx, shape, plan, qr, kp, vp)
+    assert ctx.errors() == 0
+    C = R.Cache.__new__(R.Cache)
+    C.k, C.v, C.cu, C.lens, C.new = [k], [v], [0, new], [L], [new]
+    C.check(qr, out)
 
 
 # All together -----------------------------------------------------------------------------------------

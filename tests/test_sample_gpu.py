@@ -116,6 +116,40 @@ def test_sampling_odd_rows(ops, ctx, kind, V):
     check(ops, ctx, x.cuda(), rng.random(n, dtype=np.float32).tolist(), t, k, p, m)
 
 
+@pytest.mark.parametrize("V", [163841, 262147, 1000003])
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+def test_sampling_rows_beyond_shared_memory(ops, ctx, V, dtype):
+    """Rows too long to be kept on chip are read again in every pass."""
+    rng = np.random.default_rng(V)
+    x = torch.randn(5, V, generator=torch.Generator().manual_seed(V)) * 3
+    for rep in range(3):
+        t, k, p, m = settings(rng, 5)
+        check(ops, ctx, x.to(getattr(torch, dtype)).cuda(), rng.random(5, dtype=np.float32).tolist(), t, k, p, m)
+
+
+def test_sampling_many_rows(ops, ctx):
+    """More rows than clusters fit the device at once."""
+    n, V = 1500, 2003
+    rng = np.random.default_rng(2)
+    t, k, p, m = settings(rng, n)
+    check(ops, ctx, torch.randn(n, V, generator=torch.Generator().manual_seed(2)).cuda() * 3,
+          rng.random(n, dtype=np.float32).tolist(), t, k, p, m)
+
+
+def test_sampling_undefined_and_infinite_settings(ops, ctx):
+    """Settings outside the definition's ranges end in a token of the row or -1."""
+    x = torch.randn(6, 5003, generator=torch.Generator().manual_seed(4)).cuda()
+    nan, inf = float("nan"), float("inf")
+    f = lambda a: torch.tensor(a, dtype=torch.float32, device="cuda")
+    k = torch.tensor([0, 7, 0, 3000, -1, 2 ** 31 - 1], dtype=torch.int32, device="cuda")
+    for t, p, m, u in ((inf, 0.9, 0.0, 0.5), (nan, 0.9, 0.1, 0.5), (1e-40, 0.9, 0.0, 0.5), (0.8, nan, 0.0, 0.5),
+                       (0.8, 0.9, nan, 0.5), (0.8, 0.9, 0.0, nan), (0.8, 0.9, 0.0, -3.0), (0.8, 0.9, 0.0, inf),
+                       (0.8, -1.0, 0.0, 0.5), (0.8, 0.9, -1.0, 2.0), (-inf, inf, inf, 0.5), (0.8, 1e-30, 0.0, 0.5)):
+        tok = ops.sample_rows(ctx, x, f([u] * 6), f([t] * 6), k, f([p] * 6), f([m] * 6))
+        assert bool(((tok >= -1) & (tok < 5003)).all()), (t, p, m, u, tok)
+    assert ctx.errors() == 0
+
+
 def test_sampling_rows_without_a_token(ops, ctx):
     x = torch.full((3, 5000), -float("inf"), device="cuda")
     x[1] = float("nan")

@@ -180,7 +180,7 @@ def lib():
             "trx_matvec_fp_rows": ([_vp, E, _vp, _vp, ctypes.c_int32, _vp, _vp, _vp], ctypes.c_int),
             "trx_matvec_f_rows_multi": ([_vp, E, ctypes.c_int, _vp, _vp, ctypes.c_int, _vp, ctypes.c_float, _vp, _vp,
                                          _vp], ctypes.c_int),
-            "trx_paged_plan": ([_vp, P, _vp, _vp, _vp, _vp, _vp], ctypes.c_int),
+            "trx_paged_plan": ([_vp, P, _vp, _vp, _vp, ctypes.c_uint32, _vp, _vp], ctypes.c_int),
             "trx_paged_release": ([_vp, P, _vp, _vp, _vp, _vp, _vp], ctypes.c_int),
             "trx_paged_append": ([_vp, PS, P, _vp, ctypes.c_uint64, _vp, ctypes.c_uint64, _vp, ctypes.c_uint64, _vp,
                                   _vp, _vp, _vp, _vp, ctypes.c_int32, _vp, ctypes.c_int32, _vp], ctypes.c_int),

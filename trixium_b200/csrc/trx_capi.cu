@@ -927,13 +927,13 @@ static trx_status check_paged_types(int32_t cache_type, int32_t q_type) {
 }
 
 trx_status trx_paged_plan(trx_ctx *ctx, const trx_pages *pages, const int32_t *d_cached, const int32_t *d_new,
-                          const int32_t *d_free, const int32_t *d_n_free, cudaStream_t stream) {
+                          const int32_t *d_free, uint32_t free_cap, const int32_t *d_n_free, cudaStream_t stream) {
     if (!ctx) return TRX_ERR_ARG;
     if (trx_status s = check_pages(pages)) return s;
     if (!d_cached || !d_new || !d_free || !d_n_free || !pages->lens || !pages->cu || !pages->slots || !pages->pos ||
         !pages->last || !pages->n_free)
         return TRX_ERR_ARG;
-    return trx::launch_paged_plan(*pages, d_cached, d_new, d_free, d_n_free, ctx->err, stream);
+    return trx::launch_paged_plan(*pages, d_cached, d_new, d_free, free_cap, d_n_free, ctx->err, stream);
 }
 
 trx_status trx_paged_release(trx_ctx *ctx, const trx_pages *pages, const int32_t *d_done, int32_t *d_lens,

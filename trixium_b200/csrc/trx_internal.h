@@ -253,7 +253,7 @@ struct PgAttnArgs {
     float scale_log2;          // log2(e) / sqrt(hd)
 };
 trx_status launch_paged_plan(const trx_pages &P, const int *cached, const int *fresh, const int *free_pages,
-                             const int *n_free, uint32_t *err, cudaStream_t st);
+                             uint32_t free_cap, const int *n_free, uint32_t *err, cudaStream_t st);
 trx_status launch_paged_release(const trx_pages &P, const int *done, int *lens, int *free_pages, int *n_free,
                                 uint32_t *err, cudaStream_t st);
 struct PgAppendArgs {

@@ -46,7 +46,7 @@ __device__ __forceinline__ int find_le(const int *a, int n, int v) {  // a[i] <=
 
 __global__ void __launch_bounds__(kPlanThreads)
     paged_plan_kernel(const trx_pages P, int shift, const int *cached, const int *fresh, const int *free_pages,
-                      const int *n_free, uint32_t *err) {
+                      uint32_t free_cap, const int *n_free, uint32_t *err) {
     __shared__ PlanSmem sm;
     cg::cluster_group cluster = cg::this_cluster();
     const int tid = threadIdx.x, nseq = (int)P.nseq;
@@ -78,7 +78,7 @@ __global__ void __launch_bounds__(kPlanThreads)
         sm.pg[tid] = (int)(ex >> kPlanRowBits);
     }
     int bad = sm.bad;
-    if (nf < 0 || nf > (int)P.n_pages || rows > (long long)P.max_rows) bad |= TRX_DEV_RANGE;
+    if (nf < 0 || (uint32_t)nf > min(P.n_pages, free_cap) || rows > (long long)P.max_rows) bad |= TRX_DEV_RANGE;
     if (!bad && taken > nf) bad = TRX_DEV_PAGES;
     if (tid == 0) {
         sm.cu[nseq] = bad ? 0 : (int)rows;
@@ -768,7 +768,7 @@ int shift_of(uint32_t page) {
 }  // namespace
 
 trx_status launch_paged_plan(const trx_pages &P, const int *cached, const int *fresh, const int *free_pages,
-                             const int *n_free, uint32_t *err, cudaStream_t st) {
+                             uint32_t free_cap, const int *n_free, uint32_t *err, cudaStream_t st) {
     // Blocks: one per 2048 rows, at most a portable cluster.
     int nb = 1;
     while (nb < 8 && (uint32_t)nb * 2048 < P.max_rows) nb *= 2;
@@ -785,7 +785,8 @@ trx_status launch_paged_plan(const trx_pages &P, const int *cached, const int *f
     attr[1].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = attr;
     cfg.numAttrs = pdl_enabled() ? 2 : 1;
-    return note_cuda(cudaLaunchKernelEx(&cfg, paged_plan_kernel, P, shift_of(P.page), cached, fresh, free_pages, n_free, err));
+    return note_cuda(cudaLaunchKernelEx(&cfg, paged_plan_kernel, P, shift_of(P.page), cached, fresh, free_pages, free_cap,
+                                        n_free, err));
 }
 
 trx_status launch_paged_release(const trx_pages &P, const int *done, int *lens, int *free_pages, int *n_free,

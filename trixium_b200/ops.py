@@ -602,12 +602,14 @@ _TYPES = {torch.float32: _lib.TYPE_F32, torch.float16: _lib.TYPE_F16, torch.bflo
 _raw_stream, _current_device = torch._C._cuda_getCurrentRawStream, torch._C._cuda_getDevice
 
 
-def _stream_of(ctx):
+def _stream_of(ctx, on=None):
     """The current stream of the context's device, which has to be the current device (the library
-    launches on it)."""
+    launches on it) and the one that a plan's tensors are on."""
     dev = ctx.device.index or 0
     if _current_device() != dev:
         raise ValueError(f"the context is on {ctx.device}, the current device is cuda:{_current_device()}")
+    if on is not None and (on.type != "cuda" or on.index != dev):
+        raise ValueError(f"the context is on {ctx.device}, the plan on {on}")
     return _raw_stream(dev)
 
 
@@ -638,15 +640,21 @@ class PagedPlan:
     """The block tables of nseq sequences over a pool of n_pages pages of `page` positions, and the
     buffers that paged_plan fills for a step of at most max_rows new rows (trx_pages): tables
     [nseq, max_pages] (-1 at first), lens [nseq], cu [nseq + 1], slots and pos [max_rows], last [nseq],
-    n_free [1], int32."""
+    n_free [1], int32.  The buffers are written in place (by the calls, or with copy_), never replaced."""
+
+    def __setattr__(self, name, value):
+        if "_c" in self.__dict__:  # trx_pages hold the buffers' addresses
+            raise AttributeError(f"PagedPlan: {name} is fixed; write into its buffers in place")
+        self.__dict__[name] = value
 
     def __init__(self, nseq, max_rows, max_pages, page, n_pages, device=None):
-        dev = self.device = torch.device("cuda", torch.cuda.current_device()) if device is None else torch.device(device)
+        dev = torch.device("cuda", torch.cuda.current_device()) if device is None else torch.device(device)
         if min(nseq, max_rows, max_pages, n_pages) < 1 or page < 16 or page & (page - 1):
             raise ValueError("PagedPlan: sizes must be positive and the page a power of two of at least 16")
         self.nseq, self.max_rows, self.max_pages, self.page, self.n_pages = nseq, max_rows, max_pages, page, n_pages
         i32 = lambda *s: torch.zeros(*s, dtype=torch.int32, device=dev)
         self.tables = torch.full((nseq, max_pages), -1, dtype=torch.int32, device=dev)
+        self.device = self.tables.device
         self.lens, self.cu, self.last, self.n_free = i32(nseq), i32(nseq + 1), i32(nseq), i32(1)
         self.slots = torch.full((max_rows,), -1, dtype=torch.int32, device=dev)
         self.pos = torch.full((max_rows,), -1, dtype=torch.int32, device=dev)
@@ -670,14 +678,14 @@ def paged_shape(n_head, n_kv, head_dim, rope_dims=None, gated=False, eps=1e-6, w
 
 def paged_plan(ctx, plan, cached, new, free, n_free):
     """The plan of a step (trx_paged_plan): cached and new [nseq] int32, the positions every sequence has
-    in the cache and the rows it brings; free [n_pages] and n_free [1] int32, the stack of free pages and
-    its height.  Fills plan's buffers and returns it.  cached may be plan.lens and n_free plan.n_free (in
+    in the cache and the rows it brings; free [up to n_pages] and n_free [1] int32, the stack of free pages
+    and its height.  Fills plan's buffers and returns it.  cached may be plan.lens and n_free plan.n_free (in
     place); free is not changed."""
     dev = plan.device
     _lib.check(_lib.lib().trx_paged_plan(
         ctx.h, plan.pages(), _buf(cached, torch.int32, plan.nseq, "cached", dev),
-        _buf(new, torch.int32, plan.nseq, "new", dev), _buf(free, torch.int32, 1, "free", dev),
-        _buf(n_free, torch.int32, 1, "n_free", dev), _stream_of(ctx)), "trx_paged_plan")
+        _buf(new, torch.int32, plan.nseq, "new", dev), _buf(free, torch.int32, 1, "free", dev), free.numel(),
+        _buf(n_free, torch.int32, 1, "n_free", dev), _stream_of(ctx, dev)), "trx_paged_plan")
     return plan
 
 
@@ -688,7 +696,7 @@ def paged_release(ctx, plan, done, lens, free, n_free):
     _lib.check(_lib.lib().trx_paged_release(
         ctx.h, plan.pages(), _buf(done, torch.int32, plan.nseq, "done", dev),
         _buf(lens, torch.int32, plan.nseq, "lens", dev), _buf(free, torch.int32, plan.n_pages, "free", dev),
-        _buf(n_free, torch.int32, 1, "n_free", dev), _stream_of(ctx)), "trx_paged_release")
+        _buf(n_free, torch.int32, 1, "n_free", dev), _stream_of(ctx, dev)), "trx_paged_release")
 
 
 def _pools(shape, plan, kpages, vpages):
@@ -722,7 +730,7 @@ def paged_append(ctx, shape, plan, q, k, v, q_norm, k_norm, rope_freq, kpages, v
         ctx.h, shape, plan.pages(rows), qp, q_ld, kk, k_ld, vv, v_ld, _buf(q_norm, f32, hd, "q_norm", dev),
         _buf(k_norm, f32, hd, "k_norm", dev),
         _buf(rope_freq, f32, shape.rope_dims // 2, "rope_freq", dev) if shape.rope_dims else None, kp, vp, ct,
-        _buf(q_out, qt, rows * n_head * hd, "q_out", dev), _TYPES[qt], _stream_of(ctx)), "trx_paged_append")
+        _buf(q_out, qt, rows * n_head * hd, "q_out", dev), _TYPES[qt], _stream_of(ctx, dev)), "trx_paged_append")
     return q_out
 
 
@@ -746,8 +754,8 @@ def attn_paged(ctx, shape, plan, q, kpages, vpages, gate=None, max_new=None, out
         return out
     _lib.check(_lib.lib().trx_attn_paged(
         ctx.h, shape, plan.pages(rows), _buf(q, qt, rows * width, "q", dev), _TYPES[qt], gp, g_ld, kp, vp, ct,
-        rows if max_new is None else max_new, _buf(out, qt, rows * width, "out", dev), _stream_of(ctx)),
-        "trx_attn_paged")
+        rows if max_new is None else max_new, _buf(out, qt, rows * width, "out", dev),
+        _stream_of(ctx, dev)), "trx_attn_paged")
     return out
 
 
