@@ -89,8 +89,8 @@ def test_window_and_sinks_that_cover_everything_change_nothing():
     assert not torch.equal(run(window=4)[1], logits)  # (a random model's greedy tokens need not change)
 
 
-def test_refusals_and_running_out_of_pages():
-    from trixium_b200 import _lib, decoder as D
+def test_refusals():
+    from trixium_b200 import decoder as D
     with pytest.raises(ValueError, match="DeltaNet"):
         D.PagedDecoder(weights("tiny-hybrid"), 2)
     w = weights("tiny")
@@ -107,7 +107,28 @@ def test_refusals_and_running_out_of_pages():
         pd.step([[1]])
     with pytest.raises(ValueError):
         pd.generate([[1] * 33], 1)
+    with pytest.raises(ValueError, match="pass max_pos"):
+        pd.generate([[1] * 14], 4)  # 17 positions, one page of 16
+
+
+def test_few_pages():
+    """With a page for one sequence only, prompts wait for it; a step that needs a second one is refused and
+    changes nothing; capturing with every page taken works."""
+    from trixium_b200 import decoder as D
+    w = weights("tiny")
+    want = [D.Decoder(w, max_pos=32).generate(p, 4) for p in ([1, 2], [3])]
     pd = D.PagedDecoder(w, 2, max_pos=32, max_rows=16, n_pages=1)
-    with pytest.raises(_lib.TrxDeviceError) as e:
-        pd.generate([[1, 2], [3]], 4)
-    assert e.value.bits & _lib.DEV_PAGES
+    assert pd.generate([[1, 2], [3]], 4) == want
+    pd.step([[1, 2], []])
+    with pytest.raises(ValueError, match="pool"):
+        pd.step([None, [3]])
+    got = [int(pd.tok[0])]
+    pd.capture()
+    for _ in range(3):
+        pd.step([None, []])
+        got.append(int(pd.tok[0]))
+    assert got == want[0]
+    assert pd.plan.n_free.item() == 0 and pd.lens == [5, 0]
+    pd.finish([0])
+    assert pd.plan.n_free.item() == 1
+    pd.ctx.raise_on_error()

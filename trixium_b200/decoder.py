@@ -519,7 +519,8 @@ class PagedDecoder:
     append (trx_paged_append) and one attention call for all rows (trx_attn_paged, queries in fp32 as the
     other decoders keep them), then the LM head over every sequence's last row and the sampler
     (trx_sample_rows; temperature 0, the default, is the greedy token).  window and sinks limit what a row
-    sees (trx_paged_shape).  finish() returns a slot's pages to the pool."""
+    sees (trx_paged_shape).  finish() returns a slot's pages to the pool; a step that would need more pages
+    than are free is refused."""
 
     def __init__(self, weights: SyntheticWeights, nseq, ctx=None, max_pos=4096, page=16, n_pages=None, max_rows=256,
                  window=0, sinks=0):
@@ -613,6 +614,8 @@ class PagedDecoder:
                              f"{self.max_rows} rows")
         if any(n + c > self.max_pos for n, c in zip(self.lens, counts)):
             raise ValueError(f"PagedDecoder: a sequence would pass max_pos = {self.max_pos}")
+        if self._pages(n + c for n, c in zip(self.lens, counts)) > self.n_pages:
+            raise ValueError(f"PagedDecoder: the step needs more than the pool's {self.n_pages} pages (finish a slot)")
         if rows == 0:
             return
         self.lens = [n + c for n, c in zip(self.lens, counts)]
@@ -629,6 +632,9 @@ class PagedDecoder:
             self.rows_tok[idx[0]] = self.tok[idx[1]]
         self.enqueue_step(rows, top)
 
+    def _pages(self, lens):
+        return sum(-(-n // self.plan.page) for n in lens)
+
     def finish(self, slots):
         """Return the pages of these slots to the pool; the slots are empty again."""
         done = torch.zeros(self.nseq, dtype=torch.int32)
@@ -643,17 +649,14 @@ class PagedDecoder:
         def one():
             self.rows_tok[:self.nseq].copy_(self.tok)
             self.enqueue_step(self.nseq, 1)
-        self.new.fill_(1)
         s = torch.cuda.Stream()
         s.wait_stream(torch.cuda.current_stream())
-        live = [self.plan.lens, self.plan.tables, self.plan.n_free, self.tok]
-        saved = [t.clone() for t in live]
+        tok = self.tok.clone()
         with torch.cuda.stream(s):
-            self.plan.lens.zero_()  # the warm-up writes to pages of the free stack only
+            self.new.zero_()  # the warm-up brings no rows: it takes no page and writes to none
             one()
             torch.cuda.synchronize()
-        for t, c in zip(live, saved):
-            t.copy_(c)
+        self.tok.copy_(tok)
         self.graph = torch.cuda.CUDAGraph()
         with torch.cuda.stream(s):
             with torch.cuda.graph(self.graph, stream=s):
@@ -664,13 +667,18 @@ class PagedDecoder:
 
     def generate(self, prompts, n_new, sampling=None, seed=0):
         """n_new tokens after every prompt (any number of them, any lengths): prompts enter free slots in
-        order, in chunks that share the steps' rows with the decoding slots; a finished sequence's slot and
-        pages go to the next prompt.  sampling: per prompt a dict for set_sampling (None: greedy), the
+        order, as soon as the pool has the pages for all their tokens beside the sequences already in, in chunks
+        that share the steps' rows with the decoding slots; a finished sequence's slot and pages go to the next
+        prompt.  sampling: per prompt a dict for set_sampling (None: greedy), the
         random numbers from `seed`.  Returns [prompts][n_new] ids."""
         if any(len(p) == 0 for p in prompts) or n_new < 1:
             raise ValueError("PagedDecoder: prompts must hold a token, and n_new be at least 1")
         if any(self.lens):
             raise ValueError("PagedDecoder: generate needs empty slots (finish)")
+        total = [len(p) + n_new - 1 for p in prompts]  # positions at the end: the last token is not fed
+        if any(n > self.max_pos or self._pages([n]) > self.n_pages for n in total):
+            raise ValueError(f"PagedDecoder: a prompt and its {n_new} tokens pass max_pos = {self.max_pos} or the pool's "
+                             f"{self.n_pages} pages")
         gen = torch.Generator(device=self.tok.device)
         gen.manual_seed(seed)
         out = torch.empty(len(prompts), n_new, dtype=torch.int32, device=self.tok.device)
@@ -678,7 +686,8 @@ class PagedDecoder:
         waiting = list(range(len(prompts)))
         while waiting or any(slots):
             for s in range(self.nseq):
-                if slots[s] is None and waiting:
+                held = self._pages(total[t[0]] for t in slots if t)
+                if slots[s] is None and waiting and held + self._pages([total[waiting[0]]]) <= self.n_pages:
                     i = waiting.pop(0)
                     slots[s] = [i, 0, 0]
                     self.set_sampling(s, **((sampling[i] if sampling else None) or {}))
