@@ -314,18 +314,14 @@ __global__ void __launch_bounds__(kThreadsS, 2) sample_kernel(SampleArgs A, int 
             __syncthreads();
             return f;
         };
-        // This block's tokens of the row for which in(logit) holds into block 0's list (at most kList in all;
+        // Tokens of this block that are set aside in a pass, then handed to block 0's list (at most kList in all;
         // nall counts them all).
-        auto collect = [&](auto &&in) {
-            u64 *const mine = rank ? sm.list : sm.sorted;
-            if (tid == 0) sm.got = 0;
-            __syncthreads();
-            each([&](int i, float v) {
-                if (in(v)) {
-                    const uint32_t at = atomicAdd(&sm.got, 1u);
-                    if (at < kList) mine[at] = ((u64)key_of(v) << 32) | (0xffffffffu - (uint32_t)i);
-                }
-            });
+        u64 *const mine = rank ? sm.list : sm.sorted;
+        auto set_aside = [&](int i, float v) {
+            const uint32_t at = atomicAdd(&sm.got, 1u);
+            if (at < kList) mine[at] = ((u64)key_of(v) << 32) | (0xffffffffu - (uint32_t)i);
+        };
+        auto hand_over = [&] {
             __syncthreads();
             SmemS *const s0 = cluster.map_shared_rank(&sm, 0);
             const int got = min((int)sm.got, kList);
@@ -425,7 +421,10 @@ __global__ void __launch_bounds__(kThreadsS, 2) sample_kernel(SampleArgs A, int 
         if (need_k) bin_k = cross(false, (u64)k, 0.0, 0, 0);
         if (bin_k < kBins && sm.nlist <= kList) {
             // 3. The first k are among few tokens: block 0 finishes the row.
-            collect([&](float v) { return v != -INFINITY && bin_of(v) <= bin_k; });
+            each([&](int i, float v) {
+                if (v != -INFINITY && bin_of(v) <= bin_k) set_aside(i, v);
+            });
+            hand_over();
             cluster.sync();
             if (rank) return;
             const int n = rank_list(), nk = min(n, k);
@@ -510,6 +509,8 @@ __global__ void __launch_bounds__(kThreadsS, 2) sample_kernel(SampleArgs A, int 
             double target;
             for (int tries = 0;; ++tries) {
                 // Exactly: the weight kept by k, above the step, in the step; and the step's tokens.
+                if (tid == 0) sm.got = 0;
+                __syncthreads();
                 u64 sa = 0, sb = 0, sc = 0;
                 each([&](int i, float v) {
                     const int b = bin_of(v);
@@ -517,7 +518,10 @@ __global__ void __launch_bounds__(kThreadsS, 2) sample_kernel(SampleArgs A, int 
                         const u64 w = W(v);
                         if (key_of(v) > thr) sa += w;
                         if (b < guess) sb += w;
-                        if (b == guess) sc += w;
+                        if (b == guess) {
+                            sc += w;
+                            if (v != -INFINITY) set_aside(i, v);
+                        }
                     }
                 });
                 sa = warp_sum(sa);
@@ -536,7 +540,7 @@ __global__ void __launch_bounds__(kThreadsS, 2) sample_kernel(SampleArgs A, int 
                         if (lane < C) *cluster.map_shared_rank(&sm.sum[rank][q], lane) = v;
                     }
                 }
-                collect([&](float v) { return v != -INFINITY && bin_of(v) == guess; });
+                hand_over();
                 cluster.sync();
                 joined = false;
                 all = wk;
@@ -656,10 +660,46 @@ __global__ void __launch_bounds__(kThreadsS, 2) sample_kernel(SampleArgs A, int 
         return;
     }
     if (owner / kWarpsS != rank || owner % kWarpsS != warp) return;
+    // A lane sums a 32nd of the part, in index order by lane; the lane that holds the token follows from the
+    // sums, and all look for it in that lane's share.  (Scans of 32 tokens at a time along the whole part took
+    // 15,000 cycles.)
     u64 run = sm.base_mass, seen = sm.base_cnt;
-    bool done = false;
-    each([&](int i, float v) {
-        if (done) return;
+    const int share = part / 32;
+    auto at = [&](int i) {
+        if constexpr (CACHED) return cache[i];
+        return i < w1 ? fetch(i) : -INFINITY;
+    };
+    u64 s = 0;
+    uint32_t n = 0;
+    for (int i = w0 + lane * share; i < w0 + (lane + 1) * share; ++i) {
+        const float v = at(i);
+        const uint32_t key = key_of(v);
+        if (key > thr) {
+            const u64 w = W(v);
+            if (W.enough(w)) s += w;
+        } else if (key == thr && v != -INFINITY) {
+            ++n;
+        }
+    }
+    auto scan = [&](u64 v) {
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const u64 y = __shfl_up_sync(0xffffffffu, v, o);
+            if (lane >= o) v += y;
+        }
+        return v;
+    };
+    const u64 before = seen + scan(n) - n;
+    s += (before >= ties ? 0 : min((u64)ties - before, (u64)n)) * wt;
+    const u64 upto = run + scan(s);
+    const int holder = __ffs(__ballot_sync(0xffffffffu, upto > goal)) - 1;
+    if (holder < 0) return;  // (the part's own sum is past the goal)
+    run = __shfl_sync(0xffffffffu, upto - s, holder);
+    seen = __shfl_sync(0xffffffffu, before, holder);
+    const int i0 = w0 + holder * share;
+    for (int j = 0; j < share; j += 32) {
+        const int i = i0 + j + lane;
+        const float v = j + lane < share ? at(i) : -INFINITY;
         const uint32_t key = key_of(v);
         const bool tie = key == thr && v != -INFINITY;
         const unsigned bal = __ballot_sync(0xffffffffu, tie);
@@ -670,21 +710,15 @@ __global__ void __launch_bounds__(kThreadsS, 2) sample_kernel(SampleArgs A, int 
         } else if (tie && seen + __popc(bal & ((1u << lane) - 1u)) < ties) {
             w = wt;
         }
-        u64 s = w;
-#pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-            const u64 y = __shfl_up_sync(0xffffffffu, s, o);
-            if (lane >= o) s += y;
-        }
-        const unsigned hit = __ballot_sync(0xffffffffu, run + s > goal);
+        const u64 e = scan(w);
+        const unsigned hit = __ballot_sync(0xffffffffu, run + e > goal);
         if (hit) {
             if (lane == __ffs(hit) - 1) A.tokens[row] = i;
-            done = true;
             return;
         }
-        run += __shfl_sync(0xffffffffu, s, 31);
+        run += __shfl_sync(0xffffffffu, e, 31);
         seen += __popc(bal);
-    });
+    }
 }
 
 template <typename T, bool CACHED>
