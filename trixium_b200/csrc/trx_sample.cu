@@ -92,11 +92,9 @@ struct Weigh {
     int S;
     const uint2 *tab;
     __device__ __forceinline__ u64 operator()(float x) const {
-        if (x == mx) return 1ull << S;
         const float d = x - mx, c = d - x, dl = (x - (d - c)) - (mx + c);
-        const float t = d * kh;
-        if (!(t > lowest)) return 0;  // also x = -inf
-        const float tl = fmaf(d, kh, -t) + fmaf(d, kl, dl * kh);
+        const float p = d * kh, t = fmaxf(p, lowest);  // lowest also for x = -inf
+        const float tl = fmaf(d, kh, -p) + fmaf(d, kl, dl * kh);
         const float magic = 12582912.f, big = t + magic;  // the nearest whole number in its low bits
         const int n = __float_as_int(big) - __float_as_int(magic);
         const float r = (t - (big - magic)) + tl;
@@ -104,7 +102,8 @@ struct Weigh {
         const float q = fmaf(y * y, fmaf(y, fmaf(y, 1.f / 24, 1.f / 6), 0.5f), y);
         const uint2 e = tab[n & 31];
         const uint32_t m = e.x + (uint32_t)__float2int_rn(q * __uint_as_float(e.y));
-        return ((u64)m << 31) >> (62 - S - (n >> 5));
+        const u64 w = ((u64)m << 31) >> (62 - S - (n >> 5));
+        return x == mx ? 1ull << S : (p > lowest ? w : 0);
     }
     __device__ __forceinline__ bool enough(u64 w) const { return w >= minw; }
 };
@@ -205,6 +204,22 @@ __global__ void __launch_bounds__(kThreadsS, 2) sample_kernel(SampleArgs A, int 
                 f(i, cache[i]);
             else
                 f(i, i < w1 ? fetch(i) : -INFINITY);
+        }
+    };
+    // The same four at a time: f(index of the first, logits), the next 32 tokens further on each.  Sums of weights
+    // go this way: without branches between them four weights are worked on together.
+    auto each4 = [&](auto &&f) {
+        for (int i = w0 + lane; i < w0 + part; i += 128) {
+            float v[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const int j = i + 32 * e;
+                if constexpr (CACHED)
+                    v[e] = j < w0 + part ? cache[j] : -INFINITY;
+                else
+                    v[e] = j < w1 ? fetch(j) : -INFINITY;
+            }
+            f(i, v);
         }
     };
     {
@@ -421,8 +436,14 @@ __global__ void __launch_bounds__(kThreadsS, 2) sample_kernel(SampleArgs A, int 
         if (need_k) bin_k = cross(false, (u64)k, 0.0, 0, 0);
         if (bin_k < kBins && sm.nlist <= kList) {
             // 3. The first k are among few tokens: block 0 finishes the row.
-            each([&](int i, float v) {
-                if (v != -INFINITY && bin_of(v) <= bin_k) set_aside(i, v);
+            each4([&](int i, const float (&v)[4]) {
+                unsigned in = 0;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) in |= (v[e] != -INFINITY && bin_of(v[e]) <= bin_k ? 1u : 0u) << e;
+                for (; in; in &= in - 1) {
+                    const int e = __ffs(in) - 1;
+                    set_aside(i + 32 * e, e < 2 ? (e ? v[1] : v[0]) : (e > 2 ? v[3] : v[2]));
+                }
             });
             hand_over();
             cluster.sync();
@@ -512,16 +533,20 @@ __global__ void __launch_bounds__(kThreadsS, 2) sample_kernel(SampleArgs A, int 
                 if (tid == 0) sm.got = 0;
                 __syncthreads();
                 u64 sa = 0, sb = 0, sc = 0;
-                each([&](int i, float v) {
-                    const int b = bin_of(v);
-                    if (key_of(v) > thr || b == guess) {
-                        const u64 w = W(v);
-                        if (key_of(v) > thr) sa += w;
-                        if (b < guess) sb += w;
-                        if (b == guess) {
-                            sc += w;
-                            if (v != -INFINITY) set_aside(i, v);
-                        }
+                each4([&](int i, const float (&v)[4]) {
+                    unsigned in = 0;
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        const int b = bin_of(v[e]);
+                        const u64 w = W(v[e]);
+                        sa += key_of(v[e]) > thr ? w : 0;
+                        sb += b < guess ? w : 0;
+                        sc += b == guess ? w : 0;
+                        in |= (b == guess && v[e] != -INFINITY ? 1u : 0u) << e;
+                    }
+                    for (; in; in &= in - 1) {
+                        const int e = __ffs(in) - 1;
+                        set_aside(i + 32 * e, e < 2 ? (e ? v[1] : v[0]) : (e > 2 ? v[3] : v[2]));
                     }
                 });
                 sa = warp_sum(sa);
@@ -616,13 +641,19 @@ __global__ void __launch_bounds__(kThreadsS, 2) sample_kernel(SampleArgs A, int 
     // 4. The draw over the row.
     u64 mass = 0;
     uint32_t nt = 0;
-    each([&](int i, float v) {
-        const uint32_t key = key_of(v);
-        if (key > thr) {
-            const u64 w = W(v);
-            if (W.enough(w)) mass += w;
-        } else if (key == thr && v != -INFINITY) {
-            ++nt;
+    each4([&](int, const float (&v)[4]) {
+        bool any = false;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            any |= key_of(v[e]) > thr;
+            nt += key_of(v[e]) == thr && v[e] != -INFINITY ? 1u : 0u;
+        }
+        if (any) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const u64 w = W(v[e]);
+                mass += key_of(v[e]) > thr && W.enough(w) ? w : 0;
+            }
         }
     });
     mass = warp_sum(mass);
@@ -671,15 +702,13 @@ __global__ void __launch_bounds__(kThreadsS, 2) sample_kernel(SampleArgs A, int 
     };
     u64 s = 0;
     uint32_t n = 0;
+#pragma unroll 4
     for (int i = w0 + lane * share; i < w0 + (lane + 1) * share; ++i) {
         const float v = at(i);
         const uint32_t key = key_of(v);
-        if (key > thr) {
-            const u64 w = W(v);
-            if (W.enough(w)) s += w;
-        } else if (key == thr && v != -INFINITY) {
-            ++n;
-        }
+        const u64 w = W(v);
+        s += key > thr && W.enough(w) ? w : 0;
+        n += key == thr && v != -INFINITY ? 1u : 0u;
     }
     auto scan = [&](u64 v) {
 #pragma unroll
