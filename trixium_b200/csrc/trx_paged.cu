@@ -170,9 +170,11 @@ __global__ void __launch_bounds__(kPlanThreads)
 // A unit is 8 elements of a head: for u < half / 4 the pairs 4u..4u+3 and half+4u.. that the rotation
 // mixes, else 8 consecutive dims behind the rotated ones; hd / 8 neighbouring lanes hold a head, so the
 // norm is a shuffle over them and a rotation needs no exchange.  A block takes one row and a share of
-// its heads (y): its loads go out first, and meanwhile one thread per pair computes the row's cosines
-// and sines, which all heads share, into shared memory.  HBM-bound for chunks: 4 bytes in and 2 (or 4)
-// out per element.
+// its heads (y): its first loads go out, and meanwhile one thread per pair computes the row's cosines
+// and sines, which all heads share, into shared memory; then each head's loads go out a head ahead.
+// HBM-bound for chunks: 4 bytes in and 2 (or 4) out per element.  2,602 rows of 24 + 2 x 4 gated heads of
+// 256 take 26 us, 4.9 TB/s; one head's loads at a time, behind the table, and the norms' weights kept in
+// registers (4 blocks per SM for 5) took 32.  Few rows are latency: 16 of 48 heads of 128 take 2.6 us.
 constexpr int kAppThreads = 256;
 
 template <typename T> __device__ __forceinline__ void store4(T *p, float4 v) {
@@ -188,7 +190,7 @@ __device__ __forceinline__ float4 mul4(float4 a, float4 b) {
 __device__ __forceinline__ float dot4(float4 a) { return a.x * a.x + a.y * a.y + a.z * a.z + a.w * a.w; }
 
 template <typename CT, typename QT, int HD>
-__global__ void __launch_bounds__(kAppThreads) paged_append_kernel(PgAppendArgs A, uint32_t *err) {
+__global__ void __launch_bounds__(kAppThreads, 5) paged_append_kernel(PgAppendArgs A, uint32_t *err) {
     constexpr int UPH = HD / 8;               // lanes (units) per head
     constexpr int HPB = kAppThreads / UPH;    // heads a block takes at a time
     __shared__ __align__(16) float cs[HD / 2], sn[HD / 2];
@@ -198,8 +200,6 @@ __global__ void __launch_bounds__(kAppThreads) paged_append_kernel(PgAppendArgs 
     const int d0 = rot ? 4 * u : 2 * A.half + 8 * (u - A.half / 4), d1 = rot ? A.half + 4 * u : d0 + 4;
     const int heads = A.H + 2 * A.Hkv;
     pdl_wait();
-    const float4 qw0 = *reinterpret_cast<const float4 *>(A.qn + d0), qw1 = *reinterpret_cast<const float4 *>(A.qn + d1);
-    const float4 kw0 = *reinterpret_cast<const float4 *>(A.kn + d0), kw1 = *reinterpret_cast<const float4 *>(A.kn + d1);
     int rows = A.cu[A.nseq];
     if (rows > A.max_rows || rows < 0) {
         if (tid == 0 && blockIdx.x == 0 && blockIdx.y == 0) atomicOr(err, TRX_DEV_RANGE);
@@ -209,31 +209,43 @@ __global__ void __launch_bounds__(kAppThreads) paged_append_kernel(PgAppendArgs 
         const int slot = A.slots[row], pos = A.pos[row];
         const bool live = (unsigned)slot < (unsigned)A.n_slots;
         if (!live && tid == 0 && blockIdx.y == 0) atomicOr(err, TRX_DEV_RANGE);
+        // Whole groups of UPH lanes share a head; heads past the end do nothing but the shuffles.
+        auto load = [&](int h, float4 &a, float4 &b) {
+            const float *src = h < A.H ? A.q + row * A.q_ld + (long long)h * HD * (A.gated ? 2 : 1)
+                                       : (h < A.H + A.Hkv ? A.k + row * A.k_ld + (long long)(h - A.H) * HD
+                                                          : A.v + row * A.v_ld + (long long)(h - A.H - A.Hkv) * HD);
+            a = b = make_float4(0.f, 0.f, 0.f, 0.f);
+            if (h < heads) {
+                a = *reinterpret_cast<const float4 *>(src + d0);
+                b = *reinterpret_cast<const float4 *>(src + d1);
+            }
+        };
+        int h = blockIdx.y * HPB + tid / UPH;
+        float4 a, b, wa, wb;  // a head's elements, and the norm's weights (in L1 after the first row)
+        auto weights = [&](int h) {
+            const float *w = h < A.H ? A.qn : A.kn;
+            wa = __ldg(reinterpret_cast<const float4 *>(w + d0));
+            wb = __ldg(reinterpret_cast<const float4 *>(w + d1));
+        };
+        load(h, a, b);
+        weights(h);
         __syncthreads();  // the previous row's table is done with
         if (tid < A.half) {
             const float ang = __fmul_rn((float)pos, __ldg(A.freq + tid));
             sincosf(ang, &sn[tid], &cs[tid]);
         }
         __syncthreads();
-        for (int h = blockIdx.y * HPB + tid / UPH; h < (heads + HPB - 1) / HPB * HPB; h += gridDim.y * HPB) {
-            // Whole groups of UPH lanes share a head; heads past the end do nothing but the shuffles.
+        for (; h < (heads + HPB - 1) / HPB * HPB; h += gridDim.y * HPB) {
             const bool on = h < heads, is_q = h < A.H, is_k = !is_q && h < A.H + A.Hkv;
-            const float *src = is_q ? A.q + row * A.q_ld + (long long)h * HD * (A.gated ? 2 : 1)
-                                    : (is_k ? A.k + row * A.k_ld + (long long)(h - A.H) * HD
-                                            : A.v + row * A.v_ld + (long long)(h - A.H - A.Hkv) * HD);
-            float4 a = make_float4(0.f, 0.f, 0.f, 0.f), b = a;
-            if (on) {
-                a = *reinterpret_cast<const float4 *>(src + d0);
-                b = *reinterpret_cast<const float4 *>(src + d1);
-            }
+            float4 na, nb;  // the next head's, meanwhile
+            load(h + gridDim.y * HPB, na, nb);
             float ss = dot4(a) + dot4(b);
 #pragma unroll
             for (int o = UPH / 2; o; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
-            if (!on) continue;
-            if (is_q || is_k) {
+            if (on && (is_q || is_k)) {
                 const float r = __fdiv_rn(1.0f, __fsqrt_rn(__fadd_rn(__fdiv_rn(ss, (float)HD), A.eps)));
-                a = mul4(mul4(a, r), is_q ? qw0 : kw0);
-                b = mul4(mul4(b, r), is_q ? qw1 : kw1);
+                a = mul4(mul4(a, r), wa);
+                b = mul4(mul4(b, r), wb);
                 if (rot) {
                     const float4 c = *reinterpret_cast<const float4 *>(cs + 4 * u);
                     const float4 s = *reinterpret_cast<const float4 *>(sn + 4 * u);
@@ -244,16 +256,19 @@ __global__ void __launch_bounds__(kAppThreads) paged_append_kernel(PgAppendArgs 
                                     x.w * s.w + y.w * c.w);
                 }
             }
-            if (is_q) {
+            if (on && is_q) {
                 QT *dst = reinterpret_cast<QT *>(A.q_out) + ((size_t)row * A.H + h) * HD;
                 store4<QT>(dst + d0, a);
                 store4<QT>(dst + d1, b);
-            } else if (live) {
+            } else if (on && live) {
                 const int kh = is_k ? h - A.H : h - A.H - A.Hkv;
                 CT *dst = reinterpret_cast<CT *>(is_k ? A.kp : A.vp) + ((size_t)slot * A.Hkv + kh) * HD;
                 store4<CT>(dst + d0, a);
                 store4<CT>(dst + d1, b);
             }
+            a = na;
+            b = nb;
+            weights(h + gridDim.y * HPB);
         }
     }
 }
