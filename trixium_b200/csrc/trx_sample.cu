@@ -20,7 +20,10 @@
 //     collects the step's tokens, which block 0 ranks (or the step is narrowed, if they are too many).  Should
 //     the end lie in a neighbouring step after all, the pass is repeated there.
 //  4. Unless block 0 has drawn: the draw over the whole row: each warp sums its contiguous part, the
-//     parts' prefix tells which warp holds the token, and that warp scans its part again.
+//     parts' prefix tells which warp holds the token, and that warp sums its part again, a lane at a time.
+// Bound by the arithmetic of the weights (about 50 instructions each, twice 32 bits of sum) and of the counts, and
+// by the cluster's barriers: one row of 151,936 takes 18 us, 32 of them 51 us (19 MB; the bytes alone 3 us), 333
+// rows of 32,003 68 us.  A cluster per row keeps the row on chip between its three to five passes.
 #include <cstdint>
 #include <cooperative_groups.h>
 #include <cuda_bf16.h>
