@@ -205,9 +205,11 @@ __device__ __forceinline__ void pg_schedule(const PgAttnArgs &A, PgSchedSmem &sm
     if (A.nseq <= 32) {
         if (tid < 32) {
             bool bad = false;
-            int q = 0;
-            if (lane < A.nseq) q = (pg_seq(A, lane, bad).n + A.tq - 1) / A.tq;
+            PgSeq seq{};
+            if (lane < A.nseq) seq = pg_seq(A, lane, bad);
+            const int q = (seq.n + A.tq - 1) / A.tq;
             if (__any_sync(0xffffffffu, bad) && lane == 0 && blockIdx.x == 0) atomicOr(err, TRX_DEV_RANGE);
+            const bool single = !__any_sync(0xffffffffu, q > 1);  // at most one query tile each: a lane has its own
             int x = q;
 #pragma unroll
             for (int o = 1; o < 32; o <<= 1) {
@@ -221,7 +223,17 @@ __device__ __forceinline__ void pg_schedule(const PgAttnArgs &A, PgSchedSmem &sm
             if (NQ <= 32) {
                 int b = 0, t = 0;
                 PgRange R{};
-                long long u = lane < NQ ? pg_units(A, sm.qpre, lane, b, t, R) : 0, v = u;
+                long long u = 0;
+                if (single) {
+                    b = lane;
+                    if (q) {
+                        R = pg_range(A, seq, 0);
+                        u = (long long)R.cnt * A.Hkv;
+                    }
+                } else if (lane < NQ) {
+                    u = pg_units(A, sm.qpre, lane, b, t, R);
+                }
+                long long v = u;
 #pragma unroll
                 for (int o = 1; o < 32; o <<= 1) {
                     const long long y = __shfl_up_sync(0xffffffffu, v, o);
