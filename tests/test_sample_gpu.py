@@ -116,15 +116,16 @@ def test_sampling_odd_rows(ops, ctx, kind, V):
     check(ops, ctx, x.cuda(), rng.random(n, dtype=np.float32).tolist(), t, k, p, m)
 
 
+@pytest.mark.parametrize("n", [2, 5])
 @pytest.mark.parametrize("V", [163841, 262147, 1000003])
 @pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
-def test_sampling_rows_beyond_shared_memory(ops, ctx, V, dtype):
-    """Rows too long to be kept on chip are read again in every pass."""
+def test_sampling_rows_beyond_shared_memory(ops, ctx, n, V, dtype):
+    """Rows too long to be kept on chip are read again in every pass (few rows: kept by larger clusters)."""
     rng = np.random.default_rng(V)
-    x = torch.randn(5, V, generator=torch.Generator().manual_seed(V)) * 3
+    x = torch.randn(n, V, generator=torch.Generator().manual_seed(V)) * 3
     for rep in range(3):
-        t, k, p, m = settings(rng, 5)
-        check(ops, ctx, x.to(getattr(torch, dtype)).cuda(), rng.random(5, dtype=np.float32).tolist(), t, k, p, m)
+        t, k, p, m = settings(rng, n)
+        check(ops, ctx, x.to(getattr(torch, dtype)).cuda(), rng.random(n, dtype=np.float32).tolist(), t, k, p, m)
 
 
 def test_sampling_many_rows(ops, ctx):

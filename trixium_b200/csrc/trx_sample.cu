@@ -22,7 +22,7 @@
 //  4. Unless block 0 has drawn: the draw over the whole row: each warp sums its contiguous part, the
 //     parts' prefix tells which warp holds the token, and that warp sums its part again, a lane at a time.
 // Bound by the arithmetic of the weights (about 50 instructions each, twice 32 bits of sum) and of the counts, and
-// by the cluster's barriers: one row of 151,936 takes 18 us, 32 of them 51 us (19 MB; the bytes alone 3 us), 333
+// by the cluster's barriers: one row of 151,936 takes 17 us, 32 of them 51 us (19 MB; the bytes alone 3 us), 333
 // rows of 32,003 68 us.  A cluster per row keeps the row on chip between its three to five passes.
 #include <cstdint>
 #include <cooperative_groups.h>
@@ -42,7 +42,7 @@ constexpr int kThreadsS = 512;
 constexpr int kWarpsS = kThreadsS / 32;
 constexpr int kBins = kThreadsS;  // a thread has one
 constexpr int kList = 1024;
-constexpr int kMaxCluster = 8;
+constexpr int kMaxCluster = 16;
 constexpr size_t kCacheMax = 80 * 1024;  // a block's part of the row: two blocks fit an SM
 
 // Order-preserving bits of a float.
@@ -757,8 +757,9 @@ template <typename T, bool CACHED>
 cudaError_t launch_e(const SampleArgs &A, int S, int C, size_t cache, cudaStream_t st) {
     static DevBits configured{0};
     cudaError_t e = once_per_device(configured, [] {
-        return cudaFuncSetAttribute(sample_kernel<T, CACHED>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                    (int)(sizeof(SmemS) + kCacheMax));
+        const cudaError_t e = cudaFuncSetAttribute(sample_kernel<T, CACHED>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+        return e != cudaSuccess ? e : cudaFuncSetAttribute(sample_kernel<T, CACHED>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                                           (int)(sizeof(SmemS) + kCacheMax));
     });
     if (e != cudaSuccess) return e;
     cudaLaunchConfig_t cfg{};
@@ -788,8 +789,11 @@ trx_status launch_t(const SampleArgs &A, cudaStream_t st) {
     auto bytes = [&](int C) {  // of a block's part of the row
         return (size_t)((A.V + C * kWarpsS - 1) / (C * kWarpsS) + 31) / 32 * 32 * kWarpsS * 4;
     };
+    // Sixteen blocks (not 8) only while they leave half of the SMs free: 2 rows of 151,936 take 11.6 us (16.6), 3 of
+    // 600,001 45 us (71), but 9 rows 22.8 us (20.4).
+    const int most = A.nrows * kMaxCluster * 2 <= device_sms() ? kMaxCluster : 8;
     int C = 1;
-    while (C < kMaxCluster && A.V > C * 2 * kThreadsS && ((long long)A.nrows * C < device_sms() || bytes(C) > kCacheMax))
+    while (C < most && A.V > C * 2 * kThreadsS && ((long long)A.nrows * C < device_sms() || bytes(C) > kCacheMax))
         C *= 2;
     return note_cuda(bytes(C) <= kCacheMax ? launch_e<T, true>(A, S, C, bytes(C), st) : launch_e<T, false>(A, S, C, 0, st));
 }
