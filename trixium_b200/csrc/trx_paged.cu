@@ -287,7 +287,7 @@ __global__ void __launch_bounds__(kAppThreads, 5) paged_append_kernel(PgAppendAr
 // Bound by the K/V stream: rep tokens' work per byte is far below the tensor cores' rate even with 16 rows
 // padded, so the ring (64 to 192 KB per SM in flight) and short ends of pieces are what matters.
 // 3 sequences, 371 MB of fp16 K and V (16 query, 8 kv heads of 128, fp32 queries): 70 us, 5.3 TB/s.  16 sequences
-// of 900 tokens, 63 MB: 18.7 us, of which the stream is 10; the rest is the start (schedule, tables, first
+// of 900 tokens, 63 MB: 18.5 us, of which the stream is 10; the rest is the start (schedule, tables, first
 // tiles: 4 us) and the joins of cut items.
 constexpr int kDecThreads = 160;
 constexpr int kDecWarps = 4;
@@ -824,7 +824,7 @@ trx_status launch_paged_append(const PgAppendArgs &A, int cache_type, int q_type
 trx_status launch_attn_paged(const PgAttnArgs &A, int hd, int cache_type, int q_type, size_t part_cap, int cnt_cap,
                              uint32_t *err, cudaStream_t st) {
     // More query rows per kv head than the 16 of one mma.sync tile: the tcgen05 kernel, whose 128-row tiles would
-    // be mostly padding below.  16 sequences of 900 tokens, 4 (or 16) rows per kv head: 18.8 (24.2) us here, 24.6
+    // be mostly padding below.  16 sequences of 900 tokens, 4 (or 16) rows per kv head: 18.5 (24.2) us here, 24.6
     // (24.7) there; 3 sequences of 30,000 tokens, fp32 queries: 70 us here, 109 there.
     if ((long long)A.max_new * A.rep > 16) return launch_attn_paged_tc(A, hd, cache_type, q_type, part_cap, cnt_cap, err, st);
     if (cache_type == TRX_TYPE_BF16)
