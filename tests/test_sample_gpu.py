@@ -82,7 +82,7 @@ def test_sampling_matches_definition(ops, ctx, V, dtype, n):
 
 
 @pytest.mark.parametrize("kind", ["equal", "two_values", "one_high", "wide", "narrow", "minus_inf", "nan", "plus_inf",
-                                  "zeros", "lowest"])
+                                  "zeros", "signed_zeros", "lowest"])
 @pytest.mark.parametrize("V", [700, 60001])
 def test_sampling_odd_rows(ops, ctx, kind, V):
     """Ties across every border, rows with masked, infinite and undefined logits."""
@@ -110,6 +110,8 @@ def test_sampling_odd_rows(ops, ctx, kind, V):
         x = torch.zeros(n, V)
         x[:, ::2] = -0.0
         x = x + 0.0
+    elif kind == "signed_zeros":  # equal: ties by index
+        x = torch.round(x * 0.6)
     else:
         x[x < 1.2] = torch.finfo(torch.float32).min
     t, k, p, m = settings(rng, n)

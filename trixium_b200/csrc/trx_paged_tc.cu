@@ -25,9 +25,10 @@
 // one.
 //
 // Bound by the tensor cores and the power they draw for 16-bit heads of 128 (2,048 rows of 32 heads behind
-// 6,001 positions: 225 us, 1,050 TFLOP/s, in short runs, 272 in long ones; 1,600 cycles a tile for two CTAs, the MMAs alone 1,280); by
-// the softmax warps, one per scheduler, with fp32 queries (4,096 rows of 16 heads, a window of 1,024: 134 us);
-// by the K and V traffic between L2 and the SMs (46 bytes a cycle and SM) for heads of 256.
+// 6,001 positions: 225 us, 1,050 TFLOP/s, in short runs, 272 us in long ones; 1,600 cycles a tile for two CTAs,
+// the MMAs alone 1,280); by the softmax warps, one per scheduler, with fp32 queries (4,096 rows of 16 heads, a
+// window of 1,024: 134 us); by the K and V traffic between L2 and the SMs (46 bytes a cycle and SM) for heads of
+// 256.
 #include <algorithm>
 #include <cstdint>
 #include <cstring>

@@ -176,7 +176,7 @@ __global__ void __launch_bounds__(kThreadsS, 2) sample_kernel(SampleArgs A, int 
     float *const cache = reinterpret_cast<float *>(smem_raw + sizeof(SmemS)) + warp * part - w0;
     auto fetch = [&](int i) {
         const float v = load_f(x + i);
-        return v != v ? -INFINITY : v;  // NaN counts as -inf
+        return v != v ? -INFINITY : __fadd_rn(v, 0.f);  // NaN counts as -inf; -0 and 0 are equal (and one key)
     };
     // 1. Max (the first of equal ones), min.
     float vmax = -INFINITY, vmin = INFINITY;
