@@ -524,11 +524,11 @@ typedef struct trx_pages {
  * the cache and brings d_new[b] >= 0 more.  Its table's first ceil(cached / page) entries are read;
  * if it has new rows the entries up to ceil((cached + new) / page) are filled with pages from the
  * top of the free stack (d_free[0 .. *d_n_free), of free_cap entries at most), sequence after sequence.
- * Writes those table entries, lens, cu, slots, pos, last and n_free; slots and pos behind the last row and all other
- * table entries are left as they were, d_free too.  d_cached may be pages->lens and d_n_free
- * pages->n_free (a plan in place); otherwise the same call again gives the same plan.
- * A negative or too large length, or more rows than max_rows, or a stack higher than free_cap or n_pages, sets TRX_DEV_RANGE, too few free pages
- * TRX_DEV_PAGES: cu and last are then zero (the step's other calls do nothing), lens is d_cached,
+ * Writes those table entries, lens, cu, slots, pos, last and n_free; slots and pos behind the last row
+ * and all other table entries are left as they were, d_free too.  d_cached may be pages->lens and
+ * d_n_free pages->n_free (a plan in place); otherwise the same call again gives the same plan.
+ * A negative or too large length, more rows than max_rows, or a stack higher than free_cap or n_pages
+ * sets TRX_DEV_RANGE, too few free pages TRX_DEV_PAGES: cu and last are then zero (the step's other calls do nothing), lens is d_cached,
  * n_free is *d_n_free.  A free-stack or table entry outside [0, n_pages) sets TRX_DEV_RANGE; its rows'
  * slots are -1.
  */
@@ -538,9 +538,9 @@ trx_status trx_paged_plan(trx_ctx *ctx, const trx_pages *pages, const int32_t *d
 /*
  * Give back the pages of the sequences with d_done[b] != 0: their ceil(d_lens[b] / page) pages go on
  * top of the free stack d_free (room for n_pages) in sequence and table order, *d_n_free grows, the
- * entries become -1 and d_lens[b] 0.  A page belongs to one sequence: one that two tables name would come
- * back twice.  If the stack would overflow, or a table entry is outside
- * [0, n_pages), TRX_DEV_RANGE is set and nothing changes.  Uses pages->tables only.
+ * entries become -1 and d_lens[b] 0.  A page belongs to one sequence: one that two tables name would
+ * come back twice.  If the stack would overflow, or a table entry is outside [0, n_pages),
+ * TRX_DEV_RANGE is set and nothing changes.  Uses pages->tables only.
  */
 trx_status trx_paged_release(trx_ctx *ctx, const trx_pages *pages, const int32_t *d_done, int32_t *d_lens,
                              int32_t *d_free, int32_t *d_n_free, cudaStream_t stream);
@@ -602,9 +602,8 @@ trx_status trx_attn_paged(trx_ctx *ctx, const trx_paged_shape *shape, const trx_
  * >= min_p (the largest weight is 1).  The token is the first, in index order, at which the running
  * weight exceeds u times the weight of all kept (u in [0, 1)).  temperature <= 0: the largest logit,
  * ties to the smallest index.  0 and -0 are equal, NaN logits count as -inf; a row with no logit
- * above -inf, or (at temperature > 0) with min_p above 1, gives -1.  Weights are summed as integers (steps of
- * 2^-40 or finer of the largest),
- * so the token does not depend on the order of the sums.  V <= 2^22.  One launch, no scratch.
+ * above -inf, or (at temperature > 0) with min_p above 1, gives -1.  Weights are summed as integers
+ * (steps of 2^-40 or finer of the largest), so the token does not depend on the order of the sums.  V <= 2^22.  One launch, no scratch.
  */
 trx_status trx_sample_rows(trx_ctx *ctx, const void *d_logits, int32_t type, uint64_t ld, uint32_t V, uint32_t nrows,
                            const float *d_u, const float *d_temperature, const int32_t *d_top_k, const float *d_top_p,
