@@ -208,6 +208,31 @@ def test_append_matches_definition(ops, ctx, H, kv, hd, rope, gated, cache, qt):
     assert torch.equal(vp.view(-1, kv, hd)[rest], v0.view(-1, kv, hd)[rest])
 
 
+def test_append_more_rows_than_blocks(ops, ctx):
+    """70,000 rows: a block takes several."""
+    n, hd = 70000, 64
+    g = torch.Generator(device="cuda").manual_seed(9)
+    rnd = lambda *s: torch.randn(*s, generator=g, device="cuda")
+    plan = ops.PagedPlan(1, n, n // 16, 16, n // 16)
+    ops.paged_plan(ctx, plan, i32([0]), i32([n]), torch.arange(n // 16, dtype=torch.int32, device="cuda"), i32([n // 16]))
+    q, k, v = rnd(n, 2 * hd), rnd(n, hd), rnd(n, hd)
+    qn, kn = 1 + 0.1 * rnd(hd), 1 + 0.1 * rnd(hd)
+    freq = (1e4 ** (-torch.arange(hd // 2, dtype=torch.float64) / 32)).float().cuda()
+    kp = torch.zeros(n // 16, 16, 1, hd, dtype=torch.float16, device="cuda")
+    vp = torch.zeros_like(kp)
+    qo = ops.paged_append(ctx, ops.paged_shape(2, 1, hd), plan, q, k, v, qn, kn, freq, kp, vp, q_dtype=torch.float32)
+    assert ctx.errors() == 0
+    slots = plan.slots.long()
+    qr = R.rotate(q.view(n, 2, hd), plan.pos, freq, qn, 1e-6)
+    kr = R.rotate(k.view(n, 1, hd), plan.pos, freq, kn, 1e-6)
+    size = lambda x: (x.abs()[..., :hd // 2] + x.abs()[..., hd // 2:]).repeat(1, 1, 2)  # of a rotated pair
+    # As in test_append_matches_definition.
+    assert bool(((qo.double() - qr).abs() <= size(qr) * 2.0 ** -20 + qr.abs() * 2.0 ** -24).all())
+    kg = kp.view(n, 1, hd)[slots].double()
+    assert bool(((kg - kr).abs() <= size(kr) * 2.0 ** -20 + kr.abs() * 2.0 ** -11 + 2.0 ** -24).all())
+    assert torch.equal(vp.view(n, 1, hd)[slots], v.view(n, 1, hd).half())
+
+
 def test_append_bad_slots_store_nothing(ops, ctx):
     from trixium_b200 import _lib
     shape = ops.paged_shape(2, 1, 64)
