@@ -579,9 +579,9 @@ trx_status trx_paged_append(trx_ctx *ctx, const trx_paged_shape *shape, const tr
  * d_q [max_rows][H][head_dim] of q_type (as trx_paged_append writes it), d_out the same shape and type: d_q
  * may be read, without effect, behind the last row, up to max_rows.
  * q_type fp32 (fp16 cache only): queries and softmax weights enter the tensor cores as two fp16 parts
- * each (an element of q, below 65504, within the larger of 2^-22 of itself and 2^-25), so the result has
- * fp32 rounding; 16-bit q_type (the cache's type): the weights are rounded to
- * that type.  Sums, maxima and the output before its rounding are fp32 in both.  d_gate (NULL unless
+ * each (an element of q, below 65504, within the larger of 2^-22 of itself and 2^-25; a weight within the
+ * larger of 2^-22 of itself and 2^-39 of the row's largest), so the result has fp32 rounding; 16-bit
+ * q_type (the cache's type): the weights are rounded to that type.  Sums, maxima and the output before its rounding are fp32 in both.  d_gate (NULL unless
  * gated): the rows of d_q given to trx_paged_append, stride gate_ld floats.  max_new: a bound on the
  * new rows of any sequence (rows only; it picks the kernel).  What the pools hold behind a sequence's
  * length is never used; the positions below it have to be finite.  A sequence whose cu, lens or

@@ -460,6 +460,34 @@ def test_pages_behind_4_billion_bytes(ops, ctx, new):
     C.check(qr, out)
 
 
+@pytest.mark.parametrize("hd", [64, 128, 256])
+@pytest.mark.parametrize("new", [1, 60])
+def test_attention_small_weights_beside_a_large_one(ops, ctx, hd, new):
+    """fp32 queries: the largest weight meets zeros of V, so that the output is what the small weights (about
+    1e-6 of it) give; they keep their precision."""
+    L = 200
+    C = R.Cache(ops, [L], [new], 1, hd, 16, torch.float16, 8)
+    g = torch.Generator(device="cuda").manual_seed(3)
+    q = torch.randn(new, 4, hd, generator=g, device="cuda") * 3
+    # One key along the mean query: its score is some 14 above the others'.
+    k = torch.randn(L, 1, hd, generator=g, device="cuda") * 0.3
+    base = torch.randn(hd, generator=g, device="cuda")
+    q += base * 4
+    k[70, 0] = base * (14.0 * hd ** 0.5 / (4 * float(base @ base)))
+    k -= (k @ base)[..., None] / (base @ base) * base * (torch.arange(L, device="cuda")[:, None, None] != 70)
+    k = k.half()
+    v = torch.randn(L, 1, hd, generator=g, device="cuda").half()
+    v[70] = 0
+    for j in range(0, L, 16):
+        page = int(C.plan.tables[0, j // 16])
+        n = min(16, L - j)
+        C.kp[page, :n], C.vp[page, :n] = k[j:j + n], v[j:j + n]
+    C.k, C.v = [k], [v]
+    out = ops.attn_paged(ctx, ops.paged_shape(4, 1, hd, rope_dims=0), C.plan, q, C.kp, C.vp, max_new=max(new, 1))
+    assert ctx.errors() == 0
+    C.check(q, out)
+
+
 # All together -----------------------------------------------------------------------------------------
 
 @pytest.mark.parametrize("ct,qt", [("float16", "float32"), ("bfloat16", "bfloat16")])

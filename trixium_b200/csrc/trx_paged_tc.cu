@@ -14,7 +14,8 @@
 //    PgMaps); places behind the sequence's end come from outside the map, as zeros.
 //  * warps 5 and 6: issue the MMAs of the first and of the second product, each from one elected lane. Two
 //    warps, since one's instructions between two MMAs (waits, commits) take as long as the MMAs.
-// fp32 queries: Q = hi + lo and P = hi + lo in fp16, two MMAs per product, so products keep 2^-22; each
+// fp32 queries: Q = hi + lo and P = hi + lo in fp16 (P and its sum times 2^14, see kSplitScale), two MMAs per
+// product, so products keep 2^-22; each
 // tile's P V is added to an O in registers (head dim 256: tensor memory) by the softmax warps.
 // V is read as the N-major B operand of the second product straight from its row-major tile; the rows
 // of a sequence's last page behind its end are overwritten with zeros first (0 times what lies there
@@ -757,7 +758,7 @@ __global__ void __launch_bounds__(kTcThreads, HD == 256 || sizeof(QT) == 4 ? 1 :
                 float f = 1.f;
                 if constexpr (SPLIT) {  // O = O f + P V, tile by tile
                     const float mo = m;
-                    m = fmaxf(m, mx);
+                    m = fmaxf(m, ceilf(mx));  // a whole number: 14 - m below is exact, and f a power of two
                     f = m == -INFINITY ? 0.f : ex2f(mo - m);
                     l *= f;
                 } else if (j == j0) {
@@ -786,7 +787,7 @@ __global__ void __launch_bounds__(kTcThreads, HD == 256 || sizeof(QT) == 4 ? 1 :
                         tm_wait_st();
                     }
                 }
-                const float nm = m == -INFINITY ? 0.f : -m;
+                const float nm = m == -INFINITY ? 0.f : (SPLIT ? kSplitBits - m : -m);
                 float sum[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
                 for (int c = 0; c < KT / 32; ++c) {
