@@ -174,9 +174,8 @@ __global__ void __launch_bounds__(kThreadsS, 2) sample_kernel(SampleArgs A, int 
     const int part = ((V + C * kWarpsS - 1) / (C * kWarpsS) + 31) / 32 * 32;
     const int w0 = min(V, (rank * kWarpsS + warp) * part), w1 = min(V, w0 + part);
     float *const cache = reinterpret_cast<float *>(smem_raw + sizeof(SmemS)) + warp * part - w0;
-    auto fetch = [&](int i) {
-        const float v = load_f(x + i);
-        return v != v ? -INFINITY : __fadd_rn(v, 0.f);  // NaN counts as -inf; -0 and 0 are equal (and one key)
+    auto fetch = [&](int i) {  // NaN counts as -inf; -0 and 0 are equal (and one key)
+        return __fadd_rn(fmaxf(load_f(x + i), -INFINITY), 0.f);
     };
     // 1. Max (the first of equal ones), min.
     float vmax = -INFINITY, vmin = INFINITY;
