@@ -132,3 +132,27 @@ def test_few_pages():
     pd.finish([0])
     assert pd.plan.n_free.item() == 1
     pd.ctx.raise_on_error()
+
+
+def test_capture_behind_other_work_keeps_the_tokens(monkeypatch):
+    """Work that reaches the current stream right behind capture()'s wait for it delays nothing that the capture
+    needs: the slots go on from their own last tokens."""
+    from trixium_b200 import decoder as D
+    w = weights("tiny")
+    want = [D.Decoder(w, max_pos=64).generate(p, 4) for p in PROMPTS[:3]]
+    pd = D.PagedDecoder(w, 3, max_pos=64, max_rows=32)
+    pd.step(PROMPTS[:3])
+    got = [pd.tok.tolist()]
+    wait = torch.cuda.Stream.wait_stream
+
+    def wait_then_busy(self, stream):
+        wait(self, stream)
+        torch.cuda._sleep(200_000_000)  # some 0.1 s of a plain kernel
+    monkeypatch.setattr(torch.cuda.Stream, "wait_stream", wait_then_busy)
+    pd.capture()
+    monkeypatch.undo()
+    assert pd.tok.tolist() == got[0]
+    for _ in range(3):
+        pd.step([None] * 3)
+        got.append(pd.tok.tolist())
+    assert [list(t) for t in zip(*got)] == want

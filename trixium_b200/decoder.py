@@ -650,8 +650,8 @@ class PagedDecoder:
             self.rows_tok[:self.nseq].copy_(self.tok)
             self.enqueue_step(self.nseq, 1)
         s = torch.cuda.Stream()
+        tok = self.tok.clone()  # in front of the wait: the warm-up on the other stream writes tok
         s.wait_stream(torch.cuda.current_stream())
-        tok = self.tok.clone()
         with torch.cuda.stream(s):
             self.new.zero_()  # the warm-up brings no rows: it takes no page and writes to none
             one()
