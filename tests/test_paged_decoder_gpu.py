@@ -156,3 +156,35 @@ def test_capture_behind_other_work_keeps_the_tokens(monkeypatch):
         pd.step([None] * 3)
         got.append(pd.tok.tolist())
     assert [list(t) for t in zip(*got)] == want
+
+
+@pytest.mark.parametrize("graph", [False, True])
+def test_a_waiting_slot_keeps_its_token_and_logits(graph):
+    """A decoding slot waits while another goes on (and a third starts and ends), then goes on from its own
+    last token."""
+    from trixium_b200 import decoder as D
+    w = weights("tiny")
+    want = [D.Decoder(w, max_pos=64).generate(p, 7) for p in PROMPTS[:2]]
+    pd = D.PagedDecoder(w, 3, max_pos=64, max_rows=32)
+    got = [[], []]
+
+    def step(*tokens, took):
+        pd.step(list(tokens))
+        for s in took:
+            got[s].append(int(pd.tok[s]))
+    step(PROMPTS[0], PROMPTS[1], [], took=(0, 1))
+    logits = pd.logits[1].clone()
+    for third in ([], PROMPTS[2], None):
+        step(None, [], third, took=(0,))
+        assert int(pd.tok[1]) == got[1][-1] and torch.equal(pd.logits[1], logits)
+    pd.finish([2])
+    if graph:
+        pd.capture()
+        assert pd.tok.tolist()[:2] == [g[-1] for g in got] and torch.equal(pd.logits[1], logits)
+        pd.step([[], [], PROMPTS[3]])
+        step(None, None, None, took=(0, 1))
+    for _ in range(2):
+        step(None, None, [], took=(0, 1))
+    assert got[0] == want[0][:len(got[0])] and got[1] == want[1][:len(got[1])]
+    assert len(got[1]) == (4 if graph else 3)
+    pd.ctx.raise_on_error()

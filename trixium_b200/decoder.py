@@ -550,12 +550,12 @@ class PagedDecoder:
                                      gated=cfg.attn_gated, eps=cfg.eps, window=window, sinks=sinks)
         pool = lambda: torch.zeros(n_pages, page, cfg.n_kv, cfg.head_dim, dtype=torch.float16, device=dev)
         self.kp, self.vp = [pool() for _ in range(cfg.n_layer)], [pool() for _ in range(cfg.n_layer)]
-        self.x, self.h = f32(R, E), f32(nseq, E)
+        self.x, self.h, self.last = f32(R, E), f32(nseq, E), f32(nseq, E)
         self.q, self.k, self.v = f32(R, cfg.q_rows), f32(R, cfg.kv_rows), f32(R, cfg.kv_rows)
         self.qr, self.attn = f32(R, cfg.n_head, cfg.head_dim), f32(R, cfg.n_head, cfg.head_dim)
         self.g, self.u, self.act = f32(R, cfg.ffn), f32(R, cfg.ffn), f32(R, cfg.ffn)
         self.logits = f32(nseq, cfg.vocab)
-        self.rows_tok, self.new, self.tok = i32(R), i32(nseq), i32(nseq)
+        self.rows_tok, self.new, self.tok, self.drawn = i32(R), i32(nseq), i32(nseq), i32(nseq)
         # Sampling settings of every slot, and the step's random numbers.
         self.temperature, self.top_k, self.top_p, self.min_p = f32(nseq), i32(nseq), f32(nseq) + 1, f32(nseq)
         self.rand = f32(nseq)
@@ -595,18 +595,23 @@ class PagedDecoder:
                     ops.matvec_f_rows_kseg(ctx, lw["down"], self.act[g], out=self.x[g], resid=self.x[g])
                 else:
                     ops.matvec_f_rows(ctx, lw["down"], self.act[g], out=self.x[g], resid=self.x[g])
-        # Every slot's last row (row 0 for one without rows: its token is not used).
-        ops.embed_lookup_rows(ctx, self.x, plan.last, self.h)
+        # Every slot's last row.  A slot without rows (the plan gives it row 0, which is another's) keeps its
+        # own from the step before, and with it its logits; and its token.
+        live = self.new > 0
+        ops.embed_lookup_rows(ctx, self.x, plan.last, self.last)
+        torch.where(live[:, None], self.last, self.h, out=self.h)
         ops.rmsnorm_rows(ctx, self.h, w.out_norm, cfg.eps, y=self.x[:self.nseq])
         for r in range(0, self.nseq, 32):
             g = slice(r, min(r + 32, self.nseq))
             ops.matvec_f_rows(ctx, w.lm_head, self.x[g], out=self.logits[g])
         ops.sample_rows(ctx, self.logits, self.rand, self.temperature, self.top_k, self.top_p, self.min_p,
-                        tokens=self.tok)
+                        tokens=self.drawn)
+        torch.where(live, self.drawn, self.tok, out=self.tok)
 
     def step(self, tokens):
         """One step: tokens[s], the new tokens of slot s (a list; empty: the slot waits; None: its last
-        sampled token).  Afterwards self.tok[s] is the token that follows, on the device."""
+        sampled token).  Afterwards self.tok[s] is the token that follows, drawn from self.logits[s], on the
+        device; those of a slot that waits are as they were."""
         counts = [1 if t is None else len(t) for t in tokens]
         rows, top = sum(counts), max(counts, default=0)
         if len(counts) != self.nseq or rows > self.max_rows:
