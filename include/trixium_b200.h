@@ -601,9 +601,10 @@ trx_status trx_attn_paged(trx_ctx *ctx, const trx_paged_shape *shape, const trx_
  * shortest prefix whose share of the weight reaches top_p (>= 1: all); of those the ones with weight
  * >= min_p (the largest weight is 1).  The token is the first, in index order, at which the running
  * weight exceeds u times the weight of all kept (u in [0, 1)).  temperature <= 0: the largest logit,
- * ties to the smallest index.  0 and -0 are equal, NaN logits count as -inf; a row with no logit
- * above -inf, or (at temperature > 0) with min_p above 1, gives -1.  Weights are summed as integers
- * (steps of 2^-40 or finer of the largest), so the token does not depend on the order of the sums.  V <= 2^22.  One launch, no scratch.
+ * ties to the smallest index; one between 0 and 2^-100 counts as 2^-100.  0 and -0 are equal, NaN logits
+ * count as -inf; a row with no logit above -inf, or (at temperature > 0) with min_p above 1, gives -1.
+ * Weights are summed as integers (steps of 2^-40 or finer of the largest), so the token does not depend on
+ * the order of the sums.  V <= 2^22.  One launch, no scratch.
  */
 trx_status trx_sample_rows(trx_ctx *ctx, const void *d_logits, int32_t type, uint64_t ld, uint32_t V, uint32_t nrows,
                            const float *d_u, const float *d_temperature, const int32_t *d_top_k, const float *d_top_p,

@@ -210,3 +210,26 @@ def test_sampling_strided_rows_graph_and_stream(ops, ctx):
         want = ops.sample_rows(ctx, x, *args)
         assert tok.tolist() == want.tolist()
         check(ops, ctx, x, args[0].tolist(), [0.9] * 6, [40] * 6, [0.9] * 6, [0.0] * 6)
+
+
+@pytest.mark.parametrize("V", [700, 60001])
+@pytest.mark.parametrize("temperature", [1e-45, 1e-40, 4e-38, 1e-37, 7e-31, 1e-20])
+def test_sampling_tiny_temperatures(ops, ctx, V, temperature):
+    """The largest logits' ties alone have weight: the definition's token, cut by top-k and drawn by u."""
+    n = 24
+    rng = np.random.default_rng(V)
+    x = torch.round(torch.randn(n, V, generator=torch.Generator().manual_seed(V)) * 4)
+    x[::2] = torch.round(x[::2] / 8)  # many ties
+    _, k, p, m = settings(rng, n)
+    check(ops, ctx, x.cuda(), rng.random(n, dtype=np.float32).tolist(), [temperature] * n, k, p, m)
+
+
+@pytest.mark.parametrize("V", [700, 60001])
+@pytest.mark.parametrize("size", [1e-44, 1e-40, 1e-38, 1e-37, 1e-36, 1e-30])
+def test_sampling_logits_next_to_zero(ops, ctx, V, size):
+    """Equal weights in an order of their own, the logits' differences down to the smallest number."""
+    n = 24
+    rng = np.random.default_rng(V)
+    x = torch.randn(n, V, generator=torch.Generator().manual_seed(V)) * size
+    t, k, p, m = settings(rng, n)
+    check(ops, ctx, x.cuda(), rng.random(n, dtype=np.float32).tolist(), t, k, p, m)

@@ -24,6 +24,7 @@
 // Bound by the arithmetic of the weights (about 50 instructions each, twice 32 bits of sum) and of the counts, and
 // by the cluster's barriers: one row of 151,936 takes 17 us, 32 of them 51 us (19 MB; the bytes alone 3 us), 333
 // rows of 32,003 67 us.  A cluster per row keeps the row on chip between its three to five passes.
+#include <cfloat>
 #include <cstdint>
 #include <cooperative_groups.h>
 #include <cuda_bf16.h>
@@ -168,7 +169,10 @@ __global__ void __launch_bounds__(kThreadsS, 2) sample_kernel(SampleArgs A, int 
     }
     pdl_wait();
     const T *const x = reinterpret_cast<const T *>(A.x) + row * A.ld;
-    const float temp = A.temp[row], u = A.u[row], topp = A.top_p[row];
+    // Temperatures below 2^-100 count as that (NaN as 0): 32 log2(e) / T and steps of T stay finite, and weights
+    // change only where logits differ by less than 2^-94.
+    const float t_in = A.temp[row], temp = t_in > 0.f ? fmaxf(t_in, 0x1p-100f) : 0.f;
+    const float u = A.u[row], topp = A.top_p[row];
     const int k = A.top_k[row];
     // This warp's contiguous part, a multiple of 32 tokens; its e-th step of 32.
     const int part = ((V + C * kWarpsS - 1) / (C * kWarpsS) + 31) / 32 * 32;
@@ -262,9 +266,9 @@ __global__ void __launch_bounds__(kThreadsS, 2) sample_kernel(SampleArgs A, int 
         klo = min(klo, sm.lo[r]);
     }
     const uint32_t kmax = (uint32_t)(best >> 32);
-    const bool none = kmax <= kKeyNegInf, greedy = !(temp > 0.f) || k == 1 || topp <= 0.f;
+    const bool none = kmax <= kKeyNegInf, greedy = temp == 0.f || k == 1 || topp <= 0.f;
     const float minp = A.min_p[row];
-    if (none || (greedy && (!(temp > 0.f) || minp <= 1.f))) {
+    if (none || (greedy && (temp == 0.f || minp <= 1.f))) {
         if (rank == 0 && tid == 0) A.tokens[row] = none ? -1 : (int)(0xffffffffu - (uint32_t)best);
         return;
     }
@@ -284,7 +288,8 @@ __global__ void __launch_bounds__(kThreadsS, 2) sample_kernel(SampleArgs A, int 
         // 2. Counts over max - x.
         const float span = fminf(36.f * temp, W.mx - val_of(klo));
         // The last step ends short of kBins, so that only what rounds to no weight (or an infinity) is beyond.
-        const float step = span > 0.f && span < INFINITY ? (kBins - 0.5f) / span : 0.f;
+        // Of spans so small that this would overflow (logits next to 0) the steps fill the first places only.
+        const float step = span > 0.f && span < INFINITY ? fminf((kBins - 0.5f) / span, FLT_MAX) : 0.f;
         auto place = [&](float v) {  // in steps; kBins: beyond
             const float d = v == W.mx ? 0.f : W.mx - v;
             return fminf(d * step, (float)kBins);
