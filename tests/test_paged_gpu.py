@@ -488,6 +488,32 @@ def test_attention_small_weights_beside_a_large_one(ops, ctx, hd, new):
     C.check(q, out)
 
 
+@pytest.mark.parametrize("cache,qt", TYPES)
+@pytest.mark.parametrize("hd", [64, 128, 256])
+@pytest.mark.parametrize("new,lens", [([1, 1, 1], [1, 3000, 70]), ([3, 90, 1], [3, 2500, 70])])
+@pytest.mark.parametrize("value", [float("nan"), float("inf"), -float("inf")])
+def test_attention_undefined_queries_stay_undefined(ops, ctx, cache, qt, hd, new, lens, value):
+    """A query that is not finite gives NaN, as the definition does (whole and cut items, one visible position
+    and many), and every other row and head the bits it gives without it."""
+    C = R.Cache(ops, lens, new, 2, hd, 16, getattr(torch, cache), 4)
+    g = torch.Generator(device="cuda").manual_seed(5)
+    q = torch.randn(C.rows, 4, hd, generator=g, device="cuda").to(getattr(torch, qt))
+    shape = ops.paged_shape(4, 2, hd, rope_dims=0)
+    clean = ops.attn_paged(ctx, shape, C.plan, q, C.kp, C.vp, max_new=max(new))
+    bad = torch.zeros(C.rows, 4, dtype=torch.bool, device="cuda")
+    for r, h in [(0, 0), (C.rows // 2, 3), (C.rows - 1, 1)]:
+        bad[r, h] = True
+        q[r, h, 5] = value
+        b = next(b for b in range(3) if r < C.cu[b + 1])
+        i, first = r - C.cu[b], lens[b] - new[b]
+        ref = R.attention(q[r:r + 1], C.k[b][:first + i + 1], C.v[b][:first + i + 1], first + i)[0]
+        assert bool(torch.isnan(ref[0, h]).all())
+    out = ops.attn_paged(ctx, shape, C.plan, q, C.kp, C.vp, max_new=max(new))
+    assert ctx.errors() == 0
+    assert bool(torch.isnan(out[bad]).all())
+    assert torch.equal(out[~bad], clean[~bad])
+
+
 # All together -----------------------------------------------------------------------------------------
 
 @pytest.mark.parametrize("ct,qt", [("float16", "float32"), ("bfloat16", "bfloat16")])

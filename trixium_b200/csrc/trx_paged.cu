@@ -630,7 +630,8 @@ __global__ void __launch_bounds__(kDecThreads, HD == 256 ? 1 : 2)
         if (!ok) break;
         if (lane == 0) arrive(qfreed + 8u * (piece % QB));
         ++piece;
-        // The warps' parts of the piece, joined in their order, four rows at a time.
+        // The warps' parts of the piece, joined in their order, four rows at a time.  (A row sees its own position, so
+        // its sum is never 0 unless its query is not finite: the quotient is then NaN, as by the formula.)
 #pragma unroll
         for (int rr = 0; rr < 2; ++rr) {
             l[rr] += __shfl_xor_sync(0xffffffffu, l[rr], 1);
@@ -677,7 +678,7 @@ __global__ void __launch_bounds__(kDecThreads, HD == 256 ? 1 : 2)
                     acc = fmaf(e, sm.o[w][r][d], acc);
                 }
                 if (whole) {
-                    put_out<QT>(A, HD, row0 + tk, kh * A.rep + R - tk * A.rep, d, L > 0.f ? __fdiv_rn(acc, L) : 0.f);
+                    put_out<QT>(A, HD, row0 + tk, kh * A.rep + R - tk * A.rep, d, __fdiv_rn(acc, L));
                 } else {
                     part[32 + R * HD + d] = acc;
                     if (d == 0) {
@@ -727,7 +728,7 @@ __global__ void __launch_bounds__(kDecThreads, HD == 256 ? 1 : 2)
                     }
 #pragma unroll
                     for (int e = 0; e < 4; ++e)
-                        put_out<QT>(A, HD, row0 + tk, kh * A.rep + r - tk * A.rep, d + e, L > 0.f ? __fdiv_rn(acc[e], L) : 0.f);
+                        put_out<QT>(A, HD, row0 + tk, kh * A.rep + r - tk * A.rep, d + e, __fdiv_rn(acc[e], L));
                 }
                 if (tid == 0) A.cnt[c0] = 0u;
             }

@@ -319,7 +319,7 @@ __device__ __forceinline__ void load_query(const PgAttnArgs &A, unsigned char *s
 template <typename QT, int HD, bool REG, bool RING, typename Get>
 __device__ __forceinline__ void finish_whole(const PgAttnArgs &A, GateRing &G, Get &&get, float l, int row, int head) {
     if (!__any_sync(0xffffffffu, row >= 0)) return;
-    const float inv = l > 0.f ? __fdiv_rn(1.0f, l) : 0.f;
+    const float inv = __fdiv_rn(1.0f, l);  // l = 0 or NaN: a query that is not finite; its outputs are NaN
 #pragma unroll (REG ? HD / 32 : 1)
     for (int c = 0; c < HD / 32; ++c) {
         uint32_t v[32];
@@ -382,7 +382,7 @@ __device__ __forceinline__ void finish_cut(const PgAttnArgs &A, const PgSched &S
         }
     }
     const float Ms = M == -INFINITY ? 0.f : M;
-    const float inv = L > 0.f ? __fdiv_rn(1.0f, L) : 0.f;
+    const float inv = __fdiv_rn(1.0f, L);
     constexpr int GC = HD == 256 ? 2 : 1;  // 32 dims at a time, or 64: loads in flight
 #pragma unroll (REG ? HD / 32 : 1)
     for (int c = 0; c < HD / 32; c += GC) {
