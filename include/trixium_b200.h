@@ -63,7 +63,9 @@ typedef struct trx_ctx trx_ctx;
 trx_status trx_create(trx_ctx **ctx, int device);
 trx_status trx_destroy(trx_ctx *ctx);
 
-/* Synchronise `stream`, return the accumulated device error bits in *bits and clear them. */
+/* Synchronise `stream`, return the accumulated device error bits in *bits and clear them.  With
+ * TRX_DEV_TIMEOUT the context's scratch is put back in order too (results since that wait are not to be
+ * used): no other stream may be running the context's launches then. */
 trx_status trx_get_error(trx_ctx *ctx, cudaStream_t stream, uint32_t *bits);
 
 /* The message of the CUDA error behind the last TRX_ERR_CUDA returned on this thread. */

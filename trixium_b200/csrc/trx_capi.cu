@@ -157,6 +157,17 @@ trx_status trx_get_error(trx_ctx *ctx, cudaStream_t stream, uint32_t *bits) {
     if (cudaStreamSynchronize(stream) != cudaSuccess) return TRX_ERR_CUDA;
     *bits = v;
     if (v && cudaMemsetAsync(ctx->err, 0, 4, stream) != cudaSuccess) return TRX_ERR_CUDA;
+    if (v & TRX_DEV_TIMEOUT) {
+        // A launch that gave up may have left some of what has to be zero between launches: the arrival that
+        // clears a count did not come.
+        if (cudaMemsetAsync(ctx->attn_cnt, 0, kAttnMaxKv * 4, stream) != cudaSuccess ||
+            cudaMemsetAsync(ctx->amax_key, 0, kMaxArgmaxJobs * 8, stream) != cudaSuccess ||
+            cudaMemsetAsync(ctx->amax_cnt, 0, 16, stream) != cudaSuccess ||
+            cudaMemsetAsync(ctx->rows_acc, 0, kRowsAcc * 8, stream) != cudaSuccess ||
+            cudaMemsetAsync(ctx->rows_cnt, 0, kRowsCnt * 4, stream) != cudaSuccess ||
+            cudaStreamSynchronize(stream) != cudaSuccess)
+            return TRX_ERR_CUDA;
+    }
     return TRX_OK;
 }
 
