@@ -188,3 +188,14 @@ def test_a_waiting_slot_keeps_its_token_and_logits(graph):
     assert got[0] == want[0][:len(got[0])] and got[1] == want[1][:len(got[1])]
     assert len(got[1]) == (4 if graph else 3)
     pd.ctx.raise_on_error()
+
+
+def test_finish_takes_any_iterable():
+    from trixium_b200 import decoder as D
+    w = weights("tiny")
+    pd = D.PagedDecoder(w, 2, max_pos=32, max_rows=16, n_pages=2)
+    for slots in (iter([0, 1]), range(2), {1, 0}):
+        pd.step([[1, 2], [3]])
+        pd.finish(slots)
+        assert pd.lens == [0, 0] == pd.plan.lens.tolist() and pd.plan.n_free.item() == 2
+    assert pd.generate(PROMPTS[:1], 2) == [D.Decoder(w, max_pos=32).generate(PROMPTS[0], 2)]

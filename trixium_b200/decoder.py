@@ -642,8 +642,9 @@ class PagedDecoder:
 
     def finish(self, slots):
         """Return the pages of these slots to the pool; the slots are empty again."""
+        slots = list(slots)
         done = torch.zeros(self.nseq, dtype=torch.int32)
-        done[list(slots)] = 1
+        done[slots] = 1
         ops.paged_release(self.ctx, self.plan, done.to(self.tok.device), self.plan.lens, self.free, self.plan.n_free)
         for s in slots:
             self.lens[s] = 0
