@@ -199,3 +199,41 @@ def test_finish_takes_any_iterable():
         pd.finish(slots)
         assert pd.lens == [0, 0] == pd.plan.lens.tolist() and pd.plan.n_free.item() == 2
     assert pd.generate(PROMPTS[:1], 2) == [D.Decoder(w, max_pos=32).generate(PROMPTS[0], 2)]
+
+
+@pytest.mark.parametrize("graph", [False, True])
+def test_steps_draw_a_number_each(graph):
+    """Without numbers from the caller every step draws its own, the same ones again from the same seed, and the
+    tokens spread; a number that the caller wrote stays in use until it is taken back."""
+    from trixium_b200 import decoder as D
+    w = weights("tiny")
+
+    def run(seed):
+        pd = D.PagedDecoder(w, 3, max_pos=64, max_rows=16, seed=seed)
+        pd.set_sampling(0, temperature=1e4)  # near enough even over the vocabulary
+        pd.set_sampling(1, temperature=1e4)
+        pd.rand[1] = 0.5
+        pd.step([[1], [2], [3]])
+        if graph:
+            pd.capture()
+        toks = []
+        for _ in range(24):
+            pd.step([None] * 3)
+            toks.append(pd.tok.tolist())
+        pd.ctx.raise_on_error()
+        return np.array(toks), pd
+    a, pd = run(7)
+    V = pd.cfg.vocab
+    # 24 even draws of V tokens fall into both halves but for 2 in 2^24, and the same token twice in a row
+    # all along never; u = 1/2 of nearly even weights is near the middle.
+    assert 0 < (a[:, 0] < V // 2).sum() < 24 and len(set(a[:, 0])) > 4
+    assert (abs(a[:, 1] - V / 2) < V / 20).all()
+    b, _ = run(7)
+    assert (a == b).all()
+    assert (run(8)[0][:, 0] != a[:, 0]).any()
+    pd.rand[1] = float("nan")
+    later = []
+    for _ in range(24):
+        pd.step([None] * 3)
+        later.append(int(pd.tok[1]))
+    assert 0 < sum(t < V // 2 for t in later) < 24

@@ -520,10 +520,13 @@ class PagedDecoder:
     other decoders keep them), then the LM head over every sequence's last row and the sampler
     (trx_sample_rows; temperature 0, the default, is the greedy token).  window and sinks limit what a row
     sees (trx_paged_shape).  finish() returns a slot's pages to the pool; a step that would need more pages
-    than are free is refused."""
+    than are free is refused.
+
+    Random numbers: self.rand[s], in [0, 1), is what slot s is drawn with, in every step until it is changed;
+    NaN, as it is at first, stands for a new number in every step, from a generator that starts at `seed`."""
 
     def __init__(self, weights: SyntheticWeights, nseq, ctx=None, max_pos=4096, page=16, n_pages=None, max_rows=256,
-                 window=0, sinks=0):
+                 window=0, sinks=0, seed=0):
         cfg = self.cfg = weights.cfg
         if any(cfg.layer_type(l) == "d" for l in range(cfg.n_layer)):
             raise ValueError("PagedDecoder: DeltaNet layers have no paged form (BatchDecoder takes them)")
@@ -556,9 +559,11 @@ class PagedDecoder:
         self.g, self.u, self.act = f32(R, cfg.ffn), f32(R, cfg.ffn), f32(R, cfg.ffn)
         self.logits = f32(nseq, cfg.vocab)
         self.rows_tok, self.new, self.tok, self.drawn = i32(R), i32(nseq), i32(nseq), i32(nseq)
-        # Sampling settings of every slot, and the step's random numbers.
+        # Sampling settings of every slot, and the random numbers: the caller's and the step's own.
         self.temperature, self.top_k, self.top_p, self.min_p = f32(nseq), i32(nseq), f32(nseq) + 1, f32(nseq)
-        self.rand = f32(nseq)
+        self.rand, self.rand_step = f32(nseq) + float("nan"), f32(nseq)
+        self.gen = torch.Generator(device=dev)
+        self.gen.manual_seed(seed)
         self.lens = [0] * nseq  # host copy of plan.lens
         self.graph = None
 
@@ -604,7 +609,8 @@ class PagedDecoder:
         for r in range(0, self.nseq, 32):
             g = slice(r, min(r + 32, self.nseq))
             ops.matvec_f_rows(ctx, w.lm_head, self.x[g], out=self.logits[g])
-        ops.sample_rows(ctx, self.logits, self.rand, self.temperature, self.top_k, self.top_p, self.min_p,
+        u = torch.where(self.rand.isnan(), self.rand_step, self.rand)
+        ops.sample_rows(ctx, self.logits, u, self.temperature, self.top_k, self.top_p, self.min_p,
                         tokens=self.drawn)
         torch.where(live, self.drawn, self.tok, out=self.tok)
 
@@ -624,6 +630,7 @@ class PagedDecoder:
         if rows == 0:
             return
         self.lens = [n + c for n, c in zip(self.lens, counts)]
+        torch.rand(self.nseq, generator=self.gen, out=self.rand_step)
         if self.graph is not None and all(t is None for t in tokens):
             self.graph.replay()
             return
@@ -676,7 +683,7 @@ class PagedDecoder:
         order, as soon as the pool has the pages for all their tokens beside the sequences already in, in chunks
         that share the steps' rows with the decoding slots; a finished sequence's slot and pages go to the next
         prompt.  sampling: per prompt a dict for set_sampling (None: greedy), the
-        random numbers from `seed`.  Returns [prompts][n_new] ids."""
+        random numbers from `seed` (self.rand is NaN afterwards).  Returns [prompts][n_new] ids."""
         if any(len(p) == 0 for p in prompts) or n_new < 1:
             raise ValueError("PagedDecoder: prompts must hold a token, and n_new be at least 1")
         if any(self.lens):
@@ -685,8 +692,15 @@ class PagedDecoder:
         if any(n > self.max_pos or self._pages([n]) > self.n_pages for n in total):
             raise ValueError(f"PagedDecoder: a prompt and its {n_new} tokens pass max_pos = {self.max_pos} or the pool's "
                              f"{self.n_pages} pages")
-        gen = torch.Generator(device=self.tok.device)
-        gen.manual_seed(seed)
+        self.rand.fill_(float("nan"))
+        own, self.gen = self.gen, torch.Generator(device=self.tok.device)
+        self.gen.manual_seed(seed)
+        try:
+            return self._generate(prompts, n_new, sampling, total)
+        finally:
+            self.gen = own
+
+    def _generate(self, prompts, n_new, sampling, total):
         out = torch.empty(len(prompts), n_new, dtype=torch.int32, device=self.tok.device)
         slots = [None] * self.nseq   # (prompt, prompt tokens fed, tokens made)
         waiting = list(range(len(prompts)))
@@ -708,7 +722,6 @@ class PagedDecoder:
                     tokens[s] = prompts[t[0]][t[1]:t[1] + room]
                     t[1] += len(tokens[s])
                     room -= len(tokens[s])
-            torch.rand(self.nseq, generator=gen, out=self.rand)
             self.step(tokens)
             done = []
             for s, t in enumerate(slots):
