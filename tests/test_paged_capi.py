@@ -177,3 +177,38 @@ def test_plans_keep_their_buffers_and_device(monkeypatch):
         ops._pools(s, p, torch.zeros(10, 16, 2, 128), torch.zeros(10, 16, 2, 128))
     with pytest.raises(ValueError, match="vpages"):
         ops._pools(s, p, torch.zeros(10, 16, 2, 128).half(), torch.zeros(10, 16, 2, 128))
+
+
+def test_tensors_of_other_heads_are_refused(monkeypatch):
+    """Queries, outputs and pools whose heads are not the shape's: enough elements, in other places."""
+    from trixium_b200 import ops
+
+    class Ctx:
+        device, h = torch.device("cpu"), None
+    called = []
+    monkeypatch.setattr(ops, "_stream_of", lambda ctx, on=None: 0)
+    monkeypatch.setattr(ops._lib, "check", lambda status, what: called.append(what))
+    monkeypatch.setattr(ops._lib, "lib", lambda: type("L", (), {n: staticmethod(lambda *a: 0) for n in
+                                                                ("trx_attn_paged", "trx_paged_append")}))
+    plan = ops.PagedPlan(2, 8, 2, 16, 10, device="cpu")
+    shape = ops.paged_shape(4, 2, 64)
+    half = lambda *s: torch.zeros(*s, dtype=torch.float16)
+    pool, q = half(10, 16, 2, 64), half(8, 4, 64)
+    for bad in (half(8, 8, 64), half(8, 4, 128), half(8, 64, 4), half(32, 64), half(2048), half(8, 2, 4, 64)):
+        with pytest.raises(ValueError, match="q: expected"):
+            ops.attn_paged(Ctx, shape, plan, bad, pool, pool)
+        with pytest.raises(ValueError, match="out: expected"):
+            ops.attn_paged(Ctx, shape, plan, q, pool, pool, out=bad)
+        with pytest.raises(ValueError, match="q_out: expected"):
+            x, w = torch.zeros(8, 256), torch.zeros(64)
+            ops.paged_append(Ctx, shape, plan, x, x[:, :128], x[:, 128:], w, w, w, pool, pool, q_out=bad)
+    for bad in (half(10, 16, 4, 64), half(10, 16, 64, 2), half(10, 32, 2, 64), half(20, 16, 2, 128), half(10, 16, 128),
+                half(20480)):
+        with pytest.raises(ValueError, match="kpages: expected"):
+            ops.attn_paged(Ctx, shape, plan, q, bad, pool)
+        with pytest.raises(ValueError, match="vpages: expected"):
+            ops.attn_paged(Ctx, shape, plan, q, pool, bad)
+    assert not called
+    for ok in (q, q.view(8, 256)):
+        ops.attn_paged(Ctx, shape, plan, ok, pool, pool.view(160, 2, 64), out=q)
+    assert called == ["trx_attn_paged"] * 2

@@ -699,10 +699,25 @@ def paged_release(ctx, plan, done, lens, free, n_free):
         _buf(n_free, torch.int32, 1, "n_free", dev), _stream_of(ctx, dev)), "trx_paged_release")
 
 
+def _heads(t, n_head, hd, name):
+    """The rows of a [rows, n_head, hd] (or [rows, n_head * hd]) tensor."""
+    s = t.shape
+    n = len(s)
+    if n == 3 and s[1] == n_head and s[2] == hd or n == 2 and s[1] == n_head * hd:
+        return s[0]
+    raise ValueError(f"{name}: expected [rows, {n_head}, {hd}], got {tuple(s)}")
+
+
 def _pools(shape, plan, kpages, vpages):
-    n = plan.n_pages * plan.page * shape.n_kv * shape.head_dim
+    want = plan.n_pages, plan.page, shape.n_kv, shape.head_dim
+    n = want[0] * want[1] * want[2] * want[3]
     if kpages.dtype not in (torch.float16, torch.bfloat16):
         raise ValueError(f"kpages: expected float16 or bfloat16, got {kpages.dtype}")
+    if not kpages.shape == vpages.shape == want:  # more pages, or all slots in a row ([slots, n_kv, head_dim]), will do
+        for t, name in ((kpages, "kpages"), (vpages, "vpages")):
+            s = t.shape
+            if s[-2:] != want[2:] or not (len(s) == 3 or len(s) == 4 and s[1] == want[1]):
+                raise ValueError(f"{name}: expected {list(want)}, got {list(s)}")
     return (_buf(kpages, kpages.dtype, n, "kpages", plan.device), _buf(vpages, kpages.dtype, n, "vpages", plan.device),
             _TYPES[kpages.dtype])
 
@@ -723,7 +738,7 @@ def paged_append(ctx, shape, plan, q, k, v, q_norm, k_norm, rope_freq, kpages, v
     qt = q_out.dtype
     if qt is not f32 and qt is not kpages.dtype:
         raise ValueError(f"q_out: expected float32 or {kpages.dtype}, got {qt}")
-    rows = min(rows, q_out.shape[0])
+    rows = min(rows, _heads(q_out, n_head, hd, "q_out"))
     if rows == 0:
         return q_out
     _lib.check(_lib.lib().trx_paged_append(
@@ -741,11 +756,13 @@ def attn_paged(ctx, shape, plan, q, kpages, vpages, gate=None, max_new=None, out
     sequence (default: the rows of q).  Returns out, like q."""
     dev, width, qt = plan.device, shape.n_head * shape.head_dim, q.dtype
     kp, vp, ct = _pools(shape, plan, kpages, vpages)
-    rows = q.shape[0]
+    rows = _heads(q, shape.n_head, shape.head_dim, "q")
     if qt is not torch.float32 and qt is not kpages.dtype:
         raise ValueError(f"q: expected float32 or {kpages.dtype}, got {qt}")
     if out is None:
         out = torch.empty_like(q)
+    else:
+        _heads(out, shape.n_head, shape.head_dim, "out")
     gp, g_ld = None, 0
     if gate is not None:
         gp, g_ld, g_rows = _mat(gate, torch.float32, 2 * width, "gate", dev)
