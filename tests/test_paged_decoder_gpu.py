@@ -237,3 +237,22 @@ def test_steps_draw_a_number_each(graph):
         pd.step([None] * 3)
         later.append(int(pd.tok[1]))
     assert 0 < sum(t < V // 2 for t in later) < 24
+
+
+def test_an_empty_slot_has_no_last_token():
+    """None for a slot that holds no sequence is refused (its token is that of the one before), eager and captured,
+    and changes nothing."""
+    from trixium_b200 import decoder as D
+    pd = D.PagedDecoder(weights("tiny"), 2, max_pos=32, max_rows=16)
+    with pytest.raises(ValueError, match="empty slot"):
+        pd.step([None, [1]])
+    pd.step([[1, 2], [3]])
+    pd.capture()
+    pd.step([None, None])
+    pd.finish([1])
+    with pytest.raises(ValueError, match="empty slot"):
+        pd.step([None, None])
+    assert pd.lens == [3, 0] == pd.plan.lens.tolist()
+    pd.step([None, [5]])
+    pd.step([None, None])
+    assert pd.lens == [5, 2] == pd.plan.lens.tolist() and pd.ctx.errors() == 0

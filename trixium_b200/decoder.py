@@ -623,6 +623,8 @@ class PagedDecoder:
         if len(counts) != self.nseq or rows > self.max_rows:
             raise ValueError(f"PagedDecoder: {len(counts)} slots and {rows} rows, expected {self.nseq} slots and at most "
                              f"{self.max_rows} rows")
+        if any(t is None and n == 0 for t, n in zip(tokens, self.lens)):
+            raise ValueError("PagedDecoder: an empty slot has no last token to feed")
         if any(n + c > self.max_pos for n, c in zip(self.lens, counts)):
             raise ValueError(f"PagedDecoder: a sequence would pass max_pos = {self.max_pos}")
         if self._pages(n + c for n, c in zip(self.lens, counts)) > self.n_pages:
