@@ -256,3 +256,14 @@ def test_an_empty_slot_has_no_last_token():
     pd.step([None, [5]])
     pd.step([None, None])
     assert pd.lens == [5, 2] == pd.plan.lens.tolist() and pd.ctx.errors() == 0
+
+
+def test_settings_for_fewer_prompts_are_refused():
+    """Before anything runs: the slots stay empty and the next call works."""
+    from trixium_b200 import decoder as D
+    w = weights("tiny")
+    pd = D.PagedDecoder(w, 2, max_pos=32, max_rows=16)
+    with pytest.raises(ValueError, match="sampling has 2 entries for 4 prompts"):
+        pd.generate(PROMPTS, 3, sampling=[None, dict(temperature=1.0)])
+    assert pd.lens == [0, 0]
+    assert pd.generate(PROMPTS[:2], 3, sampling=[None, None]) == [D.Decoder(w, max_pos=32).generate(p, 3) for p in PROMPTS[:2]]

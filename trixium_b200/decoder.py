@@ -688,6 +688,8 @@ class PagedDecoder:
         random numbers from `seed` (self.rand is NaN afterwards).  Returns [prompts][n_new] ids."""
         if any(len(p) == 0 for p in prompts) or n_new < 1:
             raise ValueError("PagedDecoder: prompts must hold a token, and n_new be at least 1")
+        if sampling and len(sampling) < len(prompts):
+            raise ValueError(f"PagedDecoder: sampling has {len(sampling)} entries for {len(prompts)} prompts")
         if any(self.lens):
             raise ValueError("PagedDecoder: generate needs empty slots (finish)")
         total = [len(p) + n_new - 1 for p in prompts]  # positions at the end: the last token is not fed
