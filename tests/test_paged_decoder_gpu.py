@@ -267,3 +267,15 @@ def test_settings_for_fewer_prompts_are_refused():
         pd.generate(PROMPTS, 3, sampling=[None, dict(temperature=1.0)])
     assert pd.lens == [0, 0]
     assert pd.generate(PROMPTS[:2], 3, sampling=[None, None]) == [D.Decoder(w, max_pos=32).generate(p, 3) for p in PROMPTS[:2]]
+
+
+@pytest.mark.parametrize("bad", ["x", 2 ** 40, None])
+def test_a_step_of_no_tokens_changes_nothing(bad):
+    """Tokens that are no 32-bit integers raise before anything is done."""
+    from trixium_b200 import decoder as D
+    w = weights("tiny")
+    pd = D.PagedDecoder(w, 2, max_pos=32, max_rows=16)
+    with pytest.raises((ValueError, TypeError, RuntimeError)):
+        pd.step([[1, bad], [2]])
+    assert pd.lens == [0, 0] == pd.plan.lens.tolist()
+    assert pd.generate(PROMPTS[:1], 2) == [D.Decoder(w, max_pos=32).generate(PROMPTS[0], 2)]

@@ -631,13 +631,13 @@ class PagedDecoder:
             raise ValueError(f"PagedDecoder: the step needs more than the pool's {self.n_pages} pages (finish a slot)")
         if rows == 0:
             return
-        self.lens = [n + c for n, c in zip(self.lens, counts)]
+        host = torch.tensor([t for seq in tokens for t in ([0] if seq is None else seq)], dtype=torch.int32)
+        self.lens = [n + c for n, c in zip(self.lens, counts)]  # (tokens that are no int32 have raised by now)
         torch.rand(self.nseq, generator=self.gen, out=self.rand_step)
         if self.graph is not None and all(t is None for t in tokens):
             self.graph.replay()
             return
-        host = [t for seq in tokens for t in ([0] if seq is None else seq)]
-        self.rows_tok[:rows].copy_(torch.tensor(host, dtype=torch.int32))
+        self.rows_tok[:rows].copy_(host)
         self.new.copy_(torch.tensor(counts, dtype=torch.int32))
         fed = [s for s, t in enumerate(tokens) if t is None]
         if fed:  # rows whose token is still on the device only
