@@ -514,6 +514,25 @@ def test_attention_undefined_queries_stay_undefined(ops, ctx, cache, qt, hd, new
     assert torch.equal(out[~bad], clean[~bad])
 
 
+@pytest.mark.parametrize("new", [1, 60])
+@pytest.mark.parametrize("field,value", [("lens", -2 ** 31), ("lens", -1), ("lens", 0), ("lens", 2 ** 31 - 1),
+                                         ("cu", -2 ** 31), ("cu", 2 ** 31 - 1)])
+def test_attention_lengths_and_offsets_far_out_of_range(ops, ctx, field, value, new):
+    """The ends of 32 bits where a sequence's length or offset should be: its rows stay as they were (an offset's
+    neighbour's too), the others are right."""
+    from trixium_b200 import _lib
+    C = R.Cache(ops, [300, 200, 150], [new, new, new], 2, 64, 16, torch.float16, 3)
+    q = torch.randn(C.rows, 4, 64, device="cuda").half()
+    getattr(C.plan, field)[1] = value
+    out = torch.full_like(q, 9.0)
+    ops.attn_paged(ctx, ops.paged_shape(4, 2, 64, rope_dims=0), C.plan, q, C.kp, C.vp, out=out, max_new=new)
+    assert ctx.errors() == _lib.DEV_RANGE
+    for b in (1,) if field == "lens" else (0, 1):
+        assert bool((out[C.cu[b]:C.cu[b + 1]] == 9.0).all())
+        C.new[b] = 0
+    C.check(q, out)
+
+
 # All together -----------------------------------------------------------------------------------------
 
 @pytest.mark.parametrize("ct,qt", [("float16", "float32"), ("bfloat16", "bfloat16")])

@@ -74,16 +74,17 @@ struct PgSeq {
 // The sequence's rows and positions, or n = 0 for one whose offsets or length are out of range
 // (bad is then set; nothing outside the buffers is read or written for it).
 __device__ __forceinline__ PgSeq pg_seq(const PgAttnArgs &A, int b, bool &bad) {
-    PgSeq S;
+    PgSeq S{};
     const int c0 = A.cu[b], c1 = A.cu[b + 1], len = A.lens[b];
+    // Compared before it is subtracted: no difference of what passes leaves 32 bits.
+    if (c0 < 0 || c1 < c0 || c1 > A.max_rows || c1 - c0 > A.max_new || len < c1 - c0 ||
+        (c1 > c0 && (long long)len > (long long)A.max_pages << A.page_shift)) {
+        bad = true;
+        return S;
+    }
     S.row0 = c0;
     S.n = c1 - c0;
     S.p0 = len - S.n;
-    if (c0 < 0 || c1 < c0 || c1 > A.max_rows || S.n > A.max_new || S.p0 < 0 ||
-        (S.n && (long long)len > (long long)A.max_pages << A.page_shift)) {
-        bad = true;
-        S.n = 0;
-    }
     return S;
 }
 
