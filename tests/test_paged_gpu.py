@@ -533,6 +533,42 @@ def test_attention_lengths_and_offsets_far_out_of_range(ops, ctx, field, value, 
     C.check(q, out)
 
 
+@pytest.mark.parametrize("cache,qt,size", [(*t, s) for t in TYPES for s in (0.5, 4.0, 32.0, 256.0, 4096.0)] +
+                         [("bfloat16", "bfloat16", 2.0 ** 40)])
+@pytest.mark.parametrize("hd", [64, 128, 256])
+@pytest.mark.parametrize("new", [1, 150])
+@pytest.mark.parametrize("window,sinks", [(0, 0), (50, 3)])
+def test_attention_large_scores(ops, ctx, cache, qt, size, hd, new, window, sinks):
+    """Scores up to 2^30 (bf16: 2^58), far beyond what their rounding leaves of a weight's exponent: every next
+    key scores higher by more than that rounding, so the softmax is the last visible key's alone (the keys of the
+    bf16 case come in fours of equal keys with equal values) and the output its value."""
+    L, dt = 400, getattr(torch, cache)
+    C = R.Cache(ops, [L], [new], 1, hd, 16, dt, 8)
+    g = torch.Generator(device="cuda").manual_seed(3)
+    sign = (torch.rand(hd, generator=g, device="cuda") < 0.5).float() * 2 - 1
+    at = torch.arange(L, device="cuda")
+    k = ((4096 + (8 * at if cache == "float16" else 32 * (at // 4)))[:, None, None].float() * sign).to(dt)  # exact
+    v = torch.randn(L, 1, hd, generator=g, device="cuda").to(dt)
+    if cache != "float16":
+        v = v[at // 4 * 4]
+    for j in range(0, L, 16):
+        page = int(C.plan.tables[0, j // 16])
+        C.kp[page], C.vp[page] = k[j:j + 16], v[j:j + 16]
+    # Scores of one row differ by at least 8 * size * hd (32 for bf16) / sqrt(hd) from key to key: 32 for the smallest,
+    # a weight of 2^-46.  Rounded to 32 bits a score is off by 16 * 2^-23 of at most 2 * 7300 * size * sqrt(hd), less
+    # than 1 / 250 of that difference.
+    q = ((1 + torch.rand(new, 4, 1, generator=g, device="cuda")) * size * sign).to(getattr(torch, qt))
+    shape = ops.paged_shape(4, 1, hd, rope_dims=0, window=window, sinks=sinks)
+    out = ops.attn_paged(ctx, shape, C.plan, q, C.kp, C.vp, max_new=new)
+    assert ctx.errors() == 0
+    want = v[L - new:].expand(new, 4, hd).double()
+    # The weight and the output are rounded to the type (fp32 queries: the weight to 2^-22), sums and quotient to 2^-20.
+    h = torch.finfo(q.dtype).eps / 2
+    tol = want.abs() * (2 * h + h * h + 2.0 ** -20) + 2.0 ** -40 * float(v.abs().max()) + \
+        (torch.finfo(dt).tiny * torch.finfo(dt).eps if q.dtype == dt else 0)
+    assert bool(((out.double() - want).abs() <= tol).all())
+
+
 # All together -----------------------------------------------------------------------------------------
 
 @pytest.mark.parametrize("ct,qt", [("float16", "float32"), ("bfloat16", "bfloat16")])

@@ -430,6 +430,46 @@ __device__ __forceinline__ void finish_cut(const PgAttnArgs &A, const PgSched &S
     if (lane == 0) *cnt = 0u;
 }
 
+// A tile's weights where scores lie beyond kFar (in powers of 2).  One FMA gives a weight's exponent elsewhere, and
+// m was rounded to 32 bits: from there on that is no longer a small common factor of the row's weights, but 2^16 and
+// more, or 2^-64.  So the products are rounded as m was, the largest to m itself.  A function, reading the row of S
+// again (visible: e <= hi and (e >= lo or e < sk)): in the loop this cost 12 % of a long chunk with fp32 queries.
+constexpr float kFar = 0x1p20f;
+template <typename CT, bool SPLIT>
+__device__ __noinline__ float far_weights(uint32_t ts, bool far, float m, float nm, float scale, int hi, int lo, int sk) {
+    float sum[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 1
+    for (int c = 0; c < 2; ++c) {
+        uint32_t v[32], ph[16];
+        // Column 32 c of S is read before anything is written there.
+        tm_ld32(ts + 32 * c, v);
+        tm_wait_ld();
+#pragma unroll
+        for (int e = 0; e < 32; ++e) {
+            const int k = 32 * c + e;
+            const float x = k > hi || (k < lo && k >= sk) ? -INFINITY : __uint_as_float(v[e]);
+            const float near = fmaf(x, scale, nm);
+            const float p = ex2f(far ? __fadd_rn(__fsub_rn(__fmul_rn(x, scale), m), SPLIT ? kSplitBits : 0.f) : near);
+            v[e] = __float_as_uint(p);
+            sum[e & 3] += p;
+        }
+#pragma unroll
+        for (int e = 0; e < 16; ++e) ph[e] = PgCvt<CT>::pack(__uint_as_float(v[2 * e]), __uint_as_float(v[2 * e + 1]));
+        if constexpr (SPLIT) {
+            tm_st16(ts + 32 * c, ph);
+#pragma unroll
+            for (int e = 0; e < 16; ++e) {
+                const float2 b = PgCvt<CT>::unpack(ph[e]);
+                ph[e] = PgCvt<CT>::pack(__uint_as_float(v[2 * e]) - b.x, __uint_as_float(v[2 * e + 1]) - b.y);
+            }
+            tm_st16(ts + 32 * c + 16, ph);
+        } else {
+            tm_st16(ts + 16 * c, ph);
+        }
+    }
+    return (sum[0] + sum[1]) + (sum[2] + sum[3]);
+}
+
 template <typename CT, typename QT, int HD>
 __global__ void __launch_bounds__(kTcThreads, HD == 256 || sizeof(QT) == 4 ? 1 : 2)
     attn_paged_tc_kernel(const __grid_constant__ PgMaps maps, const __grid_constant__ PgAttnArgs A, uint32_t *err) {
@@ -764,7 +804,7 @@ __global__ void __launch_bounds__(kTcThreads, HD == 256 || sizeof(QT) == 4 ? 1 :
                 } else if (j == j0) {
                     m = mx;
                 } else {
-                    const bool grow = mx > m + 8.f;
+                    const bool grow = mx - m > 8.f;  // (m + 8 would round to m for large scores)
                     if (__any_sync(0xffffffffu, grow)) {
                         if (!wait2(odone, j - 1)) {
                             ok = false;
@@ -788,33 +828,39 @@ __global__ void __launch_bounds__(kTcThreads, HD == 256 || sizeof(QT) == 4 ? 1 :
                     }
                 }
                 const float nm = m == -INFINITY ? 0.f : (SPLIT ? kSplitBits - m : -m);
-                float sum[4] = {0.f, 0.f, 0.f, 0.f};
+                const bool far = fabsf(mx) >= kFar && mx != -INFINITY;
+                if (__any_sync(0xffffffffu, far)) {
+                    const int hi = qpos - k0, lo = A.window ? hi - A.window + 1 : -1, sk = A.sinks - k0;
+                    l += far_weights<CT, SPLIT>(ts, far, m, nm, A.scale_log2, open ? KT : hi, open ? -1 : lo, sk);
+                } else {
+                    float sum[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-                for (int c = 0; c < KT / 32; ++c) {
-                    uint32_t ph[16];
+                    for (int c = 0; c < KT / 32; ++c) {
+                        uint32_t ph[16];
 #pragma unroll
-                    for (int e = 32 * c; e < 32 * c + 32; ++e) {
-                        const float p = ex2f(fmaf(__uint_as_float(v[e]), A.scale_log2, nm));
-                        v[e] = __float_as_uint(p);
-                        sum[e & 3] += p;
-                    }
-#pragma unroll
-                    for (int e = 0; e < 16; ++e)
-                        ph[e] = PgCvt<CT>::pack(__uint_as_float(v[32 * c + 2 * e]), __uint_as_float(v[32 * c + 2 * e + 1]));
-                    if constexpr (SPLIT) {
-                        tm_st16(ts + 32 * c, ph);
-#pragma unroll
-                        for (int e = 0; e < 16; ++e) {
-                            const float2 b = PgCvt<CT>::unpack(ph[e]);
-                            ph[e] = PgCvt<CT>::pack(__uint_as_float(v[32 * c + 2 * e]) - b.x,
-                                                    __uint_as_float(v[32 * c + 2 * e + 1]) - b.y);
+                        for (int e = 32 * c; e < 32 * c + 32; ++e) {
+                            const float p = ex2f(fmaf(__uint_as_float(v[e]), A.scale_log2, nm));
+                            v[e] = __float_as_uint(p);
+                            sum[e & 3] += p;
                         }
-                        tm_st16(ts + 32 * c + 16, ph);
-                    } else {
-                        tm_st16(ts + 16 * c, ph);
+#pragma unroll
+                        for (int e = 0; e < 16; ++e)
+                            ph[e] = PgCvt<CT>::pack(__uint_as_float(v[32 * c + 2 * e]), __uint_as_float(v[32 * c + 2 * e + 1]));
+                        if constexpr (SPLIT) {
+                            tm_st16(ts + 32 * c, ph);
+#pragma unroll
+                            for (int e = 0; e < 16; ++e) {
+                                const float2 b = PgCvt<CT>::unpack(ph[e]);
+                                ph[e] = PgCvt<CT>::pack(__uint_as_float(v[32 * c + 2 * e]) - b.x,
+                                                        __uint_as_float(v[32 * c + 2 * e + 1]) - b.y);
+                            }
+                            tm_st16(ts + 32 * c + 16, ph);
+                        } else {
+                            tm_st16(ts + 16 * c, ph);
+                        }
                     }
+                    l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
                 }
-                l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
                 if (k0 + KT > len) {  // the rows of V behind the sequence's end
                     if (!wait(vfull + 8u * (j % KST), (uint32_t)(j / KST))) {
                         ok = false;
