@@ -1,6 +1,7 @@
 """The paged KV cache on the GPU: the plan (trx_paged_plan, trx_paged_release), the append
 (trx_paged_append) and attention over the pages (trx_attn_paged), each against a plain restatement
 (tests/paged_ref.py), and a run of them together against the batch decoder's arithmetic."""
+import math
 import random
 
 import pytest
@@ -551,9 +552,7 @@ def test_attention_large_scores(ops, ctx, cache, qt, size, hd, new, window, sink
     v = torch.randn(L, 1, hd, generator=g, device="cuda").to(dt)
     if cache != "float16":
         v = v[at // 4 * 4]
-    for j in range(0, L, 16):
-        page = int(C.plan.tables[0, j // 16])
-        C.kp[page], C.vp[page] = k[j:j + 16], v[j:j + 16]
+    put_pages(C, k, v)
     # Scores of one row differ by at least 8 * size * hd (32 for bf16) / sqrt(hd) from key to key: 32 for the smallest,
     # a weight of 2^-46.  Rounded to 32 bits a score is off by 16 * 2^-23 of at most 2 * 7300 * size * sqrt(hd), less
     # than 1 / 250 of that difference.
@@ -567,6 +566,42 @@ def test_attention_large_scores(ops, ctx, cache, qt, size, hd, new, window, sink
     tol = want.abs() * (2 * h + h * h + 2.0 ** -20) + 2.0 ** -40 * float(v.abs().max()) + \
         (torch.finfo(dt).tiny * torch.finfo(dt).eps if q.dtype == dt else 0)
     assert bool(((out.double() - want).abs() <= tol).all())
+
+
+def put_pages(C, k, v):
+    """The pools' positions of a cache of one sequence."""
+    for j in range(0, len(k), 16):
+        page, n = int(C.plan.tables[0, j // 16]), min(16, len(k) - j)
+        C.kp[page, :n], C.vp[page, :n] = k[j:j + n], v[j:j + n]
+
+
+@pytest.mark.parametrize("hd", [64, 128, 256])
+@pytest.mark.parametrize("new", [1, 150])
+def test_attention_smallest_weights_of_fp32_queries(ops, ctx, hd, new):
+    """In every sixteen positions one of a large weight whose value is 0: the output is what the small weights give,
+    2^-24 to 2^-34 of the large ones and equal, so that their errors add up: each is within the larger of 2^-22 of
+    itself and 2^-39 of the row's largest."""
+    L = 400
+    C = R.Cache(ops, [L], [new], 1, hd, 16, torch.float16, 8)
+    g = torch.Generator(device="cuda").manual_seed(3)
+    base = torch.randn(hd, generator=g, device="cuda").half()
+    k = (base.float() / 8).half().expand(L, 1, hd).clone()
+    k[::16, 0] = base
+    v = torch.full((L, 1, hd), 1024.0, dtype=torch.float16, device="cuda")
+    v[::16] = 0
+    put_pages(C, k, v)
+    seen = torch.arange(L - new, L, device="cuda").double()[:, None, None] + 1
+    large = torch.ceil(seen / 16)
+    for rep in range(1 if new > 1 else 60):
+        d = (24 + 10 * torch.rand(new, 4, 1, generator=g, device="cuda")) * 8 / 7  # 7/8 of it: log2 of large over small
+        q = base.float() * (d * math.log(2) * math.sqrt(hd) / float(base.float() @ base.float()))
+        out = ops.attn_paged(ctx, ops.paged_shape(4, 1, hd, rope_dims=0), C.plan, q, C.kp, C.vp, max_new=new)
+        assert ctx.errors() == 0
+        ref, mag, smax = R.attention(q, k, v, L - new)
+        ds = smax * (17 * 2.0 ** -23 + 2.0 ** -22)
+        tol = mag * (2.0 ** -22 + 2 * ds + 2.0 ** -19 + L * 2.0 ** -26) + 2.0 ** -39 / large * (seen - large) * 1024
+        worst = float(((out.double() - ref).abs() / tol).max())
+        assert worst <= 1.0, worst
 
 
 # All together -----------------------------------------------------------------------------------------

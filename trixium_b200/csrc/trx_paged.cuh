@@ -61,10 +61,12 @@ __device__ __forceinline__ float ex2f(float x) {
     return y;
 }
 
-// Softmax weights that are split into two fp16 parts are scaled by 2^14 first (their sum too, so the quotient is the
-// same): the parts then keep 2^-22 of a weight down to 2^-28 of the row's largest, and 2^-39 of that below, where
-// unscaled ones kept 2^-25: too little where the largest weight meets values near 0.
-constexpr float kSplitBits = 14.f, kSplitScale = 16384.f;
+// Softmax weights that are split into two fp16 parts are scaled by 2^15 first (their sum too, so the quotient is the
+// same).  The parts' last place is 2^-24 at the least, so they keep 2^-22 of a scaled weight down to 2^-3 and are within
+// 2^-25 below.  The largest is 2^15, or in the tcgen05 kernel, whose maxima are whole numbers rounded up, above 2^14:
+// 2^-22 of a weight down to 2^-17 of the row's largest, and 2^-39 of the largest below, where unscaled ones would keep
+// 2^-25: too little where the largest weight meets values near 0.
+constexpr float kSplitBits = 15.f, kSplitScale = 32768.f;
 
 // One sequence of an attention launch: its new rows [row0, row0 + n) at positions [p0, p0 + n).
 struct PgSeq {

@@ -14,7 +14,7 @@
 //    PgMaps); places behind the sequence's end come from outside the map, as zeros.
 //  * warps 5 and 6: issue the MMAs of the first and of the second product, each from one elected lane. Two
 //    warps, since one's instructions between two MMAs (waits, commits) take as long as the MMAs.
-// fp32 queries: Q = hi + lo and P = hi + lo in fp16 (P and its sum times 2^14, see kSplitScale), two MMAs per
+// fp32 queries: Q = hi + lo and P = hi + lo in fp16 (P and its sum times 2^15, see kSplitScale), two MMAs per
 // product, so products keep 2^-22; each
 // tile's P V is added to an O in registers (head dim 256: tensor memory) by the softmax warps.
 // V is read as the N-major B operand of the second product straight from its row-major tile; the rows
@@ -798,7 +798,7 @@ __global__ void __launch_bounds__(kTcThreads, HD == 256 || sizeof(QT) == 4 ? 1 :
                 float f = 1.f;
                 if constexpr (SPLIT) {  // O = O f + P V, tile by tile
                     const float mo = m;
-                    m = fmaxf(m, ceilf(mx));  // a whole number: 14 - m below is exact, and f a power of two
+                    m = fmaxf(m, ceilf(mx));  // a whole number: 15 - m below is exact, and f a power of two
                     f = m == -INFINITY ? 0.f : ex2f(mo - m);
                     l *= f;
                 } else if (j == j0) {
