@@ -583,14 +583,15 @@ trx_status trx_paged_append(trx_ctx *ctx, const trx_paged_shape *shape, const tr
  * q_type fp32 (fp16 cache only): queries and softmax weights enter the tensor cores as two fp16 parts
  * each (an element of q, below 65504, within the larger of 2^-22 of itself and 2^-25; a weight within the
  * larger of 2^-22 of itself and 2^-39 of the row's largest), so the result has fp32 rounding; 16-bit
- * q_type (the cache's type): the weights are rounded to that type.  Sums, maxima and the output before its rounding are fp32 in both.  d_gate (NULL unless
- * gated): the rows of d_q given to trx_paged_append, stride gate_ld floats.  max_new: a bound on the
- * new rows of any sequence (rows only; it picks the kernel).  What the pools hold behind a sequence's
- * length is never used; the positions below it have to be finite.  A head of a row of q with an element that is
- * not finite (in fp16, for fp32 queries) gives NaN, and the other rows and heads as ever.  A sequence whose cu, lens or
- * max_new do not fit sets TRX_DEV_RANGE and its rows are left as they were; a table entry outside
- * [0, n_pages) sets TRX_DEV_RANGE and reads as zeros.  Rows behind the last are left as they were.
- * Launches on the context's scratch: calls on one context must not overlap.
+ * q_type (the cache's type): the weights are rounded to that type (bf16: 2^-8 of itself; fp16: the larger of 2^-11
+ * of itself and 2^-32 of the row's largest).  Sums, maxima and the output before its rounding are fp32 in
+ * both.  d_gate (NULL unless gated): the rows of d_q given to trx_paged_append, stride gate_ld floats.
+ * max_new: a bound on the new rows of any sequence (rows only; it picks the kernel).  What the pools hold
+ * behind a sequence's length is never used; the positions below it have to be finite.  A head of a row of q
+ * with an element that is not finite (in fp16, for fp32 queries) gives NaN, and the other rows and heads as
+ * ever.  A sequence whose cu, lens or max_new do not fit sets TRX_DEV_RANGE and its rows are left as they
+ * were; a table entry outside [0, n_pages) sets TRX_DEV_RANGE and reads as zeros.  Rows behind the last are
+ * left as they were.  Launches on the context's scratch: calls on one context must not overlap.
  */
 trx_status trx_attn_paged(trx_ctx *ctx, const trx_paged_shape *shape, const trx_pages *pages, const void *d_q,
                           int32_t q_type, const float *d_gate, uint64_t gate_ld, const void *d_kpages,

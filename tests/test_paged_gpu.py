@@ -575,6 +575,40 @@ def put_pages(C, k, v):
         C.kp[page, :n], C.vp[page, :n] = k[j:j + n], v[j:j + n]
 
 
+@pytest.mark.parametrize("cache,qt", [("float16", "float16"), ("bfloat16", "bfloat16")])
+@pytest.mark.parametrize("hd", [64, 128, 256])
+@pytest.mark.parametrize("new", [1, 60])
+def test_attention_small_weights_of_16_bit_queries(ops, ctx, cache, qt, hd, new):
+    """In every sixteen positions one of a large weight whose value is 0: the output is what the small weights
+    (about 2^-23 of the large ones) give.  A weight is kept to half a step of the type, in fp16 or 2^-32 of the
+    row's largest."""
+    L, dt = 200, getattr(torch, cache)
+    C = R.Cache(ops, [L], [new], 1, hd, 16, dt, 8)
+    g = torch.Generator(device="cuda").manual_seed(3)
+    base = torch.randn(hd, generator=g, device="cuda")
+    base /= base.norm()
+    q = (base * 8 + torch.randn(new, 4, hd, generator=g, device="cuda") * 0.3).to(dt)
+    k = torch.randn(L, 1, hd, generator=g, device="cuda") * 0.3
+    k -= (k @ base)[..., None] * base
+    k[6::16, 0] = base * (16 * hd ** 0.5 / 8)  # a score of some 16
+    k = k.to(dt)
+    v = (torch.randn(L, 1, hd, generator=g, device="cuda") * 512).to(dt)
+    v[6::16] = 0
+    put_pages(C, k, v)
+    out = ops.attn_paged(ctx, ops.paged_shape(4, 1, hd, rope_dims=0), C.plan, q, C.kp, C.vp, max_new=new)
+    assert ctx.errors() == 0
+    ref, mag, smax = R.attention(q, k, v, L - new)
+    # As in Cache.check; in fp16 besides 2^-32 of the row's largest weight for every position that it sees.
+    h = torch.finfo(dt).eps / 2
+    ds = smax * (17 * 2.0 ** -23 + 2.0 ** -22)
+    tol = h * ref.abs() + mag * (h + 2 * ds + 2.0 ** -19 + L * 2.0 ** -26) + torch.finfo(dt).tiny * torch.finfo(dt).eps
+    if dt == torch.float16:
+        seen = R.visible(L - new, new, L, 0, 0, "cuda")[:, None]
+        s = (q.double() @ k[:, 0].double().T / math.sqrt(hd)).masked_fill(~seen, -math.inf)
+        tol = tol + 2.0 ** -32 * torch.softmax(s, -1).amax(-1, keepdim=True) * (seen.double() @ v[:, 0].double().abs())
+    assert float(((out.double() - ref).abs() / tol).max()) <= 1.0
+
+
 @pytest.mark.parametrize("hd", [64, 128, 256])
 @pytest.mark.parametrize("new", [1, 150])
 def test_attention_smallest_weights_of_fp32_queries(ops, ctx, hd, new):

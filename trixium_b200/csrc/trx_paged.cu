@@ -582,7 +582,7 @@ __global__ void __launch_bounds__(kDecThreads, HD == 256 ? 1 : 2)
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
                     p[e] = ex2f(x[e] - ms);
-                    if constexpr (SPLIT) p[e] *= kSplitScale;
+                    if constexpr (!PgIsBf16<CT>::value) p[e] *= kSplitScale;  // at most 2^15 in one part or two
                     sum += p[e];
                 }
                 l[rr] = l[rr] * al + sum;

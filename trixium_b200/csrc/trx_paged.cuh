@@ -61,12 +61,20 @@ __device__ __forceinline__ float ex2f(float x) {
     return y;
 }
 
+template <typename CT> struct PgIsBf16 { static constexpr bool value = false; };
+template <> struct PgIsBf16<__nv_bfloat16> { static constexpr bool value = true; };
+
 // Softmax weights that are split into two fp16 parts are scaled by 2^15 first (their sum too, so the quotient is the
 // same).  The parts' last place is 2^-24 at the least, so they keep 2^-22 of a scaled weight down to 2^-3 and are within
 // 2^-25 below.  The largest is 2^15, or in the tcgen05 kernel, whose maxima are whole numbers rounded up, above 2^14:
 // 2^-22 of a weight down to 2^-17 of the row's largest, and 2^-39 of the largest below, where unscaled ones would keep
 // 2^-25: too little where the largest weight meets values near 0.
 constexpr float kSplitBits = 15.f, kSplitScale = 32768.f;
+// Single fp16 weights are scaled too: by 2^15 in the mma.sync kernel, by 2^7 in the tcgen05 kernel, whose weights reach
+// 2^8 before.  They keep 2^-11 of themselves down to 2^-29 (2^-21) of the row's largest, and 2^-40 (2^-32) of the
+// largest below, where unscaled ones would lose bits from 2^-14 on and vanish at 2^-25.  bf16 ones have the range.
+template <typename CT>
+constexpr float kHalfBits = PgIsBf16<CT>::value ? 0.f : 7.f;
 
 // One sequence of an attention launch: its new rows [row0, row0 + n) at positions [p0, p0 + n).
 struct PgSeq {
@@ -359,9 +367,6 @@ struct PgWalk {
 __device__ __forceinline__ bool pg_hidden(int k, int p, int window, int sinks) {
     return k > p || (window && p - k >= window && k >= sinks);
 }
-
-template <typename CT> struct PgIsBf16 { static constexpr bool value = false; };
-template <> struct PgIsBf16<__nv_bfloat16> { static constexpr bool value = true; };
 
 template <typename CT> struct PgCvt;
 template <> struct PgCvt<__half> {

@@ -9,7 +9,8 @@
 //  * warps 0-3: one query row per thread (its TMEM lane).  They put an fp32 query tile into shared memory (a
 //    16-bit one comes by TMA), read S from tensor memory, keep the row's maximum and sum, write P (16 bits) over S as the A operand
 //    of the second product, and finish the piece.  O is rescaled only when a row's maximum has grown by
-//    more than 2^8 over the one in use: P then stays below 2^8, exact in any 16-bit float's exponent.
+//    more than 2^8 over the one in use: P then stays below 2^8 (fp16: 2^15, see kHalfBits), exact in any 16-bit
+//    float's exponent.
 //  * warp 4: the producer.  A key tile is gathered by TMA boxes of one page (or the tile's part of it, see
 //    PgMaps); places behind the sequence's end come from outside the map, as zeros.
 //  * warps 5 and 6: issue the MMAs of the first and of the second product, each from one elected lane. Two
@@ -802,9 +803,9 @@ __global__ void __launch_bounds__(kTcThreads, HD == 256 || sizeof(QT) == 4 ? 1 :
                     f = m == -INFINITY ? 0.f : ex2f(mo - m);
                     l *= f;
                 } else if (j == j0) {
-                    m = mx;
+                    m = mx - kHalfBits<CT>;  // the reference of O, l and the weights
                 } else {
-                    const bool grow = mx - m > 8.f;  // (m + 8 would round to m for large scores)
+                    const bool grow = mx - m > 8.f + kHalfBits<CT>;  // (m + 8 would round to m for large scores)
                     if (__any_sync(0xffffffffu, grow)) {
                         if (!wait2(odone, j - 1)) {
                             ok = false;
@@ -812,8 +813,9 @@ __global__ void __launch_bounds__(kTcThreads, HD == 256 || sizeof(QT) == 4 ? 1 :
                         }
                         tc_after();
                         // A row without a maximum so far has O = 0 and l = 0.
-                        f = grow && m != -INFINITY ? ex2f(m - mx) : 1.f;
-                        if (grow) m = mx;
+                        const float ref = mx - kHalfBits<CT>;
+                        f = grow && m != -INFINITY ? ex2f(m - ref) : 1.f;
+                        if (grow) m = ref;
                         l *= f;
 #pragma unroll 1
                         for (int c = 0; c < HD / 32; ++c) {
