@@ -434,10 +434,14 @@ __device__ __forceinline__ void finish_cut(const PgAttnArgs &A, const PgSched &S
 // A tile's weights where scores lie beyond kFar (in powers of 2).  One FMA gives a weight's exponent elsewhere, and
 // m was rounded to 32 bits: from there on that is no longer a small common factor of the row's weights, but 2^16 and
 // more, or 2^-64.  So the products are rounded as m was, the largest to m itself.  A function, reading the row of S
-// again (visible: e <= hi and (e >= lo or e < sk)): in the loop this cost 12 % of a long chunk with fp32 queries.
+// again (visible: k <= hi and (k >= lo or k < sk)): in the loop this cost 12 % of a long chunk with fp32 queries; this
+// way the question costs 1 to 2.5 % (2,048 rows behind 6,001 positions in fp16: 231 us in short runs, 226 without;
+// differences of scores instead of products for every tile: 243).
 constexpr float kFar = 0x1p20f;
 template <typename CT, bool SPLIT>
-__device__ __noinline__ float far_weights(uint32_t ts, bool far, float m, float nm, float scale, int hi, int lo, int sk) {
+__device__ __noinline__ float far_weights(const PgAttnArgs &A, uint32_t ts, bool far, float m, int hi, int k0) {
+    const float scale = A.scale_log2, bits = SPLIT ? kSplitBits : 0.f, nm = m == -INFINITY ? 0.f : bits - m;
+    const int lo = A.window ? hi - A.window + 1 : -1, sk = A.sinks - k0;
     float sum[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll 1
     for (int c = 0; c < 2; ++c) {
@@ -450,7 +454,7 @@ __device__ __noinline__ float far_weights(uint32_t ts, bool far, float m, float 
             const int k = 32 * c + e;
             const float x = k > hi || (k < lo && k >= sk) ? -INFINITY : __uint_as_float(v[e]);
             const float near = fmaf(x, scale, nm);
-            const float p = ex2f(far ? __fadd_rn(__fsub_rn(__fmul_rn(x, scale), m), SPLIT ? kSplitBits : 0.f) : near);
+            const float p = ex2f(far ? __fadd_rn(__fsub_rn(__fmul_rn(x, scale), m), bits) : near);
             v[e] = __float_as_uint(p);
             sum[e & 3] += p;
         }
@@ -797,16 +801,21 @@ __global__ void __launch_bounds__(kTcThreads, HD == 256 || sizeof(QT) == 4 ? 1 :
                 mx *= A.scale_log2;
                 if (r >= rows) mx = -INFINITY;
                 float f = 1.f;
+                const bool far = fabsf(mx) >= kFar && mx != -INFINITY;
+                bool any_far = false;  // of the warp's rows (asked together with what else is rare)
                 if constexpr (SPLIT) {  // O = O f + P V, tile by tile
                     const float mo = m;
                     m = fmaxf(m, ceilf(mx));  // a whole number: 15 - m below is exact, and f a power of two
                     f = m == -INFINITY ? 0.f : ex2f(mo - m);
                     l *= f;
+                    any_far = __any_sync(0xffffffffu, far);
                 } else if (j == j0) {
                     m = mx - kHalfBits<CT>;  // the reference of O, l and the weights
+                    any_far = __any_sync(0xffffffffu, far);
                 } else {
                     const bool grow = mx - m > 8.f + kHalfBits<CT>;  // (m + 8 would round to m for large scores)
-                    if (__any_sync(0xffffffffu, grow)) {
+                    if (__any_sync(0xffffffffu, grow || far)) {
+                        any_far = __any_sync(0xffffffffu, far);
                         if (!wait2(odone, j - 1)) {
                             ok = false;
                             break;
@@ -830,10 +839,8 @@ __global__ void __launch_bounds__(kTcThreads, HD == 256 || sizeof(QT) == 4 ? 1 :
                     }
                 }
                 const float nm = m == -INFINITY ? 0.f : (SPLIT ? kSplitBits - m : -m);
-                const bool far = fabsf(mx) >= kFar && mx != -INFINITY;
-                if (__any_sync(0xffffffffu, far)) {
-                    const int hi = qpos - k0, lo = A.window ? hi - A.window + 1 : -1, sk = A.sinks - k0;
-                    l += far_weights<CT, SPLIT>(ts, far, m, nm, A.scale_log2, open ? KT : hi, open ? -1 : lo, sk);
+                if (any_far) {
+                    l += far_weights<CT, SPLIT>(A, ts, far, m, qpos - k0, k0);
                 } else {
                     float sum[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
