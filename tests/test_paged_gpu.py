@@ -303,6 +303,31 @@ def test_attention_gate(ops, ctx, hd, new, lens):
     run_case(ops, ctx, 12, 4, hd, torch.float16, torch.float32, new, lens, 16, gated=True, seed=hd)
 
 
+@pytest.mark.parametrize("cache,qt", TYPES)
+@pytest.mark.parametrize("H,kv,hd", [(2, 2, 256), (12, 4, 256), (6, 1, 256), (5, 1, 256), (12, 4, 128), (8, 2, 64)])
+@pytest.mark.parametrize("new,lens", [([1, 1, 1], [1, 90, 2000]), ([700, 1, 45], [3000, 900, 45]),
+                                      ([130, 0, 3], [130, 9, 1000]), ([40] * 9, [40 + 300 * b for b in range(9)])])
+def test_attention_gate_of_every_type(ops, ctx, H, kv, hd, cache, qt, new, lens):
+    """Gates from a slice of wider rows: whole and cut items, partial tiles, several pieces of a block, groups of
+    heads that do not divide a tile; 16-bit heads of 256 take them through the ring in shared memory."""
+    dt = getattr(torch, qt)
+    C = R.Cache(ops, lens, new, kv, hd, 16, getattr(torch, cache), hd + H)
+    g = torch.Generator(device="cuda").manual_seed(H)
+    q = torch.randn(C.rows, H, hd, generator=g, device="cuda").to(dt)
+    wide = torch.randn(C.rows, 2 * H * hd + 12, generator=g, device="cuda") * 3
+    shape = ops.paged_shape(H, kv, hd, rope_dims=0, gated=True)
+    call = lambda: ops.attn_paged(ctx, shape, C.plan, q, C.kp, C.vp, gate=wide[:, 8:-4], max_new=max(new))
+    out = call()
+    assert ctx.errors() == 0
+    C.check(q, out, wide[:, 8:-4])
+    assert torch.equal(out, call())
+    wide[:, 8:-4] = 200.0  # sigmoid 1: the bits of the call without a gate
+    plain = ops.attn_paged(ctx, ops.paged_shape(H, kv, hd, rope_dims=0), C.plan, q, C.kp, C.vp, max_new=max(new))
+    assert torch.equal(call(), plain)
+    wide[:, 8:-4] = -200.0  # sigmoid 0
+    assert bool((call() == 0).all())
+
+
 @pytest.mark.parametrize("new,lens", [([1], [40000]), ([1] * 40, [37 * i + 1 for i in range(40)]), ([5, 900], [9000, 2500])])
 def test_attention_long_and_many(ops, ctx, new, lens):
     """One sequence cut among all blocks, many short ones, and long prompts."""
