@@ -19,8 +19,8 @@ namespace cg = cooperative_groups;
 // kernel is latency: a few hundred bytes in, at most some hundred KB out.  One thread block, or a
 // cluster of up to 8 when there are many rows to write; every block of the cluster repeats the sums,
 // and the cluster barrier between the last read of the lengths and the first write lets lens and
-// n_free be the inputs' own buffers.  32 decoding sequences take 3.1 us (a launch and four dependent loads),
-// 256 sequences with 23,700 rows 5.6.
+// n_free be the inputs' own buffers.  In a graph 32 decoding sequences take 3.3 us (a launch and four dependent
+// loads), 256 sequences with 23,700 rows 5.4; called from Python both take the host's 6.5.
 constexpr int kPlanThreads = 1024;
 constexpr int kPlanRowBits = 33;
 
@@ -174,8 +174,9 @@ __global__ void __launch_bounds__(kPlanThreads)
 // its heads (y): its first loads go out, and meanwhile one thread per pair computes the row's cosines
 // and sines, which all heads share, into shared memory; then each head's loads go out a head ahead.
 // HBM-bound for chunks: 4 bytes in and 2 (or 4) out per element.  2,602 rows of 24 + 2 x 4 gated heads of
-// 256 take 26 us, 4.9 TB/s; one head's loads at a time, behind the table, and the norms' weights kept in
-// registers (4 blocks per SM for 5) took 32.  Few rows are latency: 16 of 48 heads of 128 take 2.6 us.
+// 256 take 26 us in a graph (27 from Python), 5.0 TB/s; one head's loads at a time, behind the table, and the norms'
+// weights kept in registers (4 blocks per SM for 5) took 32.  Few rows are latency: 16 of 48 heads of 128 take 2.6 us
+// in a graph (11.5 from Python).
 constexpr int kAppThreads = 256;
 
 template <typename T> __device__ __forceinline__ void store4(T *p, float4 v) {
@@ -286,9 +287,9 @@ __global__ void __launch_bounds__(kAppThreads, 5) paged_append_kernel(PgAppendAr
 // fp32 queries: Q and P enter as two fp16 parts each (x = hi + lo), so that products keep 2^-22.
 // Bound by the K/V stream: rep tokens' work per byte is far below the tensor cores' rate even with 16 rows
 // padded, so the ring (64 to 192 KB per SM in flight) and short ends of pieces are what matters.
-// 3 sequences, 371 MB of fp16 K and V (16 query, 8 kv heads of 128, fp32 queries): 70 us, 5.3 TB/s.  16 sequences
-// of 900 tokens, 63 MB: 18.5 us, of which the stream is 10; the rest is the start (schedule, tables, first
-// tiles: 4 us) and the joins of cut items.
+// In a graph 3 sequences, 371 MB of fp16 K and V (16 query, 8 kv heads of 128, fp32 queries), take 70 us (76 with
+// changing inputs from Python), 5.3 TB/s; 16 sequences of 900 tokens, 63 MB, 18.2 us (22.9), of which the stream is 10: the
+// rest is the start (schedule, tables, first tiles) and the joins of cut items.
 constexpr int kDecThreads = 160;
 constexpr int kDecWarps = 4;
 constexpr int kDecTile = 64;
@@ -826,8 +827,8 @@ trx_status launch_paged_append(const PgAppendArgs &A, int cache_type, int q_type
 trx_status launch_attn_paged(const PgAttnArgs &A, int hd, int cache_type, int q_type, size_t part_cap, int cnt_cap,
                              uint32_t *err, cudaStream_t st) {
     // More query rows per kv head than the 16 of one mma.sync tile: the tcgen05 kernel, whose 128-row tiles would
-    // be mostly padding below.  16 sequences of 900 tokens, 4 (or 16) rows per kv head: 18.5 (24.2) us here, 24.6
-    // (24.7) there; 3 sequences of 30,000 tokens, fp32 queries: 70 us here, 109 there.
+    // be mostly padding below.  In a graph 16 sequences of 900 tokens, 4 (or 16) rows per kv head, take 18.5 (24.2) us
+    // here, 24.6 (24.7) there; 3 sequences of 30,000 tokens, fp32 queries: 70 us here, 109 there.
     if ((long long)A.max_new * A.rep > 16) return launch_attn_paged_tc(A, hd, cache_type, q_type, part_cap, cnt_cap, err, st);
     if (cache_type == TRX_TYPE_BF16)
         return launch_dec_hd<__nv_bfloat16, __nv_bfloat16>(A, hd, part_cap, cnt_cap, err, st);

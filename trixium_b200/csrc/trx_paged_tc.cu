@@ -7,8 +7,8 @@
 // (query tile, kv head).  Per key tile S = Q K^T (M = 128, N = KT), the softmax in 32 bits, O += P V
 // (M = 128, N = head dim).  Warp roles:
 //  * warps 0-3: one query row per thread (its TMEM lane).  They put an fp32 query tile into shared memory (a
-//    16-bit one comes by TMA), read S from tensor memory, keep the row's maximum and sum, write P (16 bits) over S as the A operand
-//    of the second product, and finish the piece.  O is rescaled only when a row's maximum has grown by
+//    16-bit one comes by TMA), read S from tensor memory, keep the row's maximum and sum, write P (16 bits) over
+//    S as the A operand of the second product, and finish the piece.  O is rescaled only when a row's maximum has grown by
 //    more than 2^8 over the one in use: P then stays below 2^8 (fp16: 2^15, see kHalfBits), exact in any 16-bit
 //    float's exponent.
 //  * warp 4: the producer.  A key tile is gathered by TMA boxes of one page (or the tile's part of it, see
@@ -16,8 +16,8 @@
 //  * warps 5 and 6: issue the MMAs of the first and of the second product, each from one elected lane. Two
 //    warps, since one's instructions between two MMAs (waits, commits) take as long as the MMAs.
 // fp32 queries: Q = hi + lo and P = hi + lo in fp16 (P and its sum times 2^15, see kSplitScale), two MMAs per
-// product, so products keep 2^-22; each
-// tile's P V is added to an O in registers (head dim 256: tensor memory) by the softmax warps.
+// product, so products keep 2^-22; each tile's P V is added to an O in registers (head dim 256: tensor memory)
+// by the softmax warps.
 // V is read as the N-major B operand of the second product straight from its row-major tile; the rows
 // of a sequence's last page behind its end are overwritten with zeros first (0 times what lies there
 // would not be 0 if it is not finite).
@@ -26,11 +26,14 @@
 // two CTAs per SM (at most 113 KB of shared memory, 256 TMEM columns each), head dim 256 and fp32 queries
 // one.
 //
-// Bound by the tensor cores and the power they draw for 16-bit heads of 128 (2,048 rows of 32 heads behind
-// 6,001 positions: 225 us, 1,050 TFLOP/s, in short runs, 272 us in long ones; 1,600 cycles a tile for two CTAs,
-// the MMAs alone 1,280); by the softmax warps, one per scheduler, with fp32 queries (4,096 rows of 16 heads, a
-// window of 1,024: 134 us); by the K and V traffic between L2 and the SMs (46 bytes a cycle and SM) for heads of
-// 256.
+// What bounds it (launches in a row or in a graph; tensor pipe and cycles by ncu):
+//  - 16-bit heads of 128: the products and the power they draw.  2,048 rows of 32 heads behind 6,001 positions: 231 us,
+//    1,020 TFLOP/s, in short runs, 276 us in long ones.  1,032 cycles a tile of 128 x 64, its MMAs' math 512 (pipe at
+//    50 %): S, 64 keys wide, reads 6 KB of shared memory (48 cycles) for 32 cycles of math, so 640 at least.
+//  - fp32 queries: the softmax warps, one per scheduler.  4,096 rows of 16 heads, a window of 1,024: 137 to 141 us,
+//    3,750 cycles a tile, ends of pieces included, its MMAs 1,024 (27 %).
+//  - heads of 256: the ends of pieces, and K and V from L2 (64 KB a tile).  1,137 rows of 24 gated heads, 9 sequences:
+//    101 us, 3,470 cycles a tile, its MMAs 1,024 (30 %); 32 bytes a cycle and SM from L2 over the whole launch.
 #include <algorithm>
 #include <cstdint>
 #include <cstring>
@@ -181,9 +184,9 @@ __device__ __forceinline__ void tm_wait_ld() { asm volatile("tcgen05.wait::ld.sy
 __device__ __forceinline__ void tm_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
 // The gates of a piece on their way to a warp's ring: 16 dims of its 32 rows at a time, each row's 64 bytes read
-// by four lanes together, kept swizzled so that a lane per row reads them without conflicts.  Loads by the thread
-// of a row at the time of use (32 lines per access, one round trip per 32 dims) made the end of a piece of 128
-// gated rows x 256 dims take 38,000 cycles; this way 25,000 (1,137 rows of 24 gated heads: 114 to 101 us).
+// by four lanes together, kept swizzled so that a lane per row reads them without conflicts.  With loads by the
+// thread of a row at the time of use (32 lines per access, one round trip per 32 dims) 1,137 rows of 24 gated heads of
+// 256 took 114 us, this way 101.
 struct GateRing {
     uint32_t at;       // shared address of the warp's ring
     long long row0;    // the piece's first row and head, its rows

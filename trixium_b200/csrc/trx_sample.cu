@@ -22,8 +22,9 @@
 //  4. Unless block 0 has drawn: the draw over the whole row: each warp sums its contiguous part, the
 //     parts' prefix tells which warp holds the token, and that warp sums its part again, a lane at a time.
 // Bound by the arithmetic of the weights (about 50 instructions each, twice 32 bits of sum) and of the counts, and
-// by the cluster's barriers: one row of 151,936 takes 17 us, 32 of them 51 us (19 MB; the bytes alone 3 us), 333
-// rows of 32,003 67 us.  A cluster per row keeps the row on chip between its three to five passes.
+// by the cluster's barriers: in a graph one row of 151,936 takes 17 us, 32 of them 51 us (54 to 65 from Python, by their
+// settings; 19 MB, the bytes alone 3 us), 333 rows of 32,003 68 us.  A cluster per row keeps the row on chip between
+// its three to five passes.
 #include <cfloat>
 #include <cstdint>
 #include <cooperative_groups.h>
